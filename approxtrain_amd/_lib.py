@@ -23,6 +23,11 @@ def lib_path():
 
 _i, _i64, _sz, _p, _f = C.c_int, C.c_int64, C.c_size_t, C.c_void_p, C.c_void_p
 
+class AdamWHyper(C.Structure):
+    """amsim_adamw_hyper of include/amsim.h."""
+    _fields_ = [("step", C.c_int64)] + [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+
+
 # name -> (restype, argtypes); mirrors include/amsim.h and include/amsim_bench.h declaration by declaration
 SIGNATURES = {
     "amsim_status_string": (C.c_char_p, [_i]),
@@ -74,6 +79,15 @@ SIGNATURES = {
     "amsim_attention_grad_f32": (_i, [_p, _f, _f, _f, _f, _f] + [_i] * 5 + [C.c_float, _f, _f, _f, _p, _sz, _p]),
     "amsim_epilogue_grad_workspace_bytes": (_sz, [_i64, _i]),
     "amsim_epilogue_grad_f32": (_i, [_f, _f, _i64, _i, _i, _f, _f, _p, _sz, _p]),
+    "amsim_mxfp4_operand_workspace_bytes": (_sz, [_i64, _i64]),
+    "amsim_mxfp4_quantize": (_i, [_p, _i, _i64, _i64, _i64, _p, _p, _p]),
+    "amsim_mxfp4_dequantize": (_i, [_p, _i64, _i64, _i, _p, _p]),
+    "amsim_mxfp4_matmul_workspace_bytes": (_sz, [_i64] * 3),
+    "amsim_mxfp4_matmul": (_i, [_p, _p, _i64, _i64, _i64, _p, _i, _i, _p, _i, _p, _sz, _p]),
+    "amsim_mxfp4_linear_workspace_bytes": (_sz, [_i64] * 3),
+    "amsim_mxfp4_linear": (_i, [_p, _i, _i64, _p, _i64, _i64, _i64, _p, _i, _i, _p, _p, _sz, _p]),
+    "amsim_adamw_step": (_i, [_i, _p, _p, _p, _i, _i, _i, _p, _p, _f, _f, _p, _f, _p]),
+    "amsim_adamw_state_values": (_i, [_p, _f, _i64, _i, _f, _p]),
     "amsim_conv_geometry": (_i, [_i, _i, _i, _i, C.POINTER(_i), C.POINTER(_i)]),
     "amsim_set_split_k": (_i, [_i]),
     "amsim_set_engine": (_i, [_i]),

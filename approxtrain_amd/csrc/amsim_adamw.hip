@@ -1,0 +1,306 @@
+// One AdamW step over many tensors, with the moments in 32 bits or in 8.
+//
+//   g = grad [* grad_scale]      m' = beta1 m + (1 - beta1) g      v' = beta2 v + ((1 - beta2) g) g
+//   p' = p (1 - lr decay) - (m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)) * lr / (1 - beta1^t)
+//
+// Every operation is one rounding in 32 bits (no contraction), in this order.  Bound by memory: 28 bytes per
+// element with 32-bit parameters, gradients and moments, 16 with 8-bit moments, each read and written once.
+// One launch serves as many tensors as its arguments hold: a tensor is an entry of 24 bytes, and the moments of
+// all tensors lie in one buffer, each tensor from a multiple of 256 elements on, so that no table has to be
+// sent to the device ahead of the kernel.
+//
+// 8-bit moments: a wavefront's 256 elements share a 32-bit scale, the largest magnitude among them.  m is held as
+// sign, 4 bits of exponent and 3 of mantissa of |m| / scale; v as its root r = sqrt(v), which halves the binades
+// to cover, with 4 and 4 bits.  A code is the upper bits of the relative magnitude's 32-bit form, rounded to nearest-even,
+// counted down from 1.0 at the largest code: 16 binades.  An |m| below half the smallest code becomes 0, an
+// r above 0 never does: its element would otherwise be divided by eps alone.
+#include "amsim_mx.h"
+
+#include <cmath>
+
+namespace amsim {
+
+namespace {
+
+constexpr int WG = 256;
+constexpr int BLOCK = 256;             // elements that share a scale
+constexpr int CHUNK_BLOCKS = 16;       // blocks of a workgroup: four per wavefront
+constexpr int TABLE = 120;             // tensors per launch (arguments: below 4 KB)
+
+struct Entry {
+    void *p;
+    const void *g;
+    int64_t n;
+};
+struct AdamWArgs {
+    Entry t[TABLE];
+    int first_chunk[TABLE + 1];        // workgroups before each tensor's
+    int blocks_before[TABLE];          // blocks of the moments' buffer from first_block to each tensor's
+    int count;
+    int64_t first_block;               // of the moments' buffer, where this launch's tensors begin
+    void *m, *v;
+    float *m_scale, *v_scale;
+    const float *grad_scale;
+    float keep, beta1, grad1, beta2, grad2, inv_root2, step_size, eps;
+};
+
+__device__ __forceinline__ float wave_max(float v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const float w = __shfl_xor(v, o, 64);
+        v = __float_as_uint(w) > __float_as_uint(v) ? w : v;  // (magnitudes: a NaN is above all others)
+    }
+    return v;
+}
+
+template <int SHIFT, int BASE> __device__ __forceinline__ float magnitude(uint32_t code)
+{
+    return code ? __uint_as_float((code + BASE) << SHIFT) : 0.0f;
+}
+template <int SHIFT, int BASE, int LARGEST> __device__ __forceinline__ uint32_t code_of(float t)
+{
+    const uint32_t bits = __float_as_uint(t);
+    const int c = (int)((bits + ((1u << (SHIFT - 1)) - 1) + ((bits >> SHIFT) & 1)) >> SHIFT) - BASE;
+    return (uint32_t)min(max(c, 1), LARGEST);
+}
+constexpr int M_SHIFT = 20, M_BASE = 889, M_LARGEST = 127;    // 1.0 is 1016 << 20
+constexpr int R_SHIFT = 19, R_BASE = 1777, R_LARGEST = 255;   // 1.0 is 2032 << 19
+
+__device__ __forceinline__ float m_value(uint32_t c, float scale)
+{
+    const float v = magnitude<M_SHIFT, M_BASE>(c & 127) * scale;
+    return c & 128 ? -v : v;
+}
+__device__ __forceinline__ float r_value(uint32_t c, float scale) { return magnitude<R_SHIFT, R_BASE>(c) * scale; }
+__device__ __forceinline__ uint32_t m_code(float m, float scale)
+{
+    const float t = scale > 0.0f ? fabsf(m) / scale : 0.0f;
+    const uint32_t c = t < magnitude<M_SHIFT, M_BASE>(1) * 0.5f ? 0 : code_of<M_SHIFT, M_BASE, M_LARGEST>(t);
+    return m < 0.0f ? c | 128 : c;
+}
+__device__ __forceinline__ uint32_t r_code(float r, float scale)
+{
+    const float t = scale > 0.0f ? r / scale : 0.0f;
+    return t == 0.0f ? 0 : code_of<R_SHIFT, R_BASE, R_LARGEST>(t);
+}
+
+// four neighbouring elements, of which `count` exist
+template <typename T> __device__ __forceinline__ void load4(const T *p, int count, float (&v)[4])
+{
+    T t[4] = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
+    if (count == 4 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0) {
+        __builtin_memcpy(t, __builtin_assume_aligned(p, 4 * sizeof(T)), sizeof(t));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < count) t[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = to_float(t[i]);
+}
+template <typename T> __device__ __forceinline__ void store4(T *p, int count, const float (&v)[4])
+{
+    T t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = from_float<T>(v[i]);
+    if (count == 4 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0) {
+        __builtin_memcpy(__builtin_assume_aligned(p, 4 * sizeof(T)), t, sizeof(t));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < count) p[i] = t[i];
+    }
+}
+
+template <typename P, typename G, bool BITS8>
+__global__ __launch_bounds__(WG) void adamw_kernel(AdamWArgs a)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int lo = 0, hi = a.count;  // the tensor whose chunk this is: first_chunk[lo] <= blockIdx.x < first_chunk[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if ((int)blockIdx.x >= a.first_chunk[mid]) lo = mid;
+        else hi = mid;
+    }
+    const Entry t = a.t[lo];
+    const int64_t before = a.first_block + a.blocks_before[lo];
+    const float scale_g = a.grad_scale ? *a.grad_scale : 1.0f;
+    const int64_t blocks = (t.n + BLOCK - 1) / BLOCK, chunk = (int64_t)((int)blockIdx.x - a.first_chunk[lo]) * CHUNK_BLOCKS;
+    for (int64_t b = chunk + wave; b < chunk + CHUNK_BLOCKS && b < blocks; b += WG / 64) {
+        const int64_t i = b * BLOCK + lane * 4, s = (before + b) * BLOCK + lane * 4;
+        const int count = (int)(t.n - i >= 4 ? 4 : t.n - i > 0 ? t.n - i : 0);
+        float p[4], g[4], m[4], v[4];
+        load4((const P *)t.p + i, count, p);
+        load4((const G *)t.g + i, count, g);
+        uint32_t mc = 0, rc = 0;
+        float ms = 0, rs = 0;
+        if (BITS8) {
+            mc = *(const uint32_t *)((const uint8_t *)a.m + s);
+            rc = *(const uint32_t *)((const uint8_t *)a.v + s);
+            ms = a.m_scale[before + b];
+            rs = a.v_scale[before + b];
+        } else {
+            const v4f mv = *(const v4f *)((const float *)a.m + s), vv = *(const v4f *)((const float *)a.v + s);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[e] = mv[e], v[e] = vv[e];
+        }
+        float r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (BITS8) {
+                m[e] = m_value((mc >> (8 * e)) & 255, ms);
+                v[e] = r_value((rc >> (8 * e)) & 255, rs);
+                v[e] = v[e] * v[e];
+            }
+            if (a.grad_scale) g[e] = g[e] * scale_g;
+            m[e] = m[e] * a.beta1 + g[e] * a.grad1;
+            v[e] = v[e] * a.beta2 + (g[e] * a.grad2) * g[e];
+            r[e] = sqrtf(v[e]);
+            const float denominator = r[e] * a.inv_root2 + a.eps;
+            p[e] = p[e] * a.keep - (m[e] / denominator) * a.step_size;
+        }
+        store4((P *)t.p + i, count, p);
+        if (BITS8) {
+            float mx = 0, rx = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (e >= count) m[e] = r[e] = 0.0f;
+                const float am = fabsf(m[e]), ar = fabsf(r[e]);
+                mx = __float_as_uint(am) > __float_as_uint(mx) ? am : mx;
+                rx = __float_as_uint(ar) > __float_as_uint(rx) ? ar : rx;
+            }
+            mx = wave_max(mx);
+            rx = wave_max(rx);
+            mc = rc = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                mc |= m_code(m[e], mx) << (8 * e);
+                rc |= r_code(r[e], rx) << (8 * e);
+            }
+            *(uint32_t *)((uint8_t *)a.m + s) = mc;
+            *(uint32_t *)((uint8_t *)a.v + s) = rc;
+            if (lane == 0) {
+                a.m_scale[before + b] = mx;
+                a.v_scale[before + b] = rx;
+            }
+        } else {
+            v4f mv, vv;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mv[e] = e < count ? m[e] : 0.0f, vv[e] = e < count ? v[e] : 0.0f;
+            *(v4f *)((float *)a.m + s) = mv;
+            *(v4f *)((float *)a.v + s) = vv;
+        }
+    }
+}
+
+template <bool ROOTS>
+__global__ __launch_bounds__(WG) void state_values_kernel(const uint8_t *codes, const float *scales, int64_t quads, float *out)
+{
+    const int64_t q = (int64_t)blockIdx.x * WG + threadIdx.x;
+    if (q >= quads) return;
+    const uint32_t c = ((const uint32_t *)codes)[q];
+    const float s = scales[q / (BLOCK / 4)];
+    v4f v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = ROOTS ? r_value((c >> (8 * e)) & 255, s) : m_value((c >> (8 * e)) & 255, s);
+    ((v4f *)out)[q] = v;
+}
+
+template <typename P, typename G> void launch_adamw(const AdamWArgs &a, int state_bits, hipStream_t stream)
+{
+    const unsigned chunks = (unsigned)a.first_chunk[a.count];
+    if (state_bits == 8) adamw_kernel<P, G, true><<<chunks, WG, 0, stream>>>(a);
+    else adamw_kernel<P, G, false><<<chunks, WG, 0, stream>>>(a);
+}
+template <typename P> void launch_adamw_grad(const AdamWArgs &a, int grad_dtype, int state_bits, hipStream_t stream)
+{
+    switch (grad_dtype) {
+    case AMSIM_DTYPE_F32: launch_adamw<P, float>(a, state_bits, stream); break;
+    case AMSIM_DTYPE_BF16: launch_adamw<P, __bf16>(a, state_bits, stream); break;
+    default: launch_adamw<P, _Float16>(a, state_bits, stream); break;
+    }
+}
+
+}  // namespace
+
+}  // namespace amsim
+
+using namespace amsim;
+
+extern "C" {
+
+int amsim_adamw_step(int count, void *const *params, const void *const *grads, const int64_t *sizes, int param_dtype, int grad_dtype,
+                     int state_bits, void *m, void *v, float *m_scale, float *v_scale, const amsim_adamw_hyper *hyper,
+                     const float *grad_scale, void *stream)
+{
+    if (!known_dtype(param_dtype) || !known_dtype(grad_dtype)) return fail(AMSIM_ERR_INVALID, "adamw: unknown element type");
+    if (state_bits != 32 && state_bits != 8) return fail(AMSIM_ERR_INVALID, "adamw: states have 32 or 8 bits");
+    if (count < 0 || !hyper || (count && (!params || !grads || !sizes))) return fail(AMSIM_ERR_INVALID, "adamw: negative count or null pointer");
+    const double lr = hyper->lr, beta1 = hyper->beta1, beta2 = hyper->beta2, eps = hyper->eps, weight_decay = hyper->weight_decay;
+    const int64_t step = hyper->step;
+    if (step < 1) return fail(AMSIM_ERR_INVALID, "adamw: step below 1");
+    if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0)) return fail(AMSIM_ERR_INVALID, "adamw: betas or eps out of range");
+    int64_t chunks = 0;
+    for (int i = 0; i < count; ++i) {
+        if (sizes[i] < 0) return fail(AMSIM_ERR_INVALID, "adamw: negative size");
+        if (sizes[i] && !params[i]) return fail(AMSIM_ERR_INVALID, "adamw: null pointer");
+        if (((uintptr_t)params[i] & (element_bytes(param_dtype) - 1)) || ((uintptr_t)grads[i] & (element_bytes(grad_dtype) - 1)))
+            return fail(AMSIM_ERR_INVALID, "adamw: misaligned pointer");
+        if (sizes[i] > (1ll << 35)) return fail(AMSIM_ERR_UNSUPPORTED, "adamw: tensor of more than 2^35 elements");
+        chunks += ceil_div64(sizes[i], BLOCK * CHUNK_BLOCKS);
+    }
+    if (chunks == 0) return AMSIM_OK;
+    if (!m || !v || (state_bits == 8 && (!m_scale || !v_scale))) return fail(AMSIM_ERR_INVALID, "adamw: null pointer");
+    if (((uintptr_t)m & 15) || ((uintptr_t)v & 15)) return fail(AMSIM_ERR_INVALID, "adamw: misaligned pointer");
+    AdamWArgs a{};
+    a.m = m, a.v = v, a.m_scale = m_scale, a.v_scale = v_scale, a.grad_scale = grad_scale;
+    a.keep = (float)(1.0 - lr * weight_decay);
+    a.beta1 = (float)beta1, a.grad1 = (float)(1.0 - beta1), a.beta2 = (float)beta2, a.grad2 = (float)(1.0 - beta2);
+    a.inv_root2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+    a.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+    a.eps = (float)eps;
+    int64_t block = 0;
+    for (int i = 0; i < count;) {
+        a.count = 0;
+        a.first_block = block;
+        int64_t here = 0, blocks = 0;
+        for (; i < count && a.count < TABLE; ++i) {
+            const int64_t c = ceil_div64(sizes[i], BLOCK * CHUNK_BLOCKS), n = ceil_div64(sizes[i], BLOCK);
+            if (here + c >= (1ll << 24) || blocks + n >= (1ll << 31)) break;
+            if (sizes[i] && grads[i]) {
+                a.t[a.count] = Entry{params[i], grads[i], sizes[i]};
+                a.blocks_before[a.count] = (int)blocks;
+                a.first_chunk[a.count++] = (int)here;
+                here += c;
+            }
+            blocks += n;
+        }
+        block += blocks;
+        a.first_chunk[a.count] = (int)here;
+        if (a.count == 0) continue;
+        switch (param_dtype) {
+        case AMSIM_DTYPE_F32: launch_adamw_grad<float>(a, grad_dtype, state_bits, (hipStream_t)stream); break;
+        case AMSIM_DTYPE_BF16: launch_adamw_grad<__bf16>(a, grad_dtype, state_bits, (hipStream_t)stream); break;
+        default: launch_adamw_grad<_Float16>(a, grad_dtype, state_bits, (hipStream_t)stream); break;
+        }
+        AMSIM_HIP_CHECK(hipGetLastError());
+    }
+    return AMSIM_OK;
+}
+
+int amsim_adamw_state_values(const void *codes, const float *scales, int64_t blocks, int roots, float *out, void *stream)
+{
+    if (blocks < 0) return fail(AMSIM_ERR_INVALID, "adamw: negative size");
+    if (!codes || !scales || !out) return fail(AMSIM_ERR_INVALID, "adamw: null pointer");
+    if (blocks == 0) return AMSIM_OK;
+    if (((uintptr_t)codes & 3) || ((uintptr_t)out & 15)) return fail(AMSIM_ERR_INVALID, "adamw: misaligned pointer");
+    const int64_t quads = blocks * (BLOCK / 4), groups = ceil_div64(quads, WG);
+    if (groups >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "adamw: more blocks than one launch takes");
+    if (roots) state_values_kernel<true><<<(unsigned)groups, WG, 0, (hipStream_t)stream>>>((const uint8_t *)codes, scales, quads, out);
+    else state_values_kernel<false><<<(unsigned)groups, WG, 0, (hipStream_t)stream>>>((const uint8_t *)codes, scales, quads, out);
+    AMSIM_HIP_CHECK(hipGetLastError());
+    return AMSIM_OK;
+}
+
+}  // extern "C"

@@ -8,8 +8,9 @@ import functools
 
 import torch
 
-from ._lib import check, conv_geometry, load_library
+from ._lib import AdamWHyper, check, conv_geometry, load_library
 from .lut import ApproxMulLut
+from .mx import DTYPES, MXTensor
 
 
 def _dev(t, name):
@@ -355,3 +356,261 @@ def epilogue_grad_checked(grad, out, has_bias, act):
                                       ws.data_ptr() if nbytes else None, nbytes,
                                       torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())))
     return grad_z, grad_bias
+
+
+# ---- microscaled 4-bit floats and their products ---------------------------------------------------
+
+def _device_of(t, name):
+    """Index of the device that holds ``t``; the library launches on the current one."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a tensor in device memory (there is no CPU path)")
+    index = t.get_device()
+    if index != torch._C._cuda_getDevice():
+        raise ValueError(f"{name} is on device {index}, which is not the current one")
+    return index
+
+
+def _mx_source(x, name="x"):
+    """(tensor, element type, rows, columns, row stride, whether rows and columns have changed places): a
+    rank-2 tensor as the library reads it, in place where either of its axes is contiguous."""
+    _device_of(x, name)
+    dtype = DTYPES.get(x.dtype)
+    if dtype is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
+    if x.dim() != 2:
+        raise ValueError(f"{name} must be a matrix")
+    rows, cols = x.shape
+    if rows == 0 or cols == 0:
+        raise ValueError(f"{name} is empty: blocks of no elements have no scale")
+    s0, s1 = x.stride()
+    if x.is_neg():
+        x = x.resolve_neg()
+        s0, s1 = x.stride()
+    if (s1 == 1 or cols == 1) and (s0 >= cols or rows == 1):
+        return x, dtype, rows, cols, s0 if rows > 1 else cols, False
+    if (s0 == 1 or rows == 1) and (s1 >= rows or cols == 1):
+        return x, dtype, cols, rows, s1 if cols > 1 else rows, True
+    return x.contiguous(), dtype, rows, cols, cols, False
+
+
+@functools.lru_cache(maxsize=1024)
+def _mx_bytes(rows, length):
+    n = load_library().amsim_mxfp4_operand_workspace_bytes(rows, length)
+    if n == 0:
+        raise ValueError(f"a {rows} x {length} tensor is out of the 4-bit products' range")
+    return n
+
+
+def _mx_empty(like, rows, length):
+    return MXTensor(torch.empty(_mx_bytes(rows, length), dtype=torch.uint8, device=like.device), rows, length)
+
+
+def _mx_quantize(x, by_rows, by_columns):
+    x, dtype, rows, cols, stride, swapped = _mx_source(x)
+    if swapped:
+        by_rows, by_columns = by_columns, by_rows
+    r = _mx_empty(x, rows, cols) if by_rows else None
+    c = _mx_empty(x, cols, rows) if by_columns else None
+    check(load_library().amsim_mxfp4_quantize(x.data_ptr(), dtype, rows, cols, stride, r.data.data_ptr() if by_rows else None,
+                                              c.data.data_ptr() if by_columns else None,
+                                              torch._C._cuda_getCurrentRawStream(x.get_device())))
+    return (c, r) if swapped else (r, c)
+
+
+def mxfp4_quantize(x, axis=-1):
+    """Matrix ``x`` (float32, bfloat16 or float16, any strides) as an MXFP4 operand whose blocks of 32 run along
+    ``axis``, the axis that a product will sum over: ``-1`` gives an operand of x's rows, ``0`` one of its
+    columns (x's transpose, read in place)."""
+    if axis in (-1, 1):
+        return _mx_quantize(x, True, False)[0]
+    if axis in (0, -2):
+        return _mx_quantize(x, False, True)[1]
+    raise ValueError("axis must be 0 or 1 (or -2 or -1)")
+
+
+def mxfp4_quantize_both(x):
+    """``(mxfp4_quantize(x, -1), mxfp4_quantize(x, 0))`` from one reading of ``x``."""
+    return _mx_quantize(x, True, True)
+
+
+def _mx_operand(q, name):
+    if not isinstance(q, MXTensor):
+        raise TypeError(f"{name} must be an MXTensor (functors.mxfp4_quantize)")
+    _device_of(q.data, name)
+    return q
+
+
+def _mx_dtype(dtype):
+    if dtype not in DTYPES:
+        raise TypeError(f"the result's type must be float32, bfloat16 or float16, got {dtype}")
+    return DTYPES[dtype]
+
+
+def mxfp4_dequantize(q, dtype=torch.float32):
+    """The values of an MXFP4 operand, ``[rows, length]``."""
+    _mx_operand(q, "q")
+    code = _mx_dtype(dtype)
+    out = torch.empty((q.rows, q.length), dtype=dtype, device=q.data.device)
+    check(load_library().amsim_mxfp4_dequantize(q.data.data_ptr(), q.rows, q.length, code, out.data_ptr(),
+                                                torch._C._cuda_getCurrentRawStream(out.get_device())))
+    return out
+
+
+def _mx_epilogue(bias, activation, units, device):
+    if activation not in ACTIVATIONS:
+        raise ValueError("fused activation must be None, 'linear' or 'relu'")
+    if bias is None:
+        return None, None, 0, ACTIVATIONS[activation]
+    if _device_of(bias, "bias") != device:
+        raise ValueError("bias must be on the operands' device")
+    if bias.dtype not in DTYPES:
+        raise TypeError(f"bias must be float32, bfloat16 or float16, got {bias.dtype}")
+    if bias.dim() != 1 or bias.shape[0] != units:
+        raise ValueError("bias must have one entry per output channel")
+    bias = bias.contiguous()
+    return bias, bias.data_ptr(), DTYPES[bias.dtype], ACTIVATIONS[activation]
+
+
+@functools.lru_cache(maxsize=1024)
+def _mx_matmul_workspace(m, n, k):
+    return load_library().amsim_mxfp4_matmul_workspace_bytes(m, n, k)
+
+
+@functools.lru_cache(maxsize=1024)
+def _mx_linear_workspace(m, n, k):
+    return load_library().amsim_mxfp4_linear_workspace_bytes(m, n, k)
+
+
+def _scratch(nbytes, device):
+    # (torch's allocations start on 512-byte boundaries)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def mxfp4_matmul(a, b, bias=None, activation=None, dtype=torch.float32):
+    """``activation(a . b^T + bias)`` of two MXFP4 operands of one length: ``[a.rows, b.rows]``, summed in 32
+    bits and rounded to ``dtype`` once."""
+    _mx_operand(a, "a"), _mx_operand(b, "b")
+    if a.length != b.length:
+        raise ValueError("the operands' lengths differ")
+    code = _mx_dtype(dtype)
+    keep, bptr, bcode, act = _mx_epilogue(bias, activation, b.rows, a.data.get_device())
+    out = torch.empty((a.rows, b.rows), dtype=dtype, device=a.data.device)
+    nbytes = _mx_matmul_workspace(a.rows, b.rows, a.length)
+    ws = _scratch(nbytes, out.device)
+    check(load_library().amsim_mxfp4_matmul(a.data.data_ptr(), b.data.data_ptr(), a.rows, b.rows, a.length, bptr, bcode, act,
+                                            out.data_ptr(), code, ws.data_ptr() if nbytes else None, nbytes,
+                                            torch._C._cuda_getCurrentRawStream(out.get_device())))
+    return out
+
+
+def mxfp4_linear(x, weights, bias=None, activation=None):
+    """``activation(Q(x) . weights^T + bias)`` for activations ``x`` ``[..., length]``, which are quantised on the
+    way, and weights that lie in MXFP4: ``mxfp4_quantize(kernel, axis=0)`` of a ``[length, units]`` kernel.  The
+    result has x's type."""
+    w = _mx_operand(weights, "weights")
+    if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] != w.length:
+        raise ValueError("x's last axis must have the weights' length")
+    flat = x if x.dim() == 2 else x.reshape(-1, w.length)
+    if flat.shape[0] == 0:
+        return x.new_empty(tuple(x.shape[:-1]) + (w.rows,))
+    flat, dtype, m, k, stride, swapped = _mx_source(flat)
+    if swapped:
+        flat, m, k, stride = flat.contiguous(), k, m, m
+    keep, bptr, bcode, act = _mx_epilogue(bias, activation, w.rows, flat.get_device())
+    out = torch.empty((m, w.rows), dtype=flat.dtype, device=flat.device)
+    nbytes = _mx_linear_workspace(m, w.rows, k)
+    ws = _scratch(nbytes, out.device)
+    check(load_library().amsim_mxfp4_linear(flat.data_ptr(), dtype, stride, w.data.data_ptr(), m, w.rows, k, bptr, bcode, act,
+                                            out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes,
+                                            torch._C._cuda_getCurrentRawStream(out.get_device())))
+    return out if x.dim() == 2 else out.reshape(tuple(x.shape[:-1]) + (w.rows,))
+
+
+# ---- AdamW over many tensors -----------------------------------------------------------------------
+
+class AdamWState:
+    """Moments of a list of tensors (one type, one device, contiguous) for ``adamw_step``, in one buffer: each tensor's
+    begin at a multiple of 256 elements.  ``state_bits`` 32: ``m`` and ``v`` are float32.  8: ``m`` and ``v``
+    (the latter's square roots) are bytes relative to ``m_scale`` and ``v_scale``, one float32 per 256."""
+
+    BLOCK = 256
+
+    def __init__(self, params, state_bits=32):
+        params = list(params)
+        if state_bits not in (32, 8):
+            raise ValueError("state_bits must be 32 or 8")
+        if not params:
+            raise ValueError("no tensors to hold moments of")
+        self.device_index = _device_of(params[0], "params[0]")
+        self.dtype = params[0].dtype
+        if self.dtype not in DTYPES:
+            raise TypeError(f"parameters must be float32, bfloat16 or float16, got {self.dtype}")
+        self.params, self.state_bits = params, state_bits
+        self.sizes = [p.numel() for p in params]
+        self._check(params, "params", self.dtype)
+        self.starts, at = [], 0
+        for n in self.sizes:
+            self.starts.append(at)
+            at += -(-n // self.BLOCK) * self.BLOCK
+        device = params[0].device
+        kind = torch.float32 if state_bits == 32 else torch.uint8
+        self.m, self.v = torch.zeros(at, dtype=kind, device=device), torch.zeros(at, dtype=kind, device=device)
+        scales = at // self.BLOCK if state_bits == 8 else 0
+        self.m_scale, self.v_scale = torch.zeros(scales, device=device), torch.zeros(scales, device=device)
+        self._c_sizes = (C.c_int64 * len(params))(*self.sizes)
+        self._pointers = C.c_void_p * len(params)
+
+    def _check(self, tensors, name, dtype):
+        index = self.device_index
+        for i, (t, n) in enumerate(zip(tensors, self.sizes)):
+            if t is not None and (t.dtype is not dtype or t.numel() != n or t.get_device() != index or not t.is_contiguous() or t.is_neg()):
+                raise ValueError(f"{name}[{i}] must be a contiguous {dtype} tensor of {n} elements on device {index}")
+
+    def _values(self, codes, scales, roots):
+        out = torch.empty(codes.numel(), device=codes.device)
+        if out.numel():
+            check(load_library().amsim_adamw_state_values(codes.data_ptr(), scales.data_ptr(), scales.numel(), roots, out.data_ptr(),
+                                                          torch._C._cuda_getCurrentRawStream(_device_of(codes, "codes"))))
+        return out
+
+    def first_moments(self):
+        """The values of the first moments in the buffer's order, float32."""
+        return self.m if self.state_bits == 32 else self._values(self.m, self.m_scale, 0)
+
+    def second_roots(self):
+        """The square roots of the second moments in the buffer's order, float32."""
+        return self.v.sqrt() if self.state_bits == 32 else self._values(self.v, self.v_scale, 1)
+
+
+def adamw_step(state, grads, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, grad_scale=None):
+    """Updates ``state.params`` and the moments in place by one AdamW step, the ``step``-th from 1 on, in one
+    launch for about a hundred tensors.  ``grads``: a contiguous tensor, or None (its parameter stays as it is), for each
+    parameter, all of one type.  ``grad_scale``: a float32 tensor of one element on the device that multiplies
+    the gradients (a clipping factor, say), or None."""
+    params = state.params
+    grads = list(grads)
+    if len(grads) != len(params):
+        raise ValueError("as many gradients as parameters are needed")
+    if torch._C._cuda_getDevice() != state.device_index:
+        raise ValueError("the parameters' device is not the current one")
+    gdtype = next((g.dtype for g in grads if g is not None), None)
+    if gdtype is None:
+        return
+    if gdtype not in DTYPES:
+        raise TypeError(f"gradients must be float32, bfloat16 or float16, got {gdtype}")
+    state._check(params, "params", state.dtype)
+    state._check(grads, "grads", gdtype)
+    if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1
+                                   or grad_scale.get_device() != state.device_index):
+        raise ValueError("grad_scale must be one float32 on the parameters' device")
+    table = state._pointers
+    hyper = AdamWHyper(step, lr, beta1, beta2, eps, weight_decay)
+    bits8 = state.state_bits == 8
+    check(load_library().amsim_adamw_step(len(params), table(*[p.data_ptr() for p in params]),
+                                          table(*[None if g is None else g.data_ptr() for g in grads]), state._c_sizes,
+                                          DTYPES[state.dtype], DTYPES[gdtype], state.state_bits, state.m.data_ptr(), state.v.data_ptr(),
+                                          state.m_scale.data_ptr() if bits8 else None, state.v_scale.data_ptr() if bits8 else None,
+                                          C.byref(hyper), grad_scale.data_ptr() if grad_scale is not None else None,
+                                          torch._C._cuda_getCurrentRawStream(state.device_index)))
+    # (written behind autograd's back: a graph that saved a parameter has to notice)
+    torch.autograd.graph.increment_version(params)

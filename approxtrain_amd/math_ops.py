@@ -77,3 +77,51 @@ def matmulam(a, b, transpose_a=False, transpose_b=False, adjoint_a=False, adjoin
     if a.dim() > 3 or b.dim() > 3:
         out = out.reshape(tuple(lead) + tuple(out.shape[-2:]))
     return out
+
+
+class _LinearMX(torch.autograd.Function):
+    """``activation(Q(x) . Q(kernel) + bias)`` in MXFP4.  Each of the three products has its operands quantised
+    along the axis it sums over, so x, the kernel and the gradient are quantised both ways, each from one
+    reading; what the backward pass needs is kept in 4 bits."""
+
+    @staticmethod
+    def forward(ctx, x, kernel, bias, activation):
+        need_x, need_kernel = ctx.needs_input_grad[:2]
+        by_rows, by_columns = functors.mxfp4_quantize_both(x) if need_kernel else (functors.mxfp4_quantize(x), None)
+        w_rows, w_columns = functors.mxfp4_quantize_both(kernel) if need_x else (None, functors.mxfp4_quantize(kernel, axis=0))
+        out = functors.mxfp4_matmul(by_rows, w_columns, bias, activation, x.dtype)
+        relu = activation == "relu"
+        ctx.save_for_backward(by_columns.data if need_kernel else None, w_rows.data if need_x else None, out if relu else None)
+        ctx.attrs = (x.shape, kernel.shape, x.dtype, kernel.dtype, None if bias is None else bias.dtype)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x_columns, w_rows, out = ctx.saved_tensors
+        (rows, width), (_, units), x_dtype, kernel_dtype, bias_dtype = ctx.attrs
+        if out is not None:
+            grad = grad * (out > 0)
+        grad_x = grad_kernel = grad_bias = None
+        g_rows, g_columns = functors.mxfp4_quantize_both(grad)
+        if ctx.needs_input_grad[0]:
+            grad_x = functors.mxfp4_matmul(g_rows, functors.MXTensor(w_rows, width, units), dtype=x_dtype)
+        if ctx.needs_input_grad[1]:
+            grad_kernel = functors.mxfp4_matmul(functors.MXTensor(x_columns, width, rows), g_columns, dtype=kernel_dtype)
+        if bias_dtype is not None and ctx.needs_input_grad[2]:
+            grad_bias = grad.sum(0, dtype=torch.float32).to(bias_dtype)
+        return grad_x, grad_kernel, grad_bias, None
+
+
+def linearmx(x, kernel, bias=None, activation=None):
+    """``activation(x . kernel + bias)`` with both operands, and in the backward pass the gradient, in microscaled
+    4-bit floating point: ``x`` ``[..., width]``, ``kernel`` ``[width, units]`` and ``bias`` ``[units]`` in float32,
+    bfloat16 or float16 each; the result has x's type, each gradient its own tensor's.  ``activation``: None,
+    'linear' or 'relu', applied as the result is stored.  (Gradients of gradients are not provided.)"""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1 or kernel.dim() != 2 or x.shape[-1] != kernel.shape[0]:
+        raise ValueError("linearmx expects x [..., width] and kernel [width, units]")
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if flat.numel() == 0 or kernel.numel() == 0:
+        raise ValueError("linearmx of no elements")
+    out = _LinearMX.apply(flat, kernel, bias, activation)
+    return out if x.dim() == 2 else out.reshape(tuple(x.shape[:-1]) + (kernel.shape[1],))

@@ -7,7 +7,7 @@
  * (the reference prints and calls exit(); cuda/error.cuh:19-27).
  *
  * Conventions
- *   - all tensors are FP32 in device memory; NHWC activations, HWIO filters,
+ *   - all tensors are FP32 in device memory (those of the 4-bit products and the optimizer's step also BF16 and FP16); NHWC activations, HWIO filters,
  *     row-major matrices (as in the reference);
  *   - `stream` is a hipStream_t passed as void* (NULL = default stream); calls
  *     are stream-ordered and never synchronise the device (the reference calls
@@ -50,6 +50,11 @@ extern "C" {
 /* output epilogue of the *_bias_act entry points */
 #define AMSIM_ACT_NONE 0
 #define AMSIM_ACT_RELU 1
+
+/* element types of the 4-bit products and of the optimizer's step (everything else is FP32) */
+#define AMSIM_DTYPE_F32 0
+#define AMSIM_DTYPE_BF16 1
+#define AMSIM_DTYPE_F16 2
 
 typedef struct amsim_lut *amsim_lut_t;
 
@@ -296,6 +301,51 @@ int amsim_attention_grad_f32(amsim_lut_t lut, const float *q, const float *k, co
 size_t amsim_epilogue_grad_workspace_bytes(int64_t rows, int cols);
 int amsim_epilogue_grad_f32(const float *grad, const float *out, int64_t rows, int cols, int act, float *grad_z,
                             float *grad_bias, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- microscaled 4-bit floats (MXFP4) and their products (no counterpart in the reference) -----------
+ * What an approximate multiplier is set against: the narrow format that the matrix cores multiply
+ * themselves.  An operand has `rows` x `length` values, the length being the reduction axis; every 32
+ * consecutive values of a row share a power of two, 2^(floor(log2 max|x|) - 2) held as one byte, and are
+ * rounded to the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times it (ties to even, saturated at 6).  A block
+ * that holds an infinity or a NaN reads back as NaN.  Operands are opaque, amsim_mxfp4_operand_workspace_bytes long (0:
+ * extents out of range) and start on 16-byte boundaries.
+ *
+ * amsim_mxfp4_quantize: x[rows][cols] of `dtype`, rows row_stride elements apart, to an operand of its rows
+ * (rows x cols), of its columns (cols x rows), or both in one pass; a direction that is not wanted is NULL.
+ * amsim_mxfp4_dequantize: the values, out[rows][length] of `dtype`.
+ * amsim_mxfp4_matmul: out[m][n] = act(sum_k a[m][k] b[n][k] + bias[n]) with 32-bit sums, rounded to out_dtype once;
+ * bias may be NULL.  amsim_mxfp4_linear: the same with a = x[m][k], quantised on the way.  Out starts on a
+ * 16-byte boundary, the workspace on a 256-byte one.  Empty extents are refused (AMSIM_ERR_INVALID). */
+size_t amsim_mxfp4_operand_workspace_bytes(int64_t rows, int64_t length);
+int amsim_mxfp4_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void *by_rows,
+                         void *by_columns, void *stream);
+int amsim_mxfp4_dequantize(const void *q, int64_t rows, int64_t length, int dtype, void *out, void *stream);
+size_t amsim_mxfp4_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int amsim_mxfp4_matmul(const void *a, const void *b, int64_t m, int64_t n, int64_t k, const void *bias, int bias_dtype,
+                       int act, void *out, int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
+size_t amsim_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int amsim_mxfp4_linear(const void *x, int dtype, int64_t row_stride, const void *w, int64_t m, int64_t n, int64_t k,
+                       const void *bias, int bias_dtype, int act, void *out, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
+/* ---- AdamW over many tensors (no counterpart in the reference: its optimizers are Keras's) ------------
+ *   g = grad [* *grad_scale]    m' = beta1 m + (1 - beta1) g    v' = beta2 v + ((1 - beta2) g) g
+ *   p' = p (1 - lr weight_decay) - (m' / (sqrt(v') / sqrt(1 - beta2^step) + eps)) lr / (1 - beta1^step)
+ * in 32 bits; params[i] and grads[i] hold sizes[i] contiguous elements of param_dtype and grad_dtype and may
+ * start anywhere.  The three tables are read before the call returns.  A NULL gradient leaves its tensor and its moments
+ * as they are.  The moments of all tensors lie in one buffer, tensor by tensor, each from a multiple of 256
+ * elements on.  state_bits 32: m and v are floats.  state_bits 8: m and sqrt(v) are bytes, and every 256 of them
+ * have a float in m_scale / v_scale, the largest magnitude among them; a byte is (sign and) 4 bits of
+ * exponent and 3 (m) or 4 (sqrt(v)) of mantissa below it.  grad_scale: one float in device memory, or NULL. */
+typedef struct amsim_adamw_hyper {
+    int64_t step;  /* of this update, from 1 on */
+    double lr, beta1, beta2, eps, weight_decay;
+} amsim_adamw_hyper;
+int amsim_adamw_step(int count, void *const *params, const void *const *grads, const int64_t *sizes, int param_dtype,
+                     int grad_dtype, int state_bits, void *m, void *v, float *m_scale, float *v_scale,
+                     const amsim_adamw_hyper *hyper, const float *grad_scale, void *stream);
+/* the values that 8-bit moments stand for, out[256 * blocks]: of m (roots 0) or of sqrt(v) (roots 1) */
+int amsim_adamw_state_values(const void *codes, const float *scales, int64_t blocks, int roots, float *out, void *stream);
 
 /* ---- op-level host logic (what the OpKernel::Compute bodies derive) ----------
  * TensorFlow 2.3 GetWindowedOutputSizeVerbose for dilation 1 as used at
