@@ -7,6 +7,8 @@
 #include "amsim_mx.h"
 
 #include <algorithm>
+#include <cmath>
+#include <utility>
 
 namespace amsim {
 
@@ -31,7 +33,7 @@ struct GemmArgs {
     int bias_dtype, act, out_dtype;
     void *out;
     float *partial;  // [splits][m][n] where the reduction is split, else null
-    int64_t tiles_n;
+    int64_t tiles_m, tiles_n;
 };
 
 template <typename T>
@@ -74,49 +76,227 @@ template <int SA, int SB> __device__ __forceinline__ v4f mfma(v4i a, v4i b, v4f 
     const v8i wa = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, wb = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, wb, c, 4, 4, SA, sa, SB, sb);
 }
-
-// Fragments straight from memory to registers: 2 x 2 waves of F x F fragments each.
-template <int F>
-__global__ __launch_bounds__(WG) void gemm_kernel(GemmArgs g)
+// fn(integral_constant 0), ... fn(integral_constant N - 1): indices that are part of an instruction
+template <typename Fn, int... I> __device__ __forceinline__ void for_each(Fn &&fn, std::integer_sequence<int, I...>)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t tm = (int64_t)blockIdx.x / g.tiles_n, tn = (int64_t)blockIdx.x % g.tiles_n;
-    const int64_t fa = (tm * 2 + wave / 2) * F, fb = (tn * 2 + wave % 2) * F;
-    const int64_t beg = blockIdx.y * g.steps_per_split, end = min(beg + g.steps_per_split, g.steps);
-    const uint8_t *pa[F], *pb[F], *sa[F], *sb[F];
+    (fn(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename Fn> __device__ __forceinline__ void for_each(Fn &&fn) { for_each(fn, std::make_integer_sequence<int, N>{}); }
+
+// Where tile number `id` of a launch lies.  Workgroups go to the eight dies in turn; each die gets a run of
+// neighbouring tiles, eight tiles high, so that its L2 serves a fragment's step to all who read it.
+__device__ __forceinline__ void place_tile(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t &tm, int64_t &tn)
+{
+    const int64_t tiles = tiles_m * tiles_n, each = tiles / 8, more = tiles % 8, die = id % 8;
+    const int64_t t = die * each + (die < more ? die : more) + id / 8;
+    const int64_t band = 8 * tiles_n, first = t / band * 8, within = t % band, high = min<int64_t>(8, tiles_m - first);
+    tm = first + within % high;
+    tn = within / high;
+}
+
+// s_waitcnt for vmcnt n outstanding loads, and for all of LDS's answers
+#define MX_WAIT_LOADS(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | 7 << 4 | 15 << 8 | ((n) >> 4) << 14)
+#define MX_WAIT_LDS() __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 0 << 8 | 3 << 14)
+
+// SIZE bytes a lane from memory to LDS, without passing through registers: lane l's bytes go to to + SIZE l.  The
+// wavefront's address and the step's offset stay in scalar registers.
+template <int SIZE> __device__ __forceinline__ void load_to_lds(const uint8_t *from, int step_offset, uint8_t *to)
+{
+#ifdef __HIP_DEVICE_COMPILE__  // (the host's compiler does not know the type)
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, 0xffffffff, 0x00020000);
+    const auto lds = (__attribute__((address_space(3))) void *)to;
+    if constexpr (SIZE == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, (threadIdx.x & 63) * 16, step_offset, 0, 0);
+    else __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 4, (threadIdx.x & 63) * 4, step_offset, 0, 0);
+#endif
+}
+
+// 16 rows of a wave's results to memory, by way of LDS: a lane's four columns lie in sixteen rows' lines, a row
+// of 16 F columns is whole ones.  The rows' padding puts sixteen rows' writes on different banks.
+template <typename T, int F> struct Rows {
+    static constexpr int COLUMNS = 16 * F, STRIDE = COLUMNS * sizeof(T) + 16, BYTES = 16 * STRIDE;
+};
+template <typename T, int F>
+__device__ __forceinline__ void store_rows(uint8_t *lds, const v4f (&acc)[F], const float (&bias)[F][4], int act, T *out, int64_t m0,
+                                           int64_t n0, int64_t M, int64_t N)
+{
+    using R = Rows<T, F>;
+    const int lane = threadIdx.x & 63;
+    if (m0 >= M) return;
+    MX_WAIT_LDS();  // (the rows before have been read)
 #pragma unroll
-    for (int i = 0; i < F; ++i) {
-        const int64_t f = min(fa + i, g.a.fragments - 1), h = min(fb + i, g.b.fragments - 1);
-        pa[i] = g.a.codes + (f * g.steps * 64 + lane) * 16;
-        pb[i] = g.b.codes + (h * g.steps * 64 + lane) * 16;
-        sa[i] = g.a.scales + (f / 4 * g.steps * 64 + lane) * 4 + f % 4;
-        sb[i] = g.b.scales + (h / 4 * g.steps * 64 + lane) * 4 + h % 4;
+    for (int j = 0; j < F; ++j) {
+        T t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = from_float<T>(activate(acc[j][e] + bias[j][e], act));
+        __builtin_memcpy(__builtin_assume_aligned(lds + lane % 16 * R::STRIDE + (16 * j + lane / 16 * 4) * sizeof(T), 4 * sizeof(T)), t, sizeof(t));
     }
-    v4f acc[F][F] = {};
-    for (int64_t s = beg; s < end; ++s) {
+    __builtin_amdgcn_wave_barrier();
+    const int rows = (int)min<int64_t>(16, M - m0), columns = (int)min<int64_t>(R::COLUMNS, N - n0);
+    T *o = out + m0 * N + n0;
+    constexpr int PIECE = 16 / sizeof(T), PIECES = R::COLUMNS / PIECE;
+    if (N % PIECE == 0) {  // (whole pieces: out starts on a 16-byte boundary)
+#pragma unroll
+        for (int i = 0; i < 16 * PIECES / 64; ++i) {
+            const int r = (i * 64 + lane) / PIECES, c = (i * 64 + lane) % PIECES * PIECE;
+            const v4i v = *(const v4i *)(lds + r * R::STRIDE + c * sizeof(T));
+            if (r < rows && c < columns) *(v4i *)(o + r * N + c) = v;
+        }
+    } else {
+#pragma unroll 4
+        for (int i = 0; i < 16 * R::COLUMNS / 64; ++i) {
+            const int r = (i * 64 + lane) / R::COLUMNS, c = (i * 64 + lane) % R::COLUMNS;
+            const T v = *(const T *)(lds + r * R::STRIDE + c * sizeof(T));
+            if (r < rows && c < columns) o[r * N + c] = v;
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A workgroup of 2 x 2 waves, F x F fragments each: a tile of 32 F rows and columns.  Steps of 128 along the
+// reduction go from memory to one of STAGES places in LDS without passing through registers (the storage is
+// what a wavefront's 16-byte loads deliver, lane by lane), and a step's fragments are read into
+// registers while the step before is multiplied.
+template <int F, int STAGES> struct Gemm {
+    static constexpr int SIDE = 2 * F, GROUPS = F >= 4 ? F / 2 : 1;       // fragments and scale groups of a tile's side
+    static constexpr int A = 0, B = SIDE * 1024, SA = 2 * SIDE * 1024, SB = SA + GROUPS * 256, BYTES = SB + GROUPS * 256;
+    static constexpr int PER_WAVE = SIDE / 4;                             // 1 KB loads of a wave from either operand
+    static constexpr int LOADS = 2 * PER_WAVE + (GROUPS == 4 ? 2 : 1);    // of a wave for a step
+    static constexpr int SCALES = F >= 4 ? F / 4 : 1;                     // dwords of four fragments' scales
+    static constexpr int READS = 2 * F + 2;                               // of LDS (scales: one instruction for two dwords)
+    struct Registers {
         v4i a[F], b[F];
-        int ca[F], cb[F];
+        int sa[SCALES], sb[SCALES];
+    };
+};
+
+template <int F, int STAGES>
+__global__ __launch_bounds__(WG, 1) void gemm_kernel(GemmArgs g)
+{
+    using K = Gemm<F, STAGES>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * K::BYTES];
+    static_assert(4 * Rows<float, F>::BYTES <= STAGES * K::BYTES, "");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / 2, wn = wave % 2;
+    int64_t tm, tn;
+    place_tile(blockIdx.x, g.tiles_m, g.tiles_n, tm, tn);
+    const int64_t beg = blockIdx.y * g.steps_per_split, end = min(beg + g.steps_per_split, g.steps);
+    const int count = (int)(end - beg);
+
+    // what this wave fetches: PER_WAVE fragments of either operand and a group of 64 rows' scales (or one of each)
+    const uint8_t *fetch[2 * K::PER_WAVE], *fetch_scales[2];
+    int to[2 * K::PER_WAVE], to_scales[2];
+#pragma unroll
+    for (int i = 0; i < K::PER_WAVE; ++i) {
+        const int64_t f = K::PER_WAVE * wave + i, fa = min(tm * K::SIDE + f, g.a.fragments - 1), fb = min(tn * K::SIDE + f, g.b.fragments - 1);
+        fetch[i] = g.a.codes + (fa * g.steps + beg) * 1024;
+        fetch[K::PER_WAVE + i] = g.b.codes + (fb * g.steps + beg) * 1024;
+        to[i] = K::A + (int)f * 1024;
+        to[K::PER_WAVE + i] = K::B + (int)f * 1024;
+    }
+    {
+        const int64_t ga = K::GROUPS == 4 ? wave : wave / 2 % K::GROUPS, gb = ga;
+        const int64_t fa = min(tm * K::SIDE / 4 + ga, g.a.groups - 1), fb = min(tn * K::SIDE / 4 + gb, g.b.groups - 1);
+        const uint8_t *pa = g.a.scales + (fa * g.steps + beg) * 256, *pb = g.b.scales + (fb * g.steps + beg) * 256;
+        const int la = K::SA + (int)ga * 256, lb = K::SB + (int)gb * 256;
+        // (fewer groups than waves: even waves fetch a's, odd ones b's)
+        fetch_scales[0] = K::GROUPS == 4 || wave % 2 == 0 ? pa : pb;
+        to_scales[0] = K::GROUPS == 4 || wave % 2 == 0 ? la : lb;
+        fetch_scales[1] = pb;
+        to_scales[1] = lb;
+    }
+    auto fetch_step = [&](int s) {
+        uint8_t *stage = lds + s % STAGES * K::BYTES;
+        const int at = min(s, count - 1);
+#pragma unroll
+        for (int i = 0; i < 2 * K::PER_WAVE; ++i)
+            load_to_lds<16>(fetch[i], at * 1024, stage + to[i]);
+#pragma unroll
+        for (int i = 0; i < (K::GROUPS == 4 ? 2 : 1); ++i)
+            load_to_lds<4>(fetch_scales[i], at * 256, stage + to_scales[i]);
+    };
+    auto read_step = [&](int s, typename K::Registers &r) {
+        const uint8_t *stage = lds + s % STAGES * K::BYTES;
 #pragma unroll
         for (int i = 0; i < F; ++i) {
-            a[i] = *(const v4i *)(pa[i] + s * 1024);
-            b[i] = *(const v4i *)(pb[i] + s * 1024);
-            ca[i] = sa[i][s * 256];
-            cb[i] = sb[i][s * 256];
+            r.a[i] = *(const v4i *)(stage + K::A + (wm * F + i) * 1024 + lane * 16);
+            r.b[i] = *(const v4i *)(stage + K::B + (wn * F + i) * 1024 + lane * 16);
         }
 #pragma unroll
-        for (int i = 0; i < F; ++i)
+        for (int i = 0; i < K::SCALES; ++i) {
+            r.sa[i] = *(const int *)(stage + K::SA + (F >= 4 ? wm * K::SCALES + i : 0) * 256 + lane * 4);
+            r.sb[i] = *(const int *)(stage + K::SB + (F >= 4 ? wn * K::SCALES + i : 0) * 256 + lane * 4);
+            if (F == 2) r.sa[i] >>= 16 * wm, r.sb[i] >>= 16 * wn;
+        }
+    };
+    v4f acc[F][F] = {};
+    auto multiply = [&](const typename K::Registers &r) {
+        for_each<F * F>([&](auto at) {
+            constexpr int i = at.value / F, j = at.value % F;
+            acc[i][j] = mfma<j % 4, i % 4>(r.b[j], r.a[i], acc[i][j], r.sb[j / 4], r.sa[i / 4]);
+        });
+    };
+    // One step: everyone has read step s and its successor's loads are in LDS; loads of step s + STAGES take the
+    // place of step s; fragments of s + 1 are read while those of s are multiplied.  (Without branches, so that the
+    // multiplications stay where they are: behind the last step it is loaded again, and not used.)
+    auto step = [&](int s, const typename K::Registers &now, typename K::Registers &next) {
+        MX_WAIT_LDS();
+        MX_WAIT_LOADS((STAGES - 2) * K::LOADS);
+        __builtin_amdgcn_s_barrier();
+        read_step(s + 1, next);
+        fetch_step(s + STAGES);
+        multiply(now);
+        // two reads of LDS behind a multiplication, then a load behind every fourth
+        for_each<K::READS / 2>([](auto) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        });
+        for_each<K::LOADS>([](auto) {
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+    };
 #pragma unroll
-            for (int j = 0; j < F; ++j) acc[i][j] = mfma<0, 0>(b[j], a[i], acc[i][j], cb[j], ca[i]);
+    for (int s = 0; s < STAGES; ++s) fetch_step(s);
+    MX_WAIT_LOADS((STAGES - 1) * K::LOADS);
+    __builtin_amdgcn_s_barrier();
+    typename K::Registers even, odd;
+    read_step(0, even);
+    int s = count & 1;
+    if (s) {
+        step(0, even, odd);
+        even = odd;
     }
+    for (; s < count; s += 2) {
+        step(s, even, odd);
+        step(s + 1, odd, even);
+    }
+    MX_WAIT_LDS();
+    MX_WAIT_LOADS(0);
+    __builtin_amdgcn_s_barrier();  // (LDS is free)
+    const int64_t m0 = (tm * K::SIDE + wm * F) * 16, n0 = (tn * K::SIDE + wn * F) * 16;
+    if (n0 >= g.b.rows) return;
+    uint8_t *mine = lds + wave * Rows<float, F>::BYTES;
+    if (g.partial) {
+        float none[F][4] = {};
+        float *out = g.partial + (int64_t)blockIdx.y * g.a.rows * g.b.rows;
+        for_each<F>([&](auto i) { store_rows<float, F>(mine, acc[i.value], none, AMSIM_ACT_NONE, out, m0 + 16 * i.value, n0, g.a.rows, g.b.rows); });
+        return;
+    }
+    float bias[F][4];
 #pragma unroll
-    for (int i = 0; i < F; ++i)
+    for (int j = 0; j < F; ++j)
 #pragma unroll
-        for (int j = 0; j < F; ++j) {
-            const int64_t m = (fa + i) * 16 + lane % 16, n = (fb + j) * 16 + lane / 16 * 4;
-            if (m >= g.a.rows || n >= g.b.rows) continue;
-            float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-            finish4(g, m, n, v);
+        for (int e = 0; e < 4; ++e) {
+            const int64_t n = n0 + 16 * j + lane / 16 * 4 + e;
+            bias[j][e] = g.bias && n < g.b.rows ? load_as_float(g.bias, g.bias_dtype, n) : 0.0f;
         }
+    auto store = [&](auto zero) {
+        using T = decltype(zero);
+        for_each<F>([&](auto i) { store_rows<T, F>(mine, acc[i.value], bias, g.act, (T *)g.out, m0 + 16 * i.value, n0, g.a.rows, g.b.rows); });
+    };
+    if (g.out_dtype == AMSIM_DTYPE_F32) store(0.0f);
+    else if (g.out_dtype == AMSIM_DTYPE_BF16) store((__bf16)0.0f);
+    else store((_Float16)0.0f);
 }
 
 // The partial sums of a split reduction, added in the order of the splits.
@@ -149,21 +329,32 @@ struct Plan {
     int64_t tiles_m, tiles_n, splits, steps_per_split;
 };
 
+// The tile and the split of the reduction that a product takes least time with, by microseconds measured on
+// products of 128 to 16384 a side.  Tiles of 256: a round of the 256 CUs takes 0.68 a step (0.6 for one tile alone), and
+// its results are stored with nothing to multiply meanwhile, 8.  Tiles of 128 share a CU and hide that, but
+// fetch twice the bytes for an operation: 0.2 a step for one tile on a CU, 0.00088 a tile and step for many.
+// Tiles of 64 four times the bytes: 0.1 and 0.00038.  A split reduction takes a second launch, 3, and its sums
+// go to memory and back.
 Plan plan(int64_t m, int64_t n, int64_t k)
 {
-    Plan p{};
     const int64_t steps = mx_steps(k);
-    for (int f = 4; f >= 1; f /= 2) {
-        p.fragments = f;
-        p.tiles_m = ceil_div64(m, 32 * f);
-        p.tiles_n = ceil_div64(n, 32 * f);
-        if (p.tiles_m * p.tiles_n >= 256) break;
+    Plan best{};
+    double least = 0;
+    for (int f = 8; f >= 2; f /= 2) {
+        const int64_t tiles_m = ceil_div64(m, 32 * f), tiles_n = ceil_div64(n, 32 * f);
+        for (int64_t s = 1; s <= 16 && (s == 1 || 2 * s <= steps); s *= 2) {
+            const int64_t each = ceil_div64(steps, s), splits = ceil_div64(steps, each);
+            const double tiles = (double)tiles_m * (double)tiles_n * (double)splits;
+            double t = f == 8 ? 2 + std::ceil(tiles / 256) * (0.68 * each + 8)
+                     : f == 4 ? 7 + std::max(0.2, 0.00088 * tiles) * each : 6 + std::max(0.1, 0.00038 * tiles) * each;
+            if (splits > 1) t += 3 + (double)splits * (double)m * (double)n * 8 / 4e6;
+            if (best.fragments == 0 || t < least) {
+                least = t;
+                best = Plan{f, tiles_m, tiles_n, splits, each};
+            }
+        }
     }
-    const int64_t tiles = p.tiles_m * p.tiles_n;
-    p.splits = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / tiles, steps / 8), 16));
-    p.steps_per_split = ceil_div64(steps, p.splits);
-    p.splits = ceil_div64(steps, p.steps_per_split);
-    return p;
+    return best;
 }
 
 size_t product_workspace(int64_t m, int64_t n, int64_t k)
@@ -179,12 +370,12 @@ int product(const Operand &a, const Operand &b, int64_t k, const void *bias, int
     const int64_t tiles = p.tiles_m * p.tiles_n, quads = a.rows * ceil_div64(b.rows, 4);
     if (tiles >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
     GemmArgs g{a, b, mx_steps(k), p.steps_per_split, bias, bias_dtype, act, out_dtype, out,
-               p.splits > 1 ? (float *)workspace : nullptr, p.tiles_n};
+               p.splits > 1 ? (float *)workspace : nullptr, p.tiles_m, p.tiles_n};
     const dim3 grid((unsigned)tiles, (unsigned)p.splits);
     switch (p.fragments) {
-    case 4: gemm_kernel<4><<<grid, WG, 0, stream>>>(g); break;
-    case 2: gemm_kernel<2><<<grid, WG, 0, stream>>>(g); break;
-    default: gemm_kernel<1><<<grid, WG, 0, stream>>>(g); break;
+    case 8: gemm_kernel<8, 4><<<grid, WG, 0, stream>>>(g); break;
+    case 4: gemm_kernel<4, 4><<<grid, WG, 0, stream>>>(g); break;
+    default: gemm_kernel<2, 4><<<grid, WG, 0, stream>>>(g); break;
     }
     AMSIM_HIP_CHECK(hipGetLastError());
     if (p.splits > 1) {
