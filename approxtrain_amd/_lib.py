@@ -86,6 +86,10 @@ SIGNATURES = {
     "amsim_mxfp4_matmul": (_i, [_p, _p, _i64, _i64, _i64, _p, _i, _i, _p, _i, _p, _sz, _p]),
     "amsim_mxfp4_linear_workspace_bytes": (_sz, [_i64] * 3),
     "amsim_mxfp4_linear": (_i, [_p, _i, _i64, _p, _i64, _i64, _i64, _p, _i, _i, _p, _p, _sz, _p]),
+    "amsim_mxfp4_dense_workspace_bytes": (_sz, [_i64] * 3),
+    "amsim_mxfp4_dense": (_i, [_p, _i, _i64] * 2 + [_i64] * 3 + [_p, _i, _i] + [_p] * 4 + [_sz, _p]),
+    "amsim_mxfp4_dense_grad_workspace_bytes": (_sz, [_i64] * 3),
+    "amsim_mxfp4_dense_grad": (_i, [_p, _i, _i64] + [_p] * 3 + [_i64] * 3 + [_p, _p, _i, _p, _i, _p, _sz, _p]),
     "amsim_adamw_step": (_i, [_i, _p, _p, _p, _i, _i, _i, _p, _p, _f, _f, _p, _f, _p]),
     "amsim_adamw_state_values": (_i, [_p, _f, _i64, _i, _f, _p]),
     "amsim_conv_geometry": (_i, [_i, _i, _i, _i, C.POINTER(_i), C.POINTER(_i)]),

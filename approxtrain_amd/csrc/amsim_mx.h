@@ -131,6 +131,63 @@ template <> struct MxBlock<_Float16> : MxBlock16<_Float16> {
     }
 };
 
+// the same for 8 values: the exponent field of their largest magnitude, and their codes
+__device__ __forceinline__ uint32_t mx_exponent_field(const float (&v)[8])
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m >> 23;
+}
+template <typename T> __device__ __forceinline__ uint32_t mx_largest16(const T (&v)[8])
+{
+    uint32_t p[4];
+    __builtin_memcpy(p, v, 16);
+    v2us m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(v2us, p[i] & 0x7fff7fffu));
+    return max((uint32_t)m.x, (uint32_t)m.y);
+}
+__device__ __forceinline__ uint32_t mx_exponent_field(const __bf16 (&v)[8]) { return mx_largest16(v) >> 7; }
+__device__ __forceinline__ uint32_t mx_exponent_field(const _Float16 (&v)[8])
+{
+    return __float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)mx_largest16(v))) >> 23;
+}
+__device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], uint32_t code)
+{
+    const float s = mx_scale_value(code == 255u ? 127u : code);
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], s, 3);
+    return code == 255u ? 0 : w;
+}
+__device__ __forceinline__ uint32_t mx_encode8(const __bf16 (&v)[8], uint32_t code)
+{
+    const float s = mx_scale_value(code == 255u ? 127u : code);
+    v2bf p[4];
+    __builtin_memcpy(p, v, 16);
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p[0], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p[1], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p[2], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p[3], s, 3);
+    return code == 255u ? 0 : w;
+}
+__device__ __forceinline__ uint32_t mx_encode8(const _Float16 (&v)[8], uint32_t code)
+{
+    const float s = mx_scale_value(code == 255u ? 127u : code);
+    v2h p[4];
+    __builtin_memcpy(p, v, 16);
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, p[0], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, p[1], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, p[2], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, p[3], s, 3);
+    return code == 255u ? 0 : w;
+}
+
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__bf16 v) { return (float)v; }
 __device__ __forceinline__ float to_float(_Float16 v) { return (float)v; }
@@ -147,8 +204,17 @@ __device__ __forceinline__ float load_as_float(const void *p, int dtype, int64_t
 // (a NaN stays one)
 __device__ __forceinline__ float activate(float v, int act) { return act == AMSIM_ACT_RELU && v < 0.0f ? 0.0f : v; }
 
-int mx_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void *by_rows, void *by_columns,
-                hipStream_t stream);
+// A tensor to be converted: the operand of its rows, of its columns, or both.
+struct MxConversion {
+    const void *x;
+    const void *positive;            // [rows][cols] of x's type, or null: where it is not above zero x counts as zero
+    int dtype;
+    int64_t rows, cols, row_stride;  // row_stride in elements
+    uint8_t *by_rows, *by_columns;   // null where that direction is not asked for
+    float *sums;                     // [ceil(rows / 32)][cols], or null: sums of every 32 rows
+};
+// One launch for one or two tensors.
+int mx_convert(const MxConversion *jobs, int count, hipStream_t stream);
 
 }  // namespace amsim
 #endif  // AMSIM_MX_H_

@@ -1,10 +1,8 @@
 // Conversion of tensors to MXFP4 operands (amsim_mx.h) and back.
 //
 // Bound by memory: an element is read once, 4 or 2 bytes, and written as 17/32 of a byte for each direction
-// asked for.  A training step multiplies the same tensor along either axis, so one pass makes both operands.
-// A workgroup owns 128 x 128 values: coalesced loads, LDS, and then each thread takes whole blocks of 32 out
-// of it, along a row or down a column, so that the largest magnitude, the scale and the 16 bytes of codes
-// are one lane's own affair.  LDS rows are padded by 16 bytes: sixteen rows' 16-byte reads meet all banks.
+// asked for.  A training step multiplies the same tensor along either axis, so one pass makes both operands, and
+// of a gradient also the sums of its columns.
 #include "amsim_mx.h"
 
 namespace amsim {
@@ -12,55 +10,128 @@ namespace amsim {
 namespace {
 
 constexpr int WG = 256;
-constexpr int TILE = 128;
 
-struct QuantizeArgs {
-    const void *x;
-    int64_t rows, cols, row_stride;  // row_stride in elements
-    uint8_t *by_rows, *by_columns;   // null where that direction is not asked for
-    int64_t column_tiles;
-    bool vectors;                    // rows start on 16-byte boundaries
+// ---- rows alone: four lanes share a block, and nothing has to be exchanged but its largest magnitude --------
+
+template <typename T> struct Eighth;  // 8 values of a block
+template <> struct Eighth<float> { float v[8]; };
+template <> struct Eighth<__bf16> { __bf16 v[8]; };
+template <> struct Eighth<_Float16> { _Float16 v[8]; };
+
+// A workgroup: 64 rows of a step of 128.  A wavefront's 64 lanes read four rows, 128 values of each; the scales of
+// the four fragments meet in LDS, as the bytes of one dword.
+template <typename T>
+__global__ __launch_bounds__(WG) void rows_kernel(const T *x, int64_t rows, int64_t cols, int64_t row_stride, uint8_t *out, bool vectors)
+{
+    __shared__ uint8_t scales[4][64];
+    const int64_t steps = mx_steps(cols), step = (int64_t)blockIdx.x % steps, row0 = (int64_t)blockIdx.x / steps * 64;
+    const int r = threadIdx.x / 16, c = threadIdx.x % 16 * 8, lane = c / 32 * 16 + r;  // of a fragment
+    const int64_t col = 128 * step + c;
+    Eighth<T> e[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+        const int64_t row = row0 + 16 * f + r;
+        const T *p = x + row * row_stride + col;
+        if (vectors && row < rows && col + 8 <= cols) {
+            __builtin_memcpy(&e[f], __builtin_assume_aligned(p, 16), sizeof(e[f]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[f].v[i] = row < rows && col + i < cols ? p[i] : (T)0.0f;
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+        uint32_t largest = mx_exponent_field(e[f].v);
+        largest = max(largest, (uint32_t)__shfl_xor((int)largest, 1, 64));
+        largest = max(largest, (uint32_t)__shfl_xor((int)largest, 2, 64));
+        const uint32_t code = mx_scale_code(largest);
+        if (threadIdx.x % 4 == 0) scales[f][lane] = (uint8_t)code;
+        if (row0 + 16 * f < rows)
+            *(uint32_t *)(out + (((row0 / 16 + f) * steps + step) * 64 + lane) * 16 + c % 32 / 2) = mx_encode8(e[f].v, code);
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    const int l = threadIdx.x;
+    const uint32_t w = scales[0][l] | scales[1][l] << 8 | scales[2][l] << 16 | (uint32_t)scales[3][l] << 24;
+    *(uint32_t *)(out + mx_code_bytes(rows, cols) + ((row0 / 64 * steps + step) * 64 + l) * 4) = w;
+}
+
+// ---- columns, or rows and columns ---------------------------------------------------------------------------
+// A workgroup owns 32 x 128 values, in LDS: of the 256 blocks of 32 along the rows and down the columns each
+// thread takes one, so that the largest magnitude, the scale and the 16 bytes of codes are its own affair.  LDS
+// rows are padded by 16 bytes: sixteen rows' 16-byte reads meet all banks.
+
+constexpr int HIGH = 32, WIDE = 128;
+
+struct TileJobs {
+    MxConversion job[2];
+    int64_t tiles[2], column_tiles[2];
+    bool vectors[2];  // rows start on 16-byte boundaries
 };
 
 template <typename T> struct Tile {
     static constexpr int PER_VEC = 16 / sizeof(T);
-    static constexpr int STRIDE = TILE + PER_VEC;  // elements of an LDS row
-    T v[TILE][STRIDE];
+    static constexpr int STRIDE = WIDE + PER_VEC;  // elements of an LDS row
+    T v[HIGH][STRIDE];
 };
 
+template <typename T> __device__ __forceinline__ T masked(T v, T y) { return to_float(y) > 0.0f ? v : (T)0.0f; }
+
 template <typename T>
-__device__ __forceinline__ void load_tile(Tile<T> &t, const QuantizeArgs &a, int64_t row0, int64_t col0)
+__device__ __forceinline__ void load_tile(Tile<T> &t, const MxConversion &j, bool vectors, int64_t row0, int64_t col0)
 {
-    constexpr int PER_VEC = Tile<T>::PER_VEC, VECS = TILE / PER_VEC;  // 16-byte pieces of a row of the tile
-    constexpr int LOADS = TILE * VECS / WG;
-    const T *x = (const T *)a.x;
-    if (a.vectors) {
-        v4i piece[LOADS];
+    constexpr int PER_VEC = Tile<T>::PER_VEC, VECS = WIDE / PER_VEC;  // 16-byte pieces of a row of the tile
+    constexpr int LOADS = HIGH * VECS / WG;
+    const T *x = (const T *)j.x, *y = (const T *)j.positive;
+    if (vectors) {
+        v4i piece[LOADS], keep[LOADS];
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int at = threadIdx.x + WG * i, r = at / VECS, c = at % VECS * PER_VEC;
             piece[i] = v4i{0, 0, 0, 0};
-            if (row0 + r >= a.rows) continue;
-            const T *p = x + (row0 + r) * a.row_stride + col0 + c;
-            if (col0 + c + PER_VEC <= a.cols) {
+            if (row0 + r >= j.rows) continue;
+            const T *p = x + (row0 + r) * j.row_stride + col0 + c, *q = y + (row0 + r) * j.cols + col0 + c;
+            if (col0 + c + PER_VEC <= j.cols) {
                 piece[i] = *(const v4i *)p;
+                if (y) keep[i] = *(const v4i *)q;
             } else {
-                T last[PER_VEC];
+                T last[PER_VEC], also[PER_VEC];
 #pragma unroll
-                for (int e = 0; e < PER_VEC; ++e) last[e] = col0 + c + e < a.cols ? p[e] : (T)0.0f;
+                for (int e = 0; e < PER_VEC; ++e) {
+                    last[e] = col0 + c + e < j.cols ? p[e] : (T)0.0f;
+                    also[e] = y && col0 + c + e < j.cols ? q[e] : (T)0.0f;
+                }
                 __builtin_memcpy(&piece[i], last, 16);
+                __builtin_memcpy(&keep[i], also, 16);
             }
         }
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int at = threadIdx.x + WG * i, r = at / VECS, c = at % VECS * PER_VEC;
+            if (y) {
+                T a[PER_VEC], b[PER_VEC];
+                __builtin_memcpy(a, &piece[i], 16);
+                __builtin_memcpy(b, &keep[i], 16);
+#pragma unroll
+                for (int e = 0; e < PER_VEC; ++e) a[e] = masked(a[e], b[e]);
+                __builtin_memcpy(&piece[i], a, 16);
+            }
             *(v4i *)&t.v[r][c] = piece[i];
         }
     } else {
-        const int c = threadIdx.x % TILE;
-#pragma unroll 16
-        for (int r = threadIdx.x / TILE; r < TILE; r += WG / TILE)
-            t.v[r][c] = row0 + r < a.rows && col0 + c < a.cols ? x[(row0 + r) * a.row_stride + col0 + c] : (T)0.0f;
+        const int c = threadIdx.x % WIDE;
+        T v[HIGH * WIDE / WG];
+#pragma unroll
+        for (int i = 0; i < HIGH * WIDE / WG; ++i) {
+            const int r = threadIdx.x / WIDE + i * (WG / WIDE);
+            v[i] = (T)0.0f;
+            if (row0 + r < j.rows && col0 + c < j.cols) {
+                v[i] = x[(row0 + r) * j.row_stride + col0 + c];
+                if (y) v[i] = masked(v[i], y[(row0 + r) * j.cols + col0 + c]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < HIGH * WIDE / WG; ++i) t.v[threadIdx.x / WIDE + i * (WG / WIDE)][c] = v[i];
     }
 }
 
@@ -75,67 +146,64 @@ template <typename T> __device__ __forceinline__ MxBlock<T> row_block(const Tile
     __builtin_memcpy(&b, piece, sizeof(b));
     return b;
 }
-// block `kb` down column `c`
-template <typename T> __device__ __forceinline__ MxBlock<T> column_block(const Tile<T> &t, int c, int kb)
-{
-    MxBlock<T> b;
-    T v[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = t.v[32 * kb + i][c];
-    __builtin_memcpy(&b, v, sizeof(b));
-    return b;
-}
 
-// Codes of the tile's 128 rows (or columns), 8 fragments of 16, to the operand; the scales to LDS.
-template <typename T, bool COLUMNS>
-__device__ __forceinline__ void encode_tile(const Tile<T> &t, uint8_t (&scales)[8][64], uint8_t *codes, int64_t rows,
-                                            int64_t row0, int64_t steps, int64_t step)
+template <typename T> __device__ __forceinline__ void convert_tile(const MxConversion &j, bool vectors, int64_t row_tile, int64_t column_tile, uint8_t *lds)
 {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int f = (threadIdx.x >> 6) + 4 * i, lane = threadIdx.x & 63;
-        if (row0 + 16 * f >= rows) continue;
-        const MxBlock<T> b = COLUMNS ? column_block(t, 16 * f + lane % 16, lane / 16) : row_block(t, 16 * f + lane % 16, lane / 16);
+    Tile<T> &t = *(Tile<T> *)lds;
+    const int64_t row0 = row_tile * HIGH, col0 = column_tile * WIDE;
+    load_tile(t, j, vectors, row0, col0);
+    __syncthreads();
+    if (threadIdx.x < 128) {  // two fragments of 16 rows
+        const int lane = threadIdx.x & 63;
+        const int64_t f = row0 / 16 + threadIdx.x / 64, steps = mx_steps(j.cols), step = column_tile;
+        if (!j.by_rows || 16 * f >= j.rows) return;
+        const MxBlock<T> b = row_block(t, threadIdx.x / 64 * 16 + lane % 16, lane / 16);
         const uint32_t code = mx_scale_code(b.exponent_field());
-        scales[f][lane] = (uint8_t)code;
-        *(v4i *)(codes + (((row0 / 16 + f) * steps + step) * 64 + lane) * 16) = b.encode(code);
+        *(v4i *)(j.by_rows + ((f * steps + step) * 64 + lane) * 16) = b.encode(code);
+        j.by_rows[mx_code_bytes(j.rows, j.cols) + ((f / 4 * steps + step) * 64 + lane) * 4 + f % 4] = (uint8_t)code;
+    } else {  // eight fragments of 16 columns, a quarter of a step of each
+        const int c = threadIdx.x - 128;
+        const int64_t f = col0 / 16 + c / 16, steps = mx_steps(j.rows), step = row0 / 128;
+        const int lane = (int)(row0 / 32 % 4) * 16 + c % 16;
+        if (16 * f >= j.cols) return;
+        T v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = t.v[i][c];
+        if (j.by_columns) {
+            MxBlock<T> b;
+            __builtin_memcpy(&b, v, sizeof(b));
+            const uint32_t code = mx_scale_code(b.exponent_field());
+            *(v4i *)(j.by_columns + ((f * steps + step) * 64 + lane) * 16) = b.encode(code);
+            j.by_columns[mx_code_bytes(j.cols, j.rows) + ((f / 4 * steps + step) * 64 + lane) * 4 + f % 4] = (uint8_t)code;
+        }
+        if (j.sums && row0 < j.rows && col0 + c < j.cols) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s += to_float(v[i]);
+            j.sums[row_tile * j.cols + col0 + c] = s;
+        }
     }
 }
-__device__ __forceinline__ void store_scales(const uint8_t (&scales)[8][64], int i, uint8_t *out, int64_t rows, int64_t row0,
-                                             int64_t steps, int64_t step)
+
+// (types are branched on here: the two tensors of a forward pass may differ in theirs, and share a launch)
+__global__ __launch_bounds__(WG) void tiles_kernel(TileJobs jobs)
 {
-    const int g = i >> 6, lane = i & 63;
-    if (row0 + 64 * g >= rows) return;
-    const uint32_t w = scales[4 * g][lane] | scales[4 * g + 1][lane] << 8 | scales[4 * g + 2][lane] << 16 | (uint32_t)scales[4 * g + 3][lane] << 24;
-    *(uint32_t *)(out + (((row0 / 64 + g) * steps + step) * 64 + lane) * 4) = w;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[sizeof(Tile<float>)];
+    const int which = (int64_t)blockIdx.x >= jobs.tiles[0];
+    const MxConversion &j = jobs.job[which];
+    const int64_t tile = (int64_t)blockIdx.x - (which ? jobs.tiles[0] : 0), columns = jobs.column_tiles[which];
+    if (j.dtype == AMSIM_DTYPE_F32) convert_tile<float>(j, jobs.vectors[which], tile / columns, tile % columns, lds);
+    else if (j.dtype == AMSIM_DTYPE_BF16) convert_tile<__bf16>(j, jobs.vectors[which], tile / columns, tile % columns, lds);
+    else convert_tile<_Float16>(j, jobs.vectors[which], tile / columns, tile % columns, lds);
 }
 
-template <typename T, bool ROWS, bool COLUMNS>
-__global__ __launch_bounds__(WG) void quantize_kernel(QuantizeArgs a)
-{
-    __shared__ Tile<T> t;
-    __shared__ uint8_t scales[2][8][64];
-    const int64_t row0 = (int64_t)blockIdx.x / a.column_tiles * TILE, col0 = (int64_t)blockIdx.x % a.column_tiles * TILE;
-    load_tile(t, a, row0, col0);
-    // (scales of fragments that do not exist are not written below; their bytes of a dword that is are zeros)
-    for (int i = threadIdx.x; i < (int)sizeof(scales) / 4; i += WG) ((uint32_t *)scales)[i] = 0;
-    __syncthreads();
-    const int64_t row_steps = mx_steps(a.cols), column_steps = mx_steps(a.rows);
-    if (ROWS) encode_tile<T, false>(t, scales[0], a.by_rows, a.rows, row0, row_steps, col0 / TILE);
-    if (COLUMNS) encode_tile<T, true>(t, scales[1], a.by_columns, a.cols, col0, column_steps, row0 / TILE);
-    __syncthreads();
-    const int i = threadIdx.x & 127;
-    if (ROWS && threadIdx.x < 128)
-        store_scales(scales[0], i, a.by_rows + mx_code_bytes(a.rows, a.cols), a.rows, row0, row_steps, col0 / TILE);
-    if (COLUMNS && threadIdx.x >= 128)
-        store_scales(scales[1], i, a.by_columns + mx_code_bytes(a.cols, a.rows), a.cols, col0, column_steps, row0 / TILE);
-}
+inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-template <typename T> void launch_quantize(const QuantizeArgs &a, unsigned tiles, hipStream_t stream)
+inline bool rows_aligned(const MxConversion &j)
 {
-    if (a.by_rows && a.by_columns) quantize_kernel<T, true, true><<<tiles, WG, 0, stream>>>(a);
-    else if (a.by_rows) quantize_kernel<T, true, false><<<tiles, WG, 0, stream>>>(a);
-    else quantize_kernel<T, false, true><<<tiles, WG, 0, stream>>>(a);
+    const int64_t bytes = element_bytes(j.dtype);
+    return aligned16(j.x) && (j.rows == 1 || j.row_stride * bytes % 16 == 0)
+        && (!j.positive || (aligned16(j.positive) && (j.rows == 1 || j.cols * bytes % 16 == 0)));
 }
 
 // A workgroup reads the 1 KB of a fragment's step and writes 16 rows of 128 values, eight per thread.
@@ -165,22 +233,38 @@ __global__ __launch_bounds__(WG) void dequantize_kernel(const uint8_t *q, int64_
     }
 }
 
-inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
-
 }  // namespace
 
-int mx_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void *by_rows, void *by_columns,
-                hipStream_t stream)
+int mx_convert(const MxConversion *jobs, int count, hipStream_t stream)
 {
-    const int64_t column_tiles = ceil_div64(cols, TILE), tiles = ceil_div64(rows, TILE) * column_tiles;
-    if (tiles >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
-    QuantizeArgs a{x, rows, cols, row_stride, (uint8_t *)by_rows, (uint8_t *)by_columns, column_tiles,
-                   aligned16(x) && (rows == 1 || row_stride * element_bytes(dtype) % 16 == 0)};
-    switch (dtype) {
-    case AMSIM_DTYPE_F32: launch_quantize<float>(a, (unsigned)tiles, stream); break;
-    case AMSIM_DTYPE_BF16: launch_quantize<__bf16>(a, (unsigned)tiles, stream); break;
-    default: launch_quantize<_Float16>(a, (unsigned)tiles, stream); break;
+    if (count == 1 && jobs[0].by_rows && !jobs[0].by_columns && !jobs[0].positive && !jobs[0].sums) {
+        const MxConversion &j = jobs[0];
+        const int64_t blocks = mx_steps(j.cols) * ceil_div64(j.rows, 64);
+        if (blocks >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
+        const unsigned n = (unsigned)blocks;
+        uint8_t *out = (uint8_t *)j.by_rows;
+        const bool vectors = rows_aligned(j);
+        switch (j.dtype) {
+        case AMSIM_DTYPE_F32: rows_kernel<float><<<n, WG, 0, stream>>>((const float *)j.x, j.rows, j.cols, j.row_stride, out, vectors); break;
+        case AMSIM_DTYPE_BF16: rows_kernel<__bf16><<<n, WG, 0, stream>>>((const __bf16 *)j.x, j.rows, j.cols, j.row_stride, out, vectors); break;
+        default: rows_kernel<_Float16><<<n, WG, 0, stream>>>((const _Float16 *)j.x, j.rows, j.cols, j.row_stride, out, vectors); break;
+        }
+        AMSIM_HIP_CHECK(hipGetLastError());
+        return AMSIM_OK;
     }
+    TileJobs t{};
+    int64_t tiles = 0;
+    for (int i = 0; i < count; ++i) {
+        const MxConversion &j = jobs[i];
+        t.job[i] = j;
+        t.vectors[i] = rows_aligned(j);
+        t.column_tiles[i] = ceil_div64(j.cols, WIDE);
+        // (down the columns the last step is filled up with zeros)
+        const int64_t row_tiles = j.by_columns ? mx_steps(j.rows) * (128 / HIGH) : ceil_div64(j.rows, HIGH);
+        tiles += t.tiles[i] = row_tiles * t.column_tiles[i];
+    }
+    if (tiles >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
+    tiles_kernel<<<(unsigned)tiles, WG, 0, stream>>>(t);
     AMSIM_HIP_CHECK(hipGetLastError());
     return AMSIM_OK;
 }
@@ -207,7 +291,8 @@ int amsim_mxfp4_quantize(const void *x, int dtype, int64_t rows, int64_t cols, i
     if (!x) return fail(AMSIM_ERR_INVALID, "mxfp4: null pointer");
     if (!aligned16(by_rows) || !aligned16(by_columns) || ((uintptr_t)x & (element_bytes(dtype) - 1)))
         return fail(AMSIM_ERR_INVALID, "mxfp4: misaligned pointer");
-    return mx_quantize(x, dtype, rows, cols, row_stride, by_rows, by_columns, (hipStream_t)stream);
+    const MxConversion job{x, nullptr, dtype, rows, cols, row_stride, (uint8_t *)by_rows, (uint8_t *)by_columns, nullptr};
+    return mx_convert(&job, 1, (hipStream_t)stream);
 }
 
 int amsim_mxfp4_dequantize(const void *q, int64_t rows, int64_t length, int dtype, void *out, void *stream)

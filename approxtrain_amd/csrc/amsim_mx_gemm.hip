@@ -324,6 +324,26 @@ __global__ __launch_bounds__(WG) void gemm_reduce_kernel(GemmArgs g, int splits)
     finish4(h, m, n, v);
 }
 
+// Sums of columns from those of every 32 rows, in order: 64 columns and 16 runs of rows to a workgroup.
+template <typename T>
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float *parts, int64_t count, int64_t n, T *out)
+{
+    __shared__ float run[16][64];
+    const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + c, each = ceil_div64(count, 16), end = min(count, each * (w + 1));
+    float s = 0.0f;
+    if (col < n) {
+#pragma unroll 8
+        for (int64_t p = each * w; p < end; ++p) s += parts[p * n + col];
+    }
+    run[w][c] = s;
+    __syncthreads();
+    if (w != 0 || col >= n) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += run[i][c];
+    out[col] = from_float<T>(s);
+}
+
 struct Plan {
     int fragments;  // per wave and direction
     int64_t tiles_m, tiles_n, splits, steps_per_split;
@@ -403,8 +423,25 @@ int check_workspace(const void *workspace, size_t have, size_t need)
     return AMSIM_OK;
 }
 
-// bytes of the quantised activations at the start of amsim_mxfp4_linear's workspace
-size_t activation_bytes(int64_t m, int64_t k) { return (size_t)(mx_code_bytes(m, k) + mx_scale_bytes(m, k)); }
+size_t operand_bytes(int64_t rows, int64_t length) { return (size_t)(mx_code_bytes(rows, length) + mx_scale_bytes(rows, length)); }
+size_t sums_bytes(int64_t m, int64_t n) { return ((size_t)ceil_div64(m, 32) * n * 4 + 255) / 256 * 256; }
+
+bool product_fits(int64_t m, int64_t n, int64_t k)
+{
+    return mx_extents_fit(m, k) && mx_extents_fit(n, k) && mx_extents_fit(m, n) && m && n && k;
+}
+
+int column_sums(const float *parts, int64_t count, int64_t n, void *out, int dtype, hipStream_t stream)
+{
+    const unsigned groups = (unsigned)ceil_div64(n, 64);
+    switch (dtype) {
+    case AMSIM_DTYPE_F32: column_sums_kernel<float><<<groups, 1024, 0, stream>>>(parts, count, n, (float *)out); break;
+    case AMSIM_DTYPE_BF16: column_sums_kernel<__bf16><<<groups, 1024, 0, stream>>>(parts, count, n, (__bf16 *)out); break;
+    default: column_sums_kernel<_Float16><<<groups, 1024, 0, stream>>>(parts, count, n, (_Float16 *)out); break;
+    }
+    AMSIM_HIP_CHECK(hipGetLastError());
+    return AMSIM_OK;
+}
 
 }  // namespace
 
@@ -416,7 +453,7 @@ extern "C" {
 
 size_t amsim_mxfp4_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k)
 {
-    return mx_extents_fit(m, k) && mx_extents_fit(n, k) && mx_extents_fit(m, n) && m && n && k ? product_workspace(m, n, k) : 0;
+    return product_fits(m, n, k) ? product_workspace(m, n, k) : 0;
 }
 
 int amsim_mxfp4_matmul(const void *a, const void *b, int64_t m, int64_t n, int64_t k, const void *bias, int bias_dtype, int act,
@@ -431,8 +468,8 @@ int amsim_mxfp4_matmul(const void *a, const void *b, int64_t m, int64_t n, int64
 
 size_t amsim_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k)
 {
-    if (!(mx_extents_fit(m, k) && mx_extents_fit(n, k) && mx_extents_fit(m, n) && m && n && k)) return 0;
-    return activation_bytes(m, k) + product_workspace(m, n, k);
+    if (!product_fits(m, n, k)) return 0;
+    return operand_bytes(m, k) + product_workspace(m, n, k);
 }
 
 int amsim_mxfp4_linear(const void *x, int dtype, int64_t row_stride, const void *w, int64_t m, int64_t n, int64_t k, const void *bias,
@@ -443,9 +480,71 @@ int amsim_mxfp4_linear(const void *x, int dtype, int64_t row_stride, const void 
     if (row_stride < k && m > 1) return fail(AMSIM_ERR_INVALID, "mxfp4: rows overlap");
     if (((uintptr_t)x & (element_bytes(dtype) - 1)) || ((uintptr_t)w & 15)) return fail(AMSIM_ERR_INVALID, "mxfp4: misaligned pointer");
     if (int rc = check_workspace(workspace, workspace_bytes, amsim_mxfp4_linear_workspace_bytes(m, n, k))) return rc;
-    if (int rc = mx_quantize(x, dtype, m, k, row_stride, workspace, nullptr, (hipStream_t)stream)) return rc;
+    const MxConversion job{x, nullptr, dtype, m, k, row_stride, (uint8_t *)workspace, nullptr, nullptr};
+    if (int rc = mx_convert(&job, 1, (hipStream_t)stream)) return rc;
     return product(operand(workspace, m, k), operand(w, n, k), k, bias, bias_dtype, act, out, dtype,
-                   (char *)workspace + activation_bytes(m, k), (hipStream_t)stream);
+                   (char *)workspace + operand_bytes(m, k), (hipStream_t)stream);
+}
+
+size_t amsim_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t k)
+{
+    return product_fits(m, n, k) ? operand_bytes(m, k) + operand_bytes(n, k) + product_workspace(m, n, k) : 0;
+}
+
+int amsim_mxfp4_dense(const void *x, int dtype, int64_t row_stride, const void *kernel, int kernel_dtype, int64_t kernel_row_stride,
+                      int64_t m, int64_t n, int64_t k, const void *bias, int bias_dtype, int act, void *out, void *x_columns,
+                      void *kernel_rows, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (int rc = check_product(m, n, k, bias, bias_dtype, act, out, dtype)) return rc;
+    if (!known_dtype(kernel_dtype)) return fail(AMSIM_ERR_INVALID, "mxfp4: unknown element type");
+    if (!x || !kernel) return fail(AMSIM_ERR_INVALID, "mxfp4: null pointer");
+    if ((row_stride < k && m > 1) || (kernel_row_stride < n && k > 1)) return fail(AMSIM_ERR_INVALID, "mxfp4: rows overlap");
+    if (((uintptr_t)x & (element_bytes(dtype) - 1)) || ((uintptr_t)kernel & (element_bytes(kernel_dtype) - 1)) || ((uintptr_t)x_columns & 15)
+        || ((uintptr_t)kernel_rows & 15))
+        return fail(AMSIM_ERR_INVALID, "mxfp4: misaligned pointer");
+    if (int rc = check_workspace(workspace, workspace_bytes, amsim_mxfp4_dense_workspace_bytes(m, n, k))) return rc;
+    uint8_t *x_rows = (uint8_t *)workspace, *kernel_columns = x_rows + operand_bytes(m, k);
+    const MxConversion jobs[2] = {{x, nullptr, dtype, m, k, row_stride, x_rows, (uint8_t *)x_columns, nullptr},
+                                  {kernel, nullptr, kernel_dtype, k, n, kernel_row_stride, (uint8_t *)kernel_rows, kernel_columns, nullptr}};
+    if (int rc = mx_convert(jobs, 2, (hipStream_t)stream)) return rc;
+    return product(operand(x_rows, m, k), operand(kernel_columns, n, k), k, bias, bias_dtype, act, out, dtype, kernel_columns + operand_bytes(n, k),
+                   (hipStream_t)stream);
+}
+
+size_t amsim_mxfp4_dense_grad_workspace_bytes(int64_t m, int64_t n, int64_t k)
+{
+    if (!product_fits(m, n, k)) return 0;
+    return operand_bytes(m, n) + operand_bytes(n, m) + sums_bytes(m, n) + std::max(product_workspace(m, k, n), product_workspace(k, n, m));
+}
+
+int amsim_mxfp4_dense_grad(const void *grad, int dtype, int64_t row_stride, const void *out, const void *x_columns, const void *kernel_rows,
+                           int64_t m, int64_t n, int64_t k, void *grad_x, void *grad_kernel, int kernel_dtype, void *grad_bias, int bias_dtype,
+                           void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!known_dtype(dtype) || (grad_kernel && !known_dtype(kernel_dtype)) || (grad_bias && !known_dtype(bias_dtype)))
+        return fail(AMSIM_ERR_INVALID, "mxfp4: unknown element type");
+    if (!mx_extents_fit(m, k) || !mx_extents_fit(n, k) || !mx_extents_fit(m, n)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: extents out of range");
+    if (m == 0 || n == 0 || k == 0) return fail(AMSIM_ERR_INVALID, "mxfp4: empty product");
+    if (row_stride < n && m > 1) return fail(AMSIM_ERR_INVALID, "mxfp4: rows overlap");
+    if (!grad || (grad_x && !kernel_rows) || (grad_kernel && !x_columns)) return fail(AMSIM_ERR_INVALID, "mxfp4: null pointer");
+    const uintptr_t element = element_bytes(dtype) - 1;
+    if (((uintptr_t)grad & element) || ((uintptr_t)out & element) || ((uintptr_t)x_columns & 15) || ((uintptr_t)kernel_rows & 15)
+        || ((uintptr_t)grad_x & 15) || ((uintptr_t)grad_kernel & 15) || (grad_bias && ((uintptr_t)grad_bias & (element_bytes(bias_dtype) - 1))))
+        return fail(AMSIM_ERR_INVALID, "mxfp4: misaligned pointer");
+    if (int rc = check_workspace(workspace, workspace_bytes, amsim_mxfp4_dense_grad_workspace_bytes(m, n, k))) return rc;
+    if (!grad_x && !grad_kernel && !grad_bias) return AMSIM_OK;
+    hipStream_t s = (hipStream_t)stream;
+    uint8_t *rows = (uint8_t *)workspace, *columns = rows + operand_bytes(m, n);
+    float *sums = (float *)(columns + operand_bytes(n, m));
+    char *partial = (char *)sums + sums_bytes(m, n);
+    const MxConversion job{grad, out, dtype, m, n, row_stride, grad_x ? rows : nullptr, grad_kernel ? columns : nullptr, grad_bias ? sums : nullptr};
+    if (int rc = mx_convert(&job, 1, s)) return rc;
+    if (grad_x)
+        if (int rc = product(operand(rows, m, n), operand(kernel_rows, k, n), n, nullptr, 0, AMSIM_ACT_NONE, grad_x, dtype, partial, s)) return rc;
+    if (grad_kernel)
+        if (int rc = product(operand(x_columns, k, m), operand(columns, n, m), m, nullptr, 0, AMSIM_ACT_NONE, grad_kernel, kernel_dtype, partial, s)) return rc;
+    if (grad_bias) return column_sums(sums, ceil_div64(m, 32), n, grad_bias, bias_dtype, s);
+    return AMSIM_OK;
 }
 
 }  // extern "C"

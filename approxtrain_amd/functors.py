@@ -526,6 +526,71 @@ def mxfp4_linear(x, weights, bias=None, activation=None):
     return out if x.dim() == 2 else out.reshape(tuple(x.shape[:-1]) + (w.rows,))
 
 
+@functools.lru_cache(maxsize=1024)
+def _mx_dense_sizes(m, n, k):
+    """Bytes: x's operand of its columns, the kernel's of its rows, and the workspaces of both directions."""
+    lib = load_library()
+    return (_mx_bytes(k, m), _mx_bytes(k, n), lib.amsim_mxfp4_dense_workspace_bytes(m, n, k),
+            lib.amsim_mxfp4_dense_grad_workspace_bytes(m, n, k))
+
+
+def _mx_rows(x, name):
+    """A matrix whose rows are contiguous, as (tensor, element type, row stride)."""
+    t, dtype, _, _, stride, swapped = _mx_source(x, name)
+    return (t, dtype, stride) if not swapped else (t.contiguous(), dtype, t.shape[1])
+
+
+def mxfp4_dense(x, kernel, bias=None, activation=None, keep_x=True, keep_kernel=True):
+    """``activation(Q(x) . Q(kernel) + bias)`` of ``x`` ``[rows, width]`` and ``kernel`` ``[width, units]``, and what the
+    backward pass multiplies by, as one buffer of bytes: x quantised along its rows' axis (``keep_x``, for the
+    kernel's gradient) and the kernel along its units (``keep_kernel``, for x's)."""
+    x, dtype, stride = _mx_rows(x, "x")
+    kernel, kernel_dtype, kernel_stride = _mx_rows(kernel, "kernel")
+    (m, k), n = x.shape, kernel.shape[1]
+    if kernel.shape[0] != k:
+        raise ValueError("the kernel must have as many rows as x has columns")
+    device = x.get_device()
+    if kernel.get_device() != device:
+        raise ValueError("x and the kernel must be on one device")
+    bias, bias_ptr, bias_dtype, act = _mx_epilogue(bias, activation, n, device)
+    x_bytes, kernel_bytes, ws_bytes, _ = _mx_dense_sizes(m, n, k)
+    out = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    kept = torch.empty((x_bytes if keep_x else 0) + (kernel_bytes if keep_kernel else 0), dtype=torch.uint8, device=x.device)
+    at = kept.data_ptr()
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+    check(load_library().amsim_mxfp4_dense(x.data_ptr(), dtype, stride, kernel.data_ptr(), kernel_dtype, kernel_stride, m, n, k, bias_ptr, bias_dtype,
+                                           act, out.data_ptr(), at if keep_x else None, (at + x_bytes if keep_x else at) if keep_kernel else None,
+                                           ws.data_ptr(), ws_bytes, torch._C._cuda_getCurrentRawStream(device)))
+    return out, kept
+
+
+def mxfp4_dense_grad(grad, kept, rows, width, units, out=None, kernel_dtype=None, bias_dtype=None, need_x=True):
+    """Gradients ``(of x, of the kernel, of the bias)`` of ``mxfp4_dense`` from ``grad`` ``[rows, units]`` and what that
+    call ``kept``; ``out``: its result, if a rectifier was applied.  A gradient of the kernel or of the bias is
+    computed where its type is given, x's (of grad's type) if ``need_x``; the others are None."""
+    grad, dtype, stride = _mx_rows(grad, "grad")
+    if tuple(grad.shape) != (rows, units):
+        raise ValueError("grad must have the result's shape")
+    if out is not None and (out.dtype is not grad.dtype or out.shape != grad.shape or not out.is_contiguous() or out.get_device() != grad.get_device()):
+        raise ValueError("out must be the contiguous result of mxfp4_dense, of grad's type and shape")
+    need_kernel = kernel_dtype is not None
+    x_bytes, kernel_bytes, _, ws_bytes = _mx_dense_sizes(rows, units, width)
+    if kept.get_device() != grad.get_device() or kept.numel() != (x_bytes if need_kernel else 0) + (kernel_bytes if need_x else 0):
+        raise ValueError("kept must be what mxfp4_dense returned for these gradients")
+    device, at = grad.device, kept.data_ptr()
+    grad_x = torch.empty((rows, width), dtype=grad.dtype, device=device) if need_x else None
+    grad_kernel = torch.empty((width, units), dtype=kernel_dtype, device=device) if need_kernel else None
+    grad_bias = torch.empty(units, dtype=bias_dtype, device=device) if bias_dtype is not None else None
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    check(load_library().amsim_mxfp4_dense_grad(
+        grad.data_ptr(), dtype, stride, None if out is None else out.data_ptr(), at if need_kernel else None,
+        (at + x_bytes if need_kernel else at) if need_x else None, rows, units, width, grad_x.data_ptr() if need_x else None,
+        grad_kernel.data_ptr() if need_kernel else None, _mx_dtype(kernel_dtype) if need_kernel else 0,
+        grad_bias.data_ptr() if grad_bias is not None else None, _mx_dtype(bias_dtype) if grad_bias is not None else 0, ws.data_ptr(), ws_bytes,
+        torch._C._cuda_getCurrentRawStream(grad.get_device())))
+    return grad_x, grad_kernel, grad_bias
+
+
 # ---- AdamW over many tensors -----------------------------------------------------------------------
 
 class AdamWState:

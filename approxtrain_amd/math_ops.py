@@ -86,31 +86,18 @@ class _LinearMX(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, kernel, bias, activation):
-        need_x, need_kernel = ctx.needs_input_grad[:2]
-        by_rows, by_columns = functors.mxfp4_quantize_both(x) if need_kernel else (functors.mxfp4_quantize(x), None)
-        w_rows, w_columns = functors.mxfp4_quantize_both(kernel) if need_x else (None, functors.mxfp4_quantize(kernel, axis=0))
-        out = functors.mxfp4_matmul(by_rows, w_columns, bias, activation, x.dtype)
-        relu = activation == "relu"
-        ctx.save_for_backward(by_columns.data if need_kernel else None, w_rows.data if need_x else None, out if relu else None)
-        ctx.attrs = (x.shape, kernel.shape, x.dtype, kernel.dtype, None if bias is None else bias.dtype)
+        need_x, need_kernel, need_bias, _ = ctx.needs_input_grad
+        out, kept = functors.mxfp4_dense(x, kernel, bias, activation, keep_x=need_kernel, keep_kernel=need_x)
+        ctx.save_for_backward(kept, out if activation == "relu" else None)
+        ctx.attrs = x.shape + (kernel.shape[1],), kernel.dtype if need_kernel else None, bias.dtype if need_bias else None, need_x
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x_columns, w_rows, out = ctx.saved_tensors
-        (rows, width), (_, units), x_dtype, kernel_dtype, bias_dtype = ctx.attrs
-        if out is not None:
-            grad = grad * (out > 0)
-        grad_x = grad_kernel = grad_bias = None
-        g_rows, g_columns = functors.mxfp4_quantize_both(grad)
-        if ctx.needs_input_grad[0]:
-            grad_x = functors.mxfp4_matmul(g_rows, functors.MXTensor(w_rows, width, units), dtype=x_dtype)
-        if ctx.needs_input_grad[1]:
-            grad_kernel = functors.mxfp4_matmul(functors.MXTensor(x_columns, width, rows), g_columns, dtype=kernel_dtype)
-        if bias_dtype is not None and ctx.needs_input_grad[2]:
-            grad_bias = grad.sum(0, dtype=torch.float32).to(bias_dtype)
-        return grad_x, grad_kernel, grad_bias, None
+        kept, out = ctx.saved_tensors
+        shape, kernel_dtype, bias_dtype, need_x = ctx.attrs
+        return functors.mxfp4_dense_grad(grad, kept, *shape, out, kernel_dtype, bias_dtype, need_x) + (None,)
 
 
 def linearmx(x, kernel, bias=None, activation=None):

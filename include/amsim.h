@@ -328,6 +328,23 @@ int amsim_mxfp4_linear(const void *x, int dtype, int64_t row_stride, const void 
                        const void *bias, int bias_dtype, int act, void *out, void *workspace, size_t workspace_bytes,
                        void *stream);
 
+/* The training step of a dense layer in MXFP4, a conversion and the products in one call each.  amsim_mxfp4_dense:
+ * out[m][n] = act(x[m][k] kernel[k][n] + bias), both operands quantised along k; for the backward pass it also
+ * keeps x quantised along m (x_columns, an operand of k x m) and the kernel along n (kernel_rows, of k x n), either of
+ * which may be NULL.  amsim_mxfp4_dense_grad, for a gradient[m][n] of x's type: with out (the forward pass's, for the
+ * rectifier) not NULL the gradient counts as zero where out is not above zero; grad_x[m][k] = grad kernel^T,
+ * grad_kernel[k][n] = x^T grad and grad_bias[n], the sums of its columns in 32 bits, each in its tensor's type and
+ * each NULL if not wanted.  No result depends on the order of arrival. */
+size_t amsim_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int amsim_mxfp4_dense(const void *x, int dtype, int64_t row_stride, const void *kernel, int kernel_dtype,
+                      int64_t kernel_row_stride, int64_t m, int64_t n, int64_t k, const void *bias, int bias_dtype, int act,
+                      void *out, void *x_columns, void *kernel_rows, void *workspace, size_t workspace_bytes, void *stream);
+size_t amsim_mxfp4_dense_grad_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int amsim_mxfp4_dense_grad(const void *grad, int dtype, int64_t row_stride, const void *out, const void *x_columns,
+                           const void *kernel_rows, int64_t m, int64_t n, int64_t k, void *grad_x, void *grad_kernel,
+                           int kernel_dtype, void *grad_bias, int bias_dtype, void *workspace, size_t workspace_bytes,
+                           void *stream);
+
 /* ---- AdamW over many tensors (no counterpart in the reference: its optimizers are Keras's) ------------
  *   g = grad [* *grad_scale]    m' = beta1 m + (1 - beta1) g    v' = beta2 v + ((1 - beta2) g) g
  *   p' = p (1 - lr weight_decay) - (m' / (sqrt(v') / sqrt(1 - beta2^step) + eps)) lr / (1 - beta1^step)
