@@ -8,7 +8,7 @@ import functools
 
 import torch
 
-from ._lib import AdamWHyper, check, conv_geometry, load_library
+from ._lib import check, conv_geometry, load_library
 from .lut import ApproxMulLut
 from .mx import DTYPES, MXTensor
 
@@ -370,120 +370,57 @@ def _device_of(t, name):
     return index
 
 
-def _mx_source(x, name="x"):
-    """(tensor, element type, rows, columns, row stride, whether rows and columns have changed places): a
-    rank-2 tensor as the library reads it, in place where either of its axes is contiguous."""
-    _device_of(x, name)
-    dtype = DTYPES.get(x.dtype)
-    if dtype is None:
-        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
-    if x.dim() != 2:
-        raise ValueError(f"{name} must be a matrix")
-    rows, cols = x.shape
-    if rows == 0 or cols == 0:
-        raise ValueError(f"{name} is empty: blocks of no elements have no scale")
-    s0, s1 = x.stride()
-    if x.is_neg():
-        x = x.resolve_neg()
-        s0, s1 = x.stride()
-    if (s1 == 1 or cols == 1) and (s0 >= cols or rows == 1):
-        return x, dtype, rows, cols, s0 if rows > 1 else cols, False
-    if (s0 == 1 or rows == 1) and (s1 >= rows or cols == 1):
-        return x, dtype, cols, rows, s1 if cols > 1 else rows, True
-    return x.contiguous(), dtype, rows, cols, cols, False
+def _native():
+    """The calls that take tensors, ``_native.so``; loud where it is not built."""
+    global _NATIVE
+    if _NATIVE is None:
+        load_library()  # (torch's copy of the HIP runtime first)
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise ImportError(f"approxtrain_amd/_native.so is not built or does not load ({e}): run `make -C approxtrain_amd/csrc`") from e
+        _NATIVE = module
+    return _NATIVE
 
 
-@functools.lru_cache(maxsize=1024)
-def _mx_bytes(rows, length):
-    n = load_library().amsim_mxfp4_operand_workspace_bytes(rows, length)
-    if n == 0:
-        raise ValueError(f"a {rows} x {length} tensor is out of the 4-bit products' range")
-    return n
+_NATIVE = None
 
 
-def _mx_empty(like, rows, length):
-    return MXTensor(torch.empty(_mx_bytes(rows, length), dtype=torch.uint8, device=like.device), rows, length)
+def _activation(activation):
+    if activation not in ACTIVATIONS:
+        raise ValueError("fused activation must be None, 'linear' or 'relu'")
+    return ACTIVATIONS[activation]
 
 
-def _mx_quantize(x, by_rows, by_columns):
-    x, dtype, rows, cols, stride, swapped = _mx_source(x)
-    if swapped:
-        by_rows, by_columns = by_columns, by_rows
-    r = _mx_empty(x, rows, cols) if by_rows else None
-    c = _mx_empty(x, cols, rows) if by_columns else None
-    check(load_library().amsim_mxfp4_quantize(x.data_ptr(), dtype, rows, cols, stride, r.data.data_ptr() if by_rows else None,
-                                              c.data.data_ptr() if by_columns else None,
-                                              torch._C._cuda_getCurrentRawStream(x.get_device())))
-    return (c, r) if swapped else (r, c)
+def _mx_operand(q, name):
+    if not isinstance(q, MXTensor):
+        raise TypeError(f"{name} must be an MXTensor (functors.mxfp4_quantize)")
+    return q
 
 
 def mxfp4_quantize(x, axis=-1):
     """Matrix ``x`` (float32, bfloat16 or float16, any strides) as an MXFP4 operand whose blocks of 32 run along
     ``axis``, the axis that a product will sum over: ``-1`` gives an operand of x's rows, ``0`` one of its
     columns (x's transpose, read in place)."""
-    if axis in (-1, 1):
-        return _mx_quantize(x, True, False)[0]
-    if axis in (0, -2):
-        return _mx_quantize(x, False, True)[1]
+    if axis == -1 or axis == 1:
+        data, _, rows, cols = _native().quantize(x, True, False)
+        return MXTensor(data, rows, cols)
+    if axis == 0 or axis == -2:
+        _, data, rows, cols = _native().quantize(x, False, True)
+        return MXTensor(data, cols, rows)
     raise ValueError("axis must be 0 or 1 (or -2 or -1)")
 
 
 def mxfp4_quantize_both(x):
     """``(mxfp4_quantize(x, -1), mxfp4_quantize(x, 0))`` from one reading of ``x``."""
-    return _mx_quantize(x, True, True)
-
-
-def _mx_operand(q, name):
-    if not isinstance(q, MXTensor):
-        raise TypeError(f"{name} must be an MXTensor (functors.mxfp4_quantize)")
-    _device_of(q.data, name)
-    return q
-
-
-def _mx_dtype(dtype):
-    if dtype not in DTYPES:
-        raise TypeError(f"the result's type must be float32, bfloat16 or float16, got {dtype}")
-    return DTYPES[dtype]
+    by_rows, by_columns, rows, cols = _native().quantize(x, True, True)
+    return MXTensor(by_rows, rows, cols), MXTensor(by_columns, cols, rows)
 
 
 def mxfp4_dequantize(q, dtype=torch.float32):
     """The values of an MXFP4 operand, ``[rows, length]``."""
-    _mx_operand(q, "q")
-    code = _mx_dtype(dtype)
-    out = torch.empty((q.rows, q.length), dtype=dtype, device=q.data.device)
-    check(load_library().amsim_mxfp4_dequantize(q.data.data_ptr(), q.rows, q.length, code, out.data_ptr(),
-                                                torch._C._cuda_getCurrentRawStream(out.get_device())))
-    return out
-
-
-def _mx_epilogue(bias, activation, units, device):
-    if activation not in ACTIVATIONS:
-        raise ValueError("fused activation must be None, 'linear' or 'relu'")
-    if bias is None:
-        return None, None, 0, ACTIVATIONS[activation]
-    if _device_of(bias, "bias") != device:
-        raise ValueError("bias must be on the operands' device")
-    if bias.dtype not in DTYPES:
-        raise TypeError(f"bias must be float32, bfloat16 or float16, got {bias.dtype}")
-    if bias.dim() != 1 or bias.shape[0] != units:
-        raise ValueError("bias must have one entry per output channel")
-    bias = bias.contiguous()
-    return bias, bias.data_ptr(), DTYPES[bias.dtype], ACTIVATIONS[activation]
-
-
-@functools.lru_cache(maxsize=1024)
-def _mx_matmul_workspace(m, n, k):
-    return load_library().amsim_mxfp4_matmul_workspace_bytes(m, n, k)
-
-
-@functools.lru_cache(maxsize=1024)
-def _mx_linear_workspace(m, n, k):
-    return load_library().amsim_mxfp4_linear_workspace_bytes(m, n, k)
-
-
-def _scratch(nbytes, device):
-    # (torch's allocations start on 512-byte boundaries)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    q = _mx_operand(q, "q")
+    return _native().dequantize(q.data, q.rows, q.length, dtype)
 
 
 def mxfp4_matmul(a, b, bias=None, activation=None, dtype=torch.float32):
@@ -492,15 +429,7 @@ def mxfp4_matmul(a, b, bias=None, activation=None, dtype=torch.float32):
     _mx_operand(a, "a"), _mx_operand(b, "b")
     if a.length != b.length:
         raise ValueError("the operands' lengths differ")
-    code = _mx_dtype(dtype)
-    keep, bptr, bcode, act = _mx_epilogue(bias, activation, b.rows, a.data.get_device())
-    out = torch.empty((a.rows, b.rows), dtype=dtype, device=a.data.device)
-    nbytes = _mx_matmul_workspace(a.rows, b.rows, a.length)
-    ws = _scratch(nbytes, out.device)
-    check(load_library().amsim_mxfp4_matmul(a.data.data_ptr(), b.data.data_ptr(), a.rows, b.rows, a.length, bptr, bcode, act,
-                                            out.data_ptr(), code, ws.data_ptr() if nbytes else None, nbytes,
-                                            torch._C._cuda_getCurrentRawStream(out.get_device())))
-    return out
+    return _native().matmul(a.data, a.rows, b.data, b.rows, a.length, bias, _activation(activation), dtype)
 
 
 def mxfp4_linear(x, weights, bias=None, activation=None):
@@ -508,87 +437,21 @@ def mxfp4_linear(x, weights, bias=None, activation=None):
     way, and weights that lie in MXFP4: ``mxfp4_quantize(kernel, axis=0)`` of a ``[length, units]`` kernel.  The
     result has x's type."""
     w = _mx_operand(weights, "weights")
-    if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] != w.length:
-        raise ValueError("x's last axis must have the weights' length")
-    flat = x if x.dim() == 2 else x.reshape(-1, w.length)
-    if flat.shape[0] == 0:
-        return x.new_empty(tuple(x.shape[:-1]) + (w.rows,))
-    flat, dtype, m, k, stride, swapped = _mx_source(flat)
-    if swapped:
-        flat, m, k, stride = flat.contiguous(), k, m, m
-    keep, bptr, bcode, act = _mx_epilogue(bias, activation, w.rows, flat.get_device())
-    out = torch.empty((m, w.rows), dtype=flat.dtype, device=flat.device)
-    nbytes = _mx_linear_workspace(m, w.rows, k)
-    ws = _scratch(nbytes, out.device)
-    check(load_library().amsim_mxfp4_linear(flat.data_ptr(), dtype, stride, w.data.data_ptr(), m, w.rows, k, bptr, bcode, act,
-                                            out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes,
-                                            torch._C._cuda_getCurrentRawStream(out.get_device())))
-    return out if x.dim() == 2 else out.reshape(tuple(x.shape[:-1]) + (w.rows,))
-
-
-@functools.lru_cache(maxsize=1024)
-def _mx_dense_sizes(m, n, k):
-    """Bytes: x's operand of its columns, the kernel's of its rows, and the workspaces of both directions."""
-    lib = load_library()
-    return (_mx_bytes(k, m), _mx_bytes(k, n), lib.amsim_mxfp4_dense_workspace_bytes(m, n, k),
-            lib.amsim_mxfp4_dense_grad_workspace_bytes(m, n, k))
-
-
-def _mx_rows(x, name):
-    """A matrix whose rows are contiguous, as (tensor, element type, row stride)."""
-    t, dtype, _, _, stride, swapped = _mx_source(x, name)
-    return (t, dtype, stride) if not swapped else (t.contiguous(), dtype, t.shape[1])
+    return _native().linear(x, w.data, w.rows, w.length, bias, _activation(activation))
 
 
 def mxfp4_dense(x, kernel, bias=None, activation=None, keep_x=True, keep_kernel=True):
     """``activation(Q(x) . Q(kernel) + bias)`` of ``x`` ``[rows, width]`` and ``kernel`` ``[width, units]``, and what the
     backward pass multiplies by, as one buffer of bytes: x quantised along its rows' axis (``keep_x``, for the
     kernel's gradient) and the kernel along its units (``keep_kernel``, for x's)."""
-    x, dtype, stride = _mx_rows(x, "x")
-    kernel, kernel_dtype, kernel_stride = _mx_rows(kernel, "kernel")
-    (m, k), n = x.shape, kernel.shape[1]
-    if kernel.shape[0] != k:
-        raise ValueError("the kernel must have as many rows as x has columns")
-    device = x.get_device()
-    if kernel.get_device() != device:
-        raise ValueError("x and the kernel must be on one device")
-    bias, bias_ptr, bias_dtype, act = _mx_epilogue(bias, activation, n, device)
-    x_bytes, kernel_bytes, ws_bytes, _ = _mx_dense_sizes(m, n, k)
-    out = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    kept = torch.empty((x_bytes if keep_x else 0) + (kernel_bytes if keep_kernel else 0), dtype=torch.uint8, device=x.device)
-    at = kept.data_ptr()
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-    check(load_library().amsim_mxfp4_dense(x.data_ptr(), dtype, stride, kernel.data_ptr(), kernel_dtype, kernel_stride, m, n, k, bias_ptr, bias_dtype,
-                                           act, out.data_ptr(), at if keep_x else None, (at + x_bytes if keep_x else at) if keep_kernel else None,
-                                           ws.data_ptr(), ws_bytes, torch._C._cuda_getCurrentRawStream(device)))
-    return out, kept
+    return _native().dense(x, kernel, bias, _activation(activation), keep_x, keep_kernel)
 
 
 def mxfp4_dense_grad(grad, kept, rows, width, units, out=None, kernel_dtype=None, bias_dtype=None, need_x=True):
     """Gradients ``(of x, of the kernel, of the bias)`` of ``mxfp4_dense`` from ``grad`` ``[rows, units]`` and what that
-    call ``kept``; ``out``: its result, if a rectifier was applied.  A gradient of the kernel or of the bias is
-    computed where its type is given, x's (of grad's type) if ``need_x``; the others are None."""
-    grad, dtype, stride = _mx_rows(grad, "grad")
-    if tuple(grad.shape) != (rows, units):
-        raise ValueError("grad must have the result's shape")
-    if out is not None and (out.dtype is not grad.dtype or out.shape != grad.shape or not out.is_contiguous() or out.get_device() != grad.get_device()):
-        raise ValueError("out must be the contiguous result of mxfp4_dense, of grad's type and shape")
-    need_kernel = kernel_dtype is not None
-    x_bytes, kernel_bytes, _, ws_bytes = _mx_dense_sizes(rows, units, width)
-    if kept.get_device() != grad.get_device() or kept.numel() != (x_bytes if need_kernel else 0) + (kernel_bytes if need_x else 0):
-        raise ValueError("kept must be what mxfp4_dense returned for these gradients")
-    device, at = grad.device, kept.data_ptr()
-    grad_x = torch.empty((rows, width), dtype=grad.dtype, device=device) if need_x else None
-    grad_kernel = torch.empty((width, units), dtype=kernel_dtype, device=device) if need_kernel else None
-    grad_bias = torch.empty(units, dtype=bias_dtype, device=device) if bias_dtype is not None else None
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-    check(load_library().amsim_mxfp4_dense_grad(
-        grad.data_ptr(), dtype, stride, None if out is None else out.data_ptr(), at if need_kernel else None,
-        (at + x_bytes if need_kernel else at) if need_x else None, rows, units, width, grad_x.data_ptr() if need_x else None,
-        grad_kernel.data_ptr() if need_kernel else None, _mx_dtype(kernel_dtype) if need_kernel else 0,
-        grad_bias.data_ptr() if grad_bias is not None else None, _mx_dtype(bias_dtype) if grad_bias is not None else 0, ws.data_ptr(), ws_bytes,
-        torch._C._cuda_getCurrentRawStream(grad.get_device())))
-    return grad_x, grad_kernel, grad_bias
+    call ``kept`` for just these; ``out``: its result, if a rectifier was applied.  A gradient of the kernel or of the
+    bias is computed where its type is given, x's (of grad's type) if ``need_x``; the others are None."""
+    return _native().dense_grad(grad, kept, rows, width, units, out, kernel_dtype, bias_dtype, need_x)
 
 
 # ---- AdamW over many tensors -----------------------------------------------------------------------
@@ -622,8 +485,7 @@ class AdamWState:
         self.m, self.v = torch.zeros(at, dtype=kind, device=device), torch.zeros(at, dtype=kind, device=device)
         scales = at // self.BLOCK if state_bits == 8 else 0
         self.m_scale, self.v_scale = torch.zeros(scales, device=device), torch.zeros(scales, device=device)
-        self._c_sizes = (C.c_int64 * len(params))(*self.sizes)
-        self._pointers = C.c_void_p * len(params)
+        self._list = _native().TensorList(self.sizes, self.dtype, self.device_index)
 
     def _check(self, tensors, name, dtype):
         index = self.device_index
@@ -652,30 +514,5 @@ def adamw_step(state, grads, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, we
     launch for about a hundred tensors.  ``grads``: a contiguous tensor, or None (its parameter stays as it is), for each
     parameter, all of one type.  ``grad_scale``: a float32 tensor of one element on the device that multiplies
     the gradients (a clipping factor, say), or None."""
-    params = state.params
-    grads = list(grads)
-    if len(grads) != len(params):
-        raise ValueError("as many gradients as parameters are needed")
-    if torch._C._cuda_getDevice() != state.device_index:
-        raise ValueError("the parameters' device is not the current one")
-    gdtype = next((g.dtype for g in grads if g is not None), None)
-    if gdtype is None:
-        return
-    if gdtype not in DTYPES:
-        raise TypeError(f"gradients must be float32, bfloat16 or float16, got {gdtype}")
-    state._check(params, "params", state.dtype)
-    state._check(grads, "grads", gdtype)
-    if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1
-                                   or grad_scale.get_device() != state.device_index):
-        raise ValueError("grad_scale must be one float32 on the parameters' device")
-    table = state._pointers
-    hyper = AdamWHyper(step, lr, beta1, beta2, eps, weight_decay)
-    bits8 = state.state_bits == 8
-    check(load_library().amsim_adamw_step(len(params), table(*[p.data_ptr() for p in params]),
-                                          table(*[None if g is None else g.data_ptr() for g in grads]), state._c_sizes,
-                                          DTYPES[state.dtype], DTYPES[gdtype], state.state_bits, state.m.data_ptr(), state.v.data_ptr(),
-                                          state.m_scale.data_ptr() if bits8 else None, state.v_scale.data_ptr() if bits8 else None,
-                                          C.byref(hyper), grad_scale.data_ptr() if grad_scale is not None else None,
-                                          torch._C._cuda_getCurrentRawStream(state.device_index)))
-    # (written behind autograd's back: a graph that saved a parameter has to notice)
-    torch.autograd.graph.increment_version(params)
+    _native().adamw_step(state._list, state.params, grads if type(grads) is list else list(grads), state.state_bits, state.m, state.v, state.m_scale,
+                         state.v_scale, step, lr, beta1, beta2, eps, weight_decay, grad_scale)

@@ -79,36 +79,9 @@ def matmulam(a, b, transpose_a=False, transpose_b=False, adjoint_a=False, adjoin
     return out
 
 
-class _LinearMX(torch.autograd.Function):
-    """``activation(Q(x) . Q(kernel) + bias)`` in MXFP4.  Each of the three products has its operands quantised
-    along the axis it sums over, so x, the kernel and the gradient are quantised both ways, each from one
-    reading; what the backward pass needs is kept in 4 bits."""
-
-    @staticmethod
-    def forward(ctx, x, kernel, bias, activation):
-        need_x, need_kernel, need_bias, _ = ctx.needs_input_grad
-        out, kept = functors.mxfp4_dense(x, kernel, bias, activation, keep_x=need_kernel, keep_kernel=need_x)
-        ctx.save_for_backward(kept, out if activation == "relu" else None)
-        ctx.attrs = x.shape + (kernel.shape[1],), kernel.dtype if need_kernel else None, bias.dtype if need_bias else None, need_x
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        kept, out = ctx.saved_tensors
-        shape, kernel_dtype, bias_dtype, need_x = ctx.attrs
-        return functors.mxfp4_dense_grad(grad, kept, *shape, out, kernel_dtype, bias_dtype, need_x) + (None,)
-
-
 def linearmx(x, kernel, bias=None, activation=None):
     """``activation(x . kernel + bias)`` with both operands, and in the backward pass the gradient, in microscaled
     4-bit floating point: ``x`` ``[..., width]``, ``kernel`` ``[width, units]`` and ``bias`` ``[units]`` in float32,
     bfloat16 or float16 each; the result has x's type, each gradient its own tensor's.  ``activation``: None,
     'linear' or 'relu', applied as the result is stored.  (Gradients of gradients are not provided.)"""
-    if not isinstance(x, torch.Tensor) or x.dim() < 1 or kernel.dim() != 2 or x.shape[-1] != kernel.shape[0]:
-        raise ValueError("linearmx expects x [..., width] and kernel [width, units]")
-    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if flat.numel() == 0 or kernel.numel() == 0:
-        raise ValueError("linearmx of no elements")
-    out = _LinearMX.apply(flat, kernel, bias, activation)
-    return out if x.dim() == 2 else out.reshape(tuple(x.shape[:-1]) + (kernel.shape[1],))
+    return functors._native().linearmx(x, kernel, bias, functors._activation(activation))
