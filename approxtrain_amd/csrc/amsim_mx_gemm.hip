@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <utility>
 
 namespace amsim {
@@ -52,23 +53,18 @@ __device__ __forceinline__ void store4(T *o, const float (&v)[4], int count, boo
 }
 
 // columns n .. n + 3 of row m, bias and activation included
-__device__ __forceinline__ void finish4(const GemmArgs &g, int64_t m, int64_t n, float (&v)[4])
+__device__ __forceinline__ void finish4(const void *bias, int bias_dtype, int act, void *out, int out_dtype, int64_t m, int64_t n, int64_t N, float (&v)[4])
 {
-    const int64_t N = g.b.rows;
     const int count = (int)(N - n < 4 ? N - n : 4);
     const bool vector = N % 4 == 0;
-    if (g.partial) {
-        store4(g.partial + ((int64_t)blockIdx.y * g.a.rows + m) * N + n, v, count, vector);
-        return;
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if (g.bias && i < count) v[i] += load_as_float(g.bias, g.bias_dtype, n + i);
-        v[i] = activate(v[i], g.act);
+        if (bias && i < count) v[i] += load_as_float(bias, bias_dtype, n + i);
+        v[i] = activate(v[i], act);
     }
-    if (g.out_dtype == AMSIM_DTYPE_F32) store4((float *)g.out + m * N + n, v, count, vector);
-    else if (g.out_dtype == AMSIM_DTYPE_BF16) store4((__bf16 *)g.out + m * N + n, v, count, vector);
-    else store4((_Float16 *)g.out + m * N + n, v, count, vector);
+    if (out_dtype == AMSIM_DTYPE_F32) store4((float *)out + m * N + n, v, count, vector);
+    else if (out_dtype == AMSIM_DTYPE_BF16) store4((__bf16 *)out + m * N + n, v, count, vector);
+    else store4((_Float16 *)out + m * N + n, v, count, vector);
 }
 
 template <int SA, int SB> __device__ __forceinline__ v4f mfma(v4i a, v4i b, v4f c, int sa, int sb)
@@ -299,6 +295,136 @@ __global__ __launch_bounds__(WG, 1) void gemm_kernel(GemmArgs g)
     else store((_Float16)0.0f);
 }
 
+// Few rows: bound by the reading of b, and for one layer of one token by latency alone.  A workgroup takes 16
+// of b's rows and the whole reduction, its waves every n-th step each; their sums meet in LDS and are added in order.
+struct FewArgs {
+    Operand b, a;            // a: of few_kernel
+    const void *x;           // of raw_kernel: [rows][k], rows row_stride elements apart
+    int64_t row_stride, rows, k, steps;
+    const void *bias;
+    int bias_dtype, act, out_dtype;
+    void *out;
+};
+constexpr int AHEAD = 4;     // steps of b that a wave has under way at once
+
+// (behind the last step it is loaded again, and not used)
+struct FewSteps {
+    v4i codes[AHEAD];
+    int scales[AHEAD];
+    __device__ __forceinline__ void load(const FewArgs &g, int64_t f, int64_t s, int waves)
+    {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h) {
+            const int64_t t = min<int64_t>(s + h * waves, g.steps - 1);
+            codes[h] = *(const v4i *)(g.b.codes + ((f * g.steps + t) * 64 + lane) * 16);
+            scales[h] = g.b.scales[((f / 4 * g.steps + t) * 64 + lane) * 4 + f % 4];
+        }
+    }
+};
+
+// the fragments' sums over the waves and their results, a fragment to a wave
+template <int FA> __device__ __forceinline__ void finish_few(const FewArgs &g, int64_t f, v4f (&sums)[16][FA][64], const v4f (&acc)[FA])
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+#pragma unroll
+    for (int i = 0; i < FA; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < FA; i += waves) {
+        v4f z = sums[0][i][lane];
+        for (int w = 1; w < waves; ++w) z += sums[w][i][lane];
+        const int64_t m = 16 * i + lane % 16, n = f * 16 + lane / 16 * 4, N = g.b.rows;
+        if (m >= g.rows || n >= N) continue;
+        float v[4] = {z[0], z[1], z[2], z[3]};
+        finish4(g.bias, g.bias_dtype, g.act, g.out, g.out_dtype, m, n, N, v);
+    }
+}
+
+// FA fragments of converted rows.
+template <int FA>
+__global__ __launch_bounds__(1024) void few_kernel(FewArgs g)
+{
+    __shared__ v4f sums[16][FA][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    v4f acc[FA] = {};
+    for (int64_t s = wave; s < g.steps; s += AHEAD * waves) {
+        FewSteps b;
+        b.load(g, blockIdx.x, s, waves);
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h) {
+            const int64_t t = s + h * waves;
+            if (t >= g.steps) break;
+            v4i a[FA];
+#pragma unroll
+            for (int i = 0; i < FA; ++i) a[i] = *(const v4i *)(g.a.codes + ((min<int64_t>(i, g.a.fragments - 1) * g.steps + t) * 64 + lane) * 16);
+            const int ca = *(const int *)(g.a.scales + (t * 64 + lane) * 4);
+            for_each<FA>([&](auto i) { acc[i.value] = mfma<0, i.value>(b.codes[h], a[i.value], acc[i.value], b.scales[h], ca); });
+        }
+    }
+    finish_few(g, blockIdx.x, sums, acc);
+}
+
+// Up to 16 rows as they come: every workgroup converts them for itself, into LDS, four lanes to a block, while its
+// first loads of b are under way.  That saves a launch, and for a token's layer half the time.
+constexpr int64_t RAW_VALUES = 40960;  // rows x length (in whole steps) that it holds: 22 KB of LDS
+template <typename X>
+__global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
+{
+    __shared__ v4f sums[16][1][64];
+    extern __shared__ __attribute__((aligned(16))) uint8_t converted[];  // codes [block][row][16 bytes], scales [block][row]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int rows = (int)g.rows, apart = rows | 1, blocks = (int)g.steps * 4;  // (an odd distance: a row's blocks lie in different banks)
+    uint8_t *scales = converted + blocks * apart * 16;
+    FewSteps b;
+    b.load(g, blockIdx.x, wave, waves);
+    const int eighths = blocks * 4, down = blockDim.x / eighths, across = blockDim.x % eighths;
+    int r = threadIdx.x / eighths, e8 = threadIdx.x % eighths;
+    while (r < rows) {  // (a block's four lanes stay together)
+        constexpr int BATCH = 2;
+        X v[BATCH][8] = {};
+        int row[BATCH], eighth[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            row[j] = r, eighth[j] = e8;
+            r += down, e8 += across;
+            if (e8 >= eighths) e8 -= eighths, ++r;
+            if (row[j] >= rows) continue;
+            const X *p = (const X *)g.x + row[j] * g.row_stride + eighth[j] * 8;
+            if (eighth[j] * 8 + 8 <= g.k) {
+                __builtin_memcpy(v[j], p, sizeof(v[j]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (eighth[j] * 8 + e < g.k) v[j][e] = p[e];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            if (row[j] >= rows) break;
+            uint32_t largest = mx_exponent_field(v[j]);
+            largest = max(largest, (uint32_t)__shfl_xor((int)largest, 1, 64));
+            largest = max(largest, (uint32_t)__shfl_xor((int)largest, 2, 64));
+            const uint32_t code = mx_scale_code(largest);
+            const int at = eighth[j] / 4 * apart + row[j];
+            *(uint32_t *)(converted + at * 16 + eighth[j] % 4 * 4) = mx_encode8(v[j], code);
+            if (eighth[j] % 4 == 0) scales[at] = (uint8_t)code;
+        }
+    }
+    __syncthreads();
+    const int row = min(lane % 16, rows - 1);  // (results of rows that do not exist are not stored)
+    v4f acc[1] = {};
+    for (int64_t s = wave; s < g.steps; s += AHEAD * waves) {
+        if (s != wave) b.load(g, blockIdx.x, s, waves);
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h) {
+            const int t = (int)s + h * waves, at = (4 * t + lane / 16) * apart + row;
+            if (t >= g.steps) break;
+            acc[0] = mfma<0, 0>(b.codes[h], *(const v4i *)(converted + at * 16), acc[0], b.scales[h], scales[at]);
+        }
+    }
+    finish_few(g, blockIdx.x, sums, acc);
+}
+
 // The partial sums of a split reduction, added in the order of the splits.
 __global__ __launch_bounds__(WG) void gemm_reduce_kernel(GemmArgs g, int splits)
 {
@@ -319,9 +445,7 @@ __global__ __launch_bounds__(WG) void gemm_reduce_kernel(GemmArgs g, int splits)
                 if (i < count) v[i] += p[i];
         }
     }
-    GemmArgs h = g;
-    h.partial = nullptr;
-    finish4(h, m, n, v);
+    finish4(g.bias, g.bias_dtype, g.act, g.out, g.out_dtype, m, n, N, v);
 }
 
 // Sums of columns from those of every 32 rows, in order: 64 columns and 16 runs of rows to a workgroup.
@@ -377,15 +501,33 @@ Plan plan(int64_t m, int64_t n, int64_t k)
     return best;
 }
 
+// Rows up to which few_kernel serves
+constexpr int64_t FEW = 64;
+
 size_t product_workspace(int64_t m, int64_t n, int64_t k)
 {
+    if (m <= FEW) return 0;
     const Plan p = plan(m, n, k);
     return p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
+}
+
+int launch_few(void (*kernel)(FewArgs), const FewArgs &g, int64_t lds, hipStream_t stream)
+{
+    if (g.b.fragments >= (1ll << 22)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
+    int waves = 1;
+    while (waves < 16 && waves < g.steps) waves *= 2;
+    kernel<<<(unsigned)g.b.fragments, 64 * waves, lds, stream>>>(g);
+    AMSIM_HIP_CHECK(hipGetLastError());
+    return AMSIM_OK;
 }
 
 int product(const Operand &a, const Operand &b, int64_t k, const void *bias, int bias_dtype, int act, void *out, int out_dtype,
             void *workspace, hipStream_t stream)
 {
+    if (a.rows <= FEW) {
+        const FewArgs f{b, a, nullptr, 0, a.rows, k, mx_steps(k), bias, bias_dtype, act, out_dtype, out};
+        return launch_few(a.rows <= 16 ? few_kernel<1> : a.rows <= 32 ? few_kernel<2> : few_kernel<4>, f, 0, stream);
+    }
     const Plan p = plan(a.rows, b.rows, k);
     const int64_t tiles = p.tiles_m * p.tiles_n, quads = a.rows * ceil_div64(b.rows, 4);
     if (tiles >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
@@ -421,6 +563,15 @@ int check_workspace(const void *workspace, size_t have, size_t need)
 {
     if (need && (!workspace || have < need || ((uintptr_t)workspace & 255))) return fail(AMSIM_ERR_WORKSPACE, "mxfp4: workspace missing, misaligned or too small");
     return AMSIM_OK;
+}
+
+// Whether few rows are converted by every workgroup that multiplies them, not once ahead, by a launch of 3 us.  Rows x
+// length of 32768 cost a round of 256 workgroups 2.3 us: 8 rows through 4096 x 4096 take 7.0 us so, 7.7 converted
+// ahead; 16 rows 9.6 and 7.8; 4 rows through 8192 x 8192, two rounds, 13.2 and 12.6.
+bool converts_on_the_way(int64_t m, int64_t n, int64_t k)
+{
+    const int64_t values = m * mx_steps(k) * 128;
+    return m <= 16 && values * ceil_div64(n, 4096) <= RAW_VALUES;
 }
 
 size_t operand_bytes(int64_t rows, int64_t length) { return (size_t)(mx_code_bytes(rows, length) + mx_scale_bytes(rows, length)); }
@@ -468,7 +619,7 @@ int amsim_mxfp4_matmul(const void *a, const void *b, int64_t m, int64_t n, int64
 
 size_t amsim_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k)
 {
-    if (!product_fits(m, n, k)) return 0;
+    if (!product_fits(m, n, k) || converts_on_the_way(m, n, k)) return 0;
     return operand_bytes(m, k) + product_workspace(m, n, k);
 }
 
@@ -480,6 +631,11 @@ int amsim_mxfp4_linear(const void *x, int dtype, int64_t row_stride, const void 
     if (row_stride < k && m > 1) return fail(AMSIM_ERR_INVALID, "mxfp4: rows overlap");
     if (((uintptr_t)x & (element_bytes(dtype) - 1)) || ((uintptr_t)w & 15)) return fail(AMSIM_ERR_INVALID, "mxfp4: misaligned pointer");
     if (int rc = check_workspace(workspace, workspace_bytes, amsim_mxfp4_linear_workspace_bytes(m, n, k))) return rc;
+    if (converts_on_the_way(m, n, k)) {
+        const FewArgs f{operand(w, n, k), {}, x, row_stride, m, k, mx_steps(k), bias, bias_dtype, act, dtype, out};
+        const auto kernel = dtype == AMSIM_DTYPE_F32 ? raw_kernel<float> : dtype == AMSIM_DTYPE_BF16 ? raw_kernel<__bf16> : raw_kernel<_Float16>;
+        return launch_few(kernel, f, f.steps * 4 * (m | 1) * 17, (hipStream_t)stream);
+    }
     const MxConversion job{x, nullptr, dtype, m, k, row_stride, (uint8_t *)workspace, nullptr, nullptr};
     if (int rc = mx_convert(&job, 1, (hipStream_t)stream)) return rc;
     return product(operand(workspace, m, k), operand(w, n, k), k, bias, bias_dtype, act, out, dtype,
