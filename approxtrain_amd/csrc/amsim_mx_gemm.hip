@@ -32,8 +32,7 @@ struct GemmArgs {
     int64_t steps, steps_per_split;
     const void *bias;
     int bias_dtype, act, out_dtype;
-    void *out;
-    float *partial;  // [splits][m][n] where the reduction is split, else null
+    void *out;               // where the reduction is split: [splits][m][n] partial sums
     int64_t tiles_m, tiles_n;
 };
 
@@ -106,46 +105,55 @@ template <int SIZE> __device__ __forceinline__ void load_to_lds(const uint8_t *f
 #endif
 }
 
-// 16 rows of a wave's results to memory, by way of LDS: a lane's four columns lie in sixteen rows' lines, a row
-// of 16 F columns is whole ones.  The rows' padding puts sixteen rows' writes on different banks.
+// A wave's results to memory, by way of LDS: a lane's four columns lie in sixteen rows' lines, a row of 16 F columns
+// is whole ones.  The rows' padding puts sixteen rows' writes on different banks.  A tile of 256, alone on its CU,
+// goes out in parts (16 rows of 32 bits or 32 of 16), so that its first stores are under way early: 4096^3 takes 38.7 us
+// so and 39.7 in one part; smaller tiles, which have neighbours to hide behind, in one: 42.7 and 44.1.
 template <typename T, int F> struct Rows {
-    static constexpr int COLUMNS = 16 * F, STRIDE = COLUMNS * sizeof(T) + 16, BYTES = 16 * STRIDE;
+    static constexpr int COLUMNS = 16 * F, STRIDE = COLUMNS * sizeof(T) + 16, AT_ONCE = F == 8 ? 4 / sizeof(T) : F;
+    static constexpr int BYTES = 16 * AT_ONCE * STRIDE;
 };
 template <typename T, int F>
-__device__ __forceinline__ void store_rows(uint8_t *lds, const v4f (&acc)[F], const float (&bias)[F][4], int act, T *out, int64_t m0,
+__device__ __forceinline__ void store_tile(uint8_t *lds, const v4f (&acc)[F][F], const float (&bias)[F][4], int act, T *out, int64_t m0,
                                            int64_t n0, int64_t M, int64_t N)
 {
     using R = Rows<T, F>;
-    const int lane = threadIdx.x & 63;
-    if (m0 >= M) return;
-    MX_WAIT_LDS();  // (the rows before have been read)
+    const int lane = threadIdx.x & 63, columns = (int)min<int64_t>(R::COLUMNS, N - n0);
+    for_each<F / R::AT_ONCE>([&](auto part) {
+        constexpr int first = part.value * R::AT_ONCE;
+        MX_WAIT_LDS();  // (what lay there before has been read)
+        for_each<R::AT_ONCE * F>([&](auto at) {
+            constexpr int i = at.value / F, j = at.value % F;
+            T t[4];
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
-        T t[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = from_float<T>(activate(acc[j][e] + bias[j][e], act));
-        __builtin_memcpy(__builtin_assume_aligned(lds + lane % 16 * R::STRIDE + (16 * j + lane / 16 * 4) * sizeof(T), 4 * sizeof(T)), t, sizeof(t));
-    }
-    __builtin_amdgcn_wave_barrier();
-    const int rows = (int)min<int64_t>(16, M - m0), columns = (int)min<int64_t>(R::COLUMNS, N - n0);
-    T *o = out + m0 * N + n0;
-    constexpr int PIECE = 16 / sizeof(T), PIECES = R::COLUMNS / PIECE;
-    if (N % PIECE == 0) {  // (whole pieces: out starts on a 16-byte boundary)
-#pragma unroll
-        for (int i = 0; i < 16 * PIECES / 64; ++i) {
-            const int r = (i * 64 + lane) / PIECES, c = (i * 64 + lane) % PIECES * PIECE;
-            const v4i v = *(const v4i *)(lds + r * R::STRIDE + c * sizeof(T));
-            if (r < rows && c < columns) *(v4i *)(o + r * N + c) = v;
-        }
-    } else {
+            for (int e = 0; e < 4; ++e) t[e] = from_float<T>(activate(acc[first + i][j][e] + bias[j][e], act));
+            __builtin_memcpy(__builtin_assume_aligned(lds + (16 * i + lane % 16) * R::STRIDE + (16 * j + lane / 16 * 4) * sizeof(T), 4 * sizeof(T)), t, sizeof(t));
+        });
+        __builtin_amdgcn_wave_barrier();
+        const int64_t row0 = m0 + 16 * first;
+        const int rows = (int)max<int64_t>(0, min<int64_t>(16 * R::AT_ONCE, M - row0));
+        T *o = out + row0 * N + n0;
+        constexpr int PIECE = 16 / sizeof(T), PIECES = R::COLUMNS / PIECE;
+        if (N % PIECE == 0) {  // (whole pieces: out starts on a 16-byte boundary)
+            constexpr int DOWN = 64 / PIECES;  // rows a store covers
+            const int c = lane % PIECES * PIECE;
+            const uint8_t *from = lds + lane / PIECES * R::STRIDE + c * sizeof(T);
+            T *to = o + lane / PIECES * N + c;
+#pragma unroll 8
+            for (int r = lane / PIECES; r < 16 * R::AT_ONCE; r += DOWN, from += DOWN * R::STRIDE, to += DOWN * N) {
+                const v4i v = *(const v4i *)from;
+                if (r < rows && c < columns) *(v4i *)to = v;
+            }
+        } else {
 #pragma unroll 4
-        for (int i = 0; i < 16 * R::COLUMNS / 64; ++i) {
-            const int r = (i * 64 + lane) / R::COLUMNS, c = (i * 64 + lane) % R::COLUMNS;
-            const T v = *(const T *)(lds + r * R::STRIDE + c * sizeof(T));
-            if (r < rows && c < columns) o[r * N + c] = v;
+            for (int i = 0; i < 16 * R::AT_ONCE * R::COLUMNS / 64; ++i) {
+                const int r = (i * 64 + lane) / R::COLUMNS, c = (i * 64 + lane) % R::COLUMNS;
+                const T v = *(const T *)(lds + r * R::STRIDE + c * sizeof(T));
+                if (r < rows && c < columns) o[r * N + c] = v;
+            }
         }
-    }
-    __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_wave_barrier();
+    });
 }
 
 // A workgroup of 2 x 2 waves, F x F fragments each: a tile of 32 F rows and columns.  Steps of 128 along the
@@ -170,7 +178,7 @@ __global__ __launch_bounds__(WG, 1) void gemm_kernel(GemmArgs g)
 {
     using K = Gemm<F, STAGES>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * K::BYTES];
-    static_assert(4 * Rows<float, F>::BYTES <= STAGES * K::BYTES, "");
+    static_assert(4 * Rows<float, F>::BYTES <= STAGES * K::BYTES && 4 * Rows<__bf16, F>::BYTES <= STAGES * K::BYTES, "");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / 2, wn = wave % 2;
     int64_t tm, tn;
     place_tile(blockIdx.x, g.tiles_m, g.tiles_n, tm, tn);
@@ -270,14 +278,7 @@ __global__ __launch_bounds__(WG, 1) void gemm_kernel(GemmArgs g)
     MX_WAIT_LOADS(0);
     __builtin_amdgcn_s_barrier();  // (LDS is free)
     const int64_t m0 = (tm * K::SIDE + wm * F) * 16, n0 = (tn * K::SIDE + wn * F) * 16;
-    if (n0 >= g.b.rows) return;
-    uint8_t *mine = lds + wave * Rows<float, F>::BYTES;
-    if (g.partial) {
-        float none[F][4] = {};
-        float *out = g.partial + (int64_t)blockIdx.y * g.a.rows * g.b.rows;
-        for_each<F>([&](auto i) { store_rows<float, F>(mine, acc[i.value], none, AMSIM_ACT_NONE, out, m0 + 16 * i.value, n0, g.a.rows, g.b.rows); });
-        return;
-    }
+    if (m0 >= g.a.rows || n0 >= g.b.rows) return;
     float bias[F][4];
 #pragma unroll
     for (int j = 0; j < F; ++j)
@@ -286,13 +287,13 @@ __global__ __launch_bounds__(WG, 1) void gemm_kernel(GemmArgs g)
             const int64_t n = n0 + 16 * j + lane / 16 * 4 + e;
             bias[j][e] = g.bias && n < g.b.rows ? load_as_float(g.bias, g.bias_dtype, n) : 0.0f;
         }
-    auto store = [&](auto zero) {
+    auto store = [&](auto zero, auto *out) {
         using T = decltype(zero);
-        for_each<F>([&](auto i) { store_rows<T, F>(mine, acc[i.value], bias, g.act, (T *)g.out, m0 + 16 * i.value, n0, g.a.rows, g.b.rows); });
+        store_tile<T, F>(lds + wave * Rows<T, F>::BYTES, acc, bias, g.act, out, m0, n0, g.a.rows, g.b.rows);
     };
-    if (g.out_dtype == AMSIM_DTYPE_F32) store(0.0f);
-    else if (g.out_dtype == AMSIM_DTYPE_BF16) store((__bf16)0.0f);
-    else store((_Float16)0.0f);
+    if (g.out_dtype == AMSIM_DTYPE_F32) store(0.0f, (float *)g.out + (int64_t)blockIdx.y * g.a.rows * g.b.rows);
+    else if (g.out_dtype == AMSIM_DTYPE_BF16) store((__bf16)0.0f, (__bf16 *)g.out);
+    else store((_Float16)0.0f, (_Float16 *)g.out);
 }
 
 // Few rows: bound by the reading of b, and for one layer of one token by latency alone.  A workgroup takes 16
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
 }
 
 // The partial sums of a split reduction, added in the order of the splits.
-__global__ __launch_bounds__(WG) void gemm_reduce_kernel(GemmArgs g, int splits)
+__global__ __launch_bounds__(WG) void gemm_reduce_kernel(GemmArgs g, const float *partial, int splits)
 {
     const int64_t N = g.b.rows, quads = ceil_div64(N, 4), at = (int64_t)blockIdx.x * WG + threadIdx.x;
     if (at >= g.a.rows * quads) return;
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(WG) void gemm_reduce_kernel(GemmArgs g, int splits)
     const int count = (int)(N - n < 4 ? N - n : 4);
     float v[4] = {0, 0, 0, 0};
     for (int s = 0; s < splits; ++s) {
-        const float *p = g.partial + ((int64_t)s * g.a.rows + m) * N + n;
+        const float *p = partial + ((int64_t)s * g.a.rows + m) * N + n;
         if (N % 4 == 0) {
             const v4f q = *(const v4f *)p;
 #pragma unroll
@@ -531,8 +532,8 @@ int product(const Operand &a, const Operand &b, int64_t k, const void *bias, int
     const Plan p = plan(a.rows, b.rows, k);
     const int64_t tiles = p.tiles_m * p.tiles_n, quads = a.rows * ceil_div64(b.rows, 4);
     if (tiles >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
-    GemmArgs g{a, b, mx_steps(k), p.steps_per_split, bias, bias_dtype, act, out_dtype, out,
-               p.splits > 1 ? (float *)workspace : nullptr, p.tiles_m, p.tiles_n};
+    GemmArgs g{a, b, mx_steps(k), p.steps_per_split, bias, bias_dtype, act, out_dtype, out, p.tiles_m, p.tiles_n};
+    if (p.splits > 1) g.bias = nullptr, g.act = AMSIM_ACT_NONE, g.out_dtype = AMSIM_DTYPE_F32, g.out = workspace;
     const dim3 grid((unsigned)tiles, (unsigned)p.splits);
     switch (p.fragments) {
     case 8: gemm_kernel<8, 4><<<grid, WG, 0, stream>>>(g); break;
@@ -541,7 +542,8 @@ int product(const Operand &a, const Operand &b, int64_t k, const void *bias, int
     }
     AMSIM_HIP_CHECK(hipGetLastError());
     if (p.splits > 1) {
-        gemm_reduce_kernel<<<(unsigned)ceil_div64(quads, WG), WG, 0, stream>>>(g, (int)p.splits);
+        g.bias = bias, g.act = act, g.out_dtype = out_dtype, g.out = out;
+        gemm_reduce_kernel<<<(unsigned)ceil_div64(quads, WG), WG, 0, stream>>>(g, (const float *)workspace, (int)p.splits);
         AMSIM_HIP_CHECK(hipGetLastError());
     }
     return AMSIM_OK;
