@@ -27,6 +27,11 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef unsigned short v2us __attribute__((ext_vector_type(2)));
 
+// 16 bytes at any element's address: rows need not start on 16-byte boundaries, the hardware takes such pieces too
+typedef int v4i_anywhere __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ v4i load16(const void *p) { return *(const v4i_anywhere *)p; }
+__device__ __forceinline__ void store16(void *p, v4i v) { *(v4i_anywhere *)p = v; }
+
 __host__ __device__ inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // steps of 128 along the reduction
 __host__ __device__ inline int64_t mx_steps(int64_t length) { return ceil_div64(length, 128); }

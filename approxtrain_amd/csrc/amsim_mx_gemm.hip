@@ -109,21 +109,21 @@ template <int SIZE> __device__ __forceinline__ void load_to_lds(const uint8_t *f
 // is whole ones.  The rows' padding puts sixteen rows' writes on different banks.  A tile of 256, alone on its CU,
 // goes out in parts (16 rows of 32 bits or 32 of 16), so that its first stores are under way early: 4096^3 takes 38.7 us
 // so and 39.7 in one part; smaller tiles, which have neighbours to hide behind, in one: 42.7 and 44.1.
-template <typename T, int F> struct Rows {
-    static constexpr int COLUMNS = 16 * F, STRIDE = COLUMNS * sizeof(T) + 16, AT_ONCE = F == 8 ? 4 / sizeof(T) : F;
+template <typename T, int FM, int FN> struct Rows {
+    static constexpr int COLUMNS = 16 * FN, STRIDE = COLUMNS * sizeof(T) + 16, AT_ONCE = FM == 8 ? 32 / FN / sizeof(T) : FM;
     static constexpr int BYTES = 16 * AT_ONCE * STRIDE;
 };
-template <typename T, int F>
-__device__ __forceinline__ void store_tile(uint8_t *lds, const v4f (&acc)[F][F], const float (&bias)[F][4], int act, T *out, int64_t m0,
+template <typename T, int FM, int FN>
+__device__ __forceinline__ void store_tile(uint8_t *lds, const v4f (&acc)[FM][FN], const float (&bias)[FN][4], int act, T *out, int64_t m0,
                                            int64_t n0, int64_t M, int64_t N)
 {
-    using R = Rows<T, F>;
+    using R = Rows<T, FM, FN>;
     const int lane = threadIdx.x & 63, columns = (int)min<int64_t>(R::COLUMNS, N - n0);
-    for_each<F / R::AT_ONCE>([&](auto part) {
+    for_each<FM / R::AT_ONCE>([&](auto part) {
         constexpr int first = part.value * R::AT_ONCE;
         MX_WAIT_LDS();  // (what lay there before has been read)
-        for_each<R::AT_ONCE * F>([&](auto at) {
-            constexpr int i = at.value / F, j = at.value % F;
+        for_each<R::AT_ONCE * FN>([&](auto at) {
+            constexpr int i = at.value / FN, j = at.value % FN;
             T t[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] = from_float<T>(activate(acc[first + i][j][e] + bias[j][e], act));
@@ -133,108 +133,104 @@ __device__ __forceinline__ void store_tile(uint8_t *lds, const v4f (&acc)[F][F],
         const int64_t row0 = m0 + 16 * first;
         const int rows = (int)max<int64_t>(0, min<int64_t>(16 * R::AT_ONCE, M - row0));
         T *o = out + row0 * N + n0;
-        constexpr int PIECE = 16 / sizeof(T), PIECES = R::COLUMNS / PIECE;
-        if (N % PIECE == 0) {  // (whole pieces: out starts on a 16-byte boundary)
-            constexpr int DOWN = 64 / PIECES;  // rows a store covers
-            const int c = lane % PIECES * PIECE;
-            const uint8_t *from = lds + lane / PIECES * R::STRIDE + c * sizeof(T);
-            T *to = o + lane / PIECES * N + c;
+        constexpr int PIECE = 16 / sizeof(T), PIECES = R::COLUMNS / PIECE, DOWN = 64 / PIECES;  // DOWN: rows that a store covers
+        const int c = lane % PIECES * PIECE;
+        const uint8_t *from = lds + lane / PIECES * R::STRIDE + c * sizeof(T);
+        T *to = o + lane / PIECES * N + c;
+        if (c + PIECE <= columns) {  // (rows may start on any element: the hardware takes such pieces too)
 #pragma unroll 8
             for (int r = lane / PIECES; r < 16 * R::AT_ONCE; r += DOWN, from += DOWN * R::STRIDE, to += DOWN * N) {
                 const v4i v = *(const v4i *)from;
-                if (r < rows && c < columns) *(v4i *)to = v;
+                if (r < rows) store16(to, v);
             }
-        } else {
-#pragma unroll 4
-            for (int i = 0; i < 16 * R::AT_ONCE * R::COLUMNS / 64; ++i) {
-                const int r = (i * 64 + lane) / R::COLUMNS, c = (i * 64 + lane) % R::COLUMNS;
-                const T v = *(const T *)(lds + r * R::STRIDE + c * sizeof(T));
-                if (r < rows && c < columns) o[r * N + c] = v;
-            }
+        } else if (c < columns) {
+            for (int r = lane / PIECES; r < rows; r += DOWN, from += DOWN * R::STRIDE, to += DOWN * N)
+                for (int i = 0; i < columns - c; ++i) to[i] = ((const T *)from)[i];
         }
         __builtin_amdgcn_wave_barrier();
     });
 }
 
-// A workgroup of 2 x 2 waves, F x F fragments each: a tile of 32 F rows and columns.  Steps of 128 along the
+// A workgroup of 2 x 2 waves, FM x FN fragments each: a tile of 32 FM rows and 32 FN columns.  Steps of 128 along the
 // reduction go from memory to one of STAGES places in LDS without passing through registers (the storage is
 // what a wavefront's 16-byte loads deliver, lane by lane), and a step's fragments are read into
 // registers while the step before is multiplied.
-template <int F, int STAGES> struct Gemm {
-    static constexpr int SIDE = 2 * F, GROUPS = F >= 4 ? F / 2 : 1;       // fragments and scale groups of a tile's side
-    static constexpr int A = 0, B = SIDE * 1024, SA = 2 * SIDE * 1024, SB = SA + GROUPS * 256, BYTES = SB + GROUPS * 256;
-    static constexpr int PER_WAVE = SIDE / 4;                             // 1 KB loads of a wave from either operand
-    static constexpr int LOADS = 2 * PER_WAVE + (GROUPS == 4 ? 2 : 1);    // of a wave for a step
-    static constexpr int SCALES = F >= 4 ? F / 4 : 1;                     // dwords of four fragments' scales
-    static constexpr int READS = 2 * F + 2;                               // of LDS (scales: one instruction for two dwords)
+template <int FM, int FN, int STAGES> struct Gemm {
+    static constexpr int GM = FM >= 4 ? FM / 2 : 1, GN = FN >= 4 ? FN / 2 : 1;       // scale groups of a tile's sides
+    static constexpr int A = 0, B = FM * 2048, S = B + FN * 2048, BYTES = S + (GM + GN) * 256;
+    static constexpr int CODES = (FM + FN) / 2, SCALES = (GM + GN + 3) / 4;          // loads of a wave for a step: of 1 KB, of 256 bytes
+    static constexpr int LOADS = CODES + SCALES;
+    static constexpr int SM = FM >= 4 ? FM / 4 : 1, SN = FN >= 4 ? FN / 4 : 1;       // dwords of four fragments' scales
+    static constexpr int READS = FM + FN + (SM + 1) / 2 + (SN + 1) / 2;              // of LDS (two dwords in one)
     struct Registers {
-        v4i a[F], b[F];
-        int sa[SCALES], sb[SCALES];
+        v4i a[FM], b[FN];
+        int sa[SM], sb[SN];
     };
 };
 
-template <int F, int STAGES>
-__global__ __launch_bounds__(WG, 1) void gemm_kernel(GemmArgs g)
+template <int FM, int FN, int STAGES, int RESIDENT>
+__global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmArgs g)
 {
-    using K = Gemm<F, STAGES>;
+    using K = Gemm<FM, FN, STAGES>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * K::BYTES];
-    static_assert(4 * Rows<float, F>::BYTES <= STAGES * K::BYTES && 4 * Rows<__bf16, F>::BYTES <= STAGES * K::BYTES, "");
+    static_assert(4 * Rows<float, FM, FN>::BYTES <= STAGES * K::BYTES && 4 * Rows<__bf16, FM, FN>::BYTES <= STAGES * K::BYTES, "");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / 2, wn = wave % 2;
     int64_t tm, tn;
     place_tile(blockIdx.x, g.tiles_m, g.tiles_n, tm, tn);
     const int64_t beg = blockIdx.y * g.steps_per_split, end = min(beg + g.steps_per_split, g.steps);
     const int count = (int)(end - beg);
 
-    // what this wave fetches: PER_WAVE fragments of either operand and a group of 64 rows' scales (or one of each)
-    const uint8_t *fetch[2 * K::PER_WAVE], *fetch_scales[2];
-    int to[2 * K::PER_WAVE], to_scales[2];
+    // what this wave fetches: fragments of either operand, and 64 rows' scales (where there are fewer groups than waves'
+    // loads, some twice)
+    const uint8_t *fetch[K::CODES], *fetch_scales[K::SCALES];
+    int to[K::CODES], to_scales[K::SCALES];
 #pragma unroll
-    for (int i = 0; i < K::PER_WAVE; ++i) {
-        const int64_t f = K::PER_WAVE * wave + i, fa = min(tm * K::SIDE + f, g.a.fragments - 1), fb = min(tn * K::SIDE + f, g.b.fragments - 1);
-        fetch[i] = g.a.codes + (fa * g.steps + beg) * 1024;
-        fetch[K::PER_WAVE + i] = g.b.codes + (fb * g.steps + beg) * 1024;
-        to[i] = K::A + (int)f * 1024;
-        to[K::PER_WAVE + i] = K::B + (int)f * 1024;
+    for (int i = 0; i < K::CODES; ++i) {
+        const bool of_a = i < FM / 2;
+        const int f = of_a ? FM / 2 * wave + i : FN / 2 * wave + i - FM / 2;
+        const Operand &o = of_a ? g.a : g.b;
+        const int64_t at = min((of_a ? tm * 2 * FM : tn * 2 * FN) + f, o.fragments - 1);
+        fetch[i] = o.codes + (at * g.steps + beg) * 1024;
+        to[i] = (of_a ? K::A : K::B) + f * 1024;
     }
-    {
-        const int64_t ga = K::GROUPS == 4 ? wave : wave / 2 % K::GROUPS, gb = ga;
-        const int64_t fa = min(tm * K::SIDE / 4 + ga, g.a.groups - 1), fb = min(tn * K::SIDE / 4 + gb, g.b.groups - 1);
-        const uint8_t *pa = g.a.scales + (fa * g.steps + beg) * 256, *pb = g.b.scales + (fb * g.steps + beg) * 256;
-        const int la = K::SA + (int)ga * 256, lb = K::SB + (int)gb * 256;
-        // (fewer groups than waves: even waves fetch a's, odd ones b's)
-        fetch_scales[0] = K::GROUPS == 4 || wave % 2 == 0 ? pa : pb;
-        to_scales[0] = K::GROUPS == 4 || wave % 2 == 0 ? la : lb;
-        fetch_scales[1] = pb;
-        to_scales[1] = lb;
+#pragma unroll
+    for (int i = 0; i < K::SCALES; ++i) {
+        const int group = (wave + 4 * i) % (K::GM + K::GN);
+        const bool of_a = group < K::GM;
+        const Operand &o = of_a ? g.a : g.b;
+        const int64_t at = min(of_a ? tm * FM / 2 + group : tn * FN / 2 + group - K::GM, o.groups - 1);
+        fetch_scales[i] = o.scales + (at * g.steps + beg) * 256;
+        to_scales[i] = K::S + group * 256;
     }
     auto fetch_step = [&](int s) {
         uint8_t *stage = lds + s % STAGES * K::BYTES;
         const int at = min(s, count - 1);
 #pragma unroll
-        for (int i = 0; i < 2 * K::PER_WAVE; ++i)
-            load_to_lds<16>(fetch[i], at * 1024, stage + to[i]);
+        for (int i = 0; i < K::CODES; ++i) load_to_lds<16>(fetch[i], at * 1024, stage + to[i]);
 #pragma unroll
-        for (int i = 0; i < (K::GROUPS == 4 ? 2 : 1); ++i)
-            load_to_lds<4>(fetch_scales[i], at * 256, stage + to_scales[i]);
+        for (int i = 0; i < K::SCALES; ++i) load_to_lds<4>(fetch_scales[i], at * 256, stage + to_scales[i]);
     };
     auto read_step = [&](int s, typename K::Registers &r) {
         const uint8_t *stage = lds + s % STAGES * K::BYTES;
 #pragma unroll
-        for (int i = 0; i < F; ++i) {
-            r.a[i] = *(const v4i *)(stage + K::A + (wm * F + i) * 1024 + lane * 16);
-            r.b[i] = *(const v4i *)(stage + K::B + (wn * F + i) * 1024 + lane * 16);
+        for (int i = 0; i < FM; ++i) r.a[i] = *(const v4i *)(stage + K::A + (wm * FM + i) * 1024 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) r.b[i] = *(const v4i *)(stage + K::B + (wn * FN + i) * 1024 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < K::SM; ++i) {
+            r.sa[i] = *(const int *)(stage + K::S + (FM >= 4 ? wm * K::SM + i : 0) * 256 + lane * 4);
+            if (FM == 2) r.sa[i] >>= 16 * wm;
         }
 #pragma unroll
-        for (int i = 0; i < K::SCALES; ++i) {
-            r.sa[i] = *(const int *)(stage + K::SA + (F >= 4 ? wm * K::SCALES + i : 0) * 256 + lane * 4);
-            r.sb[i] = *(const int *)(stage + K::SB + (F >= 4 ? wn * K::SCALES + i : 0) * 256 + lane * 4);
-            if (F == 2) r.sa[i] >>= 16 * wm, r.sb[i] >>= 16 * wn;
+        for (int i = 0; i < K::SN; ++i) {
+            r.sb[i] = *(const int *)(stage + K::S + (K::GM + (FN >= 4 ? wn * K::SN + i : 0)) * 256 + lane * 4);
+            if (FN == 2) r.sb[i] >>= 16 * wn;
         }
     };
-    v4f acc[F][F] = {};
+    v4f acc[FM][FN] = {};
     auto multiply = [&](const typename K::Registers &r) {
-        for_each<F * F>([&](auto at) {
-            constexpr int i = at.value / F, j = at.value % F;
+        for_each<FM * FN>([&](auto at) {
+            constexpr int i = at.value / FN, j = at.value % FN;
             acc[i][j] = mfma<j % 4, i % 4>(r.b[j], r.a[i], acc[i][j], r.sb[j / 4], r.sa[i / 4]);
         });
     };
@@ -277,11 +273,11 @@ __global__ __launch_bounds__(WG, 1) void gemm_kernel(GemmArgs g)
     MX_WAIT_LDS();
     MX_WAIT_LOADS(0);
     __builtin_amdgcn_s_barrier();  // (LDS is free)
-    const int64_t m0 = (tm * K::SIDE + wm * F) * 16, n0 = (tn * K::SIDE + wn * F) * 16;
+    const int64_t m0 = (tm * 2 + wm) * FM * 16, n0 = (tn * 2 + wn) * FN * 16;
     if (m0 >= g.a.rows || n0 >= g.b.rows) return;
-    float bias[F][4];
+    float bias[FN][4];
 #pragma unroll
-    for (int j = 0; j < F; ++j)
+    for (int j = 0; j < FN; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int64_t n = n0 + 16 * j + lane / 16 * 4 + e;
@@ -289,7 +285,7 @@ __global__ __launch_bounds__(WG, 1) void gemm_kernel(GemmArgs g)
         }
     auto store = [&](auto zero, auto *out) {
         using T = decltype(zero);
-        store_tile<T, F>(lds + wave * Rows<T, F>::BYTES, acc, bias, g.act, out, m0, n0, g.a.rows, g.b.rows);
+        store_tile<T, FM, FN>(lds + wave * Rows<T, FM, FN>::BYTES, acc, bias, g.act, out, m0, n0, g.a.rows, g.b.rows);
     };
     if (g.out_dtype == AMSIM_DTYPE_F32) store(0.0f, (float *)g.out + (int64_t)blockIdx.y * g.a.rows * g.b.rows);
     else if (g.out_dtype == AMSIM_DTYPE_BF16) store((__bf16)0.0f, (__bf16 *)g.out);
@@ -392,7 +388,10 @@ __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
             if (row[j] >= rows) continue;
             const X *p = (const X *)g.x + row[j] * g.row_stride + eighth[j] * 8;
             if (eighth[j] * 8 + 8 <= g.k) {
-                __builtin_memcpy(v[j], p, sizeof(v[j]));
+                v4i piece[sizeof(v[j]) / 16];
+#pragma unroll
+                for (int e = 0; e < (int)(sizeof(v[j]) / 16); ++e) piece[e] = load16((const char *)p + 16 * e);
+                __builtin_memcpy(v[j], piece, sizeof(v[j]));
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -469,33 +468,47 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float *parts, i
     out[col] = from_float<T>(s);
 }
 
+struct Tile {
+    int rows, cols;
+    // microseconds, as measured on products of 128 to 16384 a side: of one tile's step on a CU of its own, of a tile's step
+    // with the card full, of storing a tile, and of a round where tiles do not overlap
+    double alone, step, store, round;
+};
+// Tiles of 256 fetch least for an operation, and have their CU for themselves: what they store, nobody multiplies
+// beside.  256 x 128 share it by two (512 tiles of 32 steps: 39.3 us, 40.7 as 256 of 256, 42.2 as 1024 of 128; of 128 steps 124,
+// 115 and 136; 2048 tiles of 16 steps 84, 96, 92).  Tiles of 128 and 64 fetch two and four times the bytes, and are
+// for few results (256 tiles of 128, 16 steps: 10.0 us, 13.9 in 256 x 128; 410 of 64, 21 steps: 7.7, 10.1 in 128).
+constexpr Tile TILES[] = {{256, 256, 0.6, 0, 0, 10.9}, {256, 128, 0.4, 0.00172, 0.0106, 0}, {128, 128, 0.2, 0.00093, 0.0067, 0}, {64, 64, 0.1, 0.00039, 0.0021, 0}};
+
 struct Plan {
-    int fragments;  // per wave and direction
+    int tile;  // of TILES
     int64_t tiles_m, tiles_n, splits, steps_per_split;
 };
 
-// The tile and the split of the reduction that a product takes least time with, by microseconds measured on
-// products of 128 to 16384 a side.  Tiles of 256: a round of the 256 CUs takes 0.68 a step (0.6 for one tile alone), and
-// its results are stored with nothing to multiply meanwhile, 8.  Tiles of 128 share a CU and hide that, but
-// fetch twice the bytes for an operation: 0.2 a step for one tile on a CU, 0.00088 a tile and step for many.
-// Tiles of 64 four times the bytes: 0.1 and 0.00038.  A split reduction takes a second launch, 3, and its sums
-// go to memory and back.
+// The tile and the split of the reduction that a product takes least time with.  A split reduction takes a second
+// launch, 3 us, and its sums go to memory and back.
 Plan plan(int64_t m, int64_t n, int64_t k)
 {
     const int64_t steps = mx_steps(k);
-    Plan best{};
+    Plan best{-1};
     double least = 0;
-    for (int f = 8; f >= 2; f /= 2) {
-        const int64_t tiles_m = ceil_div64(m, 32 * f), tiles_n = ceil_div64(n, 32 * f);
+    for (int i = 0; i < 4; ++i) {
+        const Tile &t = TILES[i];
+        const int64_t tiles_m = ceil_div64(m, t.rows), tiles_n = ceil_div64(n, t.cols);
         for (int64_t s = 1; s <= 16 && (s == 1 || 2 * s <= steps); s *= 2) {
             const int64_t each = ceil_div64(steps, s), splits = ceil_div64(steps, each);
             const double tiles = (double)tiles_m * (double)tiles_n * (double)splits;
-            double t = f == 8 ? 2 + std::ceil(tiles / 256) * (0.68 * each + 8)
-                     : f == 4 ? 7 + std::max(0.2, 0.00088 * tiles) * each : 6 + std::max(0.1, 0.00038 * tiles) * each;
-            if (splits > 1) t += 3 + (double)splits * (double)m * (double)n * 8 / 4e6;
-            if (best.fragments == 0 || t < least) {
-                least = t;
-                best = Plan{f, tiles_m, tiles_n, splits, each};
+            double us;
+            if (t.round) {
+                us = 4.2 + std::ceil(tiles / 256) * (0.74 * each + t.round);
+            } else {
+                us = 6.5 + std::max(t.alone, t.step * tiles) * each + t.store * tiles;
+                if (i == 1 && tiles > 256 && tiles < 512) us = 6.5 + 0.8 * each + t.store * tiles;  // some CUs have two, others one
+            }
+            if (splits > 1) us += 3 + (double)splits * (double)m * (double)n * 8 / 4e6;
+            if (best.tile < 0 || us < least) {
+                least = us;
+                best = Plan{i, tiles_m, tiles_n, splits, each};
             }
         }
     }
@@ -536,10 +549,11 @@ int product(const Operand &a, const Operand &b, int64_t k, const void *bias, int
     GemmArgs g{a, b, mx_steps(k), p.steps_per_split, bias, bias_dtype, act, out_dtype, out, p.tiles_m, p.tiles_n};
     if (p.splits > 1) g.bias = nullptr, g.act = AMSIM_ACT_NONE, g.out_dtype = AMSIM_DTYPE_F32, g.out = workspace;
     const dim3 grid((unsigned)tiles, (unsigned)p.splits);
-    switch (p.fragments) {
-    case 8: gemm_kernel<8, 4><<<grid, WG, 0, stream>>>(g); break;
-    case 4: gemm_kernel<4, 4><<<grid, WG, 0, stream>>>(g); break;
-    default: gemm_kernel<2, 4><<<grid, WG, 0, stream>>>(g); break;
+    switch (p.tile) {
+    case 0: gemm_kernel<8, 8, 4, 1><<<grid, WG, 0, stream>>>(g); break;
+    case 1: gemm_kernel<8, 4, 3, 2><<<grid, WG, 0, stream>>>(g); break;
+    case 2: gemm_kernel<4, 4, 4, 2><<<grid, WG, 0, stream>>>(g); break;
+    default: gemm_kernel<2, 2, 4, 4><<<grid, WG, 0, stream>>>(g); break;
     }
     AMSIM_HIP_CHECK(hipGetLastError());
     if (p.splits > 1) {
