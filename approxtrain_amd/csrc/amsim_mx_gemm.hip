@@ -478,7 +478,7 @@ struct Tile {
 // beside.  256 x 128 share it by two (512 tiles of 32 steps: 39.3 us, 40.7 as 256 of 256, 42.2 as 1024 of 128; of 128 steps 124,
 // 115 and 136; 2048 tiles of 16 steps 84, 96, 92).  Tiles of 128 and 64 fetch two and four times the bytes, and are
 // for few results (256 tiles of 128, 16 steps: 10.0 us, 13.9 in 256 x 128; 410 of 64, 21 steps: 7.7, 10.1 in 128).
-constexpr Tile TILES[] = {{256, 256, 0.6, 0, 0, 10.9}, {256, 128, 0.4, 0.00172, 0.0106, 0}, {128, 128, 0.2, 0.00093, 0.0067, 0}, {64, 64, 0.1, 0.00039, 0.0021, 0}};
+constexpr Tile TILES[] = {{256, 256, 0.6, 0, 0, 12}, {256, 128, 0.4, 0.00166, 0.0106, 0}, {128, 128, 0.2, 0.00093, 0.0067, 0}, {64, 64, 0.1, 0.00039, 0.0021, 0}};
 
 struct Plan {
     int tile;  // of TILES
