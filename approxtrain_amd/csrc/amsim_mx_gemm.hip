@@ -32,8 +32,15 @@ struct GemmArgs {
     int64_t steps, steps_per_split;
     const void *bias;
     int bias_dtype, act, out_dtype;
-    void *out;               // where the reduction is split: [splits][m][n] partial sums
-    int64_t tiles_m, tiles_n;
+    void *out;
+    unsigned tiles_m, tiles_n;  // (below 2^24 together)
+    int splits;
+    float *partial;          // [splits][m][n] where the reduction is split, else null
+};
+// One or two products of a launch: a training step's backward pass has two that do not wait for each other.
+struct GemmJobs {
+    GemmArgs job[2];
+    unsigned blocks;         // of the first
 };
 
 template <typename T>
@@ -80,11 +87,11 @@ template <int N, typename Fn> __device__ __forceinline__ void for_each(Fn &&fn) 
 
 // Where tile number `id` of a launch lies.  Workgroups go to the eight dies in turn; each die gets a run of
 // neighbouring tiles, eight tiles high, so that its L2 serves a fragment's step to all who read it.
-__device__ __forceinline__ void place_tile(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t &tm, int64_t &tn)
+__device__ __forceinline__ void place_tile(unsigned id, unsigned tiles_m, unsigned tiles_n, unsigned &tm, unsigned &tn)
 {
-    const int64_t tiles = tiles_m * tiles_n, each = tiles / 8, more = tiles % 8, die = id % 8;
-    const int64_t t = die * each + (die < more ? die : more) + id / 8;
-    const int64_t band = 8 * tiles_n, first = t / band * 8, within = t % band, high = min<int64_t>(8, tiles_m - first);
+    const unsigned tiles = tiles_m * tiles_n, each = tiles / 8, more = tiles % 8, die = id % 8;
+    const unsigned t = die * each + min(die, more) + id / 8;
+    const unsigned band = 8 * tiles_n, first = t / band * 8, within = t % band, high = min(8u, tiles_m - first);
     tm = first + within % high;
     tn = within / high;
 }
@@ -169,15 +176,18 @@ template <int FM, int FN, int STAGES> struct Gemm {
 };
 
 template <int FM, int FN, int STAGES, int RESIDENT>
-__global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmArgs g)
+__global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmJobs jobs)
 {
     using K = Gemm<FM, FN, STAGES>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * K::BYTES];
     static_assert(4 * Rows<float, FM, FN>::BYTES <= STAGES * K::BYTES && 4 * Rows<__bf16, FM, FN>::BYTES <= STAGES * K::BYTES, "");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / 2, wn = wave % 2;
-    int64_t tm, tn;
-    place_tile(blockIdx.x, g.tiles_m, g.tiles_n, tm, tn);
-    const int64_t beg = blockIdx.y * g.steps_per_split, end = min(beg + g.steps_per_split, g.steps);
+    const bool other = blockIdx.x >= jobs.blocks;
+    const GemmArgs g = jobs.job[other];
+    const unsigned id = blockIdx.x - (other ? jobs.blocks : 0), tiles = g.tiles_m * g.tiles_n, split = g.splits > 1 ? id / tiles : 0;
+    unsigned tm, tn;
+    place_tile(id - split * tiles, g.tiles_m, g.tiles_n, tm, tn);
+    const int64_t beg = split * g.steps_per_split, end = min(beg + g.steps_per_split, g.steps);
     const int count = (int)(end - beg);
 
     // what this wave fetches: fragments of either operand, and 64 rows' scales (where there are fewer groups than waves'
@@ -189,7 +199,7 @@ __global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmArgs g)
         const bool of_a = i < FM / 2;
         const int f = of_a ? FM / 2 * wave + i : FN / 2 * wave + i - FM / 2;
         const Operand &o = of_a ? g.a : g.b;
-        const int64_t at = min((of_a ? tm * 2 * FM : tn * 2 * FN) + f, o.fragments - 1);
+        const int64_t at = min<int64_t>((of_a ? tm * 2 * FM : tn * 2 * FN) + f, o.fragments - 1);
         fetch[i] = o.codes + (at * g.steps + beg) * 1024;
         to[i] = (of_a ? K::A : K::B) + f * 1024;
     }
@@ -198,7 +208,7 @@ __global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmArgs g)
         const int group = (wave + 4 * i) % (K::GM + K::GN);
         const bool of_a = group < K::GM;
         const Operand &o = of_a ? g.a : g.b;
-        const int64_t at = min(of_a ? tm * FM / 2 + group : tn * FN / 2 + group - K::GM, o.groups - 1);
+        const int64_t at = min<int64_t>(of_a ? tm * FM / 2 + group : tn * FN / 2 + group - K::GM, o.groups - 1);
         fetch_scales[i] = o.scales + (at * g.steps + beg) * 256;
         to_scales[i] = K::S + group * 256;
     }
@@ -273,21 +283,22 @@ __global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmArgs g)
     MX_WAIT_LDS();
     MX_WAIT_LOADS(0);
     __builtin_amdgcn_s_barrier();  // (LDS is free)
-    const int64_t m0 = (tm * 2 + wm) * FM * 16, n0 = (tn * 2 + wn) * FN * 16;
+    const int64_t m0 = (int64_t)(tm * 2 + wm) * FM * 16, n0 = (int64_t)(tn * 2 + wn) * FN * 16;
     if (m0 >= g.a.rows || n0 >= g.b.rows) return;
+    const bool whole = !g.partial;
     float bias[FN][4];
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int64_t n = n0 + 16 * j + lane / 16 * 4 + e;
-            bias[j][e] = g.bias && n < g.b.rows ? load_as_float(g.bias, g.bias_dtype, n) : 0.0f;
+            bias[j][e] = whole && g.bias && n < g.b.rows ? load_as_float(g.bias, g.bias_dtype, n) : 0.0f;
         }
     auto store = [&](auto zero, auto *out) {
         using T = decltype(zero);
-        store_tile<T, FM, FN>(lds + wave * Rows<T, FM, FN>::BYTES, acc, bias, g.act, out, m0, n0, g.a.rows, g.b.rows);
+        store_tile<T, FM, FN>(lds + wave * Rows<T, FM, FN>::BYTES, acc, bias, whole ? g.act : AMSIM_ACT_NONE, out, m0, n0, g.a.rows, g.b.rows);
     };
-    if (g.out_dtype == AMSIM_DTYPE_F32) store(0.0f, (float *)g.out + (int64_t)blockIdx.y * g.a.rows * g.b.rows);
+    if (!whole || g.out_dtype == AMSIM_DTYPE_F32) store(0.0f, whole ? (float *)g.out : g.partial + split * g.a.rows * g.b.rows);
     else if (g.out_dtype == AMSIM_DTYPE_BF16) store((__bf16)0.0f, (__bf16 *)g.out);
     else store((_Float16)0.0f, (_Float16 *)g.out);
 }
@@ -425,47 +436,60 @@ __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
     finish_few(g, blockIdx.x, sums, acc);
 }
 
-// The partial sums of a split reduction, added in the order of the splits.
-__global__ __launch_bounds__(WG) void gemm_reduce_kernel(GemmArgs g, const float *partial, int splits)
+// What is left behind the products: partial sums of split reductions, added in the order of the splits, and a bias
+// gradient's from the sums of every 32 rows, 16 columns and 16 runs of rows to a workgroup.
+struct FinishArgs {
+    GemmJobs products;
+    unsigned blocks[2];      // of either product's sums
+    const float *sums;       // [parts][columns]
+    int64_t parts, columns;
+    void *out;
+    int out_dtype;
+};
+__global__ __launch_bounds__(WG) void finish_kernel(FinishArgs f)
 {
-    const int64_t N = g.b.rows, quads = ceil_div64(N, 4), at = (int64_t)blockIdx.x * WG + threadIdx.x;
-    if (at >= g.a.rows * quads) return;
-    const int64_t m = at / quads, n = at % quads * 4;
-    const int count = (int)(N - n < 4 ? N - n : 4);
-    float v[4] = {0, 0, 0, 0};
-    for (int s = 0; s < splits; ++s) {
-        const float *p = partial + ((int64_t)s * g.a.rows + m) * N + n;
-        if (N % 4 == 0) {
-            const v4f q = *(const v4f *)p;
+    __shared__ float run[16][16];
+    unsigned id = blockIdx.x;
+    if (id < f.blocks[0] + f.blocks[1]) {
+        const bool other = id >= f.blocks[0];
+        if (other) id -= f.blocks[0];
+        const GemmArgs &g = f.products.job[other];
+        const int64_t N = g.b.rows, quads = ceil_div64(N, 4), at = (int64_t)id * WG + threadIdx.x;
+        if (at >= g.a.rows * quads) return;
+        const int64_t m = at / quads, n = at % quads * 4;
+        const int count = (int)(N - n < 4 ? N - n : 4);
+        float v[4] = {0, 0, 0, 0};
+        for (int s = 0; s < g.splits; ++s) {
+            const float *p = g.partial + (s * g.a.rows + m) * N + n;
+            if (N % 4 == 0) {
+                const v4f q = *(const v4f *)p;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += q[i];
-        } else {
+                for (int i = 0; i < 4; ++i) v[i] += q[i];
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < count) v[i] += p[i];
+                for (int i = 0; i < 4; ++i)
+                    if (i < count) v[i] += p[i];
+            }
         }
+        finish4(g.bias, g.bias_dtype, g.act, g.out, g.out_dtype, m, n, N, v);
+        return;
     }
-    finish4(g.bias, g.bias_dtype, g.act, g.out, g.out_dtype, m, n, N, v);
-}
-
-// Sums of columns from those of every 32 rows, in order: 64 columns and 16 runs of rows to a workgroup.
-template <typename T>
-__global__ __launch_bounds__(1024) void column_sums_kernel(const float *parts, int64_t count, int64_t n, T *out)
-{
-    __shared__ float run[16][64];
-    const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + c, each = ceil_div64(count, 16), end = min(count, each * (w + 1));
+    id -= f.blocks[0] + f.blocks[1];
+    const int c = threadIdx.x & 15, w = threadIdx.x >> 4;
+    const int64_t col = (int64_t)id * 16 + c, each = ceil_div64(f.parts, 16), end = min(f.parts, each * (w + 1));
     float s = 0.0f;
-    if (col < n) {
-#pragma unroll 8
-        for (int64_t p = each * w; p < end; ++p) s += parts[p * n + col];
+    if (col < f.columns) {
+#pragma unroll 16
+        for (int64_t p = each * w; p < end; ++p) s += f.sums[p * f.columns + col];
     }
     run[w][c] = s;
     __syncthreads();
-    if (w != 0 || col >= n) return;
+    if (w != 0 || col >= f.columns) return;
 #pragma unroll
     for (int i = 1; i < 16; ++i) s += run[i][c];
-    out[col] = from_float<T>(s);
+    if (f.out_dtype == AMSIM_DTYPE_F32) ((float *)f.out)[col] = s;
+    else if (f.out_dtype == AMSIM_DTYPE_BF16) ((__bf16 *)f.out)[col] = (__bf16)s;
+    else ((_Float16 *)f.out)[col] = (_Float16)s;
 }
 
 struct Tile {
@@ -480,50 +504,109 @@ struct Tile {
 // for few results (256 tiles of 128, 16 steps: 10.0 us, 13.9 in 256 x 128; 410 of 64, 21 steps: 7.7, 10.1 in 128).
 constexpr Tile TILES[] = {{256, 256, 0.6, 0, 0, 12}, {256, 128, 0.4, 0.00166, 0.0106, 0}, {128, 128, 0.2, 0.00093, 0.0067, 0}, {64, 64, 0.1, 0.00039, 0.0021, 0}};
 
+struct Extents {
+    int64_t m, n, k;
+};
 struct Plan {
     int tile;  // of TILES
-    int64_t tiles_m, tiles_n, splits, steps_per_split;
+    struct {
+        int64_t tiles_m, tiles_n, splits, steps_per_split;
+    } of[2];
 };
 
-// The tile and the split of the reduction that a product takes least time with.  A split reduction takes a second
-// launch, 3 us, and its sums go to memory and back.
-Plan plan(int64_t m, int64_t n, int64_t k)
+// what a launch of `tiles` tiles takes, of which the products' steps add up to `work`, each tile at least `each`
+double microseconds(int tile, double tiles, double work, double each)
 {
-    const int64_t steps = mx_steps(k);
-    Plan best{-1};
+    const Tile &t = TILES[tile];
+    if (t.round) return 4.2 + std::ceil(tiles / 256) * (0.74 * work / tiles + t.round);
+    double steps = std::max(t.alone * each, t.step * work);
+    if (tile == 1 && tiles > 256 && tiles < 512) steps = std::max(steps, 0.8 * each);  // some CUs have two, others one
+    return 6.5 + steps + t.store * tiles;
+}
+
+// The tile of one or two products and the splits of their reductions that take least time.  A split reduction takes a
+// second launch, 3 us, and its sums go to memory and back.
+Plan make_plan(const Extents *e, int count)
+{
+    Plan best{-1, {}};
     double least = 0;
     for (int i = 0; i < 4; ++i) {
-        const Tile &t = TILES[i];
-        const int64_t tiles_m = ceil_div64(m, t.rows), tiles_n = ceil_div64(n, t.cols);
-        for (int64_t s = 1; s <= 16 && (s == 1 || 2 * s <= steps); s *= 2) {
-            const int64_t each = ceil_div64(steps, s), splits = ceil_div64(steps, each);
-            const double tiles = (double)tiles_m * (double)tiles_n * (double)splits;
-            double us;
-            if (t.round) {
-                us = 4.2 + std::ceil(tiles / 256) * (0.74 * each + t.round);
-            } else {
-                us = 6.5 + std::max(t.alone, t.step * tiles) * each + t.store * tiles;
-                if (i == 1 && tiles > 256 && tiles < 512) us = 6.5 + 0.8 * each + t.store * tiles;  // some CUs have two, others one
+        Plan p{i, {}};
+        double tiles = 0, work = 0, longest = 0, more = 0;
+        for (int j = 0; j < count; ++j) {
+            const int64_t steps = mx_steps(e[j].k), tiles_m = ceil_div64(e[j].m, TILES[i].rows), tiles_n = ceil_div64(e[j].n, TILES[i].cols);
+            const double area = (double)tiles_m * (double)tiles_n;
+            double quickest = 0, its_more = 0;
+            for (int64_t s = 1; s <= 16 && (s == 1 || 2 * s <= steps); s *= 2) {
+                const int64_t each = ceil_div64(steps, s), splits = ceil_div64(steps, each);
+                const double extra = splits > 1 ? 3 + (double)splits * (double)e[j].m * (double)e[j].n * 8 / 4e6 : 0;
+                const double us = microseconds(i, area * splits, area * splits * each, each) + extra;
+                if (s > 1 && us >= quickest) continue;
+                quickest = us;
+                its_more = extra;
+                p.of[j] = {tiles_m, tiles_n, splits, each};
             }
-            if (splits > 1) us += 3 + (double)splits * (double)m * (double)n * 8 / 4e6;
-            if (best.tile < 0 || us < least) {
-                least = us;
-                best = Plan{i, tiles_m, tiles_n, splits, each};
-            }
+            const double all = area * p.of[j].splits;
+            tiles += all;
+            work += all * p.of[j].steps_per_split;
+            longest = std::max(longest, (double)p.of[j].steps_per_split);
+            more += its_more;
+        }
+        const double us = microseconds(i, tiles, work, longest) + more;
+        if (best.tile < 0 || us < least) {
+            least = us;
+            best = p;
         }
     }
     return best;
+}
+
+// The same, looked up where the thread has asked for it before: a training step asks seven times, a microsecond each.
+Plan plan(const Extents *e, int count)
+{
+    struct Known {
+        Extents e[2];
+        Plan p;
+    };
+    static thread_local Known known[16] = {};
+    const Extents none{}, &f = count > 1 ? e[1] : none;
+    const uint64_t hash = ((uint64_t)e[0].m * 3 + (uint64_t)e[0].n * 5 + (uint64_t)e[0].k * 7 + (uint64_t)f.k * 11) * 0x9e3779b97f4a7c15ull;
+    Known &at = known[hash >> 60];
+    auto same = [](const Extents &x, const Extents &y) { return x.m == y.m && x.n == y.n && x.k == y.k; };
+    if (!same(at.e[0], e[0]) || !same(at.e[1], f)) at = Known{{e[0], f}, make_plan(e, count)};
+    return at.p;
 }
 
 // Whether few_kernel serves: reductions beyond 32768 need more than one workgroup's waves (64 rows by 512: 9.5 us against
 // 12.7 in tiles at 16384, 43 against 17 at 65536).
 bool few(int64_t m, int64_t k) { return m <= 64 && mx_steps(k) <= 256; }
 
+size_t partial_bytes(const Extents &e, int64_t splits) { return splits > 1 ? ((size_t)splits * e.m * e.n * 4 + 255) / 256 * 256 : 0; }
+
+// the products of a list that go in tiles, and the others
+int tiled(const Extents *e, int count, Extents *out, int *which)
+{
+    int n = 0;
+    for (int j = 0; j < count; ++j)
+        if (!few(e[j].m, e[j].k)) out[n] = e[j], which[n++] = j;
+    return n;
+}
+
+size_t products_workspace(const Extents *e, int count)
+{
+    Extents t[2];
+    int which[2];
+    const int n = tiled(e, count, t, which);
+    if (n == 0) return 0;
+    const Plan p = plan(t, n);
+    size_t bytes = 0;
+    for (int j = 0; j < n; ++j) bytes += partial_bytes(t[j], p.of[j].splits);
+    return bytes;
+}
 size_t product_workspace(int64_t m, int64_t n, int64_t k)
 {
-    if (few(m, k)) return 0;
-    const Plan p = plan(m, n, k);
-    return p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
+    const Extents e{m, n, k};
+    return products_workspace(&e, 1);
 }
 
 int launch_few(void (*kernel)(FewArgs), const FewArgs &g, int64_t lds, hipStream_t stream)
@@ -536,33 +619,64 @@ int launch_few(void (*kernel)(FewArgs), const FewArgs &g, int64_t lds, hipStream
     return AMSIM_OK;
 }
 
-int product(const Operand &a, const Operand &b, int64_t k, const void *bias, int bias_dtype, int act, void *out, int out_dtype,
-            void *workspace, hipStream_t stream)
+struct Product {
+    Operand a, b;
+    int64_t k;
+    const void *bias;
+    int bias_dtype, act;
+    void *out;
+    int out_dtype;
+};
+
+// One or two products, and the sums of `parts` rows of `columns` partial ones where `sums` is not null.
+int products(const Product *list, int count, const float *sums, int64_t parts, int64_t columns, void *out, int out_dtype, void *workspace,
+             hipStream_t stream)
 {
-    if (few(a.rows, k)) {
-        const FewArgs f{b, a, nullptr, 0, a.rows, k, mx_steps(k), bias, bias_dtype, act, out_dtype, out};
-        return launch_few(a.rows <= 16 ? few_kernel<1> : a.rows <= 32 ? few_kernel<2> : few_kernel<4>, f, 0, stream);
+    Extents e[2], t[2];
+    int which[2];
+    for (int j = 0; j < count; ++j) e[j] = {list[j].a.rows, list[j].b.rows, list[j].k};
+    const int n = tiled(e, count, t, which);
+    for (int j = 0; j < count; ++j) {
+        const Product &q = list[j];
+        if (!few(e[j].m, e[j].k)) continue;
+        const FewArgs f{q.b, q.a, nullptr, 0, q.a.rows, q.k, mx_steps(q.k), q.bias, q.bias_dtype, q.act, q.out_dtype, q.out};
+        if (int rc = launch_few(q.a.rows <= 16 ? few_kernel<1> : q.a.rows <= 32 ? few_kernel<2> : few_kernel<4>, f, 0, stream)) return rc;
     }
-    const Plan p = plan(a.rows, b.rows, k);
-    const int64_t tiles = p.tiles_m * p.tiles_n, quads = a.rows * ceil_div64(b.rows, 4);
-    if (tiles >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
-    GemmArgs g{a, b, mx_steps(k), p.steps_per_split, bias, bias_dtype, act, out_dtype, out, p.tiles_m, p.tiles_n};
-    if (p.splits > 1) g.bias = nullptr, g.act = AMSIM_ACT_NONE, g.out_dtype = AMSIM_DTYPE_F32, g.out = workspace;
-    const dim3 grid((unsigned)tiles, (unsigned)p.splits);
-    switch (p.tile) {
-    case 0: gemm_kernel<8, 8, 4, 1><<<grid, WG, 0, stream>>>(g); break;
-    case 1: gemm_kernel<8, 4, 3, 2><<<grid, WG, 0, stream>>>(g); break;
-    case 2: gemm_kernel<4, 4, 4, 2><<<grid, WG, 0, stream>>>(g); break;
-    default: gemm_kernel<2, 2, 4, 4><<<grid, WG, 0, stream>>>(g); break;
+    FinishArgs f{};
+    if (n) {
+        const Plan p = plan(t, n);
+        GemmJobs &jobs = f.products;
+        int64_t blocks = 0;
+        char *partial = (char *)workspace;
+        for (int j = 0; j < n; ++j) {
+            const Product &q = list[which[j]];
+            const auto &o = p.of[j];
+            jobs.job[j] = GemmArgs{q.a, q.b, mx_steps(q.k), o.steps_per_split, q.bias, q.bias_dtype, q.act, q.out_dtype, q.out, (unsigned)o.tiles_m,
+                                   (unsigned)o.tiles_n, (int)o.splits, o.splits > 1 ? (float *)partial : nullptr};
+            partial += partial_bytes(t[j], o.splits);
+            if (j == 0) jobs.blocks = (unsigned)std::min<int64_t>(o.tiles_m * o.tiles_n * o.splits, 1 << 30);
+            blocks += o.tiles_m * o.tiles_n * o.splits;
+            if (o.splits > 1) f.blocks[j] = (unsigned)ceil_div64(t[j].m * ceil_div64(t[j].n, 4), WG);
+            // (steps are counted in 32-bit offsets of 1 KB)
+            if (blocks >= (1ll << 24) || o.steps_per_split >= (1ll << 21)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles or steps than one launch takes");
+        }
+        switch (p.tile) {
+        case 0: gemm_kernel<8, 8, 4, 1><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
+        case 1: gemm_kernel<8, 4, 3, 2><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
+        case 2: gemm_kernel<4, 4, 4, 2><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
+        default: gemm_kernel<2, 2, 4, 4><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
+        }
+        AMSIM_HIP_CHECK(hipGetLastError());
     }
-    AMSIM_HIP_CHECK(hipGetLastError());
-    if (p.splits > 1) {
-        g.bias = bias, g.act = act, g.out_dtype = out_dtype, g.out = out;
-        gemm_reduce_kernel<<<(unsigned)ceil_div64(quads, WG), WG, 0, stream>>>(g, (const float *)workspace, (int)p.splits);
+    f.sums = sums, f.parts = parts, f.columns = columns, f.out = out, f.out_dtype = out_dtype;
+    const unsigned last = f.blocks[0] + f.blocks[1] + (sums ? (unsigned)ceil_div64(columns, 16) : 0);
+    if (last) {
+        finish_kernel<<<last, WG, 0, stream>>>(f);
         AMSIM_HIP_CHECK(hipGetLastError());
     }
     return AMSIM_OK;
 }
+int product(const Product &q, void *workspace, hipStream_t stream) { return products(&q, 1, nullptr, 0, 0, nullptr, 0, workspace, stream); }
 
 int check_product(int64_t m, int64_t n, int64_t k, const void *bias, int bias_dtype, int act, const void *out, int out_dtype)
 {
@@ -599,18 +713,6 @@ bool product_fits(int64_t m, int64_t n, int64_t k)
     return mx_extents_fit(m, k) && mx_extents_fit(n, k) && mx_extents_fit(m, n) && m && n && k;
 }
 
-int column_sums(const float *parts, int64_t count, int64_t n, void *out, int dtype, hipStream_t stream)
-{
-    const unsigned groups = (unsigned)ceil_div64(n, 64);
-    switch (dtype) {
-    case AMSIM_DTYPE_F32: column_sums_kernel<float><<<groups, 1024, 0, stream>>>(parts, count, n, (float *)out); break;
-    case AMSIM_DTYPE_BF16: column_sums_kernel<__bf16><<<groups, 1024, 0, stream>>>(parts, count, n, (__bf16 *)out); break;
-    default: column_sums_kernel<_Float16><<<groups, 1024, 0, stream>>>(parts, count, n, (_Float16 *)out); break;
-    }
-    AMSIM_HIP_CHECK(hipGetLastError());
-    return AMSIM_OK;
-}
-
 }  // namespace
 
 }  // namespace amsim
@@ -631,7 +733,7 @@ int amsim_mxfp4_matmul(const void *a, const void *b, int64_t m, int64_t n, int64
     if (!a || !b) return fail(AMSIM_ERR_INVALID, "mxfp4: null pointer");
     if (((uintptr_t)a & 15) || ((uintptr_t)b & 15)) return fail(AMSIM_ERR_INVALID, "mxfp4: misaligned pointer");
     if (int rc = check_workspace(workspace, workspace_bytes, product_workspace(m, n, k))) return rc;
-    return product(operand(a, m, k), operand(b, n, k), k, bias, bias_dtype, act, out, out_dtype, workspace, (hipStream_t)stream);
+    return product({operand(a, m, k), operand(b, n, k), k, bias, bias_dtype, act, out, out_dtype}, workspace, (hipStream_t)stream);
 }
 
 size_t amsim_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k)
@@ -655,8 +757,8 @@ int amsim_mxfp4_linear(const void *x, int dtype, int64_t row_stride, const void 
     }
     const MxConversion job{x, nullptr, dtype, m, k, row_stride, (uint8_t *)workspace, nullptr, nullptr};
     if (int rc = mx_convert(&job, 1, (hipStream_t)stream)) return rc;
-    return product(operand(workspace, m, k), operand(w, n, k), k, bias, bias_dtype, act, out, dtype,
-                   (char *)workspace + operand_bytes(m, k), (hipStream_t)stream);
+    return product({operand(workspace, m, k), operand(w, n, k), k, bias, bias_dtype, act, out, dtype}, (char *)workspace + operand_bytes(m, k),
+                   (hipStream_t)stream);
 }
 
 size_t amsim_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t k)
@@ -680,14 +782,16 @@ int amsim_mxfp4_dense(const void *x, int dtype, int64_t row_stride, const void *
     const MxConversion jobs[2] = {{x, nullptr, dtype, m, k, row_stride, x_rows, (uint8_t *)x_columns, nullptr},
                                   {kernel, nullptr, kernel_dtype, k, n, kernel_row_stride, (uint8_t *)kernel_rows, kernel_columns, nullptr}};
     if (int rc = mx_convert(jobs, 2, (hipStream_t)stream)) return rc;
-    return product(operand(x_rows, m, k), operand(kernel_columns, n, k), k, bias, bias_dtype, act, out, dtype, kernel_columns + operand_bytes(n, k),
+    return product({operand(x_rows, m, k), operand(kernel_columns, n, k), k, bias, bias_dtype, act, out, dtype}, kernel_columns + operand_bytes(n, k),
                    (hipStream_t)stream);
 }
 
 size_t amsim_mxfp4_dense_grad_workspace_bytes(int64_t m, int64_t n, int64_t k)
 {
     if (!product_fits(m, n, k)) return 0;
-    return operand_bytes(m, n) + operand_bytes(n, m) + sums_bytes(m, n) + std::max(product_workspace(m, k, n), product_workspace(k, n, m));
+    const Extents e[2] = {{m, k, n}, {k, n, m}};
+    // (the products of either gradient alone are planned by themselves)
+    return operand_bytes(m, n) + operand_bytes(n, m) + sums_bytes(m, n) + std::max({products_workspace(e, 2), products_workspace(e, 1), products_workspace(e + 1, 1)});
 }
 
 int amsim_mxfp4_dense_grad(const void *grad, int dtype, int64_t row_stride, const void *out, const void *x_columns, const void *kernel_rows,
@@ -712,12 +816,11 @@ int amsim_mxfp4_dense_grad(const void *grad, int dtype, int64_t row_stride, cons
     char *partial = (char *)sums + sums_bytes(m, n);
     const MxConversion job{grad, out, dtype, m, n, row_stride, grad_x ? rows : nullptr, grad_kernel ? columns : nullptr, grad_bias ? sums : nullptr};
     if (int rc = mx_convert(&job, 1, s)) return rc;
-    if (grad_x)
-        if (int rc = product(operand(rows, m, n), operand(kernel_rows, k, n), n, nullptr, 0, AMSIM_ACT_NONE, grad_x, dtype, partial, s)) return rc;
-    if (grad_kernel)
-        if (int rc = product(operand(x_columns, k, m), operand(columns, n, m), m, nullptr, 0, AMSIM_ACT_NONE, grad_kernel, kernel_dtype, partial, s)) return rc;
-    if (grad_bias) return column_sums(sums, ceil_div64(m, 32), n, grad_bias, bias_dtype, s);
-    return AMSIM_OK;
+    Product list[2];
+    int count = 0;
+    if (grad_x) list[count++] = {operand(rows, m, n), operand(kernel_rows, k, n), n, nullptr, 0, AMSIM_ACT_NONE, grad_x, dtype};
+    if (grad_kernel) list[count++] = {operand(x_columns, k, m), operand(columns, n, m), m, nullptr, 0, AMSIM_ACT_NONE, grad_kernel, kernel_dtype};
+    return products(list, count, grad_bias ? sums : nullptr, ceil_div64(m, 32), n, grad_bias, bias_dtype, partial, s);
 }
 
 }  // extern "C"
