@@ -6,6 +6,7 @@
 // training step of a 128 x 784 x 300 layer 125 and 80 (of which torch's own engine takes 50), the step of an
 // optimizer of 192 tensors 116 and 14.
 #include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
@@ -95,6 +96,7 @@ Source source(const Tensor &given, const char *name)
     s.rows = given.size(0), s.cols = given.size(1);
     if (s.rows == 0 || s.cols == 0) value_error(std::string(name) + " is empty: blocks of no elements have no scale");
     if (s.t.is_neg()) s.t = s.t.resolve_neg();
+    if (s.t._is_zerotensor()) s.t = at::zeros(s.t.sizes(), s.t.options());  // (zeros that take no memory)
     const int64_t s0 = s.t.stride(0), s1 = s.t.stride(1);
     if ((s1 == 1 || s.cols == 1) && (s0 >= s.cols || s.rows == 1)) {
         s.stride = s.rows > 1 ? s0 : s.cols;
@@ -148,7 +150,7 @@ Bias bias_of(const std::optional<Tensor> &b, int64_t units, const Tensor &like)
     if (b->get_device() != like.get_device()) value_error("bias must be on the operands' device");
     const int dtype = known(b->scalar_type(), "bias");
     if (b->dim() != 1 || b->size(0) != units) value_error("bias must have one entry per output channel");
-    return {b->contiguous().resolve_neg(), dtype};
+    return {b->_is_zerotensor() ? at::zeros(b->sizes(), b->options()) : b->contiguous().resolve_neg(), dtype};
 }
 
 // ---- conversions and products -----------------------------------------------------------------------------------
@@ -327,6 +329,8 @@ Tensor linearmx(py::handle x_, py::handle kernel_, py::handle bias_, int act)
     const std::optional<Tensor> bias = maybe_tensor(bias_, "bias");
     if (x.dim() < 1 || kernel.dim() != 2 || x.size(-1) != kernel.size(0)) value_error("linearmx expects x [..., width] and kernel [width, units]");
     if (x.numel() == 0 || kernel.numel() == 0) value_error("linearmx of no elements");
+    if (x._fw_grad(0).defined() || kernel._fw_grad(0).defined() || (bias && bias->_fw_grad(0).defined()))
+        throw py::type_error("linearmx has no forward-mode derivative");
     const Tensor flat = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
     const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || kernel.requires_grad() || (bias && bias->requires_grad()));
     const Tensor out = graph ? LinearMX::apply(flat, kernel, bias, (int64_t)act) : dense(flat, kernel, bias, act, false, false).first;
@@ -356,7 +360,7 @@ struct TensorList {
             if (good) {
                 const Tensor &t = THPVariable_Unpack(o);
                 good = t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == type && t.numel() == sizes[i] && t.get_device() == device
-                    && t.is_contiguous() && !t.is_neg();
+                    && t.is_contiguous() && !t.is_neg() && !t._is_zerotensor();
                 if (good) out[i] = t.data_ptr();
             }
             if (!good)

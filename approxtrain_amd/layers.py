@@ -13,7 +13,7 @@ from torch.autograd import forward_ad
 
 from . import functors
 from .amnn_ops import amconvolution_v2
-from .math_ops import matmulam
+from .math_ops import linearmx, matmulam
 
 
 # Keras vocabulary of the reference's layers (activations.get / initializers.get,
@@ -393,6 +393,69 @@ class denseam(nn.Module, _KerasLayerArgs):
 
     def get_config(self):
         return {"units": self.units, "use_bias": self.use_bias, "mant_mul_lut": self.mant_mul_lut}
+
+
+class densemx(nn.Module, _KerasLayerArgs):
+    """``denseam`` with the format that the matrix cores multiply in place of a table: ``activation(inputs . kernel +
+    bias)`` in microscaled 4-bit floating point (``math_ops.linearmx``), the constructor as ``denseam``'s but for
+    the table.  The parameters are 32-bit floats, activations float32, bfloat16 or float16.  ``pack()`` gives the
+    layer as it is served, with weights of 4 bits."""
+
+    def __init__(self, units, activation=None, use_bias=True, kernel_initializer="glorot_uniform",
+                 bias_initializer="zeros", kernel_regularizer=None, bias_regularizer=None, activity_regularizer=None,
+                 kernel_constraint=None, bias_constraint=None, input_dim=None, **kwargs):
+        super().__init__()
+        if int(units) < 1:
+            raise ValueError(f"Received an invalid value for `units`, expected a positive integer, got {units}.")
+        self.units, self.use_bias = int(units), use_bias
+        self.activation = _get_activation(activation)
+        self.kernel_initializer, self.bias_initializer = kernel_initializer, bias_initializer
+        input_shape = self._keras_args(kernel_regularizer, bias_regularizer, activity_regularizer, kernel_constraint,
+                                       bias_constraint, kwargs)
+        self.kernel = None
+        self.bias = None
+        if input_dim is None and input_shape is not None:
+            input_dim = input_shape[-1]
+        if input_dim is not None:
+            self.build(input_dim)
+
+    build = denseam.build
+
+    def forward(self, inputs):
+        if self.kernel is None:
+            self.build(inputs.shape[-1], inputs.device)
+        act = _fusable(self.activation)
+        out = linearmx(inputs, self.kernel, self.bias, activation=act)
+        return self._track_activity(self.activation(out) if act is None else out)
+
+    def pack(self):
+        """The layer for inference, as a ``packed_densemx`` that holds its weights in 4 bits."""
+        if self.kernel is None:
+            raise ValueError("the layer has no weights yet: call it, or give input_dim")
+        return packed_densemx(self.kernel, self.bias, self.activation)
+
+    def get_config(self):
+        return {"units": self.units, "use_bias": self.use_bias}
+
+
+class packed_densemx(nn.Module):
+    """A dense layer for inference: ``kernel`` ``[width, units]`` is converted to 4 bits once, the activations on
+    the way (``functors.mxfp4_linear``).  Its outputs are those of the ``densemx`` layer it was packed from, up to the order
+    of the sums."""
+
+    def __init__(self, kernel, bias=None, activation=None):
+        super().__init__()
+        self.activation = _get_activation(activation)
+        with torch.no_grad():
+            weights = functors.mxfp4_quantize(kernel.detach(), axis=0)
+        self.units, self.width = weights.shape
+        self.register_buffer("weights", weights.data)
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+
+    def forward(self, inputs):
+        act = _fusable(self.activation)
+        out = functors.mxfp4_linear(inputs, functors.MXTensor(self.weights, self.units, self.width), self.bias, act)
+        return self.activation(out) if act is None else out
 
 
 class _Attention(torch.autograd.Function):
