@@ -437,7 +437,8 @@ __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
 }
 
 // What is left behind the products: partial sums of split reductions, added in the order of the splits, and a bias
-// gradient's from the sums of every 32 rows, 16 columns and 16 runs of rows to a workgroup.
+// gradient's from the sums of every 32 rows, 16 columns and 64 runs of rows to a workgroup, the runs joined in pairs.
+constexpr int FINISH_WG = 1024, MOST_SPLITS = 16;
 struct FinishArgs {
     GemmJobs products;
     unsigned blocks[2];      // of either product's sums
@@ -446,63 +447,73 @@ struct FinishArgs {
     void *out;
     int out_dtype;
 };
-__global__ __launch_bounds__(WG) void finish_kernel(FinishArgs f)
+__global__ __launch_bounds__(FINISH_WG) void finish_kernel(FinishArgs f)
 {
-    __shared__ float run[16][16];
+    constexpr int RUNS = FINISH_WG / 16;
+    __shared__ float run[RUNS][16];
     unsigned id = blockIdx.x;
     if (id < f.blocks[0] + f.blocks[1]) {
         const bool other = id >= f.blocks[0];
         if (other) id -= f.blocks[0];
         const GemmArgs &g = f.products.job[other];
-        const int64_t N = g.b.rows, quads = ceil_div64(N, 4), at = (int64_t)id * WG + threadIdx.x;
+        const int64_t N = g.b.rows, quads = ceil_div64(N, 4), at = (int64_t)id * FINISH_WG + threadIdx.x;
         if (at >= g.a.rows * quads) return;
         const int64_t m = at / quads, n = at % quads * 4;
         const int count = (int)(N - n < 4 ? N - n : 4);
-        float v[4] = {0, 0, 0, 0};
-        for (int s = 0; s < g.splits; ++s) {
-            const float *p = g.partial + (s * g.a.rows + m) * N + n;
-            if (N % 4 == 0) {
-                const v4f q = *(const v4f *)p;
+        const float *p = g.partial + m * N + n;
+        const int64_t apart = g.a.rows * N;
+        v4f part[MOST_SPLITS];  // (all under way at once: one after the other they take a microsecond each)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] += q[i];
+        for (int s = 0; s < MOST_SPLITS; ++s) {
+            part[s] = v4f{0, 0, 0, 0};
+            if (s >= g.splits) continue;
+            if (count == 4) {
+                part[s] = __builtin_bit_cast(v4f, load16(p + s * apart));
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i < count) v[i] += p[i];
+                for (int i = 0; i < 3; ++i)
+                    if (i < count) part[s][i] = p[s * apart + i];
             }
         }
+        float v[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < MOST_SPLITS; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += part[s][i];
         finish4(g.bias, g.bias_dtype, g.act, g.out, g.out_dtype, m, n, N, v);
         return;
     }
     id -= f.blocks[0] + f.blocks[1];
     const int c = threadIdx.x & 15, w = threadIdx.x >> 4;
-    const int64_t col = (int64_t)id * 16 + c, each = ceil_div64(f.parts, 16), end = min(f.parts, each * (w + 1));
+    const int64_t col = (int64_t)id * 16 + c, each = ceil_div64(f.parts, RUNS), end = min(f.parts, each * (w + 1));
     float s = 0.0f;
     if (col < f.columns) {
-#pragma unroll 16
+#pragma unroll 8
         for (int64_t p = each * w; p < end; ++p) s += f.sums[p * f.columns + col];
     }
     run[w][c] = s;
-    __syncthreads();
+    for (int half = RUNS / 2; half; half /= 2) {
+        __syncthreads();
+        if (w < half) run[w][c] += run[w + half][c];
+    }
     if (w != 0 || col >= f.columns) return;
-#pragma unroll
-    for (int i = 1; i < 16; ++i) s += run[i][c];
+    s = run[0][c];
     if (f.out_dtype == AMSIM_DTYPE_F32) ((float *)f.out)[col] = s;
     else if (f.out_dtype == AMSIM_DTYPE_BF16) ((__bf16 *)f.out)[col] = (__bf16)s;
     else ((_Float16 *)f.out)[col] = (_Float16)s;
 }
 
 struct Tile {
-    int rows, cols;
-    // microseconds, as measured on products of 128 to 16384 a side: of one tile's step on a CU of its own, of a tile's step
-    // with the card full, of storing a tile, and of a round where tiles do not overlap
-    double alone, step, store, round;
+    int rows, cols, slots;  // slots: tiles that the card holds at once
+    // microseconds, as measured on products of 128 to 16384 a side: of a step where a tile has a CU for itself, and
+    // where all slots are taken; of storing a tile
+    double alone, full, store;
 };
 // Tiles of 256 fetch least for an operation, and have their CU for themselves: what they store, nobody multiplies
 // beside.  256 x 128 share it by two (512 tiles of 32 steps: 39.3 us, 40.7 as 256 of 256, 42.2 as 1024 of 128; of 128 steps 124,
 // 115 and 136; 2048 tiles of 16 steps 84, 96, 92).  Tiles of 128 and 64 fetch two and four times the bytes, and are
 // for few results (256 tiles of 128, 16 steps: 10.0 us, 13.9 in 256 x 128; 410 of 64, 21 steps: 7.7, 10.1 in 128).
-constexpr Tile TILES[] = {{256, 256, 0.6, 0, 0, 12}, {256, 128, 0.4, 0.00166, 0.0106, 0}, {128, 128, 0.2, 0.00093, 0.0067, 0}, {64, 64, 0.1, 0.00039, 0.0021, 0}};
+constexpr Tile TILES[] = {{256, 256, 256, 0.74, 0.74, 0}, {256, 128, 512, 0.45, 0.85, 0.0106}, {128, 128, 512, 0.2, 0.476, 0.0067}, {64, 64, 1024, 0.1, 0.4, 0.0021}};
 
 struct Extents {
     int64_t m, n, k;
@@ -514,14 +525,16 @@ struct Plan {
     } of[2];
 };
 
-// what a launch of `tiles` tiles takes, of which the products' steps add up to `work`, each tile at least `each`
-double microseconds(int tile, double tiles, double work, double each)
+// What a launch of `tiles` tiles takes whose steps add up to `work` and are at most `longest`: rounds of all slots, and a
+// last one in which a CU has one tile or a few.
+double microseconds(int tile, double tiles, double work, double longest)
 {
     const Tile &t = TILES[tile];
-    if (t.round) return 4.2 + std::ceil(tiles / 256) * (0.74 * work / tiles + t.round);
-    double steps = std::max(t.alone * each, t.step * work);
-    if (tile == 1 && tiles > 256 && tiles < 512) steps = std::max(steps, 0.8 * each);  // some CUs have two, others one
-    return 6.5 + steps + t.store * tiles;
+    const double mean = work / tiles, rounds = std::floor(tiles / t.slots), rest = tiles - rounds * t.slots;
+    if (tile == 0) return 4.2 + (rounds + (rest > 0)) * (t.full * mean + 12);
+    double last = rest > 0 ? std::max(t.alone, t.full * rest / t.slots) : 0;
+    if (tile == 1 && rest > 256) last = t.full;
+    return 6.5 + std::max(rounds * t.full * mean + last * mean, t.alone * longest) + t.store * tiles;
 }
 
 // The tile of one or two products and the splits of their reductions that take least time.  A split reduction takes a
@@ -537,7 +550,7 @@ Plan make_plan(const Extents *e, int count)
             const int64_t steps = mx_steps(e[j].k), tiles_m = ceil_div64(e[j].m, TILES[i].rows), tiles_n = ceil_div64(e[j].n, TILES[i].cols);
             const double area = (double)tiles_m * (double)tiles_n;
             double quickest = 0, its_more = 0;
-            for (int64_t s = 1; s <= 16 && (s == 1 || 2 * s <= steps); s *= 2) {
+            for (int64_t s = 1; s <= MOST_SPLITS && (s == 1 || 2 * s <= steps); s *= 2) {
                 const int64_t each = ceil_div64(steps, s), splits = ceil_div64(steps, each);
                 const double extra = splits > 1 ? 3 + (double)splits * (double)e[j].m * (double)e[j].n * 8 / 4e6 : 0;
                 const double us = microseconds(i, area * splits, area * splits * each, each) + extra;
@@ -644,7 +657,9 @@ int products(const Product *list, int count, const float *sums, int64_t parts, i
     }
     FinishArgs f{};
     if (n) {
-        const Plan p = plan(t, n);
+        Plan p = plan(t, n);
+        if (n == 2 && p.of[1].steps_per_split > p.of[0].steps_per_split)  // the tiles that take longest go first
+            std::swap(t[0], t[1]), std::swap(which[0], which[1]), std::swap(p.of[0], p.of[1]);
         GemmJobs &jobs = f.products;
         int64_t blocks = 0;
         char *partial = (char *)workspace;
@@ -656,7 +671,7 @@ int products(const Product *list, int count, const float *sums, int64_t parts, i
             partial += partial_bytes(t[j], o.splits);
             if (j == 0) jobs.blocks = (unsigned)std::min<int64_t>(o.tiles_m * o.tiles_n * o.splits, 1 << 30);
             blocks += o.tiles_m * o.tiles_n * o.splits;
-            if (o.splits > 1) f.blocks[j] = (unsigned)ceil_div64(t[j].m * ceil_div64(t[j].n, 4), WG);
+            if (o.splits > 1) f.blocks[j] = (unsigned)ceil_div64(t[j].m * ceil_div64(t[j].n, 4), FINISH_WG);
             // (steps are counted in 32-bit offsets of 1 KB)
             if (blocks >= (1ll << 24) || o.steps_per_split >= (1ll << 21)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles or steps than one launch takes");
         }
@@ -671,7 +686,7 @@ int products(const Product *list, int count, const float *sums, int64_t parts, i
     f.sums = sums, f.parts = parts, f.columns = columns, f.out = out, f.out_dtype = out_dtype;
     const unsigned last = f.blocks[0] + f.blocks[1] + (sums ? (unsigned)ceil_div64(columns, 16) : 0);
     if (last) {
-        finish_kernel<<<last, WG, 0, stream>>>(f);
+        finish_kernel<<<last, FINISH_WG, 0, stream>>>(f);
         AMSIM_HIP_CHECK(hipGetLastError());
     }
     return AMSIM_OK;
