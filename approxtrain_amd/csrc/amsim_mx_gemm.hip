@@ -99,6 +99,20 @@ __device__ __forceinline__ void place_tile(unsigned id, unsigned tiles_m, unsign
 // s_waitcnt for vmcnt n outstanding loads, and for all of LDS's answers
 #define MX_WAIT_LOADS(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | 7 << 4 | 15 << 8 | ((n) >> 4) << 14)
 #define MX_WAIT_LDS() __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 0 << 8 | 3 << 14)
+// the workgroup meets without waiting for anything else; no access to memory moves across it
+__device__ __forceinline__ void meet()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// what a wavefront wrote to LDS is read by its other lanes after this (LDS answers a wavefront in order)
+__device__ __forceinline__ void lanes_meet()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
 
 // SIZE bytes a lane from memory to LDS, without passing through registers: lane l's bytes go to to + SIZE l.  The
 // wavefront's address and the step's offset stay in scalar registers.
@@ -136,7 +150,7 @@ __device__ __forceinline__ void store_tile(uint8_t *lds, const v4f (&acc)[FM][FN
             for (int e = 0; e < 4; ++e) t[e] = from_float<T>(activate(acc[first + i][j][e] + bias[j][e], act));
             __builtin_memcpy(__builtin_assume_aligned(lds + (16 * i + lane % 16) * R::STRIDE + (16 * j + lane / 16 * 4) * sizeof(T), 4 * sizeof(T)), t, sizeof(t));
         });
-        __builtin_amdgcn_wave_barrier();
+        lanes_meet();
         const int64_t row0 = m0 + 16 * first;
         const int rows = (int)max<int64_t>(0, min<int64_t>(16 * R::AT_ONCE, M - row0));
         T *o = out + row0 * N + n0;
@@ -154,7 +168,7 @@ __device__ __forceinline__ void store_tile(uint8_t *lds, const v4f (&acc)[FM][FN
             for (int r = lane / PIECES; r < rows; r += DOWN, from += DOWN * R::STRIDE, to += DOWN * N)
                 for (int i = 0; i < columns - c; ++i) to[i] = ((const T *)from)[i];
         }
-        __builtin_amdgcn_wave_barrier();
+        lanes_meet();
     });
 }
 
@@ -250,25 +264,25 @@ __global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmJobs jobs)
     auto step = [&](int s, const typename K::Registers &now, typename K::Registers &next) {
         MX_WAIT_LDS();
         MX_WAIT_LOADS((STAGES - 2) * K::LOADS);
-        __builtin_amdgcn_s_barrier();
+        meet();
         read_step(s + 1, next);
         fetch_step(s + STAGES);
         multiply(now);
-        // two reads of LDS behind a multiplication, then a load behind every fourth
-        for_each<K::READS / 2>([](auto) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        // a read of LDS behind a multiplication, then a load behind every fourth (few fragments: second)
+        for_each<K::READS>([](auto) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         });
         for_each<K::LOADS>([](auto) {
             __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, FM * FN == 64 ? 4 : 2, 0);
         });
         __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) fetch_step(s);
     MX_WAIT_LOADS((STAGES - 1) * K::LOADS);
-    __builtin_amdgcn_s_barrier();
+    meet();
     typename K::Registers even, odd;
     read_step(0, even);
     int s = count & 1;
@@ -282,7 +296,7 @@ __global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmJobs jobs)
     }
     MX_WAIT_LDS();
     MX_WAIT_LOADS(0);
-    __builtin_amdgcn_s_barrier();  // (LDS is free)
+    meet();  // (LDS is free)
     const int64_t m0 = (int64_t)(tm * 2 + wm) * FM * 16, n0 = (int64_t)(tn * 2 + wn) * FN * 16;
     if (m0 >= g.a.rows || n0 >= g.b.rows) return;
     const bool whole = !g.partial;
