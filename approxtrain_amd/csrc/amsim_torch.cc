@@ -415,6 +415,18 @@ void adamw_step(const TensorList &list, py::list params, py::list grads, int sta
     }
 }
 
+// the values that a buffer of 8-bit moments stands for
+Tensor state_values(py::handle codes_, py::handle scales_, bool roots)
+{
+    const Tensor &codes = on_device(tensor(codes_, "codes"), "codes"), &scales = on_device(tensor(scales_, "scales"), "scales");
+    if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kFloat || !codes.is_contiguous() || !scales.is_contiguous()
+        || codes.numel() != scales.numel() * 256)
+        value_error("moments of 8 bits are bytes in blocks of 256 with a float32 each");
+    Tensor out = at::empty({codes.numel()}, codes.options().dtype(at::kFloat));
+    if (out.numel()) check(amsim_adamw_state_values(codes.data_ptr(), (const float *)scales.data_ptr(), scales.numel(), roots, (float *)out.data_ptr(), stream()));
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m)
@@ -427,6 +439,7 @@ PYBIND11_MODULE(_native, m)
     m.def("dense_grad", &dense_grad_call);
     m.def("linearmx", &linearmx);
     m.def("adamw_step", &adamw_step);
+    m.def("state_values", &state_values);
     py::class_<TensorList>(m, "TensorList").def(py::init([](std::vector<int64_t> sizes, py::handle dtype, int device) {
         at::ScalarType t;
         result_code(dtype, t);

@@ -493,20 +493,13 @@ class AdamWState:
             if t is not None and (t.dtype is not dtype or t.numel() != n or t.get_device() != index or not t.is_contiguous() or t.is_neg()):
                 raise ValueError(f"{name}[{i}] must be a contiguous {dtype} tensor of {n} elements on device {index}")
 
-    def _values(self, codes, scales, roots):
-        out = torch.empty(codes.numel(), device=codes.device)
-        if out.numel():
-            check(load_library().amsim_adamw_state_values(codes.data_ptr(), scales.data_ptr(), scales.numel(), roots, out.data_ptr(),
-                                                          torch._C._cuda_getCurrentRawStream(_device_of(codes, "codes"))))
-        return out
-
     def first_moments(self):
         """The values of the first moments in the buffer's order, float32."""
-        return self.m if self.state_bits == 32 else self._values(self.m, self.m_scale, 0)
+        return self.m if self.state_bits == 32 else _native().state_values(self.m, self.m_scale, False)
 
     def second_roots(self):
         """The square roots of the second moments in the buffer's order, float32."""
-        return self.v.sqrt() if self.state_bits == 32 else self._values(self.v, self.v_scale, 1)
+        return self.v.sqrt() if self.state_bits == 32 else _native().state_values(self.v, self.v_scale, True)
 
 
 def adamw_step(state, grads, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, grad_scale=None):

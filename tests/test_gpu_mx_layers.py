@@ -220,6 +220,18 @@ def test_optimizer_in_a_graph():
             assert torch.equal(a, b)
 
 
+def test_moments_of_other_buffers_are_refused():
+    p, g = torch.zeros(600, device="cuda"), torch.ones(600, device="cuda")
+    for name in ("m", "v_scale"):
+        state = functors.AdamWState([p], 8)
+        setattr(state, name, getattr(state, name)[:-1])
+        with pytest.raises(ValueError, match="buffers"):
+            functors.adamw_step(state, [g], 1)
+        with pytest.raises(ValueError, match="blocks of 256"):
+            state.first_moments() if name == "m" else state.second_roots()
+    assert not p.any()
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_example_learns(bits):
     spec = importlib.util.spec_from_file_location("lenet300_mx", os.path.join(ROOT, "examples", "lenet300_mx.py"))
