@@ -128,10 +128,10 @@ template <int SIZE> __device__ __forceinline__ void load_to_lds(const uint8_t *f
 
 // A wave's results to memory, by way of LDS: a lane's four columns lie in sixteen rows' lines, a row of 16 F columns
 // is whole ones.  The rows' padding puts sixteen rows' writes on different banks.  A tile of 256, alone on its CU,
-// goes out in parts (16 rows of 32 bits or 32 of 16), so that its first stores are under way early: 4096^3 takes 38.7 us
-// so and 39.7 in one part; smaller tiles, which have neighbours to hide behind, in one: 42.7 and 44.1.
+// goes out in parts (16 rows of 32 bits or 32 of 16), so that its first stores are under way early: 4096^3 takes 37.2 us
+// so and 37.6 in one part; tiles of 128 and less, which have neighbours to hide behind, in one: 42.7 and 44.1.
 template <typename T, int FM, int FN> struct Rows {
-    static constexpr int COLUMNS = 16 * FN, STRIDE = COLUMNS * sizeof(T) + 16, AT_ONCE = FM == 8 ? 32 / FN / sizeof(T) : FM;
+    static constexpr int COLUMNS = 16 * FN, STRIDE = COLUMNS * sizeof(T) + 16, AT_ONCE = FM * FN == 32 ? 32 / FN / sizeof(T) : FM;
     static constexpr int BYTES = 16 * AT_ONCE * STRIDE;
 };
 template <typename T, int FM, int FN>
@@ -172,14 +172,15 @@ __device__ __forceinline__ void store_tile(uint8_t *lds, const v4f (&acc)[FM][FN
     });
 }
 
-// A workgroup of 2 x 2 waves, FM x FN fragments each: a tile of 32 FM rows and 32 FN columns.  Steps of 128 along the
+// A workgroup of WM x WN waves, FM x FN fragments each: a tile of 16 FM WM rows and 16 FN WN columns.  Steps of 128 along the
 // reduction go from memory to one of STAGES places in LDS without passing through registers (the storage is
 // what a wavefront's 16-byte loads deliver, lane by lane), and a step's fragments are read into
 // registers while the step before is multiplied.
-template <int FM, int FN, int STAGES> struct Gemm {
-    static constexpr int GM = FM >= 4 ? FM / 2 : 1, GN = FN >= 4 ? FN / 2 : 1;       // scale groups of a tile's sides
-    static constexpr int A = 0, B = FM * 2048, S = B + FN * 2048, BYTES = S + (GM + GN) * 256;
-    static constexpr int CODES = (FM + FN) / 2, SCALES = (GM + GN + 3) / 4;          // loads of a wave for a step: of 1 KB, of 256 bytes
+template <int FM, int FN, int WM, int WN, int STAGES> struct Gemm {
+    static constexpr int WAVES = WM * WN, AM = FM * WM, BN = FN * WN;                // fragments of a tile's sides
+    static constexpr int GM = AM >= 4 ? AM / 4 : 1, GN = BN >= 4 ? BN / 4 : 1;       // ... and their scale groups
+    static constexpr int A = 0, B = AM * 1024, S = B + BN * 1024, BYTES = S + (GM + GN) * 256;
+    static constexpr int FROM_A = AM / WAVES, CODES = (AM + BN) / WAVES, SCALES = (GM + GN + WAVES - 1) / WAVES;  // loads of a wave for a step
     static constexpr int LOADS = CODES + SCALES;
     static constexpr int SM = FM >= 4 ? FM / 4 : 1, SN = FN >= 4 ? FN / 4 : 1;       // dwords of four fragments' scales
     static constexpr int READS = FM + FN + (SM + 1) / 2 + (SN + 1) / 2;              // of LDS (two dwords in one)
@@ -189,13 +190,13 @@ template <int FM, int FN, int STAGES> struct Gemm {
     };
 };
 
-template <int FM, int FN, int STAGES, int RESIDENT>
-__global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmJobs jobs)
+template <int FM, int FN, int WM, int WN, int STAGES, int RESIDENT>
+__global__ __launch_bounds__(64 * WM * WN, RESIDENT) void gemm_kernel(GemmJobs jobs)
 {
-    using K = Gemm<FM, FN, STAGES>;
+    using K = Gemm<FM, FN, WM, WN, STAGES>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * K::BYTES];
-    static_assert(4 * Rows<float, FM, FN>::BYTES <= STAGES * K::BYTES && 4 * Rows<__bf16, FM, FN>::BYTES <= STAGES * K::BYTES, "");
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / 2, wn = wave % 2;
+    static_assert(K::WAVES * Rows<float, FM, FN>::BYTES <= STAGES * K::BYTES && K::WAVES * Rows<__bf16, FM, FN>::BYTES <= STAGES * K::BYTES, "");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
     const bool other = blockIdx.x >= jobs.blocks;
     const GemmArgs g = jobs.job[other];
     const unsigned id = blockIdx.x - (other ? jobs.blocks : 0), tiles = g.tiles_m * g.tiles_n, split = g.splits > 1 ? id / tiles : 0;
@@ -210,19 +211,19 @@ __global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmJobs jobs)
     int to[K::CODES], to_scales[K::SCALES];
 #pragma unroll
     for (int i = 0; i < K::CODES; ++i) {
-        const bool of_a = i < FM / 2;
-        const int f = of_a ? FM / 2 * wave + i : FN / 2 * wave + i - FM / 2;
+        const bool of_a = i < K::FROM_A;
+        const int f = of_a ? K::FROM_A * wave + i : (K::CODES - K::FROM_A) * wave + i - K::FROM_A;
         const Operand &o = of_a ? g.a : g.b;
-        const int64_t at = min<int64_t>((of_a ? tm * 2 * FM : tn * 2 * FN) + f, o.fragments - 1);
+        const int64_t at = min<int64_t>((of_a ? tm * K::AM : tn * K::BN) + f, o.fragments - 1);
         fetch[i] = o.codes + (at * g.steps + beg) * 1024;
         to[i] = (of_a ? K::A : K::B) + f * 1024;
     }
 #pragma unroll
     for (int i = 0; i < K::SCALES; ++i) {
-        const int group = (wave + 4 * i) % (K::GM + K::GN);
+        const int group = (wave + K::WAVES * i) % (K::GM + K::GN);
         const bool of_a = group < K::GM;
         const Operand &o = of_a ? g.a : g.b;
-        const int64_t at = min<int64_t>(of_a ? tm * FM / 2 + group : tn * FN / 2 + group - K::GM, o.groups - 1);
+        const int64_t at = min<int64_t>(of_a ? tm * K::AM / 4 + group : tn * K::BN / 4 + group - K::GM, o.groups - 1);
         fetch_scales[i] = o.scales + (at * g.steps + beg) * 256;
         to_scales[i] = K::S + group * 256;
     }
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(WG, RESIDENT) void gemm_kernel(GemmJobs jobs)
     MX_WAIT_LDS();
     MX_WAIT_LOADS(0);
     meet();  // (LDS is free)
-    const int64_t m0 = (int64_t)(tm * 2 + wm) * FM * 16, n0 = (int64_t)(tn * 2 + wn) * FN * 16;
+    const int64_t m0 = (int64_t)(tm * WM + wm) * FM * 16, n0 = (int64_t)(tn * WN + wn) * FN * 16;
     if (m0 >= g.a.rows || n0 >= g.b.rows) return;
     const bool whole = !g.partial;
     float bias[FN][4];
@@ -519,15 +520,18 @@ __global__ __launch_bounds__(FINISH_WG) void finish_kernel(FinishArgs f)
 
 struct Tile {
     int rows, cols, slots;  // slots: tiles that the card holds at once
-    // microseconds, as measured on products of 128 to 16384 a side: of a step where a tile has a CU for itself, and
-    // where all slots are taken; of storing a tile
-    double alone, full, store;
+    // microseconds, as measured on products of 128 to 16384 a side: of a launch; of a step where a tile has a CU for itself,
+    // and where all slots are taken; of storing a tile (between results of 16 bits and of 32: workspaces are asked for
+    // before the type is known)
+    double base, alone, full, store;
 };
-// Tiles of 256 fetch least for an operation, and have their CU for themselves: what they store, nobody multiplies
-// beside.  256 x 128 share it by two (512 tiles of 32 steps: 39.3 us, 40.7 as 256 of 256, 42.2 as 1024 of 128; of 128 steps 124,
-// 115 and 136; 2048 tiles of 16 steps 84, 96, 92).  Tiles of 128 and 64 fetch two and four times the bytes, and are
-// for few results (256 tiles of 128, 16 steps: 10.0 us, 13.9 in 256 x 128; 410 of 64, 21 steps: 7.7, 10.1 in 128).
-constexpr Tile TILES[] = {{256, 256, 256, 0.74, 0.74, 0}, {256, 128, 512, 0.45, 0.85, 0.0106}, {128, 128, 512, 0.2, 0.476, 0.0067}, {64, 64, 1024, 0.1, 0.4, 0.0021}};
+// Tiles of 256 fetch least for an operation and have their CU for themselves, with eight waves (four with twice the
+// fragments: 39.8 us for 4096^3, 37.1 with eight): what they store, nobody multiplies beside.  256 x 128 share it by two (512
+// tiles of 32 steps: 38.7 us, 37.1 as 256 of 256, 42.2 as 1024 of 128; of 128 steps 124, 112 and 136; 2048 tiles of 16 steps
+// 84, 89, 92).  Tiles of 128 and 64 fetch two and four times the bytes, and are for few results (256 tiles of 128, 16
+// steps: 10.0 us, 13.9 in 256 x 128; 410 of 64, 21 steps: 7.7, 10.1 in 128).
+constexpr Tile TILES[] = {{256, 256, 256, 2.2, 0.55, 0.785, 10.8},  // (stored by a round at once)
+                          {256, 128, 512, 6.5, 0.5, 0.85, 0.0124}, {128, 128, 512, 5, 0.2, 0.46, 0.01}, {64, 64, 1024, 4, 0.1, 0.4, 0.003}};
 
 struct Extents {
     int64_t m, n, k;
@@ -545,10 +549,11 @@ double microseconds(int tile, double tiles, double work, double longest)
 {
     const Tile &t = TILES[tile];
     const double mean = work / tiles, rounds = std::floor(tiles / t.slots), rest = tiles - rounds * t.slots;
-    if (tile == 0) return 4.2 + (rounds + (rest > 0)) * (t.full * mean + 12);
     double last = rest > 0 ? std::max(t.alone, t.full * rest / t.slots) : 0;
-    if (tile == 1 && rest > 256) last = t.full;
-    return 6.5 + std::max(rounds * t.full * mean + last * mean, t.alone * longest) + t.store * tiles;
+    if (tile == 1 && rest > 256) last = 0.8;
+    const double steps = std::max(rounds * t.full * mean + last * mean, t.alone * longest);
+    if (tile == 0) return t.base + std::ceil(tiles / t.slots) * (t.store + 1.5) - 1.5 + steps;
+    return t.base + steps + t.store * tiles;
 }
 
 // The tile of one or two products and the splits of their reductions that take least time.  A split reduction takes a
@@ -595,10 +600,10 @@ Plan plan(const Extents *e, int count)
         Extents e[2];
         Plan p;
     };
-    static thread_local Known known[16] = {};
+    static thread_local Known known[64] = {};
     const Extents none{}, &f = count > 1 ? e[1] : none;
     const uint64_t hash = ((uint64_t)e[0].m * 3 + (uint64_t)e[0].n * 5 + (uint64_t)e[0].k * 7 + (uint64_t)f.k * 11) * 0x9e3779b97f4a7c15ull;
-    Known &at = known[hash >> 60];
+    Known &at = known[hash >> 58];
     auto same = [](const Extents &x, const Extents &y) { return x.m == y.m && x.n == y.n && x.k == y.k; };
     if (!same(at.e[0], e[0]) || !same(at.e[1], f)) at = Known{{e[0], f}, make_plan(e, count)};
     return at.p;
@@ -690,10 +695,10 @@ int products(const Product *list, int count, const float *sums, int64_t parts, i
             if (blocks >= (1ll << 24) || o.steps_per_split >= (1ll << 21)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles or steps than one launch takes");
         }
         switch (p.tile) {
-        case 0: gemm_kernel<8, 8, 4, 1><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
-        case 1: gemm_kernel<8, 4, 3, 2><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
-        case 2: gemm_kernel<4, 4, 4, 2><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
-        default: gemm_kernel<2, 2, 4, 4><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
+        case 0: gemm_kernel<4, 8, 4, 2, 4, 2><<<(unsigned)blocks, 512, 0, stream>>>(jobs); break;
+        case 1: gemm_kernel<8, 4, 2, 2, 3, 2><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
+        case 2: gemm_kernel<4, 4, 2, 2, 4, 2><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
+        default: gemm_kernel<2, 2, 2, 2, 4, 4><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
         }
         AMSIM_HIP_CHECK(hipGetLastError());
     }
