@@ -444,5 +444,8 @@ PYBIND11_MODULE(_native, m)
         at::ScalarType t;
         result_code(dtype, t);
         return TensorList{std::move(sizes), t, device};
-    }));
+    })).def("check", [](const TensorList &l, py::list tensors, const char *name) {
+        std::vector<void *> p;
+        l.pointers(tensors, name, l.dtype, false, p);
+    });
 }

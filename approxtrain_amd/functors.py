@@ -475,23 +475,16 @@ class AdamWState:
             raise TypeError(f"parameters must be float32, bfloat16 or float16, got {self.dtype}")
         self.params, self.state_bits = params, state_bits
         self.sizes = [p.numel() for p in params]
-        self._check(params, "params", self.dtype)
+        self._list = _native().TensorList(self.sizes, self.dtype, self.device_index)
+        self._list.check(params, "params")
         self.starts, at = [], 0
         for n in self.sizes:
             self.starts.append(at)
             at += -(-n // self.BLOCK) * self.BLOCK
         device = params[0].device
-        kind = torch.float32 if state_bits == 32 else torch.uint8
-        self.m, self.v = torch.zeros(at, dtype=kind, device=device), torch.zeros(at, dtype=kind, device=device)
+        self.m, self.v = torch.zeros((2, at), dtype=torch.float32 if state_bits == 32 else torch.uint8, device=device).unbind()
         scales = at // self.BLOCK if state_bits == 8 else 0
-        self.m_scale, self.v_scale = torch.zeros(scales, device=device), torch.zeros(scales, device=device)
-        self._list = _native().TensorList(self.sizes, self.dtype, self.device_index)
-
-    def _check(self, tensors, name, dtype):
-        index = self.device_index
-        for i, (t, n) in enumerate(zip(tensors, self.sizes)):
-            if t is not None and (t.dtype is not dtype or t.numel() != n or t.get_device() != index or not t.is_contiguous() or t.is_neg()):
-                raise ValueError(f"{name}[{i}] must be a contiguous {dtype} tensor of {n} elements on device {index}")
+        self.m_scale, self.v_scale = (torch.zeros if scales else torch.empty)((2, scales), device=device).unbind()
 
     def first_moments(self):
         """The values of the first moments in the buffer's order, float32."""
