@@ -347,15 +347,15 @@ struct FewSteps {
 };
 
 // the fragments' sums over the waves and their results, a fragment to a wave
-template <int FA> __device__ __forceinline__ void finish_few(const FewArgs &g, int64_t f, v4f (&sums)[16][FA][64], const v4f (&acc)[FA])
+template <int FA> __device__ __forceinline__ void finish_few(const FewArgs &g, int64_t f, v4f *sums, const v4f (&acc)[FA])
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
 #pragma unroll
-    for (int i = 0; i < FA; ++i) sums[wave][i][lane] = acc[i];
+    for (int i = 0; i < FA; ++i) sums[(wave * FA + i) * 64 + lane] = acc[i];
     __syncthreads();
     for (int i = wave; i < FA; i += waves) {
-        v4f z = sums[0][i][lane];
-        for (int w = 1; w < waves; ++w) z += sums[w][i][lane];
+        v4f z = sums[i * 64 + lane];
+        for (int w = 1; w < waves; ++w) z += sums[(w * FA + i) * 64 + lane];
         const int64_t m = 16 * i + lane % 16, n = f * 16 + lane / 16 * 4, N = g.b.rows;
         if (m >= g.rows || n >= N) continue;
         float v[4] = {z[0], z[1], z[2], z[3]};
@@ -367,7 +367,7 @@ template <int FA> __device__ __forceinline__ void finish_few(const FewArgs &g, i
 template <int FA>
 __global__ __launch_bounds__(1024) void few_kernel(FewArgs g)
 {
-    __shared__ v4f sums[16][FA][64];
+    __shared__ v4f sums[16 * FA * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     v4f acc[FA] = {};
     for (int64_t s = wave; s < g.steps; s += AHEAD * waves) {
@@ -387,14 +387,13 @@ __global__ __launch_bounds__(1024) void few_kernel(FewArgs g)
     finish_few(g, blockIdx.x, sums, acc);
 }
 
-// Up to 16 rows as they come: every workgroup converts them for itself, into LDS, four lanes to a block, while its
-// first loads of b are under way.  That saves a launch, and for a token's layer half the time.
-constexpr int64_t RAW_VALUES = 40960;  // rows x length (in whole steps) that it holds: 22 KB of LDS
-template <typename X>
+// FA fragments of rows as they come: every workgroup converts them for itself, into LDS, four lanes to a block, while
+// its first loads of b are under way.  That saves a launch, and for a token's layer half the time.
+constexpr int64_t RAW_VALUES = 32768;  // rows x length (in whole steps) that it converts
+template <typename X, int FA>
 __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
 {
-    __shared__ v4f sums[16][1][64];
-    extern __shared__ __attribute__((aligned(16))) uint8_t converted[];  // codes [block][row][16 bytes], scales [block][row]
+    extern __shared__ __attribute__((aligned(16))) uint8_t converted[];  // codes [block][row][16 bytes], scales [block][row]; then the sums
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int rows = (int)g.rows, apart = rows | 1, blocks = (int)g.steps * 4;  // (an odd distance: a row's blocks lie in different banks)
     uint8_t *scales = converted + blocks * apart * 16;
@@ -437,18 +436,25 @@ __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
         }
     }
     __syncthreads();
-    const int row = min(lane % 16, rows - 1);  // (results of rows that do not exist are not stored)
-    v4f acc[1] = {};
+    int row[FA];
+#pragma unroll
+    for (int i = 0; i < FA; ++i) row[i] = min(16 * i + lane % 16, rows - 1);  // (results of rows that do not exist are not stored)
+    v4f acc[FA] = {};
     for (int64_t s = wave; s < g.steps; s += AHEAD * waves) {
         if (s != wave) b.load(g, blockIdx.x, s, waves);
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) {
-            const int t = (int)s + h * waves, at = (4 * t + lane / 16) * apart + row;
+            const int t = (int)s + h * waves;
             if (t >= g.steps) break;
-            acc[0] = mfma<0, 0>(b.codes[h], *(const v4i *)(converted + at * 16), acc[0], b.scales[h], scales[at]);
+#pragma unroll
+            for (int i = 0; i < FA; ++i) {
+                const int at = (4 * t + lane / 16) * apart + row[i];
+                acc[i] = mfma<0, 0>(b.codes[h], *(const v4i *)(converted + at * 16), acc[i], b.scales[h], scales[at]);
+            }
         }
     }
-    finish_few(g, blockIdx.x, sums, acc);
+    __syncthreads();  // (the sums take the place of what was converted)
+    finish_few(g, blockIdx.x, (v4f *)converted, acc);
 }
 
 // What is left behind the products: partial sums of split reductions, added in the order of the splits, and a bias
@@ -641,14 +647,26 @@ size_t product_workspace(int64_t m, int64_t n, int64_t k)
     return products_workspace(&e, 1);
 }
 
-int launch_few(void (*kernel)(FewArgs), const FewArgs &g, int64_t lds, hipStream_t stream)
+// A wave for every step, and for 128 of the pieces of 8 values that are to be converted first (64 rows of 128: 16 waves
+// 4.7 us, one 8.7).
+int few_waves(const FewArgs &g, int64_t pieces)
+{
+    int waves = 1;
+    while (waves < 16 && (waves < g.steps || 128 * waves < pieces)) waves *= 2;
+    return waves;
+}
+int launch_few(void (*kernel)(FewArgs), const FewArgs &g, int waves, int64_t lds, hipStream_t stream)
 {
     if (g.b.fragments >= (1ll << 22)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
-    int waves = 1;
-    while (waves < 16 && waves < g.steps) waves *= 2;
     kernel<<<(unsigned)g.b.fragments, 64 * waves, lds, stream>>>(g);
     AMSIM_HIP_CHECK(hipGetLastError());
     return AMSIM_OK;
+}
+template <typename X> int launch_raw(const FewArgs &g, hipStream_t stream)
+{
+    const int fragments = g.rows <= 16 ? 1 : g.rows <= 32 ? 2 : 4, waves = few_waves(g, g.rows * g.steps * 16);
+    const int64_t lds = std::max<int64_t>(g.steps * 4 * (g.rows | 1) * 17, waves * fragments * 1024);
+    return launch_few(fragments == 1 ? raw_kernel<X, 1> : fragments == 2 ? raw_kernel<X, 2> : raw_kernel<X, 4>, g, waves, lds, stream);
 }
 
 struct Product {
@@ -672,7 +690,7 @@ int products(const Product *list, int count, const float *sums, int64_t parts, i
         const Product &q = list[j];
         if (!few(e[j].m, e[j].k)) continue;
         const FewArgs f{q.b, q.a, nullptr, 0, q.a.rows, q.k, mx_steps(q.k), q.bias, q.bias_dtype, q.act, q.out_dtype, q.out};
-        if (int rc = launch_few(q.a.rows <= 16 ? few_kernel<1> : q.a.rows <= 32 ? few_kernel<2> : few_kernel<4>, f, 0, stream)) return rc;
+        if (int rc = launch_few(q.a.rows <= 16 ? few_kernel<1> : q.a.rows <= 32 ? few_kernel<2> : few_kernel<4>, f, few_waves(f, 0), 0, stream)) return rc;
     }
     FinishArgs f{};
     if (n) {
@@ -730,13 +748,14 @@ int check_workspace(const void *workspace, size_t have, size_t need)
     return AMSIM_OK;
 }
 
-// Whether few rows are converted by every workgroup that multiplies them, not once ahead, by a launch of 3 us.  Rows x
-// length of 32768 cost a round of 256 workgroups 2.3 us: 8 rows through 4096 x 4096 take 7.0 us so, 7.7 converted
-// ahead; 16 rows 9.6 and 7.8; 4 rows through 8192 x 8192, two rounds, 13.2 and 12.6.
+// Whether few rows are converted by every workgroup that multiplies them, not once ahead, by a launch of 3 us (and as
+// much again of the host).  Rows x length of 32768 cost a round of 256 workgroups what that launch costs: 8 rows through
+// 4096 x 4096 take 7.0 us so, 7.7 converted ahead; 16 rows of 1024 x 4096 5.4 and 6.5, 32 rows 6.8 and 6.5; 24 rows of
+// 1200 x 1000 6.8 and 7.4, 32 rows 7.9 and 7.4; 48 rows of 640 x 1024 6.7 and 7.0, 64 rows 7.7 and 7.0.
 bool converts_on_the_way(int64_t m, int64_t n, int64_t k)
 {
     const int64_t values = m * mx_steps(k) * 128;
-    return m <= 16 && values * ceil_div64(n, 4096) <= RAW_VALUES;
+    return m <= 64 && values * ceil_div64(n, 4096) <= RAW_VALUES;
 }
 
 size_t operand_bytes(int64_t rows, int64_t length) { return (size_t)(mx_code_bytes(rows, length) + mx_scale_bytes(rows, length)); }
@@ -786,8 +805,11 @@ int amsim_mxfp4_linear(const void *x, int dtype, int64_t row_stride, const void 
     if (int rc = check_workspace(workspace, workspace_bytes, amsim_mxfp4_linear_workspace_bytes(m, n, k))) return rc;
     if (converts_on_the_way(m, n, k)) {
         const FewArgs f{operand(w, n, k), {}, x, row_stride, m, k, mx_steps(k), bias, bias_dtype, act, dtype, out};
-        const auto kernel = dtype == AMSIM_DTYPE_F32 ? raw_kernel<float> : dtype == AMSIM_DTYPE_BF16 ? raw_kernel<__bf16> : raw_kernel<_Float16>;
-        return launch_few(kernel, f, f.steps * 4 * (m | 1) * 17, (hipStream_t)stream);
+        switch (dtype) {
+        case AMSIM_DTYPE_F32: return launch_raw<float>(f, (hipStream_t)stream);
+        case AMSIM_DTYPE_BF16: return launch_raw<__bf16>(f, (hipStream_t)stream);
+        default: return launch_raw<_Float16>(f, (hipStream_t)stream);
+        }
     }
     const MxConversion job{x, nullptr, dtype, m, k, row_stride, (uint8_t *)workspace, nullptr, nullptr};
     if (int rc = mx_convert(&job, 1, (hipStream_t)stream)) return rc;

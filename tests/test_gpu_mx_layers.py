@@ -149,6 +149,26 @@ def test_few_rows_at_the_borders_of_their_kernels(m, k):
     assert bool(((functors.mxfp4_matmul(functors.mxfp4_quantize(x), q).double() - a @ c.t()).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(17, 10, 1), (31, 33, 33), (33, 100, 130), (50, 64, 500), (64, 1000, 128), (64, 17, 512), (18, 35, 1700)])
+def test_some_tens_of_rows_converted_on_the_way(m, n, k, dtype):
+    x, w, bias = torch.randn(m, k, device="cuda").to(dtype), torch.randn(k, n, device="cuda"), torch.randn(n, device="cuda")
+    q = functors.mxfp4_quantize(w, axis=0)
+    got = functors.mxfp4_linear(x, q, bias, "relu")
+    assert got.dtype == dtype
+    a, c, b = functors.mxfp4_quantize(x).dequantize().double(), q.dequantize().double(), bias.double()
+    want, size = torch.relu(a @ c.t() + b), a.abs() @ c.abs().t() + b.abs()
+    # sums in 32 bits, a rounding to the result's type, and of float16's small results half its smallest step
+    tol = (-(-k // 32) + 19) * 2.0 ** -23 * size + want * torch.finfo(dtype).eps / 2 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert bool(((got.double() - want).abs() <= tol).all())
+    wide = torch.full((m, k + 3), float("nan"), device="cuda", dtype=dtype)
+    wide[:, 1:k + 1] = x
+    assert torch.equal(functors.mxfp4_linear(wide[:, 1:k + 1], q, bias, "relu"), got)
+    wide[m - 1, k] = float("inf")
+    bad = torch.isnan(functors.mxfp4_linear(wide[:, 1:k + 1], q))
+    assert bool(bad[m - 1].all()) and not bool(bad[:m - 1].any())
+
+
 @pytest.mark.parametrize("m,n,k", [(256, 33000, 130), (2100, 2300, 1100), (1500, 2500, 300), (4097, 4095, 700), (300, 40000, 64)])
 def test_products_in_each_tile(m, n, k):
     """Odd extents in tiles of 256 x 256, 256 x 128 and 128, with a bias and results of 16 bits."""
