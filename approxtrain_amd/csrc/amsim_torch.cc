@@ -284,14 +284,30 @@ using torch::autograd::variable_list;
 
 // Each of a layer's three products has its operands quantised along the axis it sums over, so x, the kernel and the
 // gradient are quantised both ways, each from one reading; what the backward pass needs is kept in 4 bits.
+// A leaf has one node that adds its gradients, on the stream that it was made on, for as long as a graph of it lives.  Where
+// that is the default stream, a captured backward pass would have to wait for a captured event there, which cannot be
+// recorded and ends the process in the engine's thread: seen here first, it is an error like others.
+bool adds_on_default_stream(const Tensor &t)
+{
+    if (!t.requires_grad() || !t.is_leaf()) return false;
+    const auto node = torch::autograd::impl::grad_accumulator(t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    return stream && stream->id() == 0;
+}
+bool capturing()
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(c10::hip::getCurrentHIPStream().stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+}
+
 struct LinearMX : torch::autograd::Function<LinearMX> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &kernel, const std::optional<Tensor> &bias, int64_t act)
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &kernel, const std::optional<Tensor> &bias, int64_t act, int64_t eager)
     {
         const bool need_x = x.requires_grad(), need_kernel = kernel.requires_grad();
         auto [out, kept] = dense(x, kernel, bias, (int)act, need_kernel, need_x);
         ctx->save_for_backward(act == AMSIM_ACT_RELU ? variable_list{kept, out} : variable_list{kept});
         ctx->saved_data["shape"] = std::vector<int64_t>{x.size(0), x.size(1), kernel.size(1), need_x, need_kernel, (int64_t)kernel.scalar_type(),
-                                                        bias ? (int64_t)bias->scalar_type() : -1};
+                                                        bias ? (int64_t)bias->scalar_type() : -1, eager};
         return out;
     }
 
@@ -302,13 +318,17 @@ struct LinearMX : torch::autograd::Function<LinearMX> {
         Wanted want{s[3] && ctx->needs_input_grad(0), std::nullopt, std::nullopt};
         if (s[4] && ctx->needs_input_grad(1)) want.kernel = (at::ScalarType)s[5];
         if (s[6] >= 0 && ctx->needs_input_grad(2)) want.bias = (at::ScalarType)s[6];
+        for (int i = 0; i < 3; ++i)
+            TORCH_CHECK(!(s[7] >> i & 1) || !ctx->needs_input_grad(i) || !capturing(),
+                        "linearmx's backward pass is captured while a graph of the same leaves lives that was made on the default stream, where "
+                        "their gradients would be added: release it (its outputs and losses) before the capture");
         Tensor grads[3];
         {
             at::AutoGradMode off(false);
             const int status = dense_grad(given[0], saved[0], s[4], s[3], s[0], s[1], s[2], saved.size() > 1 ? std::optional<Tensor>(saved[1]) : std::nullopt, want, grads);
             TORCH_CHECK(status == 0, "amsim status ", status, ": ", amsim_last_error());
         }
-        variable_list result{grads[0], grads[1], grads[2], Tensor()};
+        variable_list result{grads[0], grads[1], grads[2], Tensor(), Tensor()};
         if (at::GradMode::is_enabled() && given[0].requires_grad()) {  // gradients of gradients are not provided: say so if they are asked for
             variable_list some;
             for (const Tensor &g : grads)
@@ -333,7 +353,8 @@ Tensor linearmx(py::handle x_, py::handle kernel_, py::handle bias_, int act)
         throw py::type_error("linearmx has no forward-mode derivative");
     const Tensor flat = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
     const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || kernel.requires_grad() || (bias && bias->requires_grad()));
-    const Tensor out = graph ? LinearMX::apply(flat, kernel, bias, (int64_t)act) : dense(flat, kernel, bias, act, false, false).first;
+    const int64_t eager = graph ? adds_on_default_stream(x) | adds_on_default_stream(kernel) << 1 | (bias && adds_on_default_stream(*bias)) << 2 : 0;
+    const Tensor out = graph ? LinearMX::apply(flat, kernel, bias, (int64_t)act, eager) : dense(flat, kernel, bias, act, false, false).first;
     if (x.dim() == 2) return out;
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
     shape.back() = kernel.size(1);

@@ -219,6 +219,41 @@ def test_optimizer_steps_as_the_function_does_and_goes_on_from_a_saved_state(bit
         AdamW(params, state_bits=4)
 
 
+def test_capture_beside_a_living_graph_of_the_same_leaves():
+    """A graph made on the default stream holds the nodes that add its leaves' gradients there: a captured backward pass is
+    refused while it lives, and works and replays once it is gone."""
+    x, w = torch.randn(40, 70, device="cuda"), torch.randn(70, 30, device="cuda", requires_grad=True)
+    b = torch.zeros(30, device="cuda", requires_grad=True)
+    leaves = [w, b]
+
+    def step():
+        return torch.autograd.grad(math_ops.linearmx(x, w, b, activation="relu").sum(), leaves)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    living = math_ops.linearmx(x, w, b)
+    with pytest.raises(RuntimeError, match="lives"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    torch.cuda.synchronize()
+    for got, want in zip(torch.autograd.grad(living.sum(), leaves, retain_graph=True), torch.autograd.grad(math_ops.linearmx(x, w, b).sum(), leaves)):
+        assert torch.equal(got, want)
+    del living
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(3):
+        with torch.no_grad():
+            w.normal_(generator=torch.Generator(device="cuda").manual_seed(seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(captured, step()):
+            assert torch.equal(got, want)
+
+
 def test_optimizer_in_a_graph():
     """A captured step, replayed with eager work between, steps as eager calls of the same number do."""
     p = [torch.randn(n, device="cuda") for n in (5, 300, 4097)]
