@@ -282,24 +282,24 @@ py::tuple dense_grad_call(py::handle grad, py::handle kept, int64_t rows, int64_
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// Each of a layer's three products has its operands quantised along the axis it sums over, so x, the kernel and the
-// gradient are quantised both ways, each from one reading; what the backward pass needs is kept in 4 bits.
 // A leaf has one node that adds its gradients, on the stream that it was made on, for as long as a graph of it lives.  Where
 // that is the default stream, a captured backward pass would have to wait for a captured event there, which cannot be
 // recorded and ends the process in the engine's thread: seen here first, it is an error like others.
 bool adds_on_default_stream(const Tensor &t)
 {
-    if (!t.requires_grad() || !t.is_leaf()) return false;
-    const auto node = torch::autograd::impl::grad_accumulator(t);
+    const auto node = t.requires_grad() && t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : nullptr;
     const auto stream = node ? node->stream() : std::nullopt;
     return stream && stream->id() == 0;
 }
 bool capturing()
 {
+    const auto current = c10::hip::getCurrentHIPStream();
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    return hipStreamIsCapturing(c10::hip::getCurrentHIPStream().stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+    return current.id() != 0 && hipStreamIsCapturing(current.stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
 }
 
+// Each of a layer's three products has its operands quantised along the axis it sums over, so x, the kernel and the
+// gradient are quantised both ways, each from one reading; what the backward pass needs is kept in 4 bits.
 struct LinearMX : torch::autograd::Function<LinearMX> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &kernel, const std::optional<Tensor> &bias, int64_t act, int64_t eager)
     {
@@ -353,7 +353,7 @@ Tensor linearmx(py::handle x_, py::handle kernel_, py::handle bias_, int act)
         throw py::type_error("linearmx has no forward-mode derivative");
     const Tensor flat = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
     const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || kernel.requires_grad() || (bias && bias->requires_grad()));
-    const int64_t eager = graph ? adds_on_default_stream(x) | adds_on_default_stream(kernel) << 1 | (bias && adds_on_default_stream(*bias)) << 2 : 0;
+    const int64_t eager = graph && capturing() ? adds_on_default_stream(x) | adds_on_default_stream(kernel) << 1 | (bias && adds_on_default_stream(*bias)) << 2 : 0;
     const Tensor out = graph ? LinearMX::apply(flat, kernel, bias, (int64_t)act, eager) : dense(flat, kernel, bias, act, false, false).first;
     if (x.dim() == 2) return out;
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
