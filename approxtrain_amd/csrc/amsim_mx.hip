@@ -13,6 +13,16 @@ namespace {
 
 constexpr int WG = 256;
 
+// Tensors that the last-level cache does not hold anyway go past it (AROUND), and leave it to what is read next.  In 16 bits
+// 16384 x 8192, 256 MB, take 57 us by rows so and 61 through it, both ways 67 and 74, a layer's conversion and product 583 and
+// 612; back, 47 and 74, and converted once more 104 and 147.  160 MB back take 30 and 32, but 67 and 62 with what reads
+// them; 128 MB by rows, where they may still be in the cache, 31 and 25.
+bool goes_around(double bytes) { return bytes >= 192 << 20; }
+template <bool AROUND> __device__ __forceinline__ v4i load_piece(const void *p)
+{
+    return AROUND ? __builtin_nontemporal_load((const v4i_anywhere *)p) : load16(p);
+}
+
 // ---- rows alone: four lanes share a block, and nothing has to be exchanged but its largest magnitude --------
 
 template <typename T> struct Eighth;  // 8 values of a block
@@ -22,7 +32,7 @@ template <> struct Eighth<_Float16> { _Float16 v[8]; };
 
 // A workgroup: 64 rows of a step of 128.  A wavefront's 64 lanes read four rows, 128 values of each; the scales of
 // the four fragments meet in LDS, as the bytes of one dword.
-template <typename T>
+template <typename T, bool AROUND>
 __global__ __launch_bounds__(WG) void rows_kernel(const T *x, int64_t rows, int64_t cols, int64_t row_stride, uint8_t *out)
 {
     __shared__ uint8_t scales[4][64];
@@ -37,7 +47,7 @@ __global__ __launch_bounds__(WG) void rows_kernel(const T *x, int64_t rows, int6
         if (row < rows && col + 8 <= cols) {
             v4i piece[sizeof(e[f]) / 16];
 #pragma unroll
-            for (int i = 0; i < (int)(sizeof(e[f]) / 16); ++i) piece[i] = load16((const char *)p + 16 * i);
+            for (int i = 0; i < (int)(sizeof(e[f]) / 16); ++i) piece[i] = load_piece<AROUND>((const char *)p + 16 * i);
             __builtin_memcpy(&e[f], piece, sizeof(e[f]));
         } else {
 #pragma unroll
@@ -81,7 +91,7 @@ template <typename T> struct Tile {
 
 template <typename T> __device__ __forceinline__ T masked(T v, T y) { return to_float(y) > 0.0f ? v : (T)0.0f; }
 
-template <typename T>
+template <bool AROUND, typename T>
 __device__ __forceinline__ void load_tile(Tile<T> &t, const MxConversion &j, int64_t row0, int64_t col0)
 {
     constexpr int PER_VEC = Tile<T>::PER_VEC, VECS = WIDE / PER_VEC;  // 16-byte pieces of a row of the tile
@@ -95,7 +105,7 @@ __device__ __forceinline__ void load_tile(Tile<T> &t, const MxConversion &j, int
         if (row0 + r >= j.rows) continue;
         const T *p = x + (row0 + r) * j.row_stride + col0 + c, *q = y + (row0 + r) * j.cols + col0 + c;
         if (col0 + c + PER_VEC <= j.cols) {
-            piece[i] = load16(p);
+            piece[i] = load_piece<AROUND>(p);
             if (y) keep[i] = load16(q);
         } else {
             T last[PER_VEC], also[PER_VEC];
@@ -135,11 +145,11 @@ template <typename T> __device__ __forceinline__ MxBlock<T> row_block(const Tile
     return b;
 }
 
-template <typename T> __device__ __forceinline__ void convert_tile(const MxConversion &j, int64_t row_tile, int64_t column_tile, uint8_t *lds)
+template <typename T, bool AROUND> __device__ __forceinline__ void convert_tile(const MxConversion &j, int64_t row_tile, int64_t column_tile, uint8_t *lds)
 {
     Tile<T> &t = *(Tile<T> *)lds;
     const int64_t row0 = row_tile * HIGH, col0 = column_tile * WIDE;
-    load_tile(t, j, row0, col0);
+    load_tile<AROUND>(t, j, row0, col0);
     __syncthreads();
     if (threadIdx.x < 128) {  // two fragments of 16 rows
         const int lane = threadIdx.x & 63;
@@ -174,21 +184,22 @@ template <typename T> __device__ __forceinline__ void convert_tile(const MxConve
 }
 
 // (types are branched on here: the two tensors of a forward pass may differ in theirs, and share a launch)
+template <bool AROUND>
 __global__ __launch_bounds__(WG) void tiles_kernel(TileJobs jobs)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[sizeof(Tile<float>)];
     const int which = (int64_t)blockIdx.x >= jobs.tiles[0];
     const MxConversion &j = jobs.job[which];
     const int64_t tile = (int64_t)blockIdx.x - (which ? jobs.tiles[0] : 0), columns = jobs.column_tiles[which];
-    if (j.dtype == AMSIM_DTYPE_F32) convert_tile<float>(j, tile / columns, tile % columns, lds);
-    else if (j.dtype == AMSIM_DTYPE_BF16) convert_tile<__bf16>(j, tile / columns, tile % columns, lds);
-    else convert_tile<_Float16>(j, tile / columns, tile % columns, lds);
+    if (j.dtype == AMSIM_DTYPE_F32) convert_tile<float, AROUND>(j, tile / columns, tile % columns, lds);
+    else if (j.dtype == AMSIM_DTYPE_BF16) convert_tile<__bf16, AROUND>(j, tile / columns, tile % columns, lds);
+    else convert_tile<_Float16, AROUND>(j, tile / columns, tile % columns, lds);
 }
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // A workgroup reads the 1 KB of a fragment's step and writes 16 rows of 128 values, eight per thread.
-template <typename T>
+template <typename T, bool AROUND>
 __global__ __launch_bounds__(WG) void dequantize_kernel(const uint8_t *q, int64_t rows, int64_t length, T *out)
 {
     const int64_t steps = mx_steps(length), f = (int64_t)blockIdx.x / steps, step = (int64_t)blockIdx.x % steps;
@@ -208,12 +219,27 @@ __global__ __launch_bounds__(WG) void dequantize_kernel(const uint8_t *q, int64_
         v4i piece[sizeof(v) / 16];
         __builtin_memcpy(piece, v, sizeof(v));
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(v) / 16); ++i) store16((char *)o + 16 * i, piece[i]);
+        for (int i = 0; i < (int)(sizeof(v) / 16); ++i) {
+            v4i_anywhere *to = (v4i_anywhere *)((char *)o + 16 * i);
+            if (AROUND) __builtin_nontemporal_store(piece[i], to);
+            else *to = piece[i];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (col + i < length) o[i] = v[i];
     }
+}
+
+template <typename T> void launch_rows(const MxConversion &j, unsigned blocks, hipStream_t stream)
+{
+    const auto kernel = goes_around((double)j.rows * (double)j.cols * sizeof(T)) ? rows_kernel<T, true> : rows_kernel<T, false>;
+    kernel<<<blocks, WG, 0, stream>>>((const T *)j.x, j.rows, j.cols, j.row_stride, j.by_rows);
+}
+template <typename T> void launch_dequantize(const uint8_t *q, int64_t rows, int64_t length, void *out, unsigned blocks, hipStream_t stream)
+{
+    const auto kernel = goes_around((double)rows * (double)length * sizeof(T)) ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
+    kernel<<<blocks, WG, 0, stream>>>(q, rows, length, (T *)out);
 }
 
 }  // namespace
@@ -224,18 +250,17 @@ int mx_convert(const MxConversion *jobs, int count, hipStream_t stream)
         const MxConversion &j = jobs[0];
         const int64_t blocks = mx_steps(j.cols) * ceil_div64(j.rows, 64);
         if (blocks >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
-        const unsigned n = (unsigned)blocks;
-        uint8_t *out = (uint8_t *)j.by_rows;
         switch (j.dtype) {
-        case AMSIM_DTYPE_F32: rows_kernel<float><<<n, WG, 0, stream>>>((const float *)j.x, j.rows, j.cols, j.row_stride, out); break;
-        case AMSIM_DTYPE_BF16: rows_kernel<__bf16><<<n, WG, 0, stream>>>((const __bf16 *)j.x, j.rows, j.cols, j.row_stride, out); break;
-        default: rows_kernel<_Float16><<<n, WG, 0, stream>>>((const _Float16 *)j.x, j.rows, j.cols, j.row_stride, out); break;
+        case AMSIM_DTYPE_F32: launch_rows<float>(j, (unsigned)blocks, stream); break;
+        case AMSIM_DTYPE_BF16: launch_rows<__bf16>(j, (unsigned)blocks, stream); break;
+        default: launch_rows<_Float16>(j, (unsigned)blocks, stream); break;
         }
         AMSIM_HIP_CHECK(hipGetLastError());
         return AMSIM_OK;
     }
     TileJobs t{};
     int64_t tiles = 0;
+    double bytes = 0;
     for (int i = 0; i < count; ++i) {
         const MxConversion &j = jobs[i];
         t.job[i] = j;
@@ -243,9 +268,11 @@ int mx_convert(const MxConversion *jobs, int count, hipStream_t stream)
         // (down the columns the last step is filled up with zeros)
         const int64_t row_tiles = j.by_columns ? mx_steps(j.rows) * (128 / HIGH) : ceil_div64(j.rows, HIGH);
         tiles += t.tiles[i] = row_tiles * t.column_tiles[i];
+        bytes += (double)j.rows * (double)j.cols * element_bytes(j.dtype);
     }
     if (tiles >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
-    tiles_kernel<<<(unsigned)tiles, WG, 0, stream>>>(t);
+    const auto kernel = goes_around(bytes) ? tiles_kernel<true> : tiles_kernel<false>;
+    kernel<<<(unsigned)tiles, WG, 0, stream>>>(t);
     AMSIM_HIP_CHECK(hipGetLastError());
     return AMSIM_OK;
 }
@@ -288,9 +315,9 @@ int amsim_mxfp4_dequantize(const void *q, int64_t rows, int64_t length, int dtyp
     hipStream_t s = (hipStream_t)stream;
     const uint8_t *p = (const uint8_t *)q;
     switch (dtype) {
-    case AMSIM_DTYPE_F32: dequantize_kernel<float><<<(unsigned)blocks, WG, 0, s>>>(p, rows, length, (float *)out); break;
-    case AMSIM_DTYPE_BF16: dequantize_kernel<__bf16><<<(unsigned)blocks, WG, 0, s>>>(p, rows, length, (__bf16 *)out); break;
-    default: dequantize_kernel<_Float16><<<(unsigned)blocks, WG, 0, s>>>(p, rows, length, (_Float16 *)out); break;
+    case AMSIM_DTYPE_F32: launch_dequantize<float>(p, rows, length, out, (unsigned)blocks, s); break;
+    case AMSIM_DTYPE_BF16: launch_dequantize<__bf16>(p, rows, length, out, (unsigned)blocks, s); break;
+    default: launch_dequantize<_Float16>(p, rows, length, out, (unsigned)blocks, s); break;
     }
     AMSIM_HIP_CHECK(hipGetLastError());
     return AMSIM_OK;

@@ -275,6 +275,22 @@ def test_training_step_in_a_graph():
             assert torch.equal(g, e)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tensors_larger_than_the_cache(dtype):
+    """More than 192 MB: every value as pieces of the tensor convert alone."""
+    rows, cols = (1700 if dtype == "f32" else 3300), 32003
+    x = torch.empty((rows, cols), dtype=DTYPES[dtype], device="cuda")
+    x.normal_(generator=torch.Generator(device="cuda").manual_seed(3))
+    q = functors.mxfp4_quantize(x)
+    r, c = functors.mxfp4_quantize_both(x)
+    got, both, columns = q.dequantize(x.dtype), r.dequantize(x.dtype), c.dequantize(x.dtype)
+    assert torch.equal(got, both)
+    for first in range(0, rows, 600):
+        assert torch.equal(got[first:first + 600], functors.mxfp4_quantize(x[first:first + 600]).dequantize(x.dtype))
+    for first in range(0, cols, 8000):
+        assert torch.equal(columns[first:first + 8000], functors.mxfp4_quantize(x[:, first:first + 8000], axis=0).dequantize(x.dtype))
+
+
 def test_operands_past_32_bit_offsets():
     """More than 2^32 values in one tensor: its last rows and columns convert as they do alone."""
     rows, cols = 70001, 65536
