@@ -44,6 +44,16 @@ inline bool mx_extents_fit(int64_t rows, int64_t length)
     return rows >= 0 && length >= 0 && rows < (1ll << 31) && length < (1ll << 31) && (double)rows * (double)length <= 35184372088832.0;
 }
 
+// Whether a tensor of so many bytes is read for conversion, or written, past the last-level cache: it would not be there when
+// it is read next, and keeps out what is.  In 16 bits, past the cache and through it, us:
+//   16384 x 8192 (256 MB)  by rows 57 and 61, both ways 67 and 74; back 47 and 74, and converted again 104 and 147
+//                          product of a reduction of 8192 483 and 530, of 1024 97 and 98, and converted 153 and 191
+//   14336 x 8192 (224 MB)  product 82 and 87, and converted 134 and 133, and copied 175 and 190
+//   208 MB                 product 78 and 81, and converted 126 and 122
+//   160 MB                 back 30 and 32, and converted 67 and 62
+//   64 MB                  product 30 and 29, and converted 47 and 43
+inline bool mx_goes_around(double bytes) { return bytes >= 224 << 20; }
+
 inline int element_bytes(int dtype) { return dtype == AMSIM_DTYPE_F32 ? 4 : 2; }
 inline bool known_dtype(int dtype) { return dtype == AMSIM_DTYPE_F32 || dtype == AMSIM_DTYPE_BF16 || dtype == AMSIM_DTYPE_F16; }
 

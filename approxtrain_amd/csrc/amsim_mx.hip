@@ -13,11 +13,7 @@ namespace {
 
 constexpr int WG = 256;
 
-// Tensors that the last-level cache does not hold anyway go past it (AROUND), and leave it to what is read next.  In 16 bits
-// 16384 x 8192, 256 MB, take 57 us by rows so and 61 through it, both ways 67 and 74, a layer's conversion and product 583 and
-// 612; back, 47 and 74, and converted once more 104 and 147.  160 MB back take 30 and 32, but 67 and 62 with what reads
-// them; 128 MB by rows, where they may still be in the cache, 31 and 25.
-bool goes_around(double bytes) { return bytes >= 192 << 20; }
+// (AROUND: see mx_goes_around)
 template <bool AROUND> __device__ __forceinline__ v4i load_piece(const void *p)
 {
     return AROUND ? __builtin_nontemporal_load((const v4i_anywhere *)p) : load16(p);
@@ -233,12 +229,12 @@ __global__ __launch_bounds__(WG) void dequantize_kernel(const uint8_t *q, int64_
 
 template <typename T> void launch_rows(const MxConversion &j, unsigned blocks, hipStream_t stream)
 {
-    const auto kernel = goes_around((double)j.rows * (double)j.cols * sizeof(T)) ? rows_kernel<T, true> : rows_kernel<T, false>;
+    const auto kernel = mx_goes_around((double)j.rows * (double)j.cols * sizeof(T)) ? rows_kernel<T, true> : rows_kernel<T, false>;
     kernel<<<blocks, WG, 0, stream>>>((const T *)j.x, j.rows, j.cols, j.row_stride, j.by_rows);
 }
 template <typename T> void launch_dequantize(const uint8_t *q, int64_t rows, int64_t length, void *out, unsigned blocks, hipStream_t stream)
 {
-    const auto kernel = goes_around((double)rows * (double)length * sizeof(T)) ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
+    const auto kernel = mx_goes_around((double)rows * (double)length * sizeof(T)) ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
     kernel<<<blocks, WG, 0, stream>>>(q, rows, length, (T *)out);
 }
 
@@ -271,7 +267,7 @@ int mx_convert(const MxConversion *jobs, int count, hipStream_t stream)
         bytes += (double)j.rows * (double)j.cols * element_bytes(j.dtype);
     }
     if (tiles >= (1ll << 24)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more tiles than one launch takes");
-    const auto kernel = goes_around(bytes) ? tiles_kernel<true> : tiles_kernel<false>;
+    const auto kernel = mx_goes_around(bytes) ? tiles_kernel<true> : tiles_kernel<false>;
     kernel<<<(unsigned)tiles, WG, 0, stream>>>(t);
     AMSIM_HIP_CHECK(hipGetLastError());
     return AMSIM_OK;

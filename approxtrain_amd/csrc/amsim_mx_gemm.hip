@@ -35,6 +35,7 @@ struct GemmArgs {
     void *out;
     unsigned tiles_m, tiles_n;  // (below 2^24 together)
     int splits;
+    int around;              // large results go past the last-level cache
     float *partial;          // [splits][m][n] where the reduction is split, else null
 };
 // One or two products of a launch: a training step's backward pass has two that do not wait for each other.
@@ -136,7 +137,7 @@ template <typename T, int FM, int FN> struct Rows {
 };
 template <typename T, int FM, int FN>
 __device__ __forceinline__ void store_tile(uint8_t *lds, const v4f (&acc)[FM][FN], const float (&bias)[FN][4], int act, T *out, int64_t m0,
-                                           int64_t n0, int64_t M, int64_t N)
+                                           int64_t n0, int64_t M, int64_t N, bool around)
 {
     using R = Rows<T, FM, FN>;
     const int lane = threadIdx.x & 63, columns = (int)min<int64_t>(R::COLUMNS, N - n0);
@@ -158,12 +159,19 @@ __device__ __forceinline__ void store_tile(uint8_t *lds, const v4f (&acc)[FM][FN
         const int c = lane % PIECES * PIECE;
         const uint8_t *from = lds + lane / PIECES * R::STRIDE + c * sizeof(T);
         T *to = o + lane / PIECES * N + c;
-        if (c + PIECE <= columns) {  // (rows may start on any element: the hardware takes such pieces too)
+        // (rows may start on any element: the hardware takes such pieces too)
+        auto pieces = [&](auto past) {
 #pragma unroll 8
             for (int r = lane / PIECES; r < 16 * R::AT_ONCE; r += DOWN, from += DOWN * R::STRIDE, to += DOWN * N) {
                 const v4i v = *(const v4i *)from;
-                if (r < rows) store16(to, v);
+                if (r >= rows) continue;
+                if constexpr (past.value) __builtin_nontemporal_store(v, (v4i_anywhere *)to);
+                else store16(to, v);
             }
+        };
+        if (c + PIECE <= columns) {
+            if (around) pieces(std::true_type{});
+            else pieces(std::false_type{});
         } else if (c < columns) {
             for (int r = lane / PIECES; r < rows; r += DOWN, from += DOWN * R::STRIDE, to += DOWN * N)
                 for (int i = 0; i < columns - c; ++i) to[i] = ((const T *)from)[i];
@@ -311,7 +319,8 @@ __global__ __launch_bounds__(64 * WM * WN, RESIDENT) void gemm_kernel(GemmJobs j
         }
     auto store = [&](auto zero, auto *out) {
         using T = decltype(zero);
-        store_tile<T, FM, FN>(lds + wave * Rows<T, FM, FN>::BYTES, acc, bias, whole ? g.act : AMSIM_ACT_NONE, out, m0, n0, g.a.rows, g.b.rows);
+        store_tile<T, FM, FN>(lds + wave * Rows<T, FM, FN>::BYTES, acc, bias, whole ? g.act : AMSIM_ACT_NONE, out, m0, n0, g.a.rows, g.b.rows,
+                              whole && g.around);
     };
     if (!whole || g.out_dtype == AMSIM_DTYPE_F32) store(0.0f, whole ? (float *)g.out : g.partial + split * g.a.rows * g.b.rows);
     else if (g.out_dtype == AMSIM_DTYPE_BF16) store((__bf16)0.0f, (__bf16 *)g.out);
@@ -704,7 +713,8 @@ int products(const Product *list, int count, const float *sums, int64_t parts, i
             const Product &q = list[which[j]];
             const auto &o = p.of[j];
             jobs.job[j] = GemmArgs{q.a, q.b, mx_steps(q.k), o.steps_per_split, q.bias, q.bias_dtype, q.act, q.out_dtype, q.out, (unsigned)o.tiles_m,
-                                   (unsigned)o.tiles_n, (int)o.splits, o.splits > 1 ? (float *)partial : nullptr};
+                                   (unsigned)o.tiles_n, (int)o.splits, mx_goes_around((double)t[j].m * (double)t[j].n * element_bytes(q.out_dtype)),
+                                   o.splits > 1 ? (float *)partial : nullptr};
             partial += partial_bytes(t[j], o.splits);
             if (j == 0) jobs.blocks = (unsigned)std::min<int64_t>(o.tiles_m * o.tiles_n * o.splits, 1 << 30);
             blocks += o.tiles_m * o.tiles_n * o.splits;

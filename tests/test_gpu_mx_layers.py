@@ -183,6 +183,20 @@ def test_products_in_each_tile(m, n, k):
     assert bool(((got - z).abs() <= tol * 1.01 + 2.0 ** -8 * z.abs()).all())
 
 
+@pytest.mark.parametrize("dtype,m,n", [(torch.float32, 7300, 8201), (torch.bfloat16, 14500, 8203), (torch.float16, 440, 270001)])
+def test_results_larger_than_the_cache(dtype, m, n):
+    """More than 224 MB of results, the last rows' and columns' tiles not full."""
+    k = 200
+    x, w, bias = torch.randn(m, k, device="cuda"), torch.randn(k, n, device="cuda"), torch.randn(n, device="cuda")
+    a, c = functors.mxfp4_quantize(x), functors.mxfp4_quantize(w, axis=0)
+    got = functors.mxfp4_matmul(a, c, bias, "relu", dtype=dtype)
+    left, right = a.dequantize(torch.float32).double(), c.dequantize(torch.float32).double().t()
+    for rows in torch.arange(m, device="cuda").split(500):
+        want, size = torch.relu(left[rows] @ right + bias.double()), left[rows].abs() @ right.abs() + bias.double().abs()
+        tol = (-(-k // 32) + 19) * 2.0 ** -23 * size + want * torch.finfo(dtype).eps / 2 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        assert bool(((got[rows].double() - want).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_optimizer_steps_as_the_function_does_and_goes_on_from_a_saved_state(bits):
     torch.manual_seed(3)
