@@ -9,7 +9,7 @@
 // all tensors lie in one buffer, each tensor from a multiple of 256 elements on, so that no table has to be
 // sent to the device ahead of the kernel.  A wavefront updates one block of 256 and ends (four one after the other
 // took 83 us for 25M elements in 161 tensors with 8-bit moments, one 78.5), and finds its tensor in two loads (a
-// binary search over the arguments took 502 us where this takes 441: 101M elements, 16-bit gradients, 5.9 TB/s).
+// binary search over the arguments took 502 us where this took 441, now 437: 101M elements, 16-bit gradients, 6.0 TB/s).
 // With 8-bit moments the arithmetic has to stay out of memory's way: the full divisions and roots of the
 // language and shuffles through LDS kept the vector units busy for 91% of 97 us, what is here takes 70 (5.8 TB/s).
 //
@@ -21,6 +21,7 @@
 #include "amsim_mx.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace amsim {
 
@@ -124,12 +125,29 @@ template <bool ROOTS> __device__ __forceinline__ uint32_t encode4(const float (&
     return w;
 }
 
+// Past the last-level cache, or through it.  Where all moments together are more than it holds nothing is there when a step
+// comes to it, and nothing it leaves there is read before it is displaced (us, past and through): 101M elements of 32-bit
+// moments and 16-bit gradients 449 and 491, beside other work on 512 MB 450 and 509, 112M of 8-bit moments 322 and 358, the
+// parameters read behind it 280 and 341 (that reading taken off); 28M of 32 bits, 224 MB, 144 and 147, beside others 145 and
+// 170.  Smaller states may still be there.
+template <bool AROUND, typename V> __device__ __forceinline__ V get(const void *p)
+{
+    return AROUND ? __builtin_nontemporal_load((const V *)p) : *(const V *)p;
+}
+template <bool AROUND, typename V> __device__ __forceinline__ void put(void *p, V v)
+{
+    if constexpr (AROUND) __builtin_nontemporal_store(v, (V *)p);
+    else *(V *)p = v;
+}
+
 // four neighbouring elements, of which `count` exist
-template <typename T> __device__ __forceinline__ void load4(const T *p, int count, float (&v)[4])
+template <typename T> using Quad = std::conditional_t<sizeof(T) == 4, v4i, v2i>;
+template <bool AROUND, typename T> __device__ __forceinline__ void load4(const T *p, int count, float (&v)[4])
 {
     T t[4] = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
     if (count == 4 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0) {
-        __builtin_memcpy(t, __builtin_assume_aligned(p, 4 * sizeof(T)), sizeof(t));
+        const Quad<T> q = get<AROUND, Quad<T>>(p);
+        __builtin_memcpy(t, &q, sizeof(t));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -138,13 +156,15 @@ template <typename T> __device__ __forceinline__ void load4(const T *p, int coun
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = to_float(t[i]);
 }
-template <typename T> __device__ __forceinline__ void store4(T *p, int count, const float (&v)[4])
+template <bool AROUND, typename T> __device__ __forceinline__ void store4(T *p, int count, const float (&v)[4])
 {
     T t[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) t[i] = from_float<T>(v[i]);
     if (count == 4 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0) {
-        __builtin_memcpy(__builtin_assume_aligned(p, 4 * sizeof(T)), t, sizeof(t));
+        Quad<T> q;
+        __builtin_memcpy(&q, t, sizeof(t));
+        put<AROUND>(p, q);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -152,7 +172,7 @@ template <typename T> __device__ __forceinline__ void store4(T *p, int count, co
     }
 }
 
-template <typename P, typename G, bool BITS8>
+template <typename P, typename G, bool BITS8, bool AROUND>
 __global__ __launch_bounds__(WG) void adamw_kernel(AdamWArgs a)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -168,17 +188,17 @@ __global__ __launch_bounds__(WG) void adamw_kernel(AdamWArgs a)
     const int64_t i = b * BLOCK + lane * 4, s = (before + b) * BLOCK + lane * 4;
     const int count = (int)(t.n - i >= 4 ? 4 : t.n - i > 0 ? t.n - i : 0);
     float p[4], g[4], m[4], v[4];
-    load4((const P *)t.p + i, count, p);
-    load4((const G *)t.g + i, count, g);
+    load4<AROUND>((const P *)t.p + i, count, p);
+    load4<AROUND>((const G *)t.g + i, count, g);
     uint32_t mc = 0, rc = 0;
     float ms = 0, rs = 0;
     if (BITS8) {
-        mc = *(const uint32_t *)((const uint8_t *)a.m + s);
-        rc = *(const uint32_t *)((const uint8_t *)a.v + s);
+        mc = get<AROUND, uint32_t>((const uint8_t *)a.m + s);
+        rc = get<AROUND, uint32_t>((const uint8_t *)a.v + s);
         ms = a.m_scale[before + b];
         rs = a.v_scale[before + b];
     } else {
-        const v4f mv = *(const v4f *)((const float *)a.m + s), vv = *(const v4f *)((const float *)a.v + s);
+        const v4f mv = get<AROUND, v4f>((const float *)a.m + s), vv = get<AROUND, v4f>((const float *)a.v + s);
 #pragma unroll
         for (int e = 0; e < 4; ++e) m[e] = mv[e], v[e] = vv[e];
     }
@@ -197,7 +217,7 @@ __global__ __launch_bounds__(WG) void adamw_kernel(AdamWArgs a)
         const float denominator = r[e] * a.inv_root2 + a.eps;
         p[e] = p[e] * a.keep - (m[e] / denominator) * a.step_size;
     }
-    store4((P *)t.p + i, count, p);
+    store4<AROUND>((P *)t.p + i, count, p);
     if (BITS8) {
         uint32_t mx = 0, rx = 0;
 #pragma unroll
@@ -210,8 +230,8 @@ __global__ __launch_bounds__(WG) void adamw_kernel(AdamWArgs a)
         rs = wave_max(__uint_as_float(rx));
         mc = encode4<false>(m, ms);
         rc = encode4<true>(r, rs);
-        *(uint32_t *)((uint8_t *)a.m + s) = mc;
-        *(uint32_t *)((uint8_t *)a.v + s) = rc;
+        put<AROUND>((uint8_t *)a.m + s, mc);
+        put<AROUND>((uint8_t *)a.v + s, rc);
         if (lane == 0) {
             a.m_scale[before + b] = ms;
             a.v_scale[before + b] = rs;
@@ -220,8 +240,8 @@ __global__ __launch_bounds__(WG) void adamw_kernel(AdamWArgs a)
         v4f mv, vv;
 #pragma unroll
         for (int e = 0; e < 4; ++e) mv[e] = e < count ? m[e] : 0.0f, vv[e] = e < count ? v[e] : 0.0f;
-        *(v4f *)((float *)a.m + s) = mv;
-        *(v4f *)((float *)a.v + s) = vv;
+        put<AROUND>((float *)a.m + s, mv);
+        put<AROUND>((float *)a.v + s, vv);
     }
 }
 
@@ -238,18 +258,18 @@ __global__ __launch_bounds__(WG) void state_values_kernel(const uint8_t *codes, 
     ((v4f *)out)[q] = v;
 }
 
-template <typename P, typename G> void launch_adamw(const AdamWArgs &a, int state_bits, hipStream_t stream)
+template <typename P, typename G> void launch_adamw(const AdamWArgs &a, int state_bits, bool around, hipStream_t stream)
 {
-    const unsigned chunks = (unsigned)a.first_chunk[a.count];
-    if (state_bits == 8) adamw_kernel<P, G, true><<<chunks, WG, 0, stream>>>(a);
-    else adamw_kernel<P, G, false><<<chunks, WG, 0, stream>>>(a);
+    const auto kernel = state_bits == 8 ? (around ? adamw_kernel<P, G, true, true> : adamw_kernel<P, G, true, false>)
+                                        : (around ? adamw_kernel<P, G, false, true> : adamw_kernel<P, G, false, false>);
+    kernel<<<(unsigned)a.first_chunk[a.count], WG, 0, stream>>>(a);
 }
-template <typename P> void launch_adamw_grad(const AdamWArgs &a, int grad_dtype, int state_bits, hipStream_t stream)
+template <typename P> void launch_adamw_grad(const AdamWArgs &a, int grad_dtype, int state_bits, bool around, hipStream_t stream)
 {
     switch (grad_dtype) {
-    case AMSIM_DTYPE_F32: launch_adamw<P, float>(a, state_bits, stream); break;
-    case AMSIM_DTYPE_BF16: launch_adamw<P, __bf16>(a, state_bits, stream); break;
-    default: launch_adamw<P, _Float16>(a, state_bits, stream); break;
+    case AMSIM_DTYPE_F32: launch_adamw<P, float>(a, state_bits, around, stream); break;
+    case AMSIM_DTYPE_BF16: launch_adamw<P, __bf16>(a, state_bits, around, stream); break;
+    default: launch_adamw<P, _Float16>(a, state_bits, around, stream); break;
     }
 }
 
@@ -291,6 +311,7 @@ int amsim_adamw_step(int count, void *const *params, const void *const *grads, c
     a.inv_root2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
     a.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
     a.eps = (float)eps;
+    const bool around = mx_goes_around((double)all_blocks * BLOCK * (state_bits == 8 ? 2 : 8));
     int64_t block = 0;
     for (int i = 0; i < count;) {
         a.count = 0;
@@ -311,9 +332,9 @@ int amsim_adamw_step(int count, void *const *params, const void *const *grads, c
         a.first_chunk[a.count] = (int)here;
         if (a.count == 0) continue;
         switch (param_dtype) {
-        case AMSIM_DTYPE_F32: launch_adamw_grad<float>(a, grad_dtype, state_bits, (hipStream_t)stream); break;
-        case AMSIM_DTYPE_BF16: launch_adamw_grad<__bf16>(a, grad_dtype, state_bits, (hipStream_t)stream); break;
-        default: launch_adamw_grad<_Float16>(a, grad_dtype, state_bits, (hipStream_t)stream); break;
+        case AMSIM_DTYPE_F32: launch_adamw_grad<float>(a, grad_dtype, state_bits, around, (hipStream_t)stream); break;
+        case AMSIM_DTYPE_BF16: launch_adamw_grad<__bf16>(a, grad_dtype, state_bits, around, (hipStream_t)stream); break;
+        default: launch_adamw_grad<_Float16>(a, grad_dtype, state_bits, around, (hipStream_t)stream); break;
         }
         AMSIM_HIP_CHECK(hipGetLastError());
     }

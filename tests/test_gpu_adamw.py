@@ -169,3 +169,24 @@ def test_refusals():
             functors.adamw_step(state, [g], **hyper)
     functors.adamw_step(state, [None], 1)
     assert not p.any() and not state.m.any()
+
+
+@pytest.mark.parametrize("bits,dtype,sizes", [(32, torch.float32, (15_000_001, 14_999_998)), (32, torch.bfloat16, (15_000_001, 14_999_998)),
+                                              (8, torch.bfloat16, (60_000_001, 1, 60_000_002))])
+def test_moments_larger_than_the_cache(bits, dtype, sizes):
+    """More than 224 MB of moments: every tensor as it steps alone, on addresses that four elements do and do not share."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    whole = [torch.empty(n + 1, device="cuda", dtype=dtype).normal_(generator=gen) for n in sizes]
+    params = [t[i % 2:i % 2 + n] for i, (t, n) in enumerate(zip(whole, sizes))]
+    alone = [p.clone() for p in params]
+    state, states = functors.AdamWState(params, bits), [functors.AdamWState([p], bits) for p in alone]
+    for step in (1, 2):
+        grads = [torch.empty(n, device="cuda", dtype=dtype).normal_(generator=gen) for n in sizes]
+        functors.adamw_step(state, grads, step)
+        for s, g in zip(states, grads):
+            functors.adamw_step(s, [g], step)
+    for p, q in zip(params, alone):
+        assert torch.equal(p, q)
+    assert torch.equal(state.m, torch.cat([s.m for s in states])) and torch.equal(state.v, torch.cat([s.v for s in states]))
+    if bits == 8:
+        assert torch.equal(state.m_scale, torch.cat([s.m_scale for s in states])) and torch.equal(state.v_scale, torch.cat([s.v_scale for s in states]))
