@@ -486,6 +486,14 @@ class AdamWState:
         scales = at // self.BLOCK if state_bits == 8 else 0
         self.m_scale, self.v_scale = (torch.zeros if scales else torch.empty)((2, scales), device=device).unbind()
 
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_list"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.device_index = self.params[0].get_device()
+        self._list = _native().TensorList(self.sizes, self.dtype, self.device_index)
+
     def first_moments(self):
         """The values of the first moments in the buffer's order, float32."""
         return self.m if self.state_bits == 32 else _native().state_values(self.m, self.m_scale, False)

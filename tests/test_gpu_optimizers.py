@@ -1,4 +1,7 @@
 """The optimizer class on the device: parameters that join late or miss gradients, against each stepped by itself."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -49,3 +52,22 @@ def test_late_gradients_against_torch():
     for p, q in zip(params, theirs):
         # either side rounds p and the update a dozen times a step, updates of at most 10 lr
         assert bool(((p - q).abs() <= 40 * 24 * 2.0 ** -24 * (q.abs() + 0.1)).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_copy_goes_on_as_its_original(bits):
+    params = parameters()
+    opt = AdamW(params, state_bits=bits)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    for p in params:
+        p.grad = torch.randn(p.shape, device="cuda", generator=gen).to(p.dtype)
+    opt.step()
+    for again in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        theirs = again.param_groups[0]["params"]
+        for p, q in zip(params, theirs):
+            assert p is not q and torch.equal(p, q)
+            p.grad = torch.randn(p.shape, device="cuda", generator=gen).to(p.dtype)
+            q.grad = p.grad.clone()
+        opt.step(), again.step()
+        for p, q in zip(params, theirs):
+            assert torch.equal(p, q)

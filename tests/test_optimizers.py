@@ -1,5 +1,8 @@
 """The optimizer class's host side: which parameters it steps, by which step number, what it saves.  The native calls are
 replaced by the same formulas in 64 bits on host tensors."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -148,3 +151,16 @@ def test_states_of_other_parameters_are_refused_and_change_nothing():
         AdamW([{"params": mine[:2]}, {"params": mine[2:]}]).load_state_dict(saved)
     with pytest.raises(ValueError, match="bits"):
         AdamW(mine, state_bits=8).load_state_dict(saved)
+
+
+def test_an_optimizer_that_has_stepped_can_be_copied_and_pickled():
+    mine, theirs, opt, other = pair()
+    step(mine, theirs, opt, other, 1, {0, 1, 2})
+    for again in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt)), copy.deepcopy(opt)):
+        params, (twin, reference) = again.param_groups[0]["params"], copy.deepcopy([theirs, other])
+        assert params[0] is not mine[0] and again.param_groups[0]["buckets"][0].params[0] is params[0]
+        for seed in (2, 3):
+            step(params, twin, again, reference, seed, {0, 1, 2, 3})
+        assert_same(params, twin)
+    step(mine, theirs, opt, other, 4, {1, 3})
+    assert_same(mine, theirs)
