@@ -81,6 +81,8 @@ class AdamW(torch.optim.Optimizer):
 
     def state_dict(self):
         """Hyperparameters and moments of every group, with the parameters' places in it and their numbers of steps."""
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
         groups = []
         for group in self.param_groups:
             place = {id(p): i for i, p in enumerate(group["params"])}
@@ -88,7 +90,11 @@ class AdamW(torch.optim.Optimizer):
                         "m": s.m, "v": s.v, "m_scale": s.m_scale, "v_scale": s.v_scale} for s in self._buckets(group)]
             saved = {k: v for k, v in group.items() if k not in self._NOT_SAVED}
             groups.append({**saved, "moments": moments})
-        return {"groups": groups}
+        state_dict = {"groups": groups}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
+        return state_dict
 
     def _places(self, group, saved):
         """Of each of the saved moments the parameters' places in the group, checked against it."""
@@ -110,6 +116,10 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
+        state_dict = dict(state_dict)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         groups = state_dict["groups"]
         if len(groups) != len(self.param_groups):
             raise ValueError("the saved state has another number of parameter groups")
@@ -130,3 +140,5 @@ class AdamW(torch.optim.Optimizer):
                 for k in ("m", "v", "m_scale", "v_scale"):
                     getattr(s, k).copy_(moments[k])
             group.update({k: v for k, v in saved.items() if k != "moments"})
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)

@@ -164,3 +164,24 @@ def test_an_optimizer_that_has_stepped_can_be_copied_and_pickled():
         assert_same(params, twin)
     step(mine, theirs, opt, other, 4, {1, 3})
     assert_same(mine, theirs)
+
+
+def test_registered_hooks_run_around_saving_and_loading():
+    mine, theirs, opt, other = pair()
+    step(mine, theirs, opt, other, 1, {0, 1, 2, 3})
+    seen = []
+    opt.register_state_dict_pre_hook(lambda o: seen.append(("saving", o is opt)))
+    opt.register_state_dict_post_hook(lambda o, d: {**d, "note": 5})
+    saved = opt.state_dict()
+    assert saved["note"] == 5 and seen == [("saving", True)]
+    target = AdamW(mine, lr=1.0)
+
+    def unwrap(o, d):
+        seen.append(d["note"])
+        d["note"] = None  # (a hook may change what it is given: a shallow copy)
+        return {"groups": d["groups"]}
+
+    target.register_load_state_dict_pre_hook(unwrap)
+    target.register_load_state_dict_post_hook(lambda o: seen.append(o.param_groups[0]["lr"]))
+    target.load_state_dict(saved)
+    assert seen == [("saving", True), 5, HYPER["lr"]] and saved["note"] == 5
