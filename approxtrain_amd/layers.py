@@ -441,7 +441,9 @@ class densemx(nn.Module, _KerasLayerArgs):
 class packed_densemx(nn.Module):
     """A dense layer for inference: ``kernel`` ``[width, units]`` is converted to 4 bits once, the activations on
     the way (``functors.mxfp4_linear``).  Its outputs are those of the ``densemx`` layer it was packed from, up to the order
-    of the sums."""
+    of the sums.  The saved state holds units and width besides, which the weights' bytes do not tell."""
+
+    _version = 2  # of the saved state: 1 had no extents
 
     def __init__(self, kernel, bias=None, activation=None):
         super().__init__()
@@ -451,6 +453,22 @@ class packed_densemx(nn.Module):
         self.units, self.width = weights.shape
         self.register_buffer("weights", weights.data)
         self.register_buffer("bias", None if bias is None else bias.detach().clone())
+
+    def get_extra_state(self):
+        return torch.tensor([self.units, self.width])
+
+    def set_extra_state(self, state):
+        """(compared before anything is loaded)"""
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        key = prefix + "_extra_state"
+        extents = state_dict[key].tolist() if key in state_dict else [self.units, self.width]
+        if extents != [self.units, self.width]:
+            error_msgs.append(f"{prefix}weights are those of {extents[0]} units of width {extents[1]}, not of {self.units} of width {self.width}")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if (local_metadata.get("version") or 1) < 2 and key in missing_keys:
+            missing_keys.remove(key)
 
     def forward(self, inputs):
         act = _fusable(self.activation)
