@@ -17,6 +17,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
+#include <stdexcept>
 #include <string>
 #include <vector>
 
@@ -70,6 +71,14 @@ std::optional<Tensor> maybe_tensor(py::handle h, const char *name)
 {
     if (h.is_none()) return std::nullopt;
     return tensor(h, name);
+}
+
+// for calls that are no part of a graph: what would need a derivative is refused, and not cut off without a word
+void no_derivative(const Tensor &t, const char *name, const char *call)
+{
+    if (at::GradMode::is_enabled() && t.requires_grad())
+        throw std::runtime_error(std::string(call) + " has no gradient and " + name + " requires one: train through linearmx, or call it under torch.no_grad()");
+    if (t._fw_grad(0).defined()) type_error(std::string(call) + " has no forward-mode derivative");
 }
 
 void *stream() { return c10::hip::getCurrentHIPStream().stream(); }
@@ -179,10 +188,12 @@ Tensor dequantize(py::handle data, int64_t rows, int64_t length, py::handle dtyp
 
 Tensor matmul(py::handle a_data, int64_t m, py::handle b_data, int64_t n, int64_t k, py::handle bias, int act, py::handle dtype)
 {
+    const std::optional<Tensor> given_bias = maybe_tensor(bias, "bias");
+    if (given_bias) no_derivative(*given_bias, "bias", "mxfp4_matmul");
     const Tensor &a = operand(tensor(a_data, "a"), m, k, "a"), &b = operand(tensor(b_data, "b"), n, k, "b");
     at::ScalarType t;
     const int code = result_code(dtype, t);
-    const Bias add = bias_of(maybe_tensor(bias, "bias"), n, a);
+    const Bias add = bias_of(given_bias, n, a);
     Tensor out = matrix(m, n, a, t), ws;
     const size_t need = amsim_mxfp4_matmul_workspace_bytes(m, n, k);
     if (need) ws = bytes((int64_t)need, a);
@@ -193,6 +204,9 @@ Tensor matmul(py::handle a_data, int64_t m, py::handle b_data, int64_t n, int64_
 Tensor linear(py::handle given, py::handle data, int64_t n, int64_t k, py::handle bias, int act)
 {
     const Tensor &x = tensor(given, "x");
+    const std::optional<Tensor> given_bias = maybe_tensor(bias, "bias");
+    no_derivative(x, "x", "mxfp4_linear");
+    if (given_bias) no_derivative(*given_bias, "bias", "mxfp4_linear");
     if (x.dim() < 1 || x.size(-1) != k) value_error("x's last axis must have the weights' length");
     const Tensor &w = operand(tensor(data, "weights"), n, k, "weights");
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
@@ -203,7 +217,7 @@ Tensor linear(py::handle given, py::handle data, int64_t n, int64_t k, py::handl
         return at::empty(shape, x.options());
     }
     const Source s = row_source(flat, "x");
-    const Bias add = bias_of(maybe_tensor(bias, "bias"), n, s.t);
+    const Bias add = bias_of(given_bias, n, s.t);
     Tensor out = matrix(s.rows, n, s.t, s.t.scalar_type()), ws;
     const size_t need = amsim_mxfp4_linear_workspace_bytes(s.rows, n, k);
     if (need) ws = bytes((int64_t)need, s.t);

@@ -425,7 +425,7 @@ def mxfp4_dequantize(q, dtype=torch.float32):
 
 def mxfp4_matmul(a, b, bias=None, activation=None, dtype=torch.float32):
     """``activation(a . b^T + bias)`` of two MXFP4 operands of one length: ``[a.rows, b.rows]``, summed in 32
-    bits and rounded to ``dtype`` once."""
+    bits and rounded to ``dtype`` once.  (No gradient: a bias that requires one is refused outside ``torch.no_grad``.)"""
     _mx_operand(a, "a"), _mx_operand(b, "b")
     if a.length != b.length:
         raise ValueError("the operands' lengths differ")
@@ -435,7 +435,8 @@ def mxfp4_matmul(a, b, bias=None, activation=None, dtype=torch.float32):
 def mxfp4_linear(x, weights, bias=None, activation=None):
     """``activation(Q(x) . weights^T + bias)`` for activations ``x`` ``[..., length]``, which are quantised on the
     way, and weights that lie in MXFP4: ``mxfp4_quantize(kernel, axis=0)`` of a ``[length, units]`` kernel.  The
-    result has x's type."""
+    result has x's type.  (No gradient: x or a bias that require one are refused outside ``torch.no_grad``; ``math_ops.linearmx``
+    trains.)"""
     w = _mx_operand(weights, "weights")
     return _native().linear(x, w.data, w.rows, w.length, bias, _activation(activation))
 

@@ -441,7 +441,7 @@ class densemx(nn.Module, _KerasLayerArgs):
 class packed_densemx(nn.Module):
     """A dense layer for inference: ``kernel`` ``[width, units]`` is converted to 4 bits once, the activations on
     the way (``functors.mxfp4_linear``).  Its outputs are those of the ``densemx`` layer it was packed from, up to the order
-    of the sums.  The saved state holds units and width besides, which the weights' bytes do not tell."""
+    of the sums.  Inputs that require gradients are refused outside ``torch.no_grad``.  The saved state holds units and width besides, which the weights' bytes do not tell."""
 
     _version = 2  # of the saved state: 1 had no extents
 

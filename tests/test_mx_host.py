@@ -112,3 +112,21 @@ def test_tensors_that_are_not_on_a_device_are_refused():
         math_ops.linearmx(x, torch.zeros(5, 4))
     with pytest.raises(ValueError, match="no tensors"):
         functors.AdamWState([])
+
+
+def test_calls_without_a_derivative_refuse_what_would_need_one():
+    """They came back without a graph, and a branch behind them lost its gradient without a word."""
+    x, b = torch.zeros(4, 4), torch.zeros(4)
+    w = functors.MXTensor(torch.zeros(1280, dtype=torch.uint8), 4, 4)
+    xg, bg = x.clone().requires_grad_(), b.clone().requires_grad_()
+    calls = (lambda x, b: functors.mxfp4_linear(x, w, b), lambda x, b: functors.mxfp4_matmul(w, w, b))
+    for call, args in ((calls[0], (xg, b)), (calls[0], (x, bg)), (calls[0], (xg * 2, None)), (calls[1], (None, bg))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(*args)
+        with torch.no_grad(), pytest.raises(TypeError, match="device memory"):
+            call(*args)
+    with torch.autograd.forward_ad.dual_level():
+        for call, args in ((calls[0], (torch.autograd.forward_ad.make_dual(x, x), None)), (calls[0], (x, torch.autograd.forward_ad.make_dual(b, b))),
+                           (calls[1], (None, torch.autograd.forward_ad.make_dual(b, b)))):
+            with pytest.raises(TypeError, match="forward-mode"):
+                call(*args)
