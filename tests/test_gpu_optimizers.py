@@ -62,7 +62,8 @@ def test_a_copy_goes_on_as_its_original(bits):
     for p in params:
         p.grad = torch.randn(p.shape, device="cuda", generator=gen).to(p.dtype)
     opt.step()
-    for again in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+    for make in (copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))):
+        again = make(opt)
         theirs = again.param_groups[0]["params"]
         for p, q in zip(params, theirs):
             assert p is not q and torch.equal(p, q)
