@@ -10,8 +10,8 @@
 // lines wherever they come from, and no kernel has an edge in its loads but for the last fragment of rows:
 //   codes   [rows / 16][length / 128][64 lanes][16 bytes]   lane = 16 * (block of 32 within the 128) + row % 16
 //   scales  [rows / 64][length / 128][64 lanes][4 bytes]    byte = (row / 16) % 4
-// with extents rounded up, the scales right behind the codes.  Values beyond the length are zeros.  Rows beyond
-// the last one hold zeros up to the next 16, and nothing that a product reads into a result after that.
+// with extents rounded up, the scales right behind the codes.  Values beyond the length are zeros, and so are rows
+// beyond the last one and their scales: equal values are equal bytes.
 #ifndef AMSIM_MX_H_
 #define AMSIM_MX_H_
 

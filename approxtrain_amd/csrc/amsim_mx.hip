@@ -129,6 +129,15 @@ __device__ __forceinline__ void load_tile(Tile<T> &t, const MxConversion &j, int
     }
 }
 
+// The scale of a block of fragment `f`, a byte of its group's dword; behind the last fragment the group's other bytes are zeros.
+__device__ __forceinline__ void store_scale(uint8_t *scales, int64_t rows, int64_t f, int64_t steps, int64_t step, int lane, uint32_t code)
+{
+    uint8_t *to = scales + ((f / 4 * steps + step) * 64 + lane) * 4;
+    to[f % 4] = (uint8_t)code;
+    if (16 * (f + 1) >= rows)
+        for (int i = (int)(f % 4) + 1; i < 4; ++i) to[i] = 0;
+}
+
 // block `kb` of row `r` of the tile
 template <typename T> __device__ __forceinline__ MxBlock<T> row_block(const Tile<T> &t, int r, int kb)
 {
@@ -154,7 +163,7 @@ template <typename T, bool AROUND> __device__ __forceinline__ void convert_tile(
         const MxBlock<T> b = row_block(t, threadIdx.x / 64 * 16 + lane % 16, lane / 16);
         const uint32_t code = mx_scale_code(b.exponent_field());
         *(v4i *)(j.by_rows + ((f * steps + step) * 64 + lane) * 16) = b.encode(code);
-        j.by_rows[mx_code_bytes(j.rows, j.cols) + ((f / 4 * steps + step) * 64 + lane) * 4 + f % 4] = (uint8_t)code;
+        store_scale(j.by_rows + mx_code_bytes(j.rows, j.cols), j.rows, f, steps, step, lane, code);
     } else {  // eight fragments of 16 columns, a quarter of a step of each
         const int c = threadIdx.x - 128;
         const int64_t f = col0 / 16 + c / 16, steps = mx_steps(j.rows), step = row0 / 128;
@@ -168,7 +177,7 @@ template <typename T, bool AROUND> __device__ __forceinline__ void convert_tile(
             __builtin_memcpy(&b, v, sizeof(b));
             const uint32_t code = mx_scale_code(b.exponent_field());
             *(v4i *)(j.by_columns + ((f * steps + step) * 64 + lane) * 16) = b.encode(code);
-            j.by_columns[mx_code_bytes(j.cols, j.rows) + ((f / 4 * steps + step) * 64 + lane) * 4 + f % 4] = (uint8_t)code;
+            store_scale(j.by_columns + mx_code_bytes(j.cols, j.rows), j.cols, f, steps, step, lane, code);
         }
         if (j.sums && row0 < j.rows && col0 + c < j.cols) {
             float s[4] = {};  // (four chains: fewer roundings in each)
