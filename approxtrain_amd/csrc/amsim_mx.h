@@ -233,4 +233,8 @@ struct MxConversion {
 int mx_convert(const MxConversion *jobs, int count, hipStream_t stream);
 
 }  // namespace amsim
+
+// For tests: how the products of one call would run, one (m, n, k) or the two of a backward pass, (m, k, n) and (k, n, m).
+// info = {rows and columns of the tiles, splits of either's reduction: 0 where one workgroup's waves share it}.
+extern "C" int amsim_mxfp4_plan(int count, const int64_t *extents, int64_t *info);
 #endif  // AMSIM_MX_H_

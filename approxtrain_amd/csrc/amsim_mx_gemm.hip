@@ -784,6 +784,24 @@ using namespace amsim;
 
 extern "C" {
 
+int amsim_mxfp4_plan(int count, const int64_t *extents, int64_t *info)
+{
+    if (count < 1 || count > 2 || !extents || !info) return fail(AMSIM_ERR_INVALID, "mxfp4: one or two products are planned");
+    Extents e[2], t[2];
+    int which[2];
+    for (int j = 0; j < count; ++j) {
+        e[j] = {extents[3 * j], extents[3 * j + 1], extents[3 * j + 2]};
+        if (!product_fits(e[j].m, e[j].n, e[j].k)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: extents out of range");
+    }
+    info[0] = info[1] = info[2] = info[3] = 0;
+    if (const int n = tiled(e, count, t, which)) {
+        const Plan p = plan(t, n);
+        info[0] = TILES[p.tile].rows, info[1] = TILES[p.tile].cols;
+        for (int j = 0; j < n; ++j) info[2 + which[j]] = p.of[j].splits;
+    }
+    return AMSIM_OK;
+}
+
 size_t amsim_mxfp4_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k)
 {
     return product_fits(m, n, k) ? product_workspace(m, n, k) : 0;
