@@ -130,3 +130,13 @@ def test_calls_without_a_derivative_refuse_what_would_need_one():
                            (calls[1], (None, torch.autograd.forward_ad.make_dual(b, b)))):
             with pytest.raises(TypeError, match="forward-mode"):
                 call(*args)
+
+
+@pytest.mark.parametrize("python,native", [("false", False), ("python3", True)])
+def test_the_library_builds_where_torch_is_not(python, native):
+    """From C it needs hipcc alone; the module for torch's tensors is built where torch is found."""
+    import os
+    import subprocess
+    folder = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "approxtrain_amd", "csrc")
+    run = subprocess.run(["make", "-n", "-B", f"PYTHON={python}"], cwd=folder, capture_output=True, text=True, check=True)
+    assert "-o ../libamsim.so" in run.stdout and ("-o ../_native.so" in run.stdout) == native
