@@ -887,6 +887,7 @@ int amsim_mxfp4_dense_grad(const void *grad, int dtype, int64_t row_stride, cons
     if (!mx_extents_fit(m, k) || !mx_extents_fit(n, k) || !mx_extents_fit(m, n)) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: extents out of range");
     if (m == 0 || n == 0 || k == 0) return fail(AMSIM_ERR_INVALID, "mxfp4: empty product");
     if (row_stride < n && m > 1) return fail(AMSIM_ERR_INVALID, "mxfp4: rows overlap");
+    if (grad_bias && ceil_div64(n, 16) >= (1ll << 32) / FINISH_WG) return fail(AMSIM_ERR_UNSUPPORTED, "mxfp4: more columns than one launch sums");
     if (!grad || (grad_x && !kernel_rows) || (grad_kernel && !x_columns)) return fail(AMSIM_ERR_INVALID, "mxfp4: null pointer");
     const uintptr_t element = element_bytes(dtype) - 1;
     if (((uintptr_t)grad & element) || ((uintptr_t)out & element) || ((uintptr_t)x_columns & 15) || ((uintptr_t)kernel_rows & 15)

@@ -132,6 +132,14 @@ def test_calls_without_a_derivative_refuse_what_would_need_one():
                 call(*args)
 
 
+def test_bias_gradients_of_more_columns_than_a_launch_takes_are_refused():
+    """Their sums take a workgroup of 1024 for 16 columns: the launch failed behind others that had been made."""
+    n = 1 << 26
+    need = lib().amsim_mxfp4_dense_grad_workspace_bytes(1, n, 1)
+    assert need > 0
+    assert lib().amsim_mxfp4_dense_grad(A, 0, n, None, None, None, 1, n, 1, None, None, 0, A, 0, A, need, None) == 6
+
+
 @pytest.mark.parametrize("python,native", [("false", False), ("python3", True)])
 def test_the_library_builds_where_torch_is_not(python, native):
     """From C it needs hipcc alone; the module for torch's tensors is built where torch is found."""
