@@ -474,6 +474,8 @@ class AdamWState:
         self.dtype = params[0].dtype
         if self.dtype not in DTYPES:
             raise TypeError(f"parameters must be float32, bfloat16 or float16, got {self.dtype}")
+        if params[0].is_cuda and torch.cuda.is_current_stream_capturing():  # (the fills would be the graph's: every replay would clear the moments)
+            raise RuntimeError("moments cannot be made while a graph is captured: make the state, or take a first step, ahead of the capture")
         self.params, self.state_bits = params, state_bits
         self.sizes = [p.numel() for p in params]
         self._list = _native().TensorList(self.sizes, self.dtype, self.device_index)

@@ -34,7 +34,7 @@ class AdamW(torch.optim.Optimizer):
     goes by the number of steps that it has had a gradient for, and those that had other numbers than the rest take
     a call of their own.  A parameter that is frozen at the first step has no moments until it has a gradient.
     ``state_bits``: 32, or 8 for moments of a byte each.  A step that is captured into a graph keeps its number (the
-    bias corrections) when it is replayed."""
+    bias corrections) when it is replayed, and has to be preceded by one that is not."""
 
     _NOT_SAVED = ("params", "buckets", "outside")
 

@@ -72,3 +72,29 @@ def test_a_copy_goes_on_as_its_original(bits):
         opt.step(), again.step()
         for p, q in zip(params, theirs):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_made_in_a_capture_are_refused(bits):
+    """Their clearing would be part of the graph: every replay would step from moments of zero."""
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    p.grad = torch.ones(300, device="cuda")
+    opt = AdamW([p], state_bits=bits)
+    torch.cuda.synchronize()
+    for call in (opt.step, lambda: functors.AdamWState([p], bits)):
+        with pytest.raises(RuntimeError, match="capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    torch.cuda.synchronize()
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    twin = torch.ones(300, device="cuda")
+    state = functors.AdamWState([twin], bits)
+    functors.adamw_step(state, [p.grad], 1)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        functors.adamw_step(state, [p.grad], 2)
+        assert torch.equal(p, twin)
