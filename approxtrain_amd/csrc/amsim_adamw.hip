@@ -134,11 +134,17 @@ template <bool ROOTS> __device__ __forceinline__ uint32_t encode4(const float (&
     return w;
 }
 
-// Past the last-level cache, or through it.  Where all moments together are more than it holds nothing is there when a step
-// comes to it, and nothing it leaves there is read before it is displaced (us, past and through): 101M elements of 32-bit
-// moments and 16-bit gradients 449 and 491, beside other work on 512 MB 450 and 509, 112M of 8-bit moments 322 and 358, the
-// parameters read behind it 280 and 341 (that reading taken off); 28M of 32 bits, 224 MB, 144 and 147, beside others 145 and
-// 170.  Smaller states may still be there.
+// Past the last-level cache, or through it: all that a step reads (parameters, gradients, moments) goes past it where that is
+// more than it can hold, as nothing is there then when a step comes to it, and nothing it leaves there is read before it is
+// displaced.  us of one tensor, through and past; in brackets where its gradients were written just before:
+//   MB of a step          256          280          320          336          384          400          512
+//   32 bits, f32      68/74 (88/94)              90/92 (118/115)           128/110 (147/137)          174/147 (213/182)
+//   32 bits, bf16 grads       81/85 (97/101)             112/104 (125/122)
+//   8 bits, f32                                  93/94 (127/127)                       121/118 (167/162)
+//   8 bits, bf16 grads 82/90 (103/105)           117/113 (137/137)                                     185/180 (223/216)
+// Behind 256 MB of other work (that copy's time taken in) past is quicker at all sizes: 32 bits, f32, 128 MB 96/81, 256 MB
+// 139/115.
+inline bool step_goes_around(double bytes) { return bytes >= 320 << 20; }
 template <bool AROUND, typename V> __device__ __forceinline__ V get(const void *p)
 {
     return AROUND ? __builtin_nontemporal_load((const V *)p) : *(const V *)p;
@@ -312,7 +318,7 @@ int amsim_adamw_step(int count, void *const *params, const void *const *grads, c
     const int64_t step = hyper->step;
     if (step < 1) return fail(AMSIM_ERR_INVALID, "adamw: step below 1");
     if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0)) return fail(AMSIM_ERR_INVALID, "adamw: betas or eps out of range");
-    int64_t all_blocks = 0;
+    int64_t all_blocks = 0, stepped = 0;  // (stepped: of tensors that have gradients)
     for (int i = 0; i < count; ++i) {
         if (sizes[i] < 0) return fail(AMSIM_ERR_INVALID, "adamw: negative size");
         if (sizes[i] && !params[i]) return fail(AMSIM_ERR_INVALID, "adamw: null pointer");
@@ -320,6 +326,7 @@ int amsim_adamw_step(int count, void *const *params, const void *const *grads, c
             return fail(AMSIM_ERR_INVALID, "adamw: misaligned pointer");
         if (sizes[i] > (1ll << 33)) return fail(AMSIM_ERR_UNSUPPORTED, "adamw: tensor of more than 2^33 elements");
         all_blocks += ceil_div64(sizes[i], BLOCK);
+        if (grads[i]) stepped += ceil_div64(sizes[i], BLOCK);
     }
     if (all_blocks == 0) return AMSIM_OK;
     if (!m || !v || (state_bits == 8 && (!m_scale || !v_scale))) return fail(AMSIM_ERR_INVALID, "adamw: null pointer");
@@ -331,7 +338,7 @@ int amsim_adamw_step(int count, void *const *params, const void *const *grads, c
     a.inv_root2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
     a.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
     a.eps = (float)eps;
-    const bool around = mx_goes_around((double)all_blocks * BLOCK * (state_bits == 8 ? 2 : 8));
+    const bool around = step_goes_around((double)stepped * BLOCK * (element_bytes(param_dtype) + element_bytes(grad_dtype) + (state_bits == 8 ? 2 : 8)));
     int64_t block = 0;
     for (int i = 0; i < count;) {
         a.count = 0;

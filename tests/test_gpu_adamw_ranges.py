@@ -50,3 +50,24 @@ def test_tiny_and_ordinary_blocks_side_by_side():
     for k in ("m", "v"):
         a, b = (getattr(s, k) for s in states)
         assert torch.equal(a[:256], b[:256]) and torch.equal(a[512:], b[512:])
+
+
+@pytest.mark.parametrize("bits,dtype,sizes", [(32, torch.float32, (10_500_001, 10_999_998)), (32, torch.bfloat16, (15_000_001, 14_999_998)),
+                                              (8, torch.float32, (16_000_001, 18_000_002)), (8, torch.bfloat16, (20_000_001, 1, 40_000_002))])
+def test_steps_past_the_cache_are_those_through_it(bits, dtype, sizes):
+    """All of a step's tensors are more than 320 MB; each alone, and all but one without gradients, are less."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    whole = [torch.empty(n + 1, device="cuda", dtype=dtype).normal_(generator=gen) for n in sizes]
+    params = [t[i % 2:i % 2 + n] for i, (t, n) in enumerate(zip(whole, sizes))]
+    alone = [p.clone() for p in params]
+    state, parts = functors.AdamWState(params, bits), functors.AdamWState(alone, bits)
+    for step in (1, 2):
+        grads = [torch.empty(n, device="cuda", dtype=dtype).normal_(generator=gen) for n in sizes]
+        functors.adamw_step(state, grads, step)
+        for i in range(len(sizes)):
+            functors.adamw_step(parts, [g if j == i else None for j, g in enumerate(grads)], step)
+    for p, q in zip(params, alone):
+        assert torch.equal(p, q)
+    assert torch.equal(state.m, parts.m) and torch.equal(state.v, parts.v)
+    if bits == 8:
+        assert torch.equal(state.m_scale, parts.m_scale) and torch.equal(state.v_scale, parts.v_scale)
