@@ -624,8 +624,16 @@ Plan plan(const Extents *e, int count)
     return at.p;
 }
 
-// Whether few_kernel serves: reductions beyond 32768 need more than one workgroup's waves (64 rows by 512: 9.5 us against
-// 12.7 in tiles at 16384, 43 against 17 at 65536).
+// Whether few_kernel serves, by rows and length alone: a reduction beyond 32768 needs more than one workgroup's waves.  us of
+// the product by itself, few_kernel / tiles, of 16, 32 and 64 rows:
+//   length    10 wide                          512 wide                         8192 wide
+//     2048    3.3/5.2   3.7/5.5   4.6/5.6      3.5/5.2   3.9/5.3   4.8/5.3       4.7/5.3   5.6/5.5   7.7/5.6
+//     8192    4.1/7.7   4.9/7.9   6.4/8.1      4.5/8.8   5.4/8.1   6.7/8.4       9.4/12.7  10.9/12.8 15.5/12.9
+//    16384    5.6/8.3   6.8/8.6   9.2/8.9      6.0/9.2   7.2/9.7   9.5/10.0     15.0/17.0  16.5/17.5 27.6/18.4
+//    32768    8.7/9.2  10.7/9.5  14.7/10.2     9.1/10.5 11.2/10.7 15.0/11.3     27.3/27.6  29.1/27.8 50.4/29.3
+// Of 240 such products (1, 16, 17, 32 and 64 rows, 10 to 8192 wide, lengths of 128 to 32768) it takes 1.03 times the quicker's
+// time on average.  Tiles are quicker by a tenth or more for 64 rows of a length of 128, 64 rows that are 8192 wide or of
+// 16384 and more, and at 32768 from 17 rows on where few are wide.
 bool few(int64_t m, int64_t k) { return m <= 64 && mx_steps(k) <= 256; }
 
 size_t partial_bytes(const Extents &e, int64_t splits) { return splits > 1 ? ((size_t)splits * e.m * e.n * 4 + 255) / 256 * 256 : 0; }
