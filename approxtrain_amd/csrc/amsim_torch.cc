@@ -231,7 +231,14 @@ Tensor linear(py::handle given, py::handle data, int64_t n, int64_t k, py::handl
 // (the result, what the backward pass multiplies by)
 std::pair<Tensor, Tensor> dense(const Tensor &given, const Tensor &given_kernel, const std::optional<Tensor> &bias, int act, bool keep_x, bool keep_kernel)
 {
-    const Source x = row_source(given, "x"), kernel = row_source(given_kernel, "kernel");
+    const Source kernel = row_source(given_kernel, "kernel");
+    if (given.dim() == 2 && given.size(0) == 0) {  // (a batch of nothing, as a router may leave to an expert)
+        known(on_device(given, "x").scalar_type(), "x");
+        if (kernel.rows != given.size(1)) value_error("the kernel must have as many rows as x has columns");
+        bias_of(bias, kernel.cols, given);
+        return {matrix(0, kernel.cols, given, given.scalar_type()), bytes(0, given)};
+    }
+    const Source x = row_source(given, "x");
     const int64_t m = x.rows, k = x.cols, n = kernel.cols;
     if (kernel.rows != k) value_error("the kernel must have as many rows as x has columns");
     const Bias add = bias_of(bias, n, x.t);
@@ -252,6 +259,14 @@ struct Wanted {  // the gradients' types, where they are wanted
 int dense_grad(const Tensor &given, const Tensor &kept, bool kept_x, bool kept_kernel, int64_t m, int64_t k, int64_t n, const std::optional<Tensor> &out,
                const Wanted &want, Tensor (&grads)[3])
 {
+    if (m == 0) {
+        on_device(given, "grad");
+        if (given.dim() != 2 || given.size(0) != 0 || given.size(1) != n) value_error("grad must have the result's shape");
+        if (want.x) grads[0] = matrix(0, k, given, given.scalar_type());
+        if (want.kernel) grads[1] = at::zeros({k, n}, given.options().dtype(*want.kernel));
+        if (want.bias) grads[2] = at::zeros({n}, given.options().dtype(*want.bias));
+        return 0;
+    }
     const Source grad = row_source(given, "grad");
     if (grad.rows != m || grad.cols != n) value_error("grad must have the result's shape");
     if (out && (out->scalar_type() != grad.t.scalar_type() || out->dim() != 2 || out->size(0) != m || out->size(1) != n || !out->is_contiguous()
@@ -362,7 +377,7 @@ Tensor linearmx(py::handle x_, py::handle kernel_, py::handle bias_, int act)
     const Tensor &x = THPVariable_Unpack(x_.ptr()), &kernel = THPVariable_Unpack(kernel_.ptr());
     const std::optional<Tensor> bias = maybe_tensor(bias_, "bias");
     if (x.dim() < 1 || kernel.dim() != 2 || x.size(-1) != kernel.size(0)) value_error("linearmx expects x [..., width] and kernel [width, units]");
-    if (x.numel() == 0 || kernel.numel() == 0) value_error("linearmx of no elements");
+    if (kernel.numel() == 0) value_error("linearmx of no elements");
     if (x._fw_grad(0).defined() || kernel._fw_grad(0).defined() || (bias && bias->_fw_grad(0).defined()))
         throw py::type_error("linearmx has no forward-mode derivative");
     const Tensor flat = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});

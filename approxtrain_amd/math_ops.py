@@ -83,6 +83,7 @@ def linearmx(x, kernel, bias=None, activation=None):
     """``activation(x . kernel + bias)`` with both operands, and in the backward pass the gradient, in microscaled
     4-bit floating point: ``x`` ``[..., width]``, ``kernel`` ``[width, units]`` and ``bias`` ``[units]`` in float32,
     bfloat16 or float16 each; the result has x's type, each gradient its own tensor's.  ``activation``: None,
-    'linear' or 'relu', applied as the result is stored.  (Gradients of gradients are not provided, and a backward pass
+    'linear' or 'relu', applied as the result is stored.  Of no rows the result is empty and the weights' gradients are
+    zeros.  (Gradients of gradients are not provided, and a backward pass
     cannot be captured while a graph of the same leaves from the default stream lives.)"""
     return functors._native().linearmx(x, kernel, bias, functors._activation(activation))
