@@ -3,15 +3,17 @@
 //   g = grad [* grad_scale]      m' = beta1 m + (1 - beta1) g      v' = beta2 v + ((1 - beta2) g) g
 //   p' = p (1 - lr decay) - (m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)) * lr / (1 - beta1^t)
 //
-// Every operation is one rounding in 32 bits (no contraction), in this order.  Bound by memory: 28 bytes per
-// element with 32-bit parameters, gradients and moments, 16 with 8-bit moments, each read and written once.
+// Every operation is one rounding in 32 bits (no contraction), in this order.  28 bytes per element with 32-bit
+// parameters, gradients and moments, 16 with 8-bit moments, each read and written once.
 // One launch serves as many tensors as its arguments hold: a tensor is an entry of 24 bytes, and the moments of
 // all tensors lie in one buffer, each tensor from a multiple of 256 elements on, so that no table has to be
 // sent to the device ahead of the kernel.  A wavefront updates one block of 256 and ends (four one after the other
-// took 83 us for 25M elements in 161 tensors with 8-bit moments, one 78.5), and finds its tensor in two loads (a
-// binary search over the arguments took 502 us where this took 441, now 437: 101M elements, 16-bit gradients, 6.0 TB/s).
-// With 8-bit moments the arithmetic has to stay out of memory's way: the full divisions and roots of the
-// language and shuffles through LDS kept the vector units busy for 91% of 97 us, what is here takes 70 (5.8 TB/s).
+// took 6% longer with 8-bit moments), and finds its tensor in two loads (a binary search over the arguments took 14%
+// longer with 32-bit ones).
+// 32-bit moments are bound by memory: 101M elements with 16-bit gradients 440 us, 6.0 TB/s.  With 8-bit moments the
+// arithmetic has to stay out of memory's way and just about does: 25.5M elements in 161 tensors take 69 us in a row (5.9
+// TB/s) and 79 behind other kernels, the vector units busy throughout (458 instructions a block).  The full divisions and
+// roots of the language and shuffles through LDS took 97.
 //
 // 8-bit moments: a wavefront's 256 elements share a 32-bit scale, the largest magnitude among them.  m is held as
 // sign, 4 bits of exponent and 3 of mantissa of |m| / scale; v as its root r = sqrt(v), which halves the binades

@@ -1,7 +1,7 @@
 // Conversion of tensors to MXFP4 operands (amsim_mx.h) and back.
 //
 // Rows may start on any element: pieces of 16 bytes that cross two lines cost less than elements one by one (3616 x
-// 3762 in 16 bits, both directions and back: 34 us against 50).
+// 3762 in 16 bits, both directions and back: 29 us against 50).
 // Bound by memory: an element is read once, 4 or 2 bytes, and written as 17/32 of a byte for each direction
 // asked for.  A training step multiplies the same tensor along either axis, so one pass makes both operands, and
 // of a gradient also the sums of its columns.

@@ -4,7 +4,8 @@
 ``ammha/multihead_attention.py``.  Bias add, activations, softmax, scaling and
 reshapes are plain torch ops, exactly as they are stock TF ops in the
 reference; every multiplication of activations by weights goes through the
-approximate-multiplier ops."""
+approximate-multiplier ops, but in ``densemx`` and ``packed_densemx``, which have
+no counterpart there and multiply in 4 bits."""
 import math
 
 import torch
