@@ -90,6 +90,13 @@ SIGNATURES = {
     "amsim_mxfp4_dense": (_i, [_p, _i, _i64] * 2 + [_i64] * 3 + [_p, _i, _i] + [_p] * 4 + [_sz, _p]),
     "amsim_mxfp4_dense_grad_workspace_bytes": (_sz, [_i64] * 3),
     "amsim_mxfp4_dense_grad": (_i, [_p, _i, _i64] + [_p] * 3 + [_i64] * 3 + [_p, _p, _i, _p, _i, _p, _sz, _p]),
+    "amsim_kept8_bytes": (_sz, [_i64] * 2),
+    "amsim_kept8_values": (_i, [_p, _i64, _i64, _i, _p, _p]),
+    "amsim_layer_norm": (_i, [_p, _i, _i64, _i64, _i64, _p, _p, _i, C.c_double, _p, _f, _p, _p]),
+    "amsim_layer_norm_grad_workspace_bytes": (_sz, [_i64] * 2),
+    "amsim_layer_norm_grad": (_i, [_p, _i, _i64, _i64, _i64, _p, _i64, _p, _f, _p, _i, _p, _p, _p, _p, _sz, _p]),
+    "amsim_activation": (_i, [_p, _i, _i64, _i64, _i64, _i, _p, _p, _p]),
+    "amsim_activation_grad": (_i, [_p, _i, _i64, _i64, _i64, _p, _i, _p, _p]),
     "amsim_adamw_step": (_i, [_i, _p, _p, _p, _i, _i, _i, _p, _p, _f, _f, _p, _f, _p]),
     "amsim_adamw_state_values": (_i, [_p, _f, _i64, _i, _f, _p]),
     "amsim_conv_geometry": (_i, [_i, _i, _i, _i, C.POINTER(_i), C.POINTER(_i)]),

@@ -1,0 +1,756 @@
+// Layer normalisation, forward and backward, and activations whose input is kept in 8 bits for the backward pass.
+//
+//   mean = sum x / C, var = sum (x - mean)^2 / C, rstd = 1 / sqrt(var + eps), x^ = (x - mean) rstd, y = x^ gamma + beta
+//   G = dy gamma, dx = rstd (G - sum G / C - x^ sum (G x^) / C), dgamma = sum over rows of dy x^, dbeta = ... of dy
+//
+// Everything is bound by memory: a row is read once and stays in registers, a lane holding 8 or 16 of its values, and
+// both passes over it (the sum, then the squares about the mean; the largest magnitude, then the codes) run there.
+// Statistics and sums are 32 bits.
+#include "amsim_rows.h"
+
+#include <algorithm>
+
+namespace amsim {
+
+namespace {
+
+// A row over LANES lanes of EACH values: 16 lanes for short ones (four rows a wavefront), a wavefront, four, or sixteen.
+template <int LANES_, int EACH_> struct Shape {
+    static constexpr int LANES = LANES_, EACH = EACH_, THREADS = LANES_ > 256 ? LANES_ : 256, ROWS = THREADS / LANES_;
+    static constexpr int64_t HOLDS = (int64_t)LANES_ * EACH_;
+};
+constexpr int64_t MOST_HELD = 16384;
+// fn(Shape) of the smallest that holds a row; rows beyond that are read again for every pass over them
+template <typename Fn> int with_shape(int64_t cols, Fn &&fn)
+{
+    if (cols <= 128) return fn(Shape<16, 8>{});
+    if (cols <= 512) return fn(Shape<64, 8>{});
+    if (cols <= 1024) return fn(Shape<64, 16>{});
+    if (cols <= 2048) return fn(Shape<256, 8>{});
+    if (cols <= 4096) return fn(Shape<256, 16>{});
+    if (cols <= 8192) return fn(Shape<1024, 8>{});
+    return fn(Shape<1024, 16>{});
+}
+template <typename Fn> int with_type(int dtype, Fn &&fn)
+{
+    switch (dtype) {
+    case AMSIM_DTYPE_F32: return fn(0.0f);
+    case AMSIM_DTYPE_BF16: return fn((__bf16)0.0f);
+    default: return fn((_Float16)0.0f);
+    }
+}
+
+// what a thread has of its row
+template <typename S> struct Place {
+    int lane, group;  // within the row, the row within the workgroup
+    float (*part)[RowLanes<S::LANES>::WAVES][2];
+    __device__ __forceinline__ int64_t first_row() const { return (int64_t)blockIdx.x * S::ROWS + group; }
+    __device__ __forceinline__ int64_t rows_apart() const { return (int64_t)gridDim.x * S::ROWS; }
+    __device__ __forceinline__ RowLanes<S::LANES> lanes() const { return RowLanes<S::LANES>{part}; }
+};
+#define AMSIM_PLACE(S)                                                        \
+    __shared__ float part_[2][RowLanes<S::LANES>::WAVES][2];                  \
+    const Place<S> place{(int)threadIdx.x % S::LANES, (int)threadIdx.x / S::LANES, part_}
+
+// ---- layer norm, forward ----------------------------------------------------------------------------------------------
+
+struct NormArgs {
+    const void *x;
+    int64_t rows, stride;
+    int64_t cols;
+    const void *gamma, *beta;  // null: ones, zeros
+    int param_dtype;
+    float eps;
+    void *out;
+    float *statistics;         // [rows][2], or null
+    uint8_t *codes;            // [rows][pitch], or null
+    float *scales;
+};
+
+template <typename T, typename S>
+__global__ __launch_bounds__(S::THREADS) void norm_kernel(NormArgs g)
+{
+    constexpr int N = PIECE<T>, PIECES = S::EACH / N;
+    AMSIM_PLACE(S);
+    RowLanes<S::LANES> lanes = place.lanes();
+    const int cols = (int)g.cols, pitch = (int)kept8_pitch(cols);
+    float gamma[PIECES][N], beta[PIECES][N];
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int c = (p * S::LANES + place.lane) * N;
+#pragma unroll
+        for (int i = 0; i < N; ++i) gamma[p][i] = 1.0f, beta[p][i] = 0.0f;
+        if (g.gamma) load_floats(g.gamma, g.param_dtype, c, cols - c, gamma[p]);
+        if (g.beta) load_floats(g.beta, g.param_dtype, c, cols - c, beta[p]);
+    }
+    for (int64_t row = place.first_row(); row < g.rows; row += place.rows_apart()) {
+        const T *x = (const T *)g.x + row * g.stride;
+        float v[PIECES][N], sum = 0.0f, squares = 0.0f, largest = 0.0f;
+        v4i raw[PIECES];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int c = (p * S::LANES + place.lane) * N;
+            raw[p] = load_piece(x + c, cols - c);
+        }
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            piece_floats<T>(raw[p], v[p]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                sum += v[p][i];
+                largest = MaxOf::of(largest, __uint_as_float(magnitude_bits(v[p][i])));
+            }
+        }
+        if (g.codes) lanes.template both<SumOf, MaxOf>(sum, largest);
+        else sum = lanes.template one<SumOf>(sum);
+        const float mean = sum / (float)cols;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int c = (p * S::LANES + place.lane) * N;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float d = c + i < cols ? v[p][i] - mean : 0.0f;
+                squares = __builtin_fmaf(d, d, squares);
+            }
+        }
+        squares = lanes.template one<SumOf>(squares);
+        const float rstd = 1.0f / sqrtf(squares / (float)cols + g.eps);
+        T *out = (T *)g.out + row * cols;
+        const float r = q8_multiplier(__float_as_uint(largest));
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int c = (p * S::LANES + place.lane) * N;
+            if (g.codes && c < pitch) store_codes(g.codes + row * pitch + c, v[p], r);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[p][i] = __builtin_fmaf((v[p][i] - mean) * rstd, gamma[p][i], beta[p][i]);
+            store_piece(out + c, cols - c, v[p]);
+        }
+        if (place.lane == 0) {
+            if (g.statistics) g.statistics[2 * row] = mean, g.statistics[2 * row + 1] = rstd;
+            if (g.codes) g.scales[row] = q8_scale(__float_as_uint(largest));
+        }
+    }
+}
+
+// rows that no workgroup holds: read for the sum, for the squares, and for the results
+template <typename T>
+__global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs g)
+{
+    constexpr int N = PIECE<T>;
+    using S = Shape<1024, N>;
+    AMSIM_PLACE(S);
+    RowLanes<S::LANES> lanes = place.lanes();
+    const int64_t cols = g.cols, pitch = kept8_pitch(cols);
+    for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
+        const T *x = (const T *)g.x + row * g.stride;
+        float v[N], sum = 0.0f, squares = 0.0f, largest = 0.0f;
+        for (int64_t c = place.lane * N; c < cols; c += 1024 * N) {
+            piece_floats<T>(load_piece(x + c, cols - c), v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                sum += v[i];
+                largest = MaxOf::of(largest, __uint_as_float(magnitude_bits(v[i])));
+            }
+        }
+        lanes.template both<SumOf, MaxOf>(sum, largest);
+        const float mean = sum / (float)cols;
+        for (int64_t c = place.lane * N; c < cols; c += 1024 * N) {
+            piece_floats<T>(load_piece(x + c, cols - c), v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float d = c + i < cols ? v[i] - mean : 0.0f;
+                squares = __builtin_fmaf(d, d, squares);
+            }
+        }
+        squares = lanes.template one<SumOf>(squares);
+        const float rstd = 1.0f / sqrtf(squares / (float)cols + g.eps), r = q8_multiplier(__float_as_uint(largest));
+        for (int64_t c = place.lane * N; c < pitch; c += 1024 * N) {
+            float gamma[N], beta[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) gamma[i] = 1.0f, beta[i] = 0.0f;
+            piece_floats<T>(load_piece(x + c, cols - c), v);
+            if (g.codes) store_codes(g.codes + row * pitch + c, v, r);
+            if (g.gamma) load_floats(g.gamma, g.param_dtype, c, cols - c, gamma);
+            if (g.beta) load_floats(g.beta, g.param_dtype, c, cols - c, beta);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = __builtin_fmaf((v[i] - mean) * rstd, gamma[i], beta[i]);
+            store_piece((T *)g.out + row * cols + c, cols - c, v);
+        }
+        if (place.lane == 0) {
+            if (g.statistics) g.statistics[2 * row] = mean, g.statistics[2 * row + 1] = rstd;
+            if (g.codes) g.scales[row] = q8_scale(__float_as_uint(largest));
+        }
+    }
+}
+
+// ---- layer norm, backward ---------------------------------------------------------------------------------------------
+
+struct NormGradArgs {
+    const void *grad;
+    int64_t rows, stride, cols;
+    const void *x;             // or null: codes and scales
+    int64_t x_stride;
+    const uint8_t *codes;
+    const float *scales, *statistics;
+    const void *gamma;
+    int param_dtype;
+    void *grad_x;              // or null
+    float *partial;            // [workgroups][2][cols]: of dgamma and dbeta, or null
+};
+
+// x as it was given, or as it was kept
+template <typename T, bool KEPT> __device__ __forceinline__ auto load_input(const NormGradArgs &g, int64_t row, int64_t c, int64_t pitch)
+{
+    if constexpr (KEPT) {
+        struct {
+            uint32_t w[PIECE<T> / 4];
+        } raw = {};
+        if (c < pitch) __builtin_memcpy(&raw, __builtin_assume_aligned(g.codes + row * pitch + c, PIECE<T>), PIECE<T>);
+        return raw;
+    } else {
+        return load_piece((const T *)g.x + row * g.x_stride + c, g.cols - c);
+    }
+}
+template <typename T, bool KEPT, typename Raw> __device__ __forceinline__ void input_floats(const Raw &raw, float scale, float (&v)[PIECE<T>])
+{
+    if constexpr (KEPT) code_values(raw.w, scale, v);
+    else piece_floats<T>(raw, v);
+}
+
+// The gradients of gamma and beta: a lane adds up its columns over the rows that it sees; a workgroup's go to memory
+// once, and column_sums_kernel adds those in their order.
+template <typename T, typename S, bool KEPT>
+__global__ __launch_bounds__(S::THREADS) void norm_grad_kernel(NormGradArgs g)
+{
+    constexpr int N = PIECE<T>, PIECES = S::EACH / N;
+    AMSIM_PLACE(S);
+    RowLanes<S::LANES> lanes = place.lanes();
+    const int cols = (int)g.cols, pitch = (int)kept8_pitch(cols);
+    float gamma[PIECES][N], to_gamma[PIECES][N] = {}, to_beta[PIECES][N] = {};
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int c = (p * S::LANES + place.lane) * N;
+#pragma unroll
+        for (int i = 0; i < N; ++i) gamma[p][i] = 1.0f;
+        if (g.gamma) load_floats(g.gamma, g.param_dtype, c, cols - c, gamma[p]);
+    }
+    for (int64_t row = place.first_row(); row < g.rows; row += place.rows_apart()) {
+        const T *dy = (const T *)g.grad + row * g.stride;
+        const float mean = g.statistics[2 * row], rstd = g.statistics[2 * row + 1], scale = KEPT ? g.scales[row] : 0.0f;
+        v4i raw[PIECES];
+        decltype(load_input<T, KEPT>(g, 0, 0, 0)) raw_x[PIECES];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int c = (p * S::LANES + place.lane) * N;
+            raw[p] = load_piece(dy + c, cols - c);
+            raw_x[p] = load_input<T, KEPT>(g, row, c, pitch);
+        }
+        float h[PIECES][N], d[PIECES][N], sum = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            piece_floats<T>(raw[p], d[p]);  // (zeros behind the row's end: nothing is added there)
+            input_floats<T, KEPT>(raw_x[p], scale, h[p]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                h[p][i] = (h[p][i] - mean) * rstd;
+                to_gamma[p][i] = __builtin_fmaf(d[p][i], h[p][i], to_gamma[p][i]);
+                to_beta[p][i] += d[p][i];
+                d[p][i] *= gamma[p][i];
+                sum += d[p][i];
+                dot = __builtin_fmaf(d[p][i], h[p][i], dot);
+            }
+        }
+        if (!g.grad_x) continue;
+        lanes.template both<SumOf, SumOf>(sum, dot);
+        sum /= (float)cols, dot /= (float)cols;
+        T *dx = (T *)g.grad_x + row * cols;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int c = (p * S::LANES + place.lane) * N;
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[p][i] = rstd * __builtin_fmaf(-dot, h[p][i], d[p][i] - sum);
+            store_piece(dx + c, cols - c, d[p]);
+        }
+    }
+    if (!g.partial) return;
+    float *out = g.partial + (int64_t)blockIdx.x * 2 * cols;
+    if constexpr (S::ROWS == 1) {
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int c = (p * S::LANES + place.lane) * N;
+            store_piece(out + c, cols - c < 4 ? cols - c : 4, *(const float (*)[4])&to_gamma[p][0]);
+            store_piece(out + cols + c, cols - c < 4 ? cols - c : 4, *(const float (*)[4])&to_beta[p][0]);
+            if constexpr (N == 8) {
+                store_piece(out + c + 4, cols - c - 4 < 4 ? cols - c - 4 : 4, *(const float (*)[4])&to_gamma[p][4]);
+                store_piece(out + cols + c + 4, cols - c - 4 < 4 ? cols - c - 4 : 4, *(const float (*)[4])&to_beta[p][4]);
+            }
+        }
+    } else {  // the workgroup's rows meet in LDS
+        __shared__ float sums[2][S::ROWS][S::HOLDS];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = (p * S::LANES + place.lane) * N + i;
+                sums[0][place.group][c] = to_gamma[p][i];
+                sums[1][place.group][c] = to_beta[p][i];
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < cols; c += S::THREADS)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float s = sums[k][0][c];
+#pragma unroll
+                for (int r = 1; r < S::ROWS; ++r) s += sums[k][r][c];
+                out[k * cols + c] = s;
+            }
+    }
+}
+
+// rows that no workgroup holds: dx by rows, dgamma and dbeta by columns, a slab of rows to a workgroup
+template <typename T, bool KEPT>
+__global__ __launch_bounds__(1024) void norm_grad_long_kernel(NormGradArgs g)
+{
+    constexpr int N = PIECE<T>;
+    using S = Shape<1024, N>;
+    AMSIM_PLACE(S);
+    RowLanes<S::LANES> lanes = place.lanes();
+    const int64_t cols = g.cols, pitch = kept8_pitch(cols);
+    for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
+        const T *dy = (const T *)g.grad + row * g.stride;
+        const float mean = g.statistics[2 * row], rstd = g.statistics[2 * row + 1], scale = KEPT ? g.scales[row] : 0.0f;
+        float h[N], d[N], gamma[N], sum = 0.0f, dot = 0.0f;
+        auto load = [&](int64_t c) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) gamma[i] = 1.0f;
+            piece_floats<T>(load_piece(dy + c, cols - c), d);
+            input_floats<T, KEPT>(load_input<T, KEPT>(g, row, c, pitch), scale, h);
+            if (g.gamma) load_floats(g.gamma, g.param_dtype, c, cols - c, gamma);
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] = (h[i] - mean) * rstd, d[i] *= gamma[i];
+        };
+        for (int64_t c = place.lane * N; c < cols; c += 1024 * N) {
+            load(c);
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum += d[i], dot = __builtin_fmaf(d[i], h[i], dot);
+        }
+        lanes.template both<SumOf, SumOf>(sum, dot);
+        sum /= (float)cols, dot /= (float)cols;
+        for (int64_t c = place.lane * N; c < cols; c += 1024 * N) {
+            load(c);
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[i] = rstd * __builtin_fmaf(-dot, h[i], d[i] - sum);
+            store_piece((T *)g.grad_x + row * cols + c, cols - c, d);
+        }
+    }
+}
+template <typename T, bool KEPT>
+__global__ __launch_bounds__(256) void norm_grad_columns_kernel(NormGradArgs g)
+{
+    constexpr int N = PIECE<T>;
+    const int64_t cols = g.cols, pitch = kept8_pitch(cols), c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
+    if (c >= cols) return;
+    float to_gamma[N] = {}, to_beta[N] = {};
+    for (int64_t row = blockIdx.y; row < g.rows; row += gridDim.y) {
+        float h[N], d[N];
+        const float mean = g.statistics[2 * row], rstd = g.statistics[2 * row + 1], scale = KEPT ? g.scales[row] : 0.0f;
+        piece_floats<T>(load_piece((const T *)g.grad + row * g.stride + c, cols - c), d);
+        input_floats<T, KEPT>(load_input<T, KEPT>(g, row, c, pitch), scale, h);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            to_gamma[i] = __builtin_fmaf(d[i], (h[i] - mean) * rstd, to_gamma[i]);
+            to_beta[i] += d[i];
+        }
+    }
+    float *out = g.partial + (int64_t)blockIdx.y * 2 * cols + c;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (c + i < cols) out[i] = to_gamma[i], out[cols + i] = to_beta[i];
+}
+
+// [parts][2][cols] to the two gradients: 32 columns and 32 runs of parts to a workgroup, the runs joined in pairs
+struct ColumnSums {
+    const float *partial;
+    int64_t parts, cols;
+    void *grad[2];
+    int dtype;
+};
+__global__ __launch_bounds__(1024) void column_sums_kernel(ColumnSums g)
+{
+    __shared__ float run[32][33];
+    const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + c, width = 2 * g.cols, each = ceil_div64(g.parts, 32), end = min(g.parts, each * (w + 1));
+    float s = 0.0f;
+    if (col < width) {
+#pragma unroll 8
+        for (int64_t p = each * w; p < end; ++p) s += g.partial[p * width + col];
+    }
+    run[w][c] = s;
+    for (int half = 16; half; half /= 2) {
+        __syncthreads();
+        if (w < half) run[w][c] += run[w + half][c];
+    }
+    if (w != 0 || col >= width) return;
+    const int which = col >= g.cols;
+    if (g.grad[which]) store_from_float(g.grad[which], g.dtype, col - which * g.cols, run[0][c]);
+}
+
+// ---- activations whose input is kept -------------------------------------------------------------------------------------
+
+// Phi(-|x|) = exp(-x^2 / 2) R(|x|), R by a polynomial in 1 / (1 + 0.3 |x|), least in its largest relative error, 1.6e-7, on
+// |x| <= 14.5 (the coefficients: weighted least squares on the scaled complementary error function, the weights raised
+// where the error was largest).  With the roundings Phi is within 2.5e-7.  Some 25 instructions, two of them at a quarter
+// rate: the language's erfcf takes so many more that the vector units, not memory, would be the bound.
+struct Gelu {
+    static __device__ __forceinline__ void parts(float x, float &phi, float &density)
+    {
+        const float t = fabsf(x), u = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3f, t, 1.0f));
+        float p = 0.03542371094226837f;
+        p = __builtin_fmaf(p, u, -0.15615835785865784f);
+        p = __builtin_fmaf(p, u, 0.2045566290616989f);
+        p = __builtin_fmaf(p, u, -0.05203388258814812f);
+        p = __builtin_fmaf(p, u, 0.12769170105457306f);
+        p = __builtin_fmaf(p, u, 0.10017596930265427f);
+        p = __builtin_fmaf(p, u, 0.12071213126182556f);
+        p = __builtin_fmaf(p, u, 0.11963200569152832f);
+        const float e = __builtin_amdgcn_exp2f(t * t * -0.72134752f);
+        const float tail = u * p * e;
+        phi = x < 0.0f ? tail : 1.0f - tail;
+        density = e * 0.39894228f;
+    }
+    static __device__ __forceinline__ float value(float x)
+    {
+        float phi, density;
+        parts(x, phi, density);
+        return x * phi;
+    }
+    static __device__ __forceinline__ float slope(float x)
+    {
+        float phi, density;
+        parts(x, phi, density);
+        return __builtin_fmaf(x, density, phi);
+    }
+};
+struct Swish {
+    static __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f)); }
+    static __device__ __forceinline__ float value(float x) { return x * sigmoid(x); }
+    static __device__ __forceinline__ float slope(float x)
+    {
+        const float s = sigmoid(x);
+        return __builtin_fmaf(x * s, 1.0f - s, s);
+    }
+};
+struct Linear {  // (nothing but the keeping)
+    static __device__ __forceinline__ float value(float x) { return x; }
+    static __device__ __forceinline__ float slope(float) { return 1.0f; }
+};
+
+struct ActArgs {
+    const void *x;
+    int64_t rows, stride, cols;
+    void *out;       // or null
+    uint8_t *codes;  // or null
+    float *scales;
+};
+
+template <typename T, typename S, typename F>
+__global__ __launch_bounds__(S::THREADS) void activation_kernel(ActArgs g)
+{
+    constexpr int N = PIECE<T>, PIECES = S::EACH / N;
+    AMSIM_PLACE(S);
+    RowLanes<S::LANES> lanes = place.lanes();
+    const int cols = (int)g.cols, pitch = (int)kept8_pitch(cols);
+    for (int64_t row = place.first_row(); row < g.rows; row += place.rows_apart()) {
+        const T *x = (const T *)g.x + row * g.stride;
+        v4i raw[PIECES];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int c = (p * S::LANES + place.lane) * N;
+            raw[p] = load_piece(x + c, cols - c);
+        }
+        if (g.codes) {
+            float largest = 0.0f;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) {
+                float v[N];
+                piece_floats<T>(raw[p], v);
+#pragma unroll
+                for (int i = 0; i < N; ++i) largest = MaxOf::of(largest, __uint_as_float(magnitude_bits(v[i])));
+            }
+            largest = lanes.template one<MaxOf>(largest);
+            const float r = q8_multiplier(__float_as_uint(largest));
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) {
+                const int c = (p * S::LANES + place.lane) * N;
+                float v[N];
+                piece_floats<T>(raw[p], v);
+                if (c < pitch) store_codes(g.codes + row * pitch + c, v, r);
+            }
+            if (place.lane == 0) g.scales[row] = q8_scale(__float_as_uint(largest));
+        }
+        if (!g.out) continue;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int c = (p * S::LANES + place.lane) * N;
+            float v[N];
+            piece_floats<T>(raw[p], v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = F::value(v[i]);
+            store_piece((T *)g.out + row * cols + c, cols - c, v);
+        }
+    }
+}
+template <typename T, typename F>
+__global__ __launch_bounds__(1024) void activation_long_kernel(ActArgs g)
+{
+    constexpr int N = PIECE<T>;
+    using S = Shape<1024, N>;
+    AMSIM_PLACE(S);
+    RowLanes<S::LANES> lanes = place.lanes();
+    const int64_t cols = g.cols, pitch = kept8_pitch(cols);
+    for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
+        const T *x = (const T *)g.x + row * g.stride;
+        float v[N], largest = 0.0f;
+        if (g.codes) {
+            for (int64_t c = place.lane * N; c < cols; c += 1024 * N) {
+                piece_floats<T>(load_piece(x + c, cols - c), v);
+#pragma unroll
+                for (int i = 0; i < N; ++i) largest = MaxOf::of(largest, __uint_as_float(magnitude_bits(v[i])));
+            }
+            largest = lanes.template one<MaxOf>(largest);
+        }
+        const float r = q8_multiplier(__float_as_uint(largest));
+        for (int64_t c = place.lane * N; c < pitch; c += 1024 * N) {
+            piece_floats<T>(load_piece(x + c, cols - c), v);
+            if (g.codes) store_codes(g.codes + row * pitch + c, v, r);
+            if (!g.out) continue;
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = F::value(v[i]);
+            store_piece((T *)g.out + row * cols + c, cols - c, v);
+        }
+        if (g.codes && place.lane == 0) g.scales[row] = q8_scale(__float_as_uint(largest));
+    }
+}
+
+// dx = dy f'(what was kept); without dy: what was kept
+struct ActGradArgs {
+    const void *grad;  // or null
+    int64_t rows, stride, cols;
+    const uint8_t *codes;
+    const float *scales;
+    void *grad_x;
+};
+template <typename T, typename F, int LANES>
+__global__ __launch_bounds__(256) void activation_grad_kernel(ActGradArgs g)
+{
+    constexpr int N = PIECE<T>;
+    const int64_t cols = g.cols, pitch = kept8_pitch(cols);
+    for (int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; row < g.rows; row += (int64_t)gridDim.x * (256 / LANES)) {
+        const T *dy = g.grad ? (const T *)g.grad + row * g.stride : nullptr;
+        const float scale = g.scales[row];
+#pragma unroll 4
+        for (int64_t c = (int64_t)(threadIdx.x % LANES) * N; c < cols; c += LANES * N) {
+            uint32_t w[N / 4];
+            float v[N], d[N];
+            __builtin_memcpy(w, __builtin_assume_aligned(g.codes + row * pitch + c, N), N);
+            code_values(w, scale, v);
+            if (dy) {
+                piece_floats<T>(load_piece(dy + c, cols - c), d);
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = d[i] * F::slope(v[i]);
+            }
+            store_piece((T *)g.grad_x + row * cols + c, cols - c, v);
+        }
+    }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------------------------
+
+// workgroups that go over the rows in turn: what the card holds at once
+template <typename S> unsigned workgroups(int64_t rows) { return (unsigned)std::min<int64_t>(ceil_div64(rows, S::ROWS), 256 * 2048 / S::THREADS); }
+unsigned long_workgroups(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 512); }
+// ... of the backward pass, each of which leaves 2 x cols sums to be added up
+constexpr int64_t GRAD_WORKGROUPS = 512, GRAD_SLABS = 64;
+int64_t grad_parts(int64_t rows, int64_t cols)
+{
+    if (cols > MOST_HELD) return std::min(rows, GRAD_SLABS);
+    const int64_t at_once = cols <= 128 ? 16 : cols <= 1024 ? 4 : 1;
+    return std::min(ceil_div64(rows, at_once), GRAD_WORKGROUPS);
+}
+
+template <typename T, bool KEPT> int launch_norm_grad(const NormGradArgs &g, hipStream_t stream)
+{
+    if (g.cols > MOST_HELD) {
+        if (g.grad_x) norm_grad_long_kernel<T, KEPT><<<long_workgroups(g.rows), 1024, 0, stream>>>(g);
+        if (g.partial)
+            norm_grad_columns_kernel<T, KEPT><<<dim3((unsigned)ceil_div64(g.cols, 256 * PIECE<T>), (unsigned)grad_parts(g.rows, g.cols)), 256, 0, stream>>>(g);
+    } else {
+        with_shape(g.cols, [&](auto shape) {
+            using S = decltype(shape);
+            norm_grad_kernel<T, S, KEPT><<<(unsigned)grad_parts(g.rows, g.cols), S::THREADS, 0, stream>>>(g);
+            return 0;
+        });
+    }
+    AMSIM_HIP_CHECK(hipGetLastError());
+    return AMSIM_OK;
+}
+
+template <typename F> int launch_activation(const ActArgs &g, int dtype, hipStream_t stream)
+{
+    return with_type(dtype, [&](auto zero) {
+        using T = decltype(zero);
+        if (g.cols > MOST_HELD) {
+            activation_long_kernel<T, F><<<long_workgroups(g.rows), 1024, 0, stream>>>(g);
+        } else {
+            with_shape(g.cols, [&](auto shape) {
+                using S = decltype(shape);
+                activation_kernel<T, S, F><<<workgroups<S>(g.rows), S::THREADS, 0, stream>>>(g);
+                return 0;
+            });
+        }
+        AMSIM_HIP_CHECK(hipGetLastError());
+        return (int)AMSIM_OK;
+    });
+}
+template <typename F> int launch_activation_grad(const ActGradArgs &g, int dtype, hipStream_t stream)
+{
+    return with_type(dtype, [&](auto zero) {
+        using T = decltype(zero);
+        const int64_t pieces = ceil_div64(g.cols, PIECE<T>);
+        const int lanes = pieces <= 16 ? 16 : pieces <= 64 ? 64 : 256;
+        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div64(g.rows, 256 / lanes), 1 << 20);
+        const auto kernel = lanes == 16 ? activation_grad_kernel<T, F, 16> : lanes == 64 ? activation_grad_kernel<T, F, 64> : activation_grad_kernel<T, F, 256>;
+        kernel<<<blocks, 256, 0, stream>>>(g);
+        AMSIM_HIP_CHECK(hipGetLastError());
+        return (int)AMSIM_OK;
+    });
+}
+
+int check_rows(const char *what, const void *x, int dtype, int64_t rows, int64_t cols, int64_t stride)
+{
+    const std::string w(what);
+    if (!known_dtype(dtype)) return fail(AMSIM_ERR_INVALID, w + ": unknown element type");
+    if (!mx_extents_fit(rows, cols)) return fail(AMSIM_ERR_UNSUPPORTED, w + ": extents out of range");
+    if (rows == 0 || cols == 0) return fail(AMSIM_ERR_INVALID, w + ": empty tensor");
+    if (!x) return fail(AMSIM_ERR_INVALID, w + ": null pointer");
+    if (stride < cols && rows > 1) return fail(AMSIM_ERR_INVALID, w + ": rows overlap");
+    if ((uintptr_t)x & (element_bytes(dtype) - 1)) return fail(AMSIM_ERR_INVALID, w + ": misaligned pointer");
+    return AMSIM_OK;
+}
+bool off(const void *p, uintptr_t bytes) { return (uintptr_t)p & (bytes - 1); }
+uint8_t *codes_of(void *kept) { return (uint8_t *)kept; }
+float *scales_of(void *kept, int64_t rows, int64_t cols) { return kept ? (float *)((uint8_t *)kept + rows * kept8_pitch(cols)) : nullptr; }
+
+}  // namespace
+
+}  // namespace amsim
+
+using namespace amsim;
+
+extern "C" {
+
+size_t amsim_kept8_bytes(int64_t rows, int64_t cols)
+{
+    return mx_extents_fit(rows, cols) && rows && cols ? (size_t)kept8_bytes(rows, cols) : 0;
+}
+
+int amsim_kept8_values(const void *kept, int64_t rows, int64_t cols, int dtype, void *out, void *stream)
+{
+    if (int rc = check_rows("kept8", out, dtype, rows, cols, cols)) return rc;
+    if (!kept) return fail(AMSIM_ERR_INVALID, "kept8: null pointer");
+    if (off(kept, 16)) return fail(AMSIM_ERR_INVALID, "kept8: misaligned pointer");
+    return launch_activation_grad<Linear>({nullptr, rows, cols, cols, codes_of((void *)kept), scales_of((void *)kept, rows, cols), out}, dtype, (hipStream_t)stream);
+}
+
+int amsim_layer_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, const void *gamma, const void *beta, int param_dtype,
+                     double epsilon, void *out, float *statistics, void *kept, void *stream)
+{
+    if (int rc = check_rows("layer_norm", x, dtype, rows, cols, row_stride)) return rc;
+    if ((gamma || beta) && !known_dtype(param_dtype)) return fail(AMSIM_ERR_INVALID, "layer_norm: unknown element type");
+    if (!out) return fail(AMSIM_ERR_INVALID, "layer_norm: null pointer");
+    if (!(epsilon >= 0)) return fail(AMSIM_ERR_INVALID, "layer_norm: epsilon must not be negative");
+    const uintptr_t element = element_bytes(dtype), param = element_bytes(param_dtype);
+    if (off(out, element) || off(statistics, 4) || off(kept, 16) || (gamma && off(gamma, param)) || (beta && off(beta, param)))
+        return fail(AMSIM_ERR_INVALID, "layer_norm: misaligned pointer");
+    const NormArgs g{x, rows, row_stride, cols, gamma, beta, param_dtype, (float)epsilon, out, statistics, codes_of(kept), scales_of(kept, rows, cols)};
+    return with_type(dtype, [&](auto zero) {
+        using T = decltype(zero);
+        if (cols > MOST_HELD) {
+            norm_long_kernel<T><<<long_workgroups(rows), 1024, 0, (hipStream_t)stream>>>(g);
+        } else {
+            with_shape(cols, [&](auto shape) {
+                using S = decltype(shape);
+                norm_kernel<T, S><<<workgroups<S>(rows), S::THREADS, 0, (hipStream_t)stream>>>(g);
+                return 0;
+            });
+        }
+        AMSIM_HIP_CHECK(hipGetLastError());
+        return (int)AMSIM_OK;
+    });
+}
+
+size_t amsim_layer_norm_grad_workspace_bytes(int64_t rows, int64_t cols)
+{
+    return mx_extents_fit(rows, cols) && rows && cols ? (size_t)grad_parts(rows, cols) * 2 * cols * 4 : 0;
+}
+
+int amsim_layer_norm_grad(const void *grad, int dtype, int64_t rows, int64_t cols, int64_t row_stride, const void *x, int64_t x_row_stride,
+                          const void *kept, const float *statistics, const void *gamma, int param_dtype, void *grad_x, void *grad_gamma,
+                          void *grad_beta, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (int rc = check_rows("layer_norm", grad, dtype, rows, cols, row_stride)) return rc;
+    if (!x == !kept) return fail(AMSIM_ERR_INVALID, "layer_norm: either x or what was kept of it is needed");
+    if (x)
+        if (int rc = check_rows("layer_norm", x, dtype, rows, cols, x_row_stride)) return rc;
+    if ((gamma || grad_gamma || grad_beta) && !known_dtype(param_dtype)) return fail(AMSIM_ERR_INVALID, "layer_norm: unknown element type");
+    if (!statistics) return fail(AMSIM_ERR_INVALID, "layer_norm: null pointer");
+    const uintptr_t element = element_bytes(dtype), param = element_bytes(param_dtype);
+    if (off(kept, 16) || off(statistics, 4) || off(grad_x, element) || (gamma && off(gamma, param)) || (grad_gamma && off(grad_gamma, param))
+        || (grad_beta && off(grad_beta, param)))
+        return fail(AMSIM_ERR_INVALID, "layer_norm: misaligned pointer");
+    const bool sums = grad_gamma || grad_beta;
+    if (sums && cols >= 1 << 26) return fail(AMSIM_ERR_UNSUPPORTED, "layer_norm: more columns than one launch sums");
+    if (sums && (!workspace || workspace_bytes < amsim_layer_norm_grad_workspace_bytes(rows, cols) || off(workspace, 256)))
+        return fail(AMSIM_ERR_WORKSPACE, "layer_norm: workspace missing, misaligned or too small");
+    if (!grad_x && !sums) return AMSIM_OK;
+    const NormGradArgs g{grad, rows, row_stride, cols, x, x_row_stride, codes_of((void *)kept), scales_of((void *)kept, rows, cols), statistics, gamma,
+                         param_dtype, grad_x, sums ? (float *)workspace : nullptr};
+    const int rc = with_type(dtype, [&](auto zero) {
+        using T = decltype(zero);
+        return kept ? launch_norm_grad<T, true>(g, (hipStream_t)stream) : launch_norm_grad<T, false>(g, (hipStream_t)stream);
+    });
+    if (rc || !sums) return rc;
+    column_sums_kernel<<<(unsigned)ceil_div64(2 * cols, 32), 1024, 0, (hipStream_t)stream>>>(
+        ColumnSums{(const float *)workspace, grad_parts(rows, cols), cols, {grad_gamma, grad_beta}, param_dtype});
+    AMSIM_HIP_CHECK(hipGetLastError());
+    return AMSIM_OK;
+}
+
+int amsim_activation(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int kind, void *out, void *kept, void *stream)
+{
+    if (int rc = check_rows("activation", x, dtype, rows, cols, row_stride)) return rc;
+    if (!out && !kept) return fail(AMSIM_ERR_INVALID, "activation: null pointer");
+    if (off(out, element_bytes(dtype)) || off(kept, 16)) return fail(AMSIM_ERR_INVALID, "activation: misaligned pointer");
+    const ActArgs g{x, rows, row_stride, cols, out, codes_of(kept), scales_of(kept, rows, cols)};
+    switch (kind) {
+    case AMSIM_ACT_NONE: return launch_activation<Linear>(g, dtype, (hipStream_t)stream);
+    case AMSIM_ACT_GELU: return launch_activation<Gelu>(g, dtype, (hipStream_t)stream);
+    case AMSIM_ACT_SWISH: return launch_activation<Swish>(g, dtype, (hipStream_t)stream);
+    default: return fail(AMSIM_ERR_INVALID, "activation: unknown activation");
+    }
+}
+
+int amsim_activation_grad(const void *grad, int dtype, int64_t rows, int64_t cols, int64_t row_stride, const void *kept, int kind, void *grad_x, void *stream)
+{
+    if (int rc = check_rows("activation", grad, dtype, rows, cols, row_stride)) return rc;
+    if (!kept || !grad_x) return fail(AMSIM_ERR_INVALID, "activation: null pointer");
+    if (off(kept, 16) || off(grad_x, element_bytes(dtype))) return fail(AMSIM_ERR_INVALID, "activation: misaligned pointer");
+    const ActGradArgs g{grad, rows, row_stride, cols, codes_of((void *)kept), scales_of((void *)kept, rows, cols), grad_x};
+    switch (kind) {
+    case AMSIM_ACT_GELU: return launch_activation_grad<Gelu>(g, dtype, (hipStream_t)stream);
+    case AMSIM_ACT_SWISH: return launch_activation_grad<Swish>(g, dtype, (hipStream_t)stream);
+    default: return fail(AMSIM_ERR_INVALID, "activation: unknown activation");
+    }
+}
+
+}  // extern "C"

@@ -5,132 +5,13 @@
 // library one ctypes call after another: a layer's serving call took 13 us of host time that way and takes 5 to 8 here, the
 // training step of a 128 x 784 x 300 layer 125 and 40 to 76 (most of it torch's own engine), functors.adamw_step of 192 tensors 116
 // and 12 (the optimizer's step, which gathers the gradients first, 38).
-#include <ATen/ops/empty.h>
-#include <ATen/ops/zeros.h>
-#include <c10/hip/HIPFunctions.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/variable.h>
-#include <torch/csrc/utils/pybind.h>
+#include "amsim_torch.h"
 
-#include <optional>
-#include <stdexcept>
-#include <string>
-#include <vector>
-
-#include "amsim.h"
-
-namespace py = pybind11;
-using at::Tensor;
+using namespace amsim_torch;
 
 namespace {
 
-// ---- arguments --------------------------------------------------------------------------------------------------
-
-[[noreturn]] void value_error(const std::string &what) { throw py::value_error(what); }
-[[noreturn]] void type_error(const std::string &what) { throw py::type_error(what); }
-
-int code_of(at::ScalarType t)
-{
-    return t == at::kFloat ? AMSIM_DTYPE_F32 : t == at::kBFloat16 ? AMSIM_DTYPE_BF16 : t == at::kHalf ? AMSIM_DTYPE_F16 : -1;
-}
-std::string name_of(at::ScalarType t) { return py::str(py::reinterpret_borrow<py::object>((PyObject *)torch::getTHPDtype(t))); }
-int known(at::ScalarType t, const char *name)
-{
-    const int code = code_of(t);
-    if (code < 0) type_error(std::string(name) + " must be float32, bfloat16 or float16, got " + name_of(t));
-    return code;
-}
-int result_code(py::handle dtype, at::ScalarType &t)
-{
-    if (THPDtype_Check(dtype.ptr())) {
-        t = ((THPDtype *)dtype.ptr())->scalar_type;
-        const int code = code_of(t);
-        if (code >= 0) return code;
-    }
-    type_error("the result's type must be float32, bfloat16 or float16, got " + std::string(py::str(dtype)));
-}
-
-// the library launches on the current device
-const Tensor &on_device(const Tensor &t, const char *name)
-{
-    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided) type_error(std::string(name) + " must be a tensor in device memory (there is no CPU path)");
-    if (t.get_device() != c10::hip::current_device())
-        value_error(std::string(name) + " is on device " + std::to_string(t.get_device()) + ", which is not the current one");
-    return t;
-}
-const Tensor &tensor(py::handle h, const char *name)
-{
-    if (!THPVariable_Check(h.ptr())) type_error(std::string(name) + " must be a tensor in device memory (there is no CPU path)");
-    return THPVariable_Unpack(h.ptr());
-}
-std::optional<Tensor> maybe_tensor(py::handle h, const char *name)
-{
-    if (h.is_none()) return std::nullopt;
-    return tensor(h, name);
-}
-
-// for calls that are no part of a graph: what would need a derivative is refused, and not cut off without a word
-void no_derivative(const Tensor &t, const char *name, const char *call)
-{
-    if (at::GradMode::is_enabled() && t.requires_grad())
-        throw std::runtime_error(std::string(call) + " has no gradient and " + name + " requires one: train through linearmx, or call it under torch.no_grad()");
-    if (t._fw_grad(0).defined()) type_error(std::string(call) + " has no forward-mode derivative");
-}
-
-void *stream() { return c10::hip::getCurrentHIPStream().stream(); }
-
-void check(int status)
-{
-    if (status != 0) py::module_::import("approxtrain_amd._lib").attr("check")(status);
-}
-
-Tensor bytes(int64_t n, const Tensor &like) { return at::empty({n}, like.options().dtype(at::kByte)); }
-Tensor matrix(int64_t rows, int64_t cols, const Tensor &like, at::ScalarType t) { return at::empty({rows, cols}, like.options().dtype(t)); }
-
-// A matrix as the library reads it, in place where either of its axes is contiguous: its transpose if `swapped`.
-struct Source {
-    Tensor t;
-    int dtype;
-    int64_t rows, cols, stride;
-    bool swapped;
-};
-Source source(const Tensor &given, const char *name)
-{
-    Source s{on_device(given, name), known(given.scalar_type(), name), 0, 0, 0, false};
-    if (given.dim() != 2) value_error(std::string(name) + " must be a matrix");
-    s.rows = given.size(0), s.cols = given.size(1);
-    if (s.rows == 0 || s.cols == 0) value_error(std::string(name) + " is empty: blocks of no elements have no scale");
-    if (s.t.is_neg()) s.t = s.t.resolve_neg();
-    if (s.t._is_zerotensor()) s.t = at::zeros(s.t.sizes(), s.t.options());  // (zeros that take no memory)
-    const int64_t s0 = s.t.stride(0), s1 = s.t.stride(1);
-    if ((s1 == 1 || s.cols == 1) && (s0 >= s.cols || s.rows == 1)) {
-        s.stride = s.rows > 1 ? s0 : s.cols;
-    } else if ((s0 == 1 || s.rows == 1) && (s1 >= s.rows || s.cols == 1)) {
-        s.stride = s.cols > 1 ? s1 : s.rows;
-        std::swap(s.rows, s.cols);
-        s.swapped = true;
-    } else {
-        s.t = s.t.contiguous();
-        s.stride = s.cols;
-    }
-    return s;
-}
-// ... with its rows contiguous
-Source row_source(const Tensor &given, const char *name)
-{
-    Source s = source(given, name);
-    if (s.swapped) {
-        s.t = s.t.contiguous();
-        std::swap(s.rows, s.cols);
-        s.stride = s.cols;
-        s.swapped = false;
-    }
-    return s;
-}
+// ---- operands ----------------------------------------------------------------------------------------------------
 
 int64_t operand_bytes(int64_t rows, int64_t length)
 {
@@ -145,21 +26,6 @@ const Tensor &operand(const Tensor &data, int64_t rows, int64_t length, const ch
     if (data.scalar_type() != at::kByte || !data.is_contiguous() || data.numel() != operand_bytes(rows, length))
         value_error(std::string(name) + "'s data are not those of a " + std::to_string(rows) + " x " + std::to_string(length) + " operand");
     return data;
-}
-
-struct Bias {
-    std::optional<Tensor> t;
-    int dtype = 0;
-    const void *ptr() const { return t ? t->data_ptr() : nullptr; }
-};
-Bias bias_of(const std::optional<Tensor> &b, int64_t units, const Tensor &like)
-{
-    if (!b) return {};
-    on_device(*b, "bias");
-    if (b->get_device() != like.get_device()) value_error("bias must be on the operands' device");
-    const int dtype = known(b->scalar_type(), "bias");
-    if (b->dim() != 1 || b->size(0) != units) value_error("bias must have one entry per output channel");
-    return {b->_is_zerotensor() ? at::zeros(b->sizes(), b->options()) : b->contiguous().resolve_neg(), dtype};
 }
 
 // ---- conversions and products -----------------------------------------------------------------------------------
@@ -189,7 +55,7 @@ Tensor dequantize(py::handle data, int64_t rows, int64_t length, py::handle dtyp
 Tensor matmul(py::handle a_data, int64_t m, py::handle b_data, int64_t n, int64_t k, py::handle bias, int act, py::handle dtype)
 {
     const std::optional<Tensor> given_bias = maybe_tensor(bias, "bias");
-    if (given_bias) no_derivative(*given_bias, "bias", "mxfp4_matmul");
+    if (given_bias) no_derivative(*given_bias, "bias", "mxfp4_matmul", "linearmx");
     const Tensor &a = operand(tensor(a_data, "a"), m, k, "a"), &b = operand(tensor(b_data, "b"), n, k, "b");
     at::ScalarType t;
     const int code = result_code(dtype, t);
@@ -205,8 +71,8 @@ Tensor linear(py::handle given, py::handle data, int64_t n, int64_t k, py::handl
 {
     const Tensor &x = tensor(given, "x");
     const std::optional<Tensor> given_bias = maybe_tensor(bias, "bias");
-    no_derivative(x, "x", "mxfp4_linear");
-    if (given_bias) no_derivative(*given_bias, "bias", "mxfp4_linear");
+    no_derivative(x, "x", "mxfp4_linear", "linearmx");
+    if (given_bias) no_derivative(*given_bias, "bias", "mxfp4_linear", "linearmx");
     if (x.dim() < 1 || x.size(-1) != k) value_error("x's last axis must have the weights' length");
     const Tensor &w = operand(tensor(data, "weights"), n, k, "weights");
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
@@ -308,25 +174,6 @@ py::tuple dense_grad_call(py::handle grad, py::handle kept, int64_t rows, int64_
     return py::make_tuple(cast(grads[0]), cast(grads[1]), cast(grads[2]));
 }
 
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-// A leaf has one node that adds its gradients, on the stream that it was made on, for as long as a graph of it lives.  Where
-// that is the default stream, a captured backward pass would have to wait for a captured event there, which cannot be
-// recorded and ends the process in the engine's thread: seen here first, it is an error like others.
-bool adds_on_default_stream(const Tensor &t)
-{
-    const auto node = t.requires_grad() && t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : nullptr;
-    const auto stream = node ? node->stream() : std::nullopt;
-    return stream && stream->id() == 0;
-}
-bool capturing()
-{
-    const auto current = c10::hip::getCurrentHIPStream();
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    return current.id() != 0 && hipStreamIsCapturing(current.stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
-}
-
 // Each of a layer's three products has its operands quantised along the axis it sums over, so x, the kernel and the
 // gradient are quantised both ways, each from one reading; what the backward pass needs is kept in 4 bits.
 struct LinearMX : torch::autograd::Function<LinearMX> {
@@ -358,15 +205,7 @@ struct LinearMX : torch::autograd::Function<LinearMX> {
             TORCH_CHECK(status == 0, "amsim status ", status, ": ", amsim_last_error());
         }
         variable_list result{grads[0], grads[1], grads[2], Tensor(), Tensor()};
-        if (at::GradMode::is_enabled() && given[0].requires_grad()) {  // gradients of gradients are not provided: say so if they are asked for
-            variable_list some;
-            for (const Tensor &g : grads)
-                if (g.defined()) some.push_back(g.detach().set_requires_grad(true));
-            const auto error = std::make_shared<torch::autograd::DelayedError>("gradients of linearmx's gradients are not provided", (int64_t)some.size());
-            some = (*error)(std::move(some));
-            for (size_t i = 0, j = 0; i < 3; ++i)
-                if (result[i].defined()) result[i] = some[j++];
-        }
+        no_second_derivative(result, given[0].requires_grad(), "linearmx");
         return result;
     }
 };
@@ -481,6 +320,7 @@ Tensor state_values(py::handle codes_, py::handle scales_, bool roots)
 
 PYBIND11_MODULE(_native, m)
 {
+    bind_rows(m);
     m.def("quantize", &quantize);
     m.def("dequantize", &dequantize);
     m.def("matmul", &matmul);

@@ -9,6 +9,7 @@ import functools
 import torch
 
 from ._lib import check, conv_geometry, load_library
+from .i8 import Kept8
 from .lut import ApproxMulLut
 from .mx import DTYPES, MXTensor
 
@@ -453,6 +454,34 @@ def mxfp4_dense_grad(grad, kept, rows, width, units, out=None, kernel_dtype=None
     call ``kept`` for just these; ``out``: its result, if a rectifier was applied.  A gradient of the kernel or of the
     bias is computed where its type is given, x's (of grad's type) if ``need_x``; the others are None."""
     return _native().dense_grad(grad, kept, rows, width, units, out, kernel_dtype, bias_dtype, need_x)
+
+
+# ---- layer normalisation, and tensors kept in 8 bits ------------------------------------------------
+
+KEPT_ACTIVATIONS = {"gelu": 2, "swish": 3}
+
+
+def layer_norm(x, gamma=None, beta=None, epsilon=1e-3):
+    """``(x - mean) / sqrt(var + epsilon) * gamma + beta`` over x's last axis, in x's type (float32, bfloat16 or float16; gamma
+    and beta of one type, their own), statistics in 32 bits.  (No gradient: tensors that require one are refused outside
+    ``torch.no_grad``; ``math_ops.layernorm`` trains.)"""
+    return _native().layer_norm(x, gamma, beta, epsilon)
+
+
+def keep8(x):
+    """``x`` (float32, bfloat16 or float16) as 8-bit integers with a scale for each row, as a ``Kept8``: a backward pass
+    that takes its input so holds a byte for each value.  A row that holds an infinity or a NaN reads back as NaN."""
+    data, _, _ = _native().keep8(x)
+    return Kept8(data, x.shape, x.dtype)
+
+
+def kept8_values(kept, dtype=None):
+    """The values of a ``Kept8``, in ``dtype`` (None: that of the tensor it was made of)."""
+    if not isinstance(kept, Kept8):
+        raise TypeError("kept must be a Kept8 (functors.keep8)")
+    cols = kept.shape[-1]
+    rows = kept.shape.numel() // cols
+    return _native().kept8_values(kept.data, rows, cols, kept.dtype if dtype is None else dtype).reshape(kept.shape)
 
 
 # ---- AdamW over many tensors -----------------------------------------------------------------------

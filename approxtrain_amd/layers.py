@@ -14,7 +14,7 @@ from torch.autograd import forward_ad
 
 from . import functors
 from .amnn_ops import amconvolution_v2
-from .math_ops import linearmx, matmulam
+from .math_ops import layernorm, linearmx, matmulam
 
 
 # Keras vocabulary of the reference's layers (activations.get / initializers.get,
@@ -475,6 +475,42 @@ class packed_densemx(nn.Module):
         act = _fusable(self.activation)
         out = functors.mxfp4_linear(inputs, functors.MXTensor(self.weights, self.units, self.width), self.bias, act)
         return self.activation(out) if act is None else out
+
+
+class LayerNormalization(nn.Module):
+    """Layer normalisation over the last axis with the Keras layer's vocabulary (``epsilon, center, scale`` and the
+    initializers of ``beta`` and ``gamma``); the parameters are 32-bit floats, activations float32, bfloat16 or float16.
+    ``keep_bits=8`` keeps the input for the backward pass in 8 bits (``math_ops.layernorm``)."""
+
+    def __init__(self, axis=-1, epsilon=1e-3, center=True, scale=True, beta_initializer="zeros", gamma_initializer="ones", keep_bits=None,
+                 input_dim=None):
+        super().__init__()
+        if axis != -1:
+            raise ValueError("only the last axis (-1) is normalised")
+        if not epsilon >= 0:
+            raise ValueError("epsilon must not be negative")
+        if keep_bits not in (None, 8):
+            raise ValueError("keep_bits must be None or 8")
+        self.epsilon, self.center, self.scale, self.keep_bits = epsilon, center, scale, keep_bits
+        self.beta_initializer, self.gamma_initializer = beta_initializer, gamma_initializer
+        self.gamma = None
+        self.beta = None
+        if input_dim is not None:
+            self.build(input_dim)
+
+    def build(self, input_dim, device=None):
+        if self.scale:
+            self.gamma = nn.Parameter(_initialize_(torch.empty(input_dim, device=device), self.gamma_initializer, input_dim, input_dim))
+        if self.center:
+            self.beta = nn.Parameter(_initialize_(torch.empty(input_dim, device=device), self.beta_initializer, input_dim, input_dim))
+
+    def forward(self, inputs):
+        if (self.scale and self.gamma is None) or (self.center and self.beta is None):
+            self.build(inputs.shape[-1], inputs.device)
+        return layernorm(inputs, self.gamma, self.beta, self.epsilon, self.keep_bits)
+
+    def get_config(self):
+        return {"epsilon": self.epsilon, "center": self.center, "scale": self.scale, "keep_bits": self.keep_bits}
 
 
 class _Attention(torch.autograd.Function):

@@ -87,3 +87,22 @@ def linearmx(x, kernel, bias=None, activation=None):
     zeros.  (Gradients of gradients are not provided, and a backward pass
     cannot be captured while a graph of the same leaves from the default stream lives.)"""
     return functors._native().linearmx(x, kernel, bias, functors._activation(activation))
+
+
+def layernorm(x, gamma=None, beta=None, epsilon=1e-3, keep_bits=None):
+    """Layer normalisation over x's last axis, ``(x - mean) / sqrt(var + epsilon) * gamma + beta``: ``x`` ``[..., width]`` in
+    float32, bfloat16 or float16, ``gamma`` and ``beta`` ``[width]`` of one type (None: ones, zeros); the result has x's
+    type, each gradient its own tensor's.  ``keep_bits``: what the backward pass has of x, x itself (None) or 8
+    bits for each value (``functors.keep8``), which stand in for x in its formulas; the forward pass is the same."""
+    if keep_bits not in (None, 8):
+        raise ValueError("keep_bits must be None or 8")
+    return functors._native().layernorm(x, gamma, beta, epsilon, keep_bits == 8)
+
+
+def activationi8(x, activation):
+    """``activation(x)``, 'gelu' (``x Phi(x)``) or 'swish' (``x / (1 + exp(-x))``), whose backward pass takes its derivative at
+    the values of ``functors.keep8(x)``: a byte is kept for each value.  x in float32, bfloat16 or float16, a row to
+    its last axis."""
+    if activation not in functors.KEPT_ACTIVATIONS:
+        raise ValueError("activation must be 'gelu' or 'swish'")
+    return functors._native().activationi8(x, functors.KEPT_ACTIVATIONS[activation])

@@ -50,6 +50,8 @@ extern "C" {
 /* output epilogue of the *_bias_act entry points */
 #define AMSIM_ACT_NONE 0
 #define AMSIM_ACT_RELU 1
+#define AMSIM_ACT_GELU 2   /* amsim_activation only: x Phi(x) */
+#define AMSIM_ACT_SWISH 3  /* amsim_activation only: x / (1 + exp(-x)) */
 
 /* element types of the 4-bit products and of the optimizer's step (everything else is FP32) */
 #define AMSIM_DTYPE_F32 0
@@ -344,6 +346,34 @@ int amsim_mxfp4_dense_grad(const void *grad, int dtype, int64_t row_stride, cons
                            const void *kernel_rows, int64_t m, int64_t n, int64_t k, void *grad_x, void *grad_kernel,
                            int kernel_dtype, void *grad_bias, int bias_dtype, void *workspace, size_t workspace_bytes,
                            void *stream);
+
+/* ---- rows kept in 8 bits, layer normalisation and activations (no counterpart in the reference) ------
+ * What a backward pass needs of a tensor, a byte for each value: of a row's largest magnitude a = max(|x|, 2^-119) the
+ * multiplier 127 / a and the scale a / 127, rounded to 32 bits each; a value's code is the integer nearest to its exact
+ * product with the multiplier (ties to even) and stands for code * scale.  A row that holds an infinity or a NaN reads
+ * back as NaN.  `kept` is opaque, amsim_kept8_bytes long (0: extents out of range) and starts on a 16-byte boundary.
+ *
+ * amsim_layer_norm: out = (x - mean) / sqrt(var + epsilon) * gamma + beta over each row of x[rows][cols] (rows row_stride
+ * elements apart; out is contiguous, of x's type); gamma and beta, of param_dtype, may be NULL.  For the backward pass:
+ * statistics[rows][2] (mean, 1 / sqrt(var + epsilon)) and kept, either of which may be NULL.  amsim_layer_norm_grad takes x
+ * or kept, the other NULL (kept's values then stand in for x), and gives grad_x of grad's type, grad_gamma and
+ * grad_beta of param_dtype, each NULL if not wanted; the workspace, 256-byte aligned, is for the latter two.
+ * amsim_activation: out = f(x), f GELU, SWISH or NONE; out or kept may be NULL.  amsim_activation_grad: grad_x = grad
+ * f'(kept's values).  amsim_kept8_values: those values.  No result depends on the order of arrival. */
+size_t amsim_kept8_bytes(int64_t rows, int64_t cols);
+int amsim_kept8_values(const void *kept, int64_t rows, int64_t cols, int dtype, void *out, void *stream);
+int amsim_layer_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, const void *gamma,
+                     const void *beta, int param_dtype, double epsilon, void *out, float *statistics, void *kept,
+                     void *stream);
+size_t amsim_layer_norm_grad_workspace_bytes(int64_t rows, int64_t cols);
+int amsim_layer_norm_grad(const void *grad, int dtype, int64_t rows, int64_t cols, int64_t row_stride, const void *x,
+                          int64_t x_row_stride, const void *kept, const float *statistics, const void *gamma,
+                          int param_dtype, void *grad_x, void *grad_gamma, void *grad_beta, void *workspace,
+                          size_t workspace_bytes, void *stream);
+int amsim_activation(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int kind, void *out,
+                     void *kept, void *stream);
+int amsim_activation_grad(const void *grad, int dtype, int64_t rows, int64_t cols, int64_t row_stride, const void *kept,
+                          int kind, void *grad_x, void *stream);
 
 /* ---- AdamW over many tensors (no counterpart in the reference: its optimizers are Keras's) ------------
  *   g = grad [* *grad_scale]    m' = beta1 m + (1 - beta1) g    v' = beta2 v + ((1 - beta2) g) g
