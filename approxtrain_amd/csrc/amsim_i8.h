@@ -1,0 +1,58 @@
+// Operands of the products in 8-bit integers: storage, and the conversions that write it.
+//
+// A tensor of `rows` x `length` values has a scale for every row (the length is the reduction axis of a product); codes and
+// scale are those of amsim_rows.h (Q).  Storage follows the operands of the 16x16x64 matrix instruction, so that a
+// wavefront's loads are whole lines wherever they come from:
+//   codes   [rows / 16][length / 64][64 lanes][16 bytes]   lane = 16 * (16 values within the 64) + row % 16
+//   scales  [rows] floats, right behind them
+// with extents rounded up.  Codes beyond the length and beyond the last row are zeros: equal values are equal bytes.
+#ifndef AMSIM_I8_H_
+#define AMSIM_I8_H_
+
+#include "amsim_rows.h"
+
+namespace amsim {
+
+constexpr int I8_STEP = 64;
+constexpr int64_t I8_MOST_STEPS = 131072 / I8_STEP;  // of one sum: 127^2 * 131072 < 2^31
+__host__ __device__ inline int64_t i8_steps(int64_t length) { return ceil_div64(length, I8_STEP); }
+__host__ __device__ inline int64_t i8_code_bytes(int64_t rows, int64_t length) { return ceil_div64(rows, 16) * i8_steps(length) * 1024; }
+inline int64_t i8_bytes(int64_t rows, int64_t length) { return i8_code_bytes(rows, length) + 4 * rows; }
+
+// Converts x[rows][cols].  By rows: scales over a row (of x col_factor where that is given), codes to an operand of the
+// rows, of the columns, or both.  By columns: scales over a column (of row_factor x), the same.
+struct I8Rows {
+    const void *x, *positive;        // positive: [rows][cols] of x's type, or null: where it is not above zero x counts as zero
+    int dtype;
+    int64_t rows, cols, row_stride;  // row_stride in elements
+    const float *col_factor;         // or null
+    uint8_t *by_rows, *by_columns;   // codes, or null
+    float *scales;                   // [rows]
+    // for a conversion by columns of row_factor x that follows: each 16 rows' largest magnitude, and sum of x, in every column
+    const float *row_factor;         // or null: ones
+    float *partial;                  // [ceil(rows / 16)][2][cols], or null
+};
+int i8_convert_rows(const I8Rows &j, hipStream_t stream);
+
+struct I8Columns {
+    const void *x, *positive;
+    int dtype;
+    int64_t rows, cols, row_stride;
+    const float *row_factor;
+    uint8_t *by_rows, *by_columns;
+    float *scales;                   // [cols]
+    void *sums;                      // [cols] of sums_dtype: the columns' sums, or null
+    int sums_dtype;
+    const float *partial;            // as i8_convert_rows left it, or null: columns are looked through here
+};
+// workspace: floats, i8_columns_workspace of them
+int64_t i8_columns_workspace(int64_t rows, int64_t cols);
+int i8_convert_columns(const I8Columns &j, float *workspace, hipStream_t stream);
+
+inline bool i8_extents_fit(int64_t rows, int64_t length) { return mx_extents_fit(rows, length) && length <= 16 * I8_MOST_STEPS * I8_STEP; }
+
+}  // namespace amsim
+
+// For tests: how the products of one call would run, as amsim_mxfp4_plan (amsim_mx.h).
+extern "C" int amsim_i8_plan(int count, const int64_t *extents, int64_t *info);
+#endif  // AMSIM_I8_H_

@@ -7,12 +7,7 @@
 //
 // Times in these comments compare one thing with another, launches in a row on one device; devices and neighbouring
 // kernels move them by some percent (4096^3 in 16 bits 37 to 40 us).
-#include "amsim_mx.h"
-
-#include <algorithm>
-#include <cmath>
-#include <type_traits>
-#include <utility>
+#include "amsim_tiles.h"
 
 namespace amsim {
 
@@ -47,142 +42,11 @@ struct GemmJobs {
     unsigned blocks;         // of the first
 };
 
-template <typename T>
-__device__ __forceinline__ void store4(T *o, const float (&v)[4], int count, bool vector)
-{
-    T t[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = from_float<T>(v[i]);
-    if (count == 4 && vector) {
-        __builtin_memcpy(__builtin_assume_aligned(o, 4 * sizeof(T)), t, sizeof(t));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < count) o[i] = t[i];
-    }
-}
-
-// columns n .. n + 3 of row m, bias and activation included
-__device__ __forceinline__ void finish4(const void *bias, int bias_dtype, int act, void *out, int out_dtype, int64_t m, int64_t n, int64_t N, float (&v)[4])
-{
-    const int count = (int)(N - n < 4 ? N - n : 4);
-    const bool vector = N % 4 == 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (bias && i < count) v[i] += load_as_float(bias, bias_dtype, n + i);
-        v[i] = activate(v[i], act);
-    }
-    if (out_dtype == AMSIM_DTYPE_F32) store4((float *)out + m * N + n, v, count, vector);
-    else if (out_dtype == AMSIM_DTYPE_BF16) store4((__bf16 *)out + m * N + n, v, count, vector);
-    else store4((_Float16 *)out + m * N + n, v, count, vector);
-}
-
 template <int SA, int SB> __device__ __forceinline__ v4f mfma(v4i a, v4i b, v4f c, int sa, int sb)
 {
     const v8i wa = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, wb = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, wb, c, 4, 4, SA, sa, SB, sb);
 }
-// fn(integral_constant 0), ... fn(integral_constant N - 1): indices that are part of an instruction
-template <typename Fn, int... I> __device__ __forceinline__ void for_each(Fn &&fn, std::integer_sequence<int, I...>)
-{
-    (fn(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename Fn> __device__ __forceinline__ void for_each(Fn &&fn) { for_each(fn, std::make_integer_sequence<int, N>{}); }
-
-// Where tile number `id` of a launch lies.  Workgroups go to the eight dies in turn; each die gets a run of
-// neighbouring tiles, eight tiles high, so that its L2 serves a fragment's step to all who read it.
-__device__ __forceinline__ void place_tile(unsigned id, unsigned tiles_m, unsigned tiles_n, unsigned &tm, unsigned &tn)
-{
-    const unsigned tiles = tiles_m * tiles_n, each = tiles / 8, more = tiles % 8, die = id % 8;
-    const unsigned t = die * each + min(die, more) + id / 8;
-    const unsigned band = 8 * tiles_n, first = t / band * 8, within = t % band, high = min(8u, tiles_m - first);
-    tm = first + within % high;
-    tn = within / high;
-}
-
-// s_waitcnt for vmcnt n outstanding loads, and for all of LDS's answers
-#define MX_WAIT_LOADS(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | 7 << 4 | 15 << 8 | ((n) >> 4) << 14)
-#define MX_WAIT_LDS() __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 0 << 8 | 3 << 14)
-// the workgroup meets without waiting for anything else; no access to memory moves across it
-__device__ __forceinline__ void meet()
-{
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-// what a wavefront wrote to LDS is read by its other lanes after this (LDS answers a wavefront in order)
-__device__ __forceinline__ void lanes_meet()
-{
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
-    asm volatile("" ::: "memory");
-}
-
-// SIZE bytes a lane from memory to LDS, without passing through registers: lane l's bytes go to to + SIZE l.  The
-// wavefront's address and the step's offset stay in scalar registers.
-template <int SIZE> __device__ __forceinline__ void load_to_lds(const uint8_t *from, int step_offset, uint8_t *to)
-{
-#ifdef __HIP_DEVICE_COMPILE__  // (the host's compiler does not know the type)
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, 0xffffffff, 0x00020000);
-    const auto lds = (__attribute__((address_space(3))) void *)to;
-    if constexpr (SIZE == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, (threadIdx.x & 63) * 16, step_offset, 0, 0);
-    else __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 4, (threadIdx.x & 63) * 4, step_offset, 0, 0);
-#endif
-}
-
-// A wave's results to memory, by way of LDS: a lane's four columns lie in sixteen rows' lines, a row of 16 F columns
-// is whole ones.  The rows' padding puts sixteen rows' writes on different banks.  A tile of 256, alone on its CU,
-// goes out in parts (16 rows of 32 bits or 32 of 16), so that its first stores are under way early: 4096^3 takes 37.2 us
-// so and 37.6 in one part; tiles of 128 and less, which have neighbours to hide behind, in one: 42.7 and 44.1.
-template <typename T, int FM, int FN> struct Rows {
-    static constexpr int COLUMNS = 16 * FN, STRIDE = COLUMNS * sizeof(T) + 16, AT_ONCE = FM * FN == 32 ? 32 / FN / sizeof(T) : FM;
-    static constexpr int BYTES = 16 * AT_ONCE * STRIDE;
-};
-template <typename T, int FM, int FN>
-__device__ __forceinline__ void store_tile(uint8_t *lds, const v4f (&acc)[FM][FN], const float (&bias)[FN][4], int act, T *out, int64_t m0,
-                                           int64_t n0, int64_t M, int64_t N, bool around)
-{
-    using R = Rows<T, FM, FN>;
-    const int lane = threadIdx.x & 63, columns = (int)min<int64_t>(R::COLUMNS, N - n0);
-    for_each<FM / R::AT_ONCE>([&](auto part) {
-        constexpr int first = part.value * R::AT_ONCE;
-        MX_WAIT_LDS();  // (what lay there before has been read)
-        for_each<R::AT_ONCE * FN>([&](auto at) {
-            constexpr int i = at.value / FN, j = at.value % FN;
-            T t[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = from_float<T>(activate(acc[first + i][j][e] + bias[j][e], act));
-            __builtin_memcpy(__builtin_assume_aligned(lds + (16 * i + lane % 16) * R::STRIDE + (16 * j + lane / 16 * 4) * sizeof(T), 4 * sizeof(T)), t, sizeof(t));
-        });
-        lanes_meet();
-        const int64_t row0 = m0 + 16 * first;
-        const int rows = (int)max<int64_t>(0, min<int64_t>(16 * R::AT_ONCE, M - row0));
-        T *o = out + row0 * N + n0;
-        constexpr int PIECE = 16 / sizeof(T), PIECES = R::COLUMNS / PIECE, DOWN = 64 / PIECES;  // DOWN: rows that a store covers
-        const int c = lane % PIECES * PIECE;
-        const uint8_t *from = lds + lane / PIECES * R::STRIDE + c * sizeof(T);
-        T *to = o + lane / PIECES * N + c;
-        // (rows may start on any element: the hardware takes such pieces too)
-        auto pieces = [&](auto past) {
-#pragma unroll 8
-            for (int r = lane / PIECES; r < 16 * R::AT_ONCE; r += DOWN, from += DOWN * R::STRIDE, to += DOWN * N) {
-                const v4i v = *(const v4i *)from;
-                if (r >= rows) continue;
-                if constexpr (past.value) __builtin_nontemporal_store(v, (v4i_anywhere *)to);
-                else store16(to, v);
-            }
-        };
-        if (c + PIECE <= columns) {
-            if (around) pieces(std::true_type{});
-            else pieces(std::false_type{});
-        } else if (c < columns) {
-            for (int r = lane / PIECES; r < rows; r += DOWN, from += DOWN * R::STRIDE, to += DOWN * N)
-                for (int i = 0; i < columns - c; ++i) to[i] = ((const T *)from)[i];
-        }
-        lanes_meet();
-    });
-}
-
 // A workgroup of WM x WN waves, FM x FN fragments each: a tile of 16 FM WM rows and 16 FN WN columns.  Steps of 128 along the
 // reduction go from memory to one of STAGES places in LDS without passing through registers (the storage is
 // what a wavefront's 16-byte loads deliver, lane by lane), and a step's fragments are read into
@@ -274,8 +138,8 @@ __global__ __launch_bounds__(64 * WM * WN, RESIDENT) void gemm_kernel(GemmJobs j
     // place of step s; fragments of s + 1 are read while those of s are multiplied.  (Without branches, so that the
     // multiplications stay where they are: behind the last step it is loaded again, and not used.)
     auto step = [&](int s, const typename K::Registers &now, typename K::Registers &next) {
-        MX_WAIT_LDS();
-        MX_WAIT_LOADS((STAGES - 2) * K::LOADS);
+        AMSIM_WAIT_LDS();
+        AMSIM_WAIT_LOADS((STAGES - 2) * K::LOADS);
         meet();
         read_step(s + 1, next);
         fetch_step(s + STAGES);
@@ -293,7 +157,7 @@ __global__ __launch_bounds__(64 * WM * WN, RESIDENT) void gemm_kernel(GemmJobs j
     };
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) fetch_step(s);
-    MX_WAIT_LOADS((STAGES - 1) * K::LOADS);
+    AMSIM_WAIT_LOADS((STAGES - 1) * K::LOADS);
     meet();
     typename K::Registers even, odd;
     read_step(0, even);
@@ -306,8 +170,8 @@ __global__ __launch_bounds__(64 * WM * WN, RESIDENT) void gemm_kernel(GemmJobs j
         step(s, even, odd);
         step(s + 1, odd, even);
     }
-    MX_WAIT_LDS();
-    MX_WAIT_LOADS(0);
+    AMSIM_WAIT_LDS();
+    AMSIM_WAIT_LOADS(0);
     meet();  // (LDS is free)
     const int64_t m0 = (int64_t)(tm * WM + wm) * FM * 16, n0 = (int64_t)(tn * WN + wn) * FN * 16;
     if (m0 >= g.a.rows || n0 >= g.b.rows) return;
@@ -322,8 +186,9 @@ __global__ __launch_bounds__(64 * WM * WN, RESIDENT) void gemm_kernel(GemmJobs j
         }
     auto store = [&](auto zero, auto *out) {
         using T = decltype(zero);
-        store_tile<T, FM, FN>(lds + wave * Rows<T, FM, FN>::BYTES, acc, bias, whole ? g.act : AMSIM_ACT_NONE, out, m0, n0, g.a.rows, g.b.rows,
-                              whole && g.around);
+        const int act = whole ? g.act : AMSIM_ACT_NONE;
+        store_tile<T, FM, FN>(lds + wave * Rows<T, FM, FN>::BYTES, [&](int i, int j, int e) { return from_float<T>(activate(acc[i][j][e] + bias[j][e], act)); },
+                              out, m0, n0, g.a.rows, g.b.rows, whole && g.around);
     };
     if (!whole || g.out_dtype == AMSIM_DTYPE_F32) store(0.0f, whole ? (float *)g.out : g.partial + split * g.a.rows * g.b.rows);
     else if (g.out_dtype == AMSIM_DTYPE_BF16) store((__bf16)0.0f, (__bf16 *)g.out);
@@ -471,7 +336,7 @@ __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
 
 // What is left behind the products: partial sums of split reductions, added in the order of the splits, and a bias
 // gradient's from the sums of every 32 rows, 16 columns and 64 runs of rows to a workgroup, the runs joined in pairs.
-constexpr int FINISH_WG = 1024, MOST_SPLITS = 16;
+constexpr int FINISH_WG = 1024;
 struct FinishArgs {
     GemmJobs products;
     unsigned blocks[2];      // of either product's sums
@@ -536,96 +401,16 @@ __global__ __launch_bounds__(FINISH_WG) void finish_kernel(FinishArgs f)
     else ((_Float16 *)f.out)[col] = (_Float16)s;
 }
 
-struct Tile {
-    int rows, cols, slots;  // slots: tiles that the card holds at once
-    // microseconds, as measured on products of 128 to 16384 a side: of a launch; of a step where a tile has a CU for itself,
-    // and where all slots are taken; of storing a tile (between results of 16 bits and of 32: workspaces are asked for
-    // before the type is known)
-    double base, alone, full, store;
-};
 // Tiles of 256 fetch least for an operation and have their CU for themselves, with eight waves (four with twice the
 // fragments: 39.8 us for 4096^3, 37.1 with eight): what they store, nobody multiplies beside.  256 x 128 share it by two (512
 // tiles of 32 steps: 38.7 us, 37.1 as 256 of 256, 42.2 as 1024 of 128; of 128 steps 124, 112 and 136; 2048 tiles of 16 steps
 // 84, 89, 92).  Tiles of 128 and 64 fetch two and four times the bytes, and are for few results (256 tiles of 128, 16
 // steps: 10.0 us, 13.9 in 256 x 128; 410 of 64, 21 steps: 7.7, 10.1 in 128).
-constexpr Tile TILES[] = {{256, 256, 256, 2.2, 0.55, 0.785, 10.8},  // (stored by a round at once)
-                          {256, 128, 512, 6.5, 0.5, 0.85, 0.0124}, {128, 128, 512, 5, 0.2, 0.46, 0.01}, {64, 64, 1024, 4, 0.1, 0.4, 0.003}};
-
-struct Extents {
-    int64_t m, n, k;
+struct Costs {
+    static constexpr Tile TILES[] = {{256, 256, 256, 2.2, 0.55, 0.785, 10.8},  // (stored by a round at once)
+                                 {256, 128, 512, 6.5, 0.5, 0.85, 0.0124}, {128, 128, 512, 5, 0.2, 0.46, 0.01}, {64, 64, 1024, 4, 0.1, 0.4, 0.003}};
+    static constexpr int64_t STEP = 128, MOST_STEPS = 1ll << 40;
 };
-struct Plan {
-    int tile;  // of TILES
-    struct {
-        int64_t tiles_m, tiles_n, splits, steps_per_split;
-    } of[2];
-};
-
-// What a launch of `tiles` tiles takes whose steps add up to `work` and are at most `longest`: rounds of all slots, and a
-// last one in which a CU has one tile or a few.
-double microseconds(int tile, double tiles, double work, double longest)
-{
-    const Tile &t = TILES[tile];
-    const double mean = work / tiles, rounds = std::floor(tiles / t.slots), rest = tiles - rounds * t.slots;
-    double last = rest > 0 ? std::max(t.alone, t.full * rest / t.slots) : 0;
-    if (tile == 1 && rest > 256) last = 0.8;
-    const double steps = std::max(rounds * t.full * mean + last * mean, t.alone * longest);
-    if (tile == 0) return t.base + std::ceil(tiles / t.slots) * (t.store + 1.5) - 1.5 + steps;
-    return t.base + steps + t.store * tiles;
-}
-
-// The tile of one or two products and the splits of their reductions that take least time.  A split reduction takes a
-// second launch, 3 us, and its sums go to memory and back.
-Plan make_plan(const Extents *e, int count)
-{
-    Plan best{-1, {}};
-    double least = 0;
-    for (int i = 0; i < 4; ++i) {
-        Plan p{i, {}};
-        double tiles = 0, work = 0, longest = 0, more = 0;
-        for (int j = 0; j < count; ++j) {
-            const int64_t steps = mx_steps(e[j].k), tiles_m = ceil_div64(e[j].m, TILES[i].rows), tiles_n = ceil_div64(e[j].n, TILES[i].cols);
-            const double area = (double)tiles_m * (double)tiles_n;
-            double quickest = 0, its_more = 0;
-            for (int64_t s = 1; s <= MOST_SPLITS && (s == 1 || 2 * s <= steps); s *= 2) {
-                const int64_t each = ceil_div64(steps, s), splits = ceil_div64(steps, each);
-                const double extra = splits > 1 ? 3 + (double)splits * (double)e[j].m * (double)e[j].n * 8 / 4e6 : 0;
-                const double us = microseconds(i, area * splits, area * splits * each, each) + extra;
-                if (s > 1 && us >= quickest) continue;
-                quickest = us;
-                its_more = extra;
-                p.of[j] = {tiles_m, tiles_n, splits, each};
-            }
-            const double all = area * p.of[j].splits;
-            tiles += all;
-            work += all * p.of[j].steps_per_split;
-            longest = std::max(longest, (double)p.of[j].steps_per_split);
-            more += its_more;
-        }
-        const double us = microseconds(i, tiles, work, longest) + more;
-        if (best.tile < 0 || us < least) {
-            least = us;
-            best = p;
-        }
-    }
-    return best;
-}
-
-// The same, looked up where the thread has asked for it before: a training step asks seven times, a microsecond each.
-Plan plan(const Extents *e, int count)
-{
-    struct Known {
-        Extents e[2];
-        Plan p;
-    };
-    static thread_local Known known[64] = {};
-    const Extents none{}, &f = count > 1 ? e[1] : none;
-    const uint64_t hash = ((uint64_t)e[0].m * 3 + (uint64_t)e[0].n * 5 + (uint64_t)e[0].k * 7 + (uint64_t)f.k * 11) * 0x9e3779b97f4a7c15ull;
-    Known &at = known[hash >> 58];
-    auto same = [](const Extents &x, const Extents &y) { return x.m == y.m && x.n == y.n && x.k == y.k; };
-    if (!same(at.e[0], e[0]) || !same(at.e[1], f)) at = Known{{e[0], f}, make_plan(e, count)};
-    return at.p;
-}
 
 // Whether few_kernel serves, by rows and length alone: a reduction beyond 32768 needs more than one workgroup's waves.  us of
 // the product by itself, few_kernel / tiles, of 16, 32 and 64 rows:
@@ -638,8 +423,6 @@ Plan plan(const Extents *e, int count)
 // time on average.  Tiles are quicker by a tenth or more for 64 rows of a length of 128, 64 rows that are 8192 wide or of
 // 16384 and more, and at 32768 from 17 rows on where few are wide.
 bool few(int64_t m, int64_t k) { return m <= 64 && mx_steps(k) <= 256; }
-
-size_t partial_bytes(const Extents &e, int64_t splits) { return splits > 1 ? ((size_t)splits * e.m * e.n * 4 + 255) / 256 * 256 : 0; }
 
 // the products of a list that go in tiles, and the others
 int tiled(const Extents *e, int count, Extents *out, int *which)
@@ -656,7 +439,7 @@ size_t products_workspace(const Extents *e, int count)
     int which[2];
     const int n = tiled(e, count, t, which);
     if (n == 0) return 0;
-    const Plan p = plan(t, n);
+    const Plan p = plan<Costs>(t, n);
     size_t bytes = 0;
     for (int j = 0; j < n; ++j) bytes += partial_bytes(t[j], p.of[j].splits);
     return bytes;
@@ -714,7 +497,7 @@ int products(const Product *list, int count, const float *sums, int64_t parts, i
     }
     FinishArgs f{};
     if (n) {
-        Plan p = plan(t, n);
+        Plan p = plan<Costs>(t, n);
         if (n == 2 && p.of[1].steps_per_split > p.of[0].steps_per_split)  // the tiles that take longest go first
             std::swap(t[0], t[1]), std::swap(which[0], which[1]), std::swap(p.of[0], p.of[1]);
         GemmJobs &jobs = f.products;
@@ -806,8 +589,8 @@ int amsim_mxfp4_plan(int count, const int64_t *extents, int64_t *info)
     }
     info[0] = info[1] = info[2] = info[3] = 0;
     if (const int n = tiled(e, count, t, which)) {
-        const Plan p = plan(t, n);
-        info[0] = TILES[p.tile].rows, info[1] = TILES[p.tile].cols;
+        const Plan p = plan<Costs>(t, n);
+        info[0] = Costs::TILES[p.tile].rows, info[1] = Costs::TILES[p.tile].cols;
         for (int j = 0; j < n; ++j) info[2 + which[j]] = p.of[j].splits;
     }
     return AMSIM_OK;

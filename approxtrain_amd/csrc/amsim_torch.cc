@@ -321,6 +321,7 @@ Tensor state_values(py::handle codes_, py::handle scales_, bool roots)
 PYBIND11_MODULE(_native, m)
 {
     bind_rows(m);
+    bind_i8(m);
     m.def("quantize", &quantize);
     m.def("dequantize", &dequantize);
     m.def("matmul", &matmul);

@@ -182,6 +182,7 @@ inline void no_second_derivative(variable_list &grads, bool asked, const std::st
 
 // the calls of amsim_torch_rows.cc and amsim_torch_i8.cc
 void bind_rows(py::module_ &m);
+void bind_i8(py::module_ &m);
 
 }  // namespace amsim_torch
 #endif  // AMSIM_TORCH_H_

@@ -9,7 +9,7 @@ import functools
 import torch
 
 from ._lib import check, conv_geometry, load_library
-from .i8 import Kept8
+from .i8 import I8Tensor, Kept8
 from .lut import ApproxMulLut
 from .mx import DTYPES, MXTensor
 
@@ -454,6 +454,52 @@ def mxfp4_dense_grad(grad, kept, rows, width, units, out=None, kernel_dtype=None
     call ``kept`` for just these; ``out``: its result, if a rectifier was applied.  A gradient of the kernel or of the
     bias is computed where its type is given, x's (of grad's type) if ``need_x``; the others are None."""
     return _native().dense_grad(grad, kept, rows, width, units, out, kernel_dtype, bias_dtype, need_x)
+
+
+# ---- 8-bit integers with a scale for each token and channel, and their products -----------------------
+
+def _i8_operand(q, name):
+    if not isinstance(q, I8Tensor):
+        raise TypeError(f"{name} must be an I8Tensor (functors.int8_quantize)")
+    return q
+
+
+def int8_quantize(x, axis=-1):
+    """Matrix ``x`` (float32, bfloat16 or float16, any strides) as an operand in 8-bit integers with one scale along
+    ``axis``, the axis that a product will sum over: ``-1`` gives an operand of x's rows (a scale for each token), ``0`` one
+    of its columns (a scale for each channel; x's transpose, read in place)."""
+    if axis == -1 or axis == 1:
+        data, _, rows, cols = _native().i8_quantize(x, True, False)
+        return I8Tensor(data, rows, cols)
+    if axis == 0 or axis == -2:
+        _, data, rows, cols = _native().i8_quantize(x, False, True)
+        return I8Tensor(data, cols, rows)
+    raise ValueError("axis must be 0 or 1 (or -2 or -1)")
+
+
+def int8_dequantize(q, dtype=torch.float32):
+    """The values of an operand in 8-bit integers, ``[rows, length]``."""
+    q = _i8_operand(q, "q")
+    return _native().i8_dequantize(q.data, q.rows, q.length, dtype)
+
+
+def int8_matmul(a, b, bias=None, activation=None, dtype=torch.float32):
+    """``activation(a . b^T + bias)`` of two 8-bit operands of one length: ``[a.rows, b.rows]``, the sums over the integers
+    exact, scaled in 32 bits and rounded to ``dtype`` once.  (No gradient: a bias that requires one is refused outside
+    ``torch.no_grad``.)"""
+    _i8_operand(a, "a"), _i8_operand(b, "b")
+    if a.length != b.length:
+        raise ValueError("the operands' lengths differ")
+    return _native().i8_matmul(a.data, a.rows, b.data, b.rows, a.length, bias, _activation(activation), dtype)
+
+
+def int8_linear(x, weights, bias=None, activation=None):
+    """``activation(Q(x) . weights^T + bias)`` for activations ``x`` ``[..., length]``, which are quantised on the way with a
+    scale for each token, and weights that lie in 8 bits with one for each unit: ``int8_quantize(kernel, axis=0)`` of a
+    ``[length, units]`` kernel.  The result has x's type.  (No gradient: x or a bias that require one are refused outside
+    ``torch.no_grad``; ``math_ops.lineari8`` trains.)"""
+    w = _i8_operand(weights, "weights")
+    return _native().i8_linear(x, w.data, w.rows, w.length, bias, _activation(activation))
 
 
 # ---- layer normalisation, and tensors kept in 8 bits ------------------------------------------------

@@ -5,7 +5,8 @@
 reshapes are plain torch ops, exactly as they are stock TF ops in the
 reference; every multiplication of activations by weights goes through the
 approximate-multiplier ops, but in ``densemx`` and ``packed_densemx``, which have
-no counterpart there and multiply in 4 bits."""
+no counterpart there and multiply in 4 bits, and in ``densei8`` and
+``packed_densei8``, which multiply in 8."""
 import math
 
 import torch
@@ -14,7 +15,7 @@ from torch.autograd import forward_ad
 
 from . import functors
 from .amnn_ops import amconvolution_v2
-from .math_ops import layernorm, linearmx, matmulam
+from .math_ops import activationi8, layernorm, lineari8, linearmx, matmulam
 
 
 # Keras vocabulary of the reference's layers (activations.get / initializers.get,
@@ -475,6 +476,94 @@ class packed_densemx(nn.Module):
         act = _fusable(self.activation)
         out = functors.mxfp4_linear(inputs, functors.MXTensor(self.weights, self.units, self.width), self.bias, act)
         return self.activation(out) if act is None else out
+
+
+# the activations that densei8 keeps the input of in 8 bits
+def _activate_kept(out, activation):
+    name = "gelu" if activation is nn.functional.gelu else "swish" if activation is nn.functional.silu else None
+    return activation(out) if name is None else activationi8(out, name)
+
+
+class densei8(nn.Module, _KerasLayerArgs):
+    """``denseam`` with 8-bit integers in place of a table: ``activation(inputs . kernel + bias)`` with a scale for each token and
+    each unit (``math_ops.lineari8``), the constructor as ``denseam``'s but for the table.  The parameters are 32-bit floats,
+    activations float32, bfloat16 or float16.  For the backward pass the layer keeps a byte for each value of its inputs,
+    and of what goes into a 'gelu' or 'swish' (``math_ops.activationi8``).  ``pack()`` gives the layer as it is served, with
+    weights of 8 bits."""
+
+    def __init__(self, units, activation=None, use_bias=True, kernel_initializer="glorot_uniform",
+                 bias_initializer="zeros", kernel_regularizer=None, bias_regularizer=None, activity_regularizer=None,
+                 kernel_constraint=None, bias_constraint=None, input_dim=None, **kwargs):
+        super().__init__()
+        if int(units) < 1:
+            raise ValueError(f"Received an invalid value for `units`, expected a positive integer, got {units}.")
+        self.units, self.use_bias = int(units), use_bias
+        self.activation = _get_activation(activation)
+        self.kernel_initializer, self.bias_initializer = kernel_initializer, bias_initializer
+        input_shape = self._keras_args(kernel_regularizer, bias_regularizer, activity_regularizer, kernel_constraint,
+                                       bias_constraint, kwargs)
+        self.kernel = None
+        self.bias = None
+        if input_dim is None and input_shape is not None:
+            input_dim = input_shape[-1]
+        if input_dim is not None:
+            self.build(input_dim)
+
+    build = denseam.build
+
+    def forward(self, inputs):
+        if self.kernel is None:
+            self.build(inputs.shape[-1], inputs.device)
+        act = _fusable(self.activation)
+        out = lineari8(inputs, self.kernel, self.bias, activation=act)
+        if act is None:
+            out = _activate_kept(out, self.activation)
+        return self._track_activity(out)
+
+    def pack(self):
+        """The layer for inference, as a ``packed_densei8`` that holds its weights in 8 bits."""
+        if self.kernel is None:
+            raise ValueError("the layer has no weights yet: call it, or give input_dim")
+        return packed_densei8(self.kernel, self.bias, self.activation)
+
+    def get_config(self):
+        return {"units": self.units, "use_bias": self.use_bias}
+
+
+class packed_densei8(nn.Module):
+    """A dense layer for inference: ``kernel`` ``[width, units]`` is converted to 8 bits once, the activations on
+    the way (``functors.int8_linear``).  Its outputs are those of the ``densei8`` layer it was packed from.  Inputs that require
+    gradients are refused outside ``torch.no_grad``.  The saved state holds units and width besides, which the weights' bytes do not tell."""
+
+    def __init__(self, kernel, bias=None, activation=None):
+        super().__init__()
+        self.activation = _get_activation(activation)
+        with torch.no_grad():
+            weights = functors.int8_quantize(kernel.detach(), axis=0)
+        self.units, self.width = weights.shape
+        self.register_buffer("weights", weights.data)
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+
+    def get_extra_state(self):
+        return torch.tensor([self.units, self.width])
+
+    def set_extra_state(self, state):
+        """(compared before anything is loaded)"""
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        key = prefix + "_extra_state"
+        extents = state_dict[key].tolist() if key in state_dict else [self.units, self.width]
+        if extents != [self.units, self.width]:
+            error_msgs.append(f"{prefix}weights are those of {extents[0]} units of width {extents[1]}, not of {self.units} of width {self.width}")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+
+    def forward(self, inputs):
+        act = _fusable(self.activation)
+        out = functors.int8_linear(inputs, functors.I8Tensor(self.weights, self.units, self.width), self.bias, act)
+        if act is None:
+            out = _activate_kept(out, self.activation)
+        return out
 
 
 class LayerNormalization(nn.Module):

@@ -89,6 +89,18 @@ def linearmx(x, kernel, bias=None, activation=None):
     return functors._native().linearmx(x, kernel, bias, functors._activation(activation))
 
 
+def lineari8(x, kernel, bias=None, activation=None):
+    """``activation(x . kernel + bias)`` in 8-bit integers, x with a scale for each token and the kernel with one for each unit:
+    ``x`` ``[..., width]``, ``kernel`` ``[width, units]`` and ``bias`` ``[units]`` in float32, bfloat16 or float16 each; the result
+    has x's type, each gradient its own tensor's.  ``activation``: None, 'linear' or 'relu', applied as the result is stored.
+    The backward pass keeps the integers that were multiplied, a byte for each value of x, and multiplies them by the
+    gradient in 8 bits: the kernel's scales go onto the gradient before it is quantised by token (x's gradient), x's before
+    it is quantised by unit (the kernel's); the bias's is summed in 32 bits.  Of no rows the result is empty and the weights'
+    gradients are zeros.  (Gradients of gradients are not provided, and a backward pass cannot be captured while a graph of
+    the same leaves from the default stream lives.)"""
+    return functors._native().lineari8(x, kernel, bias, functors._activation(activation))
+
+
 def layernorm(x, gamma=None, beta=None, epsilon=1e-3, keep_bits=None):
     """Layer normalisation over x's last axis, ``(x - mean) / sqrt(var + epsilon) * gamma + beta``: ``x`` ``[..., width]`` in
     float32, bfloat16 or float16, ``gamma`` and ``beta`` ``[width]`` of one type (None: ones, zeros); the result has x's

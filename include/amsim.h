@@ -347,6 +347,52 @@ int amsim_mxfp4_dense_grad(const void *grad, int dtype, int64_t row_stride, cons
                            int kernel_dtype, void *grad_bias, int bias_dtype, void *workspace, size_t workspace_bytes,
                            void *stream);
 
+/* ---- 8-bit integers with a scale for each token and channel, and their products (no counterpart) ------
+ * The other narrow format that the matrix cores multiply.  An operand has `rows` x `length` values, the length being the
+ * reduction axis, and a scale for each row: of the row's largest magnitude a = max(|x|, 2^-119) the multiplier 127 / a and the
+ * scale a / 127, rounded to 32 bits each; a value's code is the integer nearest to its exact product with the
+ * multiplier (ties to even) and stands for code * scale.  A row that holds an infinity or a NaN has the scale NaN.  Operands are
+ * opaque, amsim_i8_operand_bytes long (0: extents out of range, lengths above 2^21 among them) and start on 16-byte boundaries.
+ *
+ * amsim_i8_quantize: x[rows][cols] of `dtype`, rows row_stride elements apart, to an operand of its rows (rows x cols), of
+ * its columns (cols x rows, for which the workspace is), or both; a direction that is not wanted is NULL.
+ * amsim_i8_dequantize: the values, out[rows][length] of `dtype`.
+ * amsim_i8_matmul: out[m][n] = act(sum_k a[m][k] b[n][k] + bias[n]), the sum over the codes exact, rounded to 32 bits, scaled,
+ * and rounded to out_dtype once; bias may be NULL.  amsim_i8_linear: the same with a = x[m][k], quantised on the way.  Out
+ * starts on a 16-byte boundary, the workspace on a 256-byte one.  Empty extents are refused (AMSIM_ERR_INVALID). */
+size_t amsim_i8_operand_bytes(int64_t rows, int64_t length);
+size_t amsim_i8_quantize_workspace_bytes(int64_t rows, int64_t cols);
+int amsim_i8_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void *by_rows,
+                      void *by_columns, void *workspace, size_t workspace_bytes, void *stream);
+int amsim_i8_dequantize(const void *q, int64_t rows, int64_t length, int dtype, void *out, void *stream);
+size_t amsim_i8_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int amsim_i8_matmul(const void *a, const void *b, int64_t m, int64_t n, int64_t k, const void *bias, int bias_dtype,
+                    int act, void *out, int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
+size_t amsim_i8_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int amsim_i8_linear(const void *x, int dtype, int64_t row_stride, const void *w, int64_t m, int64_t n, int64_t k,
+                    const void *bias, int bias_dtype, int act, void *out, void *workspace, size_t workspace_bytes,
+                    void *stream);
+
+/* The training step of a dense layer in 8 bits, which keeps a byte of each activation.  amsim_i8_dense: out[m][n] = act(
+ * x[m][k] kernel[k][n] + bias), x quantised by rows (scales sx), the kernel by columns (sw); for the backward pass
+ * it keeps the codes that were multiplied, with their scales, in x_kept (amsim_i8_kept_bytes(k, m)) and kernel_kept
+ * (amsim_i8_kept_bytes(k, n)), either of which may be NULL.  amsim_i8_dense_grad, for a gradient[m][n] of x's type: with
+ * out (the forward pass's, for the rectifier) not NULL the gradient counts as zero where out is not above zero; the kept scales
+ * go onto the gradient (each product rounded to 32 bits) before that is quantised, so that the kept codes are multiplied as
+ * they are: grad_x[m][k] = Q(gradient[m][n] sw[n]) along n by the kernel's codes, grad_kernel[k][n] = x's codes by
+ * Q(gradient[m][n] sx[m]) along m, and grad_bias[n] the sums of the gradient's columns in 32 bits, each in its tensor's type
+ * and each NULL if not wanted.  No result depends on the order of arrival. */
+size_t amsim_i8_kept_bytes(int64_t rows, int64_t length);
+size_t amsim_i8_dense_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int amsim_i8_dense(const void *x, int dtype, int64_t row_stride, const void *kernel, int kernel_dtype,
+                   int64_t kernel_row_stride, int64_t m, int64_t n, int64_t k, const void *bias, int bias_dtype, int act,
+                   void *out, void *x_kept, void *kernel_kept, void *workspace, size_t workspace_bytes, void *stream);
+size_t amsim_i8_dense_grad_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int amsim_i8_dense_grad(const void *grad, int dtype, int64_t row_stride, const void *out, const void *x_kept,
+                        const void *kernel_kept, int64_t m, int64_t n, int64_t k, void *grad_x, void *grad_kernel,
+                        int kernel_dtype, void *grad_bias, int bias_dtype, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
 /* ---- rows kept in 8 bits, layer normalisation and activations (no counterpart in the reference) ------
  * What a backward pass needs of a tensor, a byte for each value: of a row's largest magnitude a = max(|x|, 2^-119) the
  * multiplier 127 / a and the scale a / 127, rounded to 32 bits each; a value's code is the integer nearest to its exact
