@@ -20,7 +20,7 @@ __host__ __device__ inline int64_t i8_code_bytes(int64_t rows, int64_t length) {
 inline int64_t i8_bytes(int64_t rows, int64_t length) { return i8_code_bytes(rows, length) + 4 * rows; }
 
 // Converts x[rows][cols].  By rows: scales over a row (of x col_factor where that is given), codes to an operand of the
-// rows, of the columns, or both.  By columns: scales over a column (of row_factor x), the same.
+// rows, of the columns, or both.  By columns: scales over a column (of row_factor x), the same, and the columns' sums.
 struct I8Rows {
     const void *x, *positive;        // positive: [rows][cols] of x's type, or null: where it is not above zero x counts as zero
     int dtype;
@@ -28,26 +28,21 @@ struct I8Rows {
     const float *col_factor;         // or null
     uint8_t *by_rows, *by_columns;   // codes, or null
     float *scales;                   // [rows]
-    // for a conversion by columns of row_factor x that follows: each 16 rows' largest magnitude, and sum of x, in every column
-    const float *row_factor;         // or null: ones
-    float *partial;                  // [ceil(rows / 16)][2][cols], or null
 };
-int i8_convert_rows(const I8Rows &j, hipStream_t stream);
-
 struct I8Columns {
     const void *x, *positive;
     int dtype;
     int64_t rows, cols, row_stride;
-    const float *row_factor;
-    uint8_t *by_rows, *by_columns;
+    const float *row_factor;         // or null: ones
+    uint8_t *by_rows, *by_columns;   // both null: sums alone
     float *scales;                   // [cols]
-    void *sums;                      // [cols] of sums_dtype: the columns' sums, or null
+    void *sums;                      // [cols] of sums_dtype, or null: of x
     int sums_dtype;
-    const float *partial;            // as i8_convert_rows left it, or null: columns are looked through here
 };
-// workspace: floats, i8_columns_workspace of them
-int64_t i8_columns_workspace(int64_t rows, int64_t cols);
-int i8_convert_columns(const I8Columns &j, float *workspace, hipStream_t stream);
+// Either or both (of one tensor or two), null where there is none: a launch that converts the rows and looks through the
+// columns, and one that converts the columns.  partial: i8_partial_floats of the columns' extents.
+int64_t i8_partial_floats(int64_t rows, int64_t cols);
+int i8_convert(const I8Rows *rows, const I8Columns *columns, float *partial, hipStream_t stream);
 
 inline bool i8_extents_fit(int64_t rows, int64_t length) { return mx_extents_fit(rows, length) && length <= 16 * I8_MOST_STEPS * I8_STEP; }
 

@@ -1,9 +1,8 @@
 // Conversions to 8-bit integers with a scale for each row or column (amsim_i8.h), and back.
 //
 // Bound by memory, and below some hundred thousand values by the launches: a scale has to be known before the first code is
-// written.  Along rows one workgroup sees 16 rows whole and holds them in registers between the two; along columns the
-// largest magnitudes are gathered first (by the conversion along rows, where there is one of the same tensor), and the
-// tensor is read again.
+// written.  Along rows one workgroup sees 16 rows whole and holds them in registers between the two; along columns slabs of
+// rows are looked through first, beside a conversion along rows where there is one, and the tensor is read again.
 //
 // A wavefront's unit is 16 rows x 64 columns, a step of one fragment: loads of 16 bytes a lane, whole lines of 128 bytes and
 // more; codes of rows go out as 1 KB in a piece.  For an operand of the columns the unit's bytes are transposed in
@@ -28,20 +27,20 @@ template <typename T> __device__ __forceinline__ int unit_row(int i) { return i 
 template <typename T> __device__ __forceinline__ int unit_col() { return lane_id() % Unit<T>::LANES * Unit<T>::N; }
 
 // rows row0 .. row0 + 15, columns col0 .. col0 + 63, zeros outside; `positive` applied
-template <typename T>
+template <bool MASK, typename T>
 __device__ __forceinline__ void load_unit(const T *x, const T *positive, int64_t rows, int64_t cols, int64_t stride, int64_t row0, int64_t col0,
                                           v4i (&raw)[Unit<T>::LOADS])
 {
     using U = Unit<T>;
     const int64_t c = col0 + unit_col<T>();
-    v4i keep[U::LOADS];
+    v4i keep[MASK ? U::LOADS : 1];
 #pragma unroll
     for (int i = 0; i < U::LOADS; ++i) {
         const int64_t r = row0 + unit_row<T>(i);
         raw[i] = load_piece(x + r * stride + c, r < rows ? cols - c : 0);
-        if (positive) keep[i] = load_piece(positive + r * cols + c, r < rows ? cols - c : 0);
+        if constexpr (MASK) keep[i] = load_piece(positive + r * cols + c, r < rows ? cols - c : 0);
     }
-    if (!positive) return;
+    if constexpr (MASK)
 #pragma unroll
     for (int i = 0; i < U::LOADS; ++i) {
         T v[U::N], y[U::N];
@@ -107,34 +106,16 @@ __device__ __forceinline__ void store_unit(const Codes<Unit<T>::N> &codes, uint3
 
 // ---- along rows -----------------------------------------------------------------------------------------------------
 
-// maxima or sums over the lanes that hold the same columns of a unit, in every one of them
-template <typename Op, typename T> __device__ __forceinline__ float down_unit(float v)
-{
-    if constexpr (Unit<T>::LANES == 8) v = with_dpp<Op, 0x128>(v);  // the other eight of sixteen
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = Op::of(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return Op::of(__uint_as_float(h[0]), __uint_as_float(h[1]));
-}
-
 // HELD units of a wave stay in registers; 0: rows are read again.
-template <typename T, int HELD>
-__global__ __launch_bounds__(WG) void rows_kernel(I8Rows g)
+template <typename T, int HELD, bool MASK> __device__ __forceinline__ void convert_rows(const I8Rows &g, uint32_t *lds)
 {
     using U = Unit<T>;
-    __shared__ uint32_t largest_of[WAVES][16];
-    __shared__ __attribute__((aligned(16))) uint32_t corners[WAVES][CORNER];
+    uint32_t (*corners)[CORNER] = (uint32_t (*)[CORNER])lds, (*largest_of)[16] = (uint32_t (*)[16])(lds + WAVES * CORNER);
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row0 = (int64_t)blockIdx.x * 16, units = i8_steps(g.cols);
     const T *x = (const T *)g.x, *positive = (const T *)g.positive;
     v4i held[HELD ? HELD : 1][U::LOADS];
     uint32_t largest[U::LOADS] = {};
-    float factor[U::LOADS];
-#pragma unroll
-    for (int i = 0; i < U::LOADS; ++i) {
-        const int64_t r = row0 + unit_row<T>(i);
-        factor[i] = g.row_factor && r < g.rows ? g.row_factor[r] : 1.0f;
-    }
     // what the unit's values are as codes are made of them
     auto floats = [&](const v4i &raw, int64_t col0, float (&v)[U::N]) {
         piece_floats<T>(raw, v);
@@ -154,43 +135,22 @@ __global__ __launch_bounds__(WG) void rows_kernel(I8Rows g)
 #pragma unroll
             for (int e = 0; e < U::N; ++e) largest[i] = max(largest[i], magnitude_bits(v[e]));
         }
-        if (!g.partial) return;
-        float most[U::N] = {}, sum[U::N] = {};
-#pragma unroll
-        for (int i = 0; i < U::LOADS; ++i) {
-            float v[U::N];
-            piece_floats<T>(raw[i], v);
-#pragma unroll
-            for (int e = 0; e < U::N; ++e) {
-                sum[e] += v[e];
-                most[e] = MaxOf::of(most[e], __uint_as_float(magnitude_bits(v[e] * factor[i])));
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < U::N; ++e) most[e] = down_unit<MaxOf, T>(most[e]), sum[e] = down_unit<SumOf, T>(sum[e]);
-        if (lane >= U::LANES) return;
-        float *to = g.partial + (int64_t)blockIdx.x * 2 * g.cols;
-        const int64_t c = col0 + unit_col<T>();
-#pragma unroll
-        for (int e = 0; e < U::N; ++e)
-            if (c + e < g.cols) to[c + e] = most[e], to[g.cols + c + e] = sum[e];
     };
     if constexpr (HELD > 0) {
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) load_unit(x, positive, g.rows, g.cols, g.row_stride, row0, (wave + h * WAVES) * 64, held[h]);
+        for (int h = 0; h < HELD; ++h) load_unit<MASK>(x, positive, g.rows, g.cols, g.row_stride, row0, (wave + h * WAVES) * 64, held[h]);
 #pragma unroll
         for (int h = 0; h < HELD; ++h)
             if (wave + h * WAVES < units) look(held[h], (wave + h * WAVES) * 64);
     } else {
         for (int64_t u = wave; u < units; u += 2 * WAVES) {
             v4i two[2][U::LOADS];
-            load_unit(x, positive, g.rows, g.cols, g.row_stride, row0, u * 64, two[0]);
-            load_unit(x, positive, g.rows, g.cols, g.row_stride, row0, (u + WAVES) * 64, two[1]);
+            load_unit<MASK>(x, positive, g.rows, g.cols, g.row_stride, row0, u * 64, two[0]);
+            load_unit<MASK>(x, positive, g.rows, g.cols, g.row_stride, row0, (u + WAVES) * 64, two[1]);
             look(two[0], u * 64);
             if (u + WAVES < units) look(two[1], (u + WAVES) * 64);
         }
     }
-    if (!g.by_rows && !g.by_columns) return;
 #pragma unroll
     for (int i = 0; i < U::LOADS; ++i) {
         float m = __uint_as_float(largest[i]);
@@ -229,51 +189,119 @@ __global__ __launch_bounds__(WG) void rows_kernel(I8Rows g)
     } else {
         for (int64_t u = wave; u < units; u += 2 * WAVES) {
             v4i two[2][U::LOADS];
-            load_unit(x, positive, g.rows, g.cols, g.row_stride, row0, u * 64, two[0]);
-            load_unit(x, positive, g.rows, g.cols, g.row_stride, row0, (u + WAVES) * 64, two[1]);
+            load_unit<MASK>(x, positive, g.rows, g.cols, g.row_stride, row0, u * 64, two[0]);
+            load_unit<MASK>(x, positive, g.rows, g.cols, g.row_stride, row0, (u + WAVES) * 64, two[1]);
             encode(two[0], u * 64);
             if (u + WAVES < units) encode(two[1], (u + WAVES) * 64);
         }
     }
 }
 
+// Rows by themselves, for few of them: sixteen to a workgroup would leave most of the card idle.  LANES lanes hold a row, EACH
+// values each (0: the row is read again), and write its 16-byte pieces of the fragments' lines.
+template <typename T, int LANES, int EACH, bool MASK> __device__ __forceinline__ void convert_single_rows(const I8Rows &g, float *lds)
+{
+    constexpr int N = PIECE<T>, PIECES = EACH ? EACH / N : 1;
+    const int in_row = threadIdx.x % LANES;
+    const int64_t row = (int64_t)blockIdx.x * (WG / LANES) + threadIdx.x / LANES, steps = i8_steps(g.cols);
+    const T *x = (const T *)g.x, *positive = (const T *)g.positive;
+    RowLanes<LANES> lanes{(float (*)[RowLanes<LANES>::WAVES][2])lds};
+    auto load = [&](int64_t c) {
+        const int64_t count = row < g.rows ? g.cols - c : 0;
+        v4i raw = load_piece(x + row * g.row_stride + c, count);
+        if constexpr (MASK) {
+            const v4i keep = load_piece(positive + row * g.cols + c, count);
+            T v[N], y[N];
+            __builtin_memcpy(v, &raw, 16);
+            __builtin_memcpy(y, &keep, 16);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = to_float(y[e]) > 0.0f ? v[e] : (T)0.0f;
+            __builtin_memcpy(&raw, v, 16);
+        }
+        return raw;
+    };
+    auto floats = [&](v4i raw, int64_t c, float (&v)[N]) {
+        piece_floats<T>(raw, v);
+        if (!g.col_factor) return;
+        float f[N];
+        load_floats(g.col_factor, AMSIM_DTYPE_F32, c, g.cols - c, f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= f[e];
+    };
+    float largest = 0.0f;
+    auto look = [&](v4i raw, int64_t c) {
+        float v[N];
+        floats(raw, c, v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) largest = MaxOf::of(largest, __uint_as_float(magnitude_bits(v[e])));
+    };
+    auto store = [&](v4i raw, int64_t c, float multiplier) {
+        if (c >= steps * I8_STEP || row >= ceil_div64(g.rows, 16) * 16) return;
+        float v[N];
+        floats(raw, c, v);
+        store_codes(g.by_rows + (row / 16 * steps + c / 64) * 1024 + (c % 64 / 16 * 16 + row % 16) * 16 + c % 16, v, multiplier);
+    };
+    v4i raw[PIECES];
+    if constexpr (EACH > 0) {
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) raw[p] = load((int64_t)(p * LANES + in_row) * N);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) look(raw[p], (int64_t)(p * LANES + in_row) * N);
+    } else {
+#pragma unroll 4
+        for (int64_t c = in_row * N; c < g.cols; c += LANES * N) look(load(c), c);
+    }
+    largest = lanes.template one<MaxOf>(largest);
+    const float multiplier = q8_multiplier(__float_as_uint(largest));
+    if (in_row == 0 && row < g.rows) g.scales[row] = q8_scale(__float_as_uint(largest));
+    if constexpr (EACH > 0) {
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) store(raw[p], (int64_t)(p * LANES + in_row) * N, multiplier);
+    } else {
+#pragma unroll 4
+        for (int64_t c = in_row * N; c < steps * I8_STEP; c += LANES * N) store(load(c), c, multiplier);
+    }
+}
+
 // ---- along columns --------------------------------------------------------------------------------------------------
 
-// the largest magnitudes (and sums) of a slab of rows: [slabs][2][cols]
+// The largest magnitudes (and sums) in every column of a slab of rows: [slabs][2][cols].  A workgroup's waves take its rows in
+// turn, four of them under way at once.
 struct Look {
     const void *x, *positive;
+    int dtype;
     int64_t rows, cols, stride;
     const float *row_factor;
-    int64_t slab;
+    bool sums;
+    int64_t slab, across;    // rows of a slab, workgroups across
     float *partial;
 };
-template <typename T>
-__global__ __launch_bounds__(256) void columns_look_kernel(Look g)
+template <typename T, bool MASK> __device__ __forceinline__ void look_through(const Look &g, int64_t id, float *lds)
 {
     constexpr int N = PIECE<T>, AHEAD = 4;
-    __shared__ float most_of[4][64 * N], sum_of[4][64 * N];
-    const int lane = lane_id(), wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 * N + lane * N, from = (int64_t)blockIdx.y * g.slab, end = min(g.rows, from + g.slab);
+    float (*most_of)[64 * N] = (float (*)[64 * N])lds, (*sum_of)[64 * N] = most_of + WAVES;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t slab = id / g.across, col0 = id % g.across * 64 * N, c = col0 + lane * N, from = slab * g.slab, end = min(g.rows, from + g.slab);
     const T *x = (const T *)g.x, *positive = (const T *)g.positive;
     float most[N] = {}, sum[N] = {};
-    for (int64_t r = from + wave; r < end; r += 4 * AHEAD) {
-        v4i raw[AHEAD], keep[AHEAD];
+    for (int64_t r = from + wave; r < end; r += WAVES * AHEAD) {
+        v4i raw[AHEAD], keep[MASK ? AHEAD : 1];
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) {
-            const int64_t at = r + 4 * h;
+            const int64_t at = r + WAVES * h;
             raw[h] = load_piece(x + at * g.stride + c, at < end ? g.cols - c : 0);
-            if (positive) keep[h] = load_piece(positive + at * g.cols + c, at < end ? g.cols - c : 0);
+            if constexpr (MASK) keep[h] = load_piece(positive + at * g.cols + c, at < end ? g.cols - c : 0);
         }
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) {
-            const int64_t at = r + 4 * h;
+            const int64_t at = r + WAVES * h;
             const float f = g.row_factor && at < end ? g.row_factor[at] : 1.0f;
             float v[N], y[N];
             piece_floats<T>(raw[h], v);
-            if (positive) piece_floats<T>(keep[h], y);
+            if constexpr (MASK) piece_floats<T>(keep[h], y);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                if (positive && !(y[e] > 0.0f)) v[e] = 0.0f;
+                if (MASK && !(y[e] > 0.0f)) v[e] = 0.0f;
                 sum[e] += v[e];
                 most[e] = MaxOf::of(most[e], __uint_as_float(magnitude_bits(v[e] * f)));
             }
@@ -282,72 +310,111 @@ __global__ __launch_bounds__(256) void columns_look_kernel(Look g)
 #pragma unroll
     for (int e = 0; e < N; ++e) most_of[wave][lane * N + e] = most[e], sum_of[wave][lane * N + e] = sum[e];
     __syncthreads();
-    float *to = g.partial + (int64_t)blockIdx.y * 2 * g.cols;
-    for (int i = threadIdx.x; i < 64 * N; i += 256) {
-        const int64_t col = (int64_t)blockIdx.x * 64 * N + i;
-        if (col >= g.cols) break;
+    float *to = g.partial + slab * 2 * g.cols;
+    for (int i = threadIdx.x; i < 64 * N; i += WG) {
+        if (col0 + i >= g.cols) break;
         float m = most_of[0][i], s = sum_of[0][i];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) m = MaxOf::of(m, most_of[w][i]), s += sum_of[w][i];
-        to[col] = m, to[g.cols + col] = s;
+        for (int w = 1; w < WAVES; ++w) m = MaxOf::of(m, most_of[w][i]), s += sum_of[w][i];
+        to[col0 + i] = m;
+        if (g.sums) to[g.cols + col0 + i] = s;
     }
 }
 
-// of [parts][2][cols]: multipliers, scales and sums.  32 columns and 32 runs of parts to a workgroup, the runs joined in pairs.
-struct Join {
-    const float *partial;
-    int64_t parts, cols;
-    float *multipliers, *scales;
-    void *sums;
-    int sums_dtype;
-};
-__global__ __launch_bounds__(1024) void columns_join_kernel(Join g)
+// How rows are converted: by sixteen with 0 to 8 units of a wave held, or by themselves.
+constexpr int LANES_64 = -1, LANES_512 = -2, LANES_512_TWICE = -3, LANES_512_AGAIN = -4;
+
+// A conversion along rows, a look through columns, or both beside each other (the two do not wait for each other).
+constexpr int LDS_FLOATS = 2 * WAVES * 64 * PIECE<__bf16>;
+template <typename T, int HOW, bool MASK> __global__ __launch_bounds__(WG, HOW == 8 && sizeof(T) == 4 ? 2 : 4) void rows_and_look_kernel(I8Rows rows, unsigned row_blocks, Look look)
 {
-    __shared__ float most_of[32][33], sum_of[32][33];
-    const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int64_t col = (int64_t)blockIdx.x * 32 + c, each = ceil_div64(g.parts, 32), end = min(g.parts, each * (w + 1));
-    float m = 0.0f, s = 0.0f;
-    if (col < g.cols) {
-#pragma unroll 4
-        for (int64_t p = each * w; p < end; ++p) {
-            m = MaxOf::of(m, g.partial[p * 2 * g.cols + col]);
-            if (g.sums) s += g.partial[(p * 2 + 1) * g.cols + col];
-        }
+    __shared__ __attribute__((aligned(16))) float lds[LDS_FLOATS];
+    static_assert(LDS_FLOATS >= WAVES * (CORNER + 16), "");
+    if (blockIdx.x < row_blocks) {
+        if constexpr (HOW >= 0) convert_rows<T, HOW, MASK>(rows, (uint32_t *)lds);
+        else if constexpr (HOW == LANES_64) convert_single_rows<T, 64, 16, MASK>(rows, lds);
+        else if constexpr (HOW == LANES_512) convert_single_rows<T, 512, 8, MASK>(rows, lds);
+        else if constexpr (HOW == LANES_512_TWICE) convert_single_rows<T, 512, 16, MASK>(rows, lds);
+        else convert_single_rows<T, 512, 0, MASK>(rows, lds);
+        return;
     }
-    most_of[w][c] = m, sum_of[w][c] = s;
-    for (int half = 16; half; half /= 2) {
-        __syncthreads();
-        if (w < half) most_of[w][c] = MaxOf::of(most_of[w][c], most_of[w + half][c]), sum_of[w][c] += sum_of[w + half][c];
+    const int64_t id = blockIdx.x - row_blocks;
+    if (look.dtype == AMSIM_DTYPE_F32) look_through<float, MASK>(look, id, lds);
+    else if (look.dtype == AMSIM_DTYPE_BF16) look_through<__bf16, MASK>(look, id, lds);
+    else look_through<_Float16, MASK>(look, id, lds);
+}
+
+// A wavefront's 64 columns over the slabs, joined by maximum or sum: 16 lanes' loads are 64 columns of a slab, four slabs
+// to a load, eight loads under way.  In every lane: those of columns 4 (lane % 16) and the three that follow.
+template <typename Op> __device__ __forceinline__ v4f over_slabs(const float *partial, int64_t slabs, int64_t cols, int64_t col0)
+{
+    constexpr int AHEAD = 8;
+    const int lane = lane_id();
+    const int64_t c = col0 + lane % 16 * 4;
+    v4f all = {0, 0, 0, 0};
+    for (int64_t p = lane / 16; p < ceil_div64(slabs, 4) * 4; p += 4 * AHEAD) {
+        v4f v[AHEAD];
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h) v[h] = __builtin_bit_cast(v4f, load_piece(partial + (p + 4 * h) * 2 * cols + c, p + 4 * h < slabs ? cols - c : 0));
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) all[e] = Op::of(all[e], v[h][e]);
     }
-    if (w != 0 || col >= g.cols) return;
-    if (g.multipliers) {
-        const uint32_t largest = __float_as_uint(most_of[0][c]);
-        g.multipliers[col] = q8_multiplier(largest);
-        g.scales[col] = q8_scale(largest);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(all[e]), __float_as_uint(all[e]), false, false);
+        all[e] = Op::of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(all[e]), __float_as_uint(all[e]), false, false);
+        all[e] = Op::of(__uint_as_float(h[0]), __uint_as_float(h[1]));
     }
-    if (g.sums) store_from_float(g.sums, g.sums_dtype, col, sum_of[0][c]);
+    return all;
 }
 
 // A workgroup of four waves takes 64 rows (a step of the columns' operand), four units in turn to a wave.
-template <typename T>
-__global__ __launch_bounds__(256) void columns_kernel(I8Columns g, const float *multipliers)
+template <typename T, bool MASK>
+__global__ __launch_bounds__(256) void columns_kernel(I8Columns g, const float *partial, int64_t slabs)
 {
     using U = Unit<T>;
     __shared__ __attribute__((aligned(16))) uint32_t corners[4][CORNER];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t units = i8_steps(g.cols), across = ceil_div64(units, 4), u = (int64_t)blockIdx.x % across * 4 + wave, step = (int64_t)blockIdx.x / across;
     if (u >= units) return;
-    const int64_t col0 = u * 64, c = col0 + unit_col<T>();
-    float multiplier[U::N];
-    load_floats(multipliers, AMSIM_DTYPE_F32, c, g.cols - c, multiplier);
+    const int64_t col0 = u * 64, first = col0 + lane * 4;
+    const bool codes = g.by_rows || g.by_columns;
     v4i raw[4][U::LOADS];
+    if (codes)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) load_unit((const T *)g.x, (const T *)g.positive, g.rows, g.cols, g.row_stride, step * 64 + 16 * q, col0, raw[q]);
+        for (int q = 0; q < 4; ++q) load_unit<MASK>((const T *)g.x, (const T *)g.positive, g.rows, g.cols, g.row_stride, step * 64 + 16 * q, col0, raw[q]);
+    if (step == 0 && g.sums) {
+        const v4f s = over_slabs<SumOf>(partial + g.cols, slabs, g.cols, col0);
+        if (lane < 16)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (first + e < g.cols) store_from_float(g.sums, g.sums_dtype, first + e, s[e]);
+    }
+    if (!codes) return;
+    const v4f most = over_slabs<MaxOf>(partial, slabs, g.cols, col0);
+    if (lane < 16) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t largest = __float_as_uint(most[e]);
+            corners[wave][4 * lane + e] = __float_as_uint(q8_multiplier(largest));
+            if (step == 0 && first + e < g.cols) g.scales[first + e] = q8_scale(largest);
+        }
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    float multiplier[U::N];
+#pragma unroll
+    for (int e = 0; e < U::N; ++e) multiplier[e] = __uint_as_float(corners[wave][unit_col<T>() + e]);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const int64_t row0 = step * 64 + 16 * q;
         if (row0 >= g.rows) break;
-        Codes<U::N> codes;
+        Codes<U::N> unit;
 #pragma unroll
         for (int i = 0; i < U::LOADS; ++i) {
             const int64_t r = row0 + unit_row<T>(i);
@@ -358,11 +425,11 @@ __global__ __launch_bounds__(256) void columns_kernel(I8Columns g, const float *
             for (int d = 0; d < U::N / 4; ++d) {
                 uint32_t b[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) b[e] = q8_code(g.row_factor ? v[4 * d + e] * f : v[4 * d + e], multiplier[4 * d + e]) & 255u;
-                codes.w[i][d] = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+                for (int e = 0; e < 4; ++e) b[e] = q8_code(g.row_factor ? v[4 * d + e] * f : v[4 * d + e], multiplier[4 * d + e]);
+                unit.w[i][d] = q8_pack(b[0], b[1], b[2], b[3]);
             }
         }
-        store_unit<T>(codes, corners[wave], g.rows, g.cols, row0, col0, g.by_rows, g.by_columns);
+        store_unit<T>(unit, corners[wave], g.rows, g.cols, row0, col0, g.by_rows, g.by_columns);
     }
 }
 
@@ -394,52 +461,63 @@ template <typename Fn> int with_type(int dtype, Fn &&fn)
     }
 }
 
+// Slabs of rows that are looked through: enough workgroups for the card beside those that convert rows, few enough for
+// every wavefront that converts columns to join them by itself.
 int64_t slab_rows(int64_t rows, int64_t cols)
 {
-    const int64_t across = ceil_div64(cols, 256), slabs = std::max<int64_t>(1, std::min<int64_t>(ceil_div64(rows, 32), 2048 / across));
-    return ceil_div64(ceil_div64(rows, slabs), 16) * 16;
+    const int64_t slabs = std::min(ceil_div64(rows, 64), std::max<int64_t>(16, 128 / ceil_div64(cols, 256)));
+    return ceil_div64(rows, slabs);
 }
 
-constexpr int64_t MOST_BLOCKS = 1 << 22;  // (of up to 1024 threads: a launch has less than 2^32)
+constexpr int64_t MOST_BLOCKS = 1 << 22;  // (of up to 512 threads: a launch has less than 2^32)
+
+// Whether rows are converted by themselves: us so, and by sixteen, of bf16 rows of 4096: 16 rows 4.9 and 7.7, 512 rows 4.5 and 8.2,
+// 1024 rows 6.8 and 8.8, 2048 rows 10.0 and 10.3, 4096 rows 17.6 and 12.9 (pieces of 16 bytes from different workgroups fill a
+// line); 2048 rows of 10000 24.9 and 21.9.
+bool single_rows(const I8Rows &j) { return !j.by_columns && j.rows <= 1024; }
+
+template <typename T, int HOW> void launch_rows_and_look(const I8Rows &rows, unsigned row_blocks, const Look &look, unsigned look_blocks, hipStream_t stream)
+{
+    const auto kernel = rows.positive || look.positive ? rows_and_look_kernel<T, HOW, true> : rows_and_look_kernel<T, HOW, false>;
+    kernel<<<row_blocks + look_blocks, WG, 0, stream>>>(rows, row_blocks, look);
+}
 
 }  // namespace
 
-int i8_convert_rows(const I8Rows &j, hipStream_t stream)
-{
-    const int64_t blocks = ceil_div64(j.rows, 16), each = ceil_div64(i8_steps(j.cols), WAVES);
-    if (blocks >= MOST_BLOCKS) return fail(AMSIM_ERR_UNSUPPORTED, "int8: more rows than one launch takes");
-    return with_type(j.dtype, [&](auto zero) {
-        using T = decltype(zero);
-        const auto kernel = each == 1 ? rows_kernel<T, 1> : each == 2 ? rows_kernel<T, 2> : each <= 4 ? rows_kernel<T, 4> : each <= 8 ? rows_kernel<T, 8> : rows_kernel<T, 0>;
-        kernel<<<(unsigned)blocks, WG, 0, stream>>>(j);
-        AMSIM_HIP_CHECK(hipGetLastError());
-        return (int)AMSIM_OK;
-    });
-}
+int64_t i8_partial_floats(int64_t rows, int64_t cols) { return ceil_div64(rows, slab_rows(rows, cols)) * 2 * cols; }
 
-int64_t i8_columns_workspace(int64_t rows, int64_t cols) { return ceil_div64(rows, slab_rows(rows, cols)) * 2 * cols + cols; }
-
-int i8_convert_columns(const I8Columns &j, float *workspace, hipStream_t stream)
+int i8_convert(const I8Rows *rows, const I8Columns *columns, float *partial, hipStream_t stream)
 {
-    const int64_t slab = slab_rows(j.rows, j.cols), slabs = ceil_div64(j.rows, slab);
-    const int64_t blocks = ceil_div64(i8_steps(j.cols), 4) * ceil_div64(j.rows, 64);
-    if (blocks >= MOST_BLOCKS || ceil_div64(j.cols, 32) >= MOST_BLOCKS) return fail(AMSIM_ERR_UNSUPPORTED, "int8: more columns than one launch takes");
-    float *multipliers = workspace, *partial = workspace + j.cols;
-    return with_type(j.dtype, [&](auto zero) {
-        using T = decltype(zero);
-        if (!j.partial) {
-            const Look look{j.x, j.positive, j.rows, j.cols, j.row_stride, j.row_factor, slab, partial};
-            columns_look_kernel<T><<<dim3((unsigned)ceil_div64(j.cols, 64 * PIECE<T>), (unsigned)slabs), 256, 0, stream>>>(look);
+    Look look{};
+    int64_t row_blocks = 0, look_blocks = 0, blocks = 0, slabs = 0;
+    if (rows) row_blocks = ceil_div64(rows->rows, 16) * (!single_rows(*rows) ? 1 : rows->cols <= 1024 ? 2 : 16);
+    if (columns) {
+        const I8Columns &c = *columns;
+        look = Look{c.x, c.positive, c.dtype, c.rows, c.cols, c.row_stride, c.row_factor, c.sums != nullptr, slab_rows(c.rows, c.cols),
+                    ceil_div64(c.cols, c.dtype == AMSIM_DTYPE_F32 ? 64 * PIECE<float> : 64 * PIECE<__bf16>), partial};
+        slabs = ceil_div64(c.rows, look.slab);
+        look_blocks = slabs * look.across;
+        blocks = ceil_div64(i8_steps(c.cols), 4) * (c.by_rows || c.by_columns ? ceil_div64(c.rows, 64) : 1);
+    }
+    if (row_blocks + look_blocks >= MOST_BLOCKS || blocks >= MOST_BLOCKS) return fail(AMSIM_ERR_UNSUPPORTED, "int8: more values than one launch takes");
+    if (const int rc = with_type(rows ? rows->dtype : AMSIM_DTYPE_F32, [&](auto zero) {
+            using T = decltype(zero);
+            const I8Rows j = rows ? *rows : I8Rows{};
+            const int64_t each = ceil_div64(i8_steps(j.cols), WAVES);  // units of a wave
+            const auto launch = rows && single_rows(j) ? j.cols <= 1024 ? launch_rows_and_look<T, LANES_64> : j.cols <= 4096 ? launch_rows_and_look<T, LANES_512>
+                                  : j.cols <= 8192 ? launch_rows_and_look<T, LANES_512_TWICE> : launch_rows_and_look<T, LANES_512_AGAIN>
+                              : each <= 1 ? launch_rows_and_look<T, 1> : each == 2 ? launch_rows_and_look<T, 2> : each <= 4 ? launch_rows_and_look<T, 4>
+                              : each <= 8 ? launch_rows_and_look<T, 8> : launch_rows_and_look<T, 0>;
+            launch(j, (unsigned)row_blocks, look, (unsigned)look_blocks, stream);
             AMSIM_HIP_CHECK(hipGetLastError());
-        }
-        const bool codes = j.by_rows || j.by_columns;
-        const Join join{j.partial ? j.partial : partial, j.partial ? ceil_div64(j.rows, 16) : slabs, j.cols, codes ? multipliers : nullptr, j.scales, j.sums, j.sums_dtype};
-        columns_join_kernel<<<(unsigned)ceil_div64(j.cols, 32), 1024, 0, stream>>>(join);
+            return (int)AMSIM_OK;
+        }))
+        return rc;
+    if (!columns) return AMSIM_OK;
+    return with_type(columns->dtype, [&](auto zero) {
+        const auto kernel = columns->positive ? columns_kernel<decltype(zero), true> : columns_kernel<decltype(zero), false>;
+        kernel<<<(unsigned)blocks, 256, 0, stream>>>(*columns, partial, slabs);
         AMSIM_HIP_CHECK(hipGetLastError());
-        if (codes) {
-            columns_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(j, multipliers);
-            AMSIM_HIP_CHECK(hipGetLastError());
-        }
         return (int)AMSIM_OK;
     });
 }
@@ -455,7 +533,7 @@ size_t amsim_i8_operand_bytes(int64_t rows, int64_t length)
     return i8_extents_fit(rows, length) && rows && length ? (size_t)i8_bytes(rows, length) : 0;
 }
 
-size_t amsim_i8_quantize_workspace_bytes(int64_t rows, int64_t cols) { return i8_extents_fit(cols, rows) && rows && cols ? (size_t)i8_columns_workspace(rows, cols) * 4 : 0; }
+size_t amsim_i8_quantize_workspace_bytes(int64_t rows, int64_t cols) { return i8_extents_fit(cols, rows) && rows && cols ? (size_t)i8_partial_floats(rows, cols) * 4 : 0; }
 
 int amsim_i8_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void *by_rows, void *by_columns, void *workspace,
                       size_t workspace_bytes, void *stream)
@@ -469,14 +547,10 @@ int amsim_i8_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int6
     if (((uintptr_t)x & (element_bytes(dtype) - 1)) || ((uintptr_t)by_rows & 15) || ((uintptr_t)by_columns & 15)) return fail(AMSIM_ERR_INVALID, "int8: misaligned pointer");
     if (by_columns && (!workspace || workspace_bytes < amsim_i8_quantize_workspace_bytes(rows, cols) || ((uintptr_t)workspace & 255)))
         return fail(AMSIM_ERR_WORKSPACE, "int8: workspace missing, misaligned or too small");
-    if (by_rows) {
-        const I8Rows j{x, nullptr, dtype, rows, cols, row_stride, nullptr, (uint8_t *)by_rows, nullptr, (float *)((uint8_t *)by_rows + i8_code_bytes(rows, cols)), nullptr, nullptr};
-        if (int rc = i8_convert_rows(j, (hipStream_t)stream)) return rc;
-    }
-    if (!by_columns) return AMSIM_OK;
-    const I8Columns j{x, nullptr, dtype, rows, cols, row_stride, nullptr, nullptr, (uint8_t *)by_columns, (float *)((uint8_t *)by_columns + i8_code_bytes(cols, rows)),
-                      nullptr, 0, nullptr};
-    return i8_convert_columns(j, (float *)workspace, (hipStream_t)stream);
+    const I8Rows r{x, nullptr, dtype, rows, cols, row_stride, nullptr, (uint8_t *)by_rows, nullptr, (float *)((uint8_t *)by_rows + i8_code_bytes(rows, cols))};
+    const I8Columns c{x, nullptr, dtype, rows, cols, row_stride, nullptr, nullptr, (uint8_t *)by_columns, (float *)((uint8_t *)by_columns + i8_code_bytes(cols, rows)),
+                      nullptr, 0};
+    return i8_convert(by_rows ? &r : nullptr, by_columns ? &c : nullptr, (float *)workspace, (hipStream_t)stream);
 }
 
 int amsim_i8_dequantize(const void *q, int64_t rows, int64_t length, int dtype, void *out, void *stream)

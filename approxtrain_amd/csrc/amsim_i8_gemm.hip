@@ -207,14 +207,28 @@ struct FewSteps {
     }
 };
 
+// What the results are scaled by and added to, under way since the kernel's start: behind the sums each would be another
+// round trip to memory.
+struct FewEnds {
+    float scale[4], bias[4];
+    __device__ __forceinline__ void load(const FewArgs &g, int64_t f)
+    {
+        const int64_t n = f * 16 + (threadIdx.x & 63) / 16 * 4, N = g.b.rows;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            scale[e] = scale_of(g.b.scales, n + e, N);
+            bias[e] = g.bias && n + e < N ? load_as_float(g.bias, g.bias_dtype, n + e) : 0.0f;
+        }
+    }
+};
+
 // the fragments' sums over the waves and their results, a fragment to a wave; row_scales: of the rows, in LDS or memory
-template <int FA> __device__ __forceinline__ void finish_few(const FewArgs &g, int64_t f, v4i *sums, const v4i (&acc)[FA], const float *row_scales)
+template <int FA>
+__device__ __forceinline__ void finish_few(const FewArgs &g, const FewEnds &ends, int64_t f, v4i *sums, const v4i (&acc)[FA], const float *row_scales)
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int64_t n = f * 16 + lane / 16 * 4, N = g.b.rows;
-    float sb[4], sa[FA];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sb[e] = scale_of(g.b.scales, n + e, N);
+    float sa[FA];
 #pragma unroll
     for (int i = 0; i < FA; ++i) sa[i] = scale_of(row_scales, 16 * i + lane % 16, g.rows);
 #pragma unroll
@@ -229,8 +243,8 @@ template <int FA> __device__ __forceinline__ void finish_few(const FewArgs &g, i
         if (m >= g.rows || n >= N) continue;
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = scaled((float)z[e], sa[i], sb[e]);
-        finish4(g.bias, g.bias_dtype, g.act, g.out, g.out_dtype, m, n, N, v);
+        for (int e = 0; e < 4; ++e) v[e] = scaled((float)z[e], sa[i], ends.scale[e]) + ends.bias[e];
+        finish4(nullptr, 0, g.act, g.out, g.out_dtype, m, n, N, v);
     }
 }
 
@@ -240,6 +254,8 @@ __global__ __launch_bounds__(1024) void few_kernel(FewArgs g)
 {
     __shared__ v4i sums[16 * FA * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    FewEnds ends;
+    ends.load(g, blockIdx.x);
     v4i acc[FA] = {};
     for (int64_t s = wave; s < g.steps; s += AHEAD * waves) {
         FewSteps b;
@@ -254,23 +270,25 @@ __global__ __launch_bounds__(1024) void few_kernel(FewArgs g)
             for_each<FA>([&](auto i) { acc[i.value] = mfma(b.codes[h], a[i.value], acc[i.value]); });
         }
     }
-    finish_few(g, blockIdx.x, sums, acc, g.a.scales);
+    finish_few(g, ends, blockIdx.x, sums, acc, g.a.scales);
 }
 
-// FA fragments of rows as they come: every workgroup converts them for itself, into LDS, while its first loads of b are
+// Up to 16 rows as they come: every workgroup converts them for itself, into LDS, while its first loads of b are
 // under way.  A row belongs to a group of waves (all of them for one row, one from nine rows on), whose lanes hold
 // its pieces of 8 values in registers between the search for the largest and the codes.
-constexpr int64_t RAW_VALUES = 32768;  // rows x length (in whole steps) that it converts
-template <typename X, int FA>
+constexpr int64_t RAW_ROWS = 16, RAW_VALUES = 32768;  // rows, and rows x length (in whole steps), that it converts
+template <typename X>
 __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t converted[];  // codes [16 values][row][16 bytes]; then the sums
-    __shared__ uint32_t largest_of[16];
-    __shared__ float row_scales[64];
+    __shared__ uint32_t largest_of[2][16];
+    __shared__ float row_scales[RAW_ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int rows = (int)g.rows, apart = rows | 1, pieces = (int)g.steps * 8;  // (an odd distance: a row's 16 values lie in different banks)
     FewSteps b;
     b.load(g, blockIdx.x, wave, waves);
+    FewEnds ends;
+    ends.load(g, blockIdx.x);
     int together = waves;  // waves to a row: a power of two
     while (together > 1 && together * rows > waves) together /= 2;
     const int group = wave / together, groups = waves / together, first = wave % together * 64 + lane;
@@ -302,10 +320,10 @@ __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
         }
         largest = __float_as_uint(over_lanes<MaxOf, 64>(__uint_as_float(largest)));
         if (together > 1) {  // (the same in every wave)
-            if (lane == 0) largest_of[wave] = largest;
+            uint32_t *of = largest_of[round & 1];  // (who writes one half has met everybody since it was read)
+            if (lane == 0) of[wave] = largest;
             __syncthreads();
-            for (int w = 0; w < together; ++w) largest = max(largest, largest_of[group * together + w]);
-            __syncthreads();
+            for (int w = 0; w < together; ++w) largest = max(largest, of[group * together + w]);
         }
         if (r >= rows) continue;
         if (first == 0) row_scales[r] = q8_scale(largest);
@@ -325,22 +343,19 @@ __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
         }
     }
     __syncthreads();
-    int row[FA];
-#pragma unroll
-    for (int i = 0; i < FA; ++i) row[i] = min(16 * i + lane % 16, rows - 1);  // (results of rows that do not exist are not stored)
-    v4i acc[FA] = {};
+    const int row = min(lane % 16, rows - 1);  // (results of rows that do not exist are not stored)
+    v4i acc[1] = {};
     for (int64_t s = wave; s < g.steps; s += AHEAD * waves) {
         if (s != wave) b.load(g, blockIdx.x, s, waves);
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) {
             const int t = (int)s + h * waves;
             if (t >= g.steps) break;
-#pragma unroll
-            for (int i = 0; i < FA; ++i) acc[i] = mfma(b.codes[h], *(const v4i *)(converted + ((4 * t + lane / 16) * apart + row[i]) * 16), acc[i]);
+            acc[0] = mfma(b.codes[h], *(const v4i *)(converted + ((4 * t + lane / 16) * apart + row) * 16), acc[0]);
         }
     }
     __syncthreads();  // (the sums take the place of what was converted)
-    finish_few(g, blockIdx.x, (v4i *)converted, acc, row_scales);
+    finish_few(g, ends, blockIdx.x, (v4i *)converted, acc, row_scales);
 }
 
 // The sums of split reductions, added in 64 bits.
@@ -386,13 +401,19 @@ __global__ __launch_bounds__(FINISH_WG) void finish_kernel(FinishArgs f)
     finish4(g.bias, g.bias_dtype, g.act, g.out, g.out_dtype, m, n, N, v);
 }
 
+// As the 4-bit products': a step is as many bytes and as long on the matrix units.  Over twenty shapes of 100 to 8192 rows, 300 to
+// 8192 columns and lengths of 128 to 16384 the choice takes at most 1.12 times the best tile's time, 1.02 on average.  Tiles of
+// 256 x 256 in waves of 128 x 64 results: 4096^3 54.5 us (2.5 POP/s), in waves of 64 x 128 55.2, of 128 x 128 (four waves) 69; 8192^3 395
+// (2.8; the instruction alone, from registers, runs at 3.5 on random operands, which the card's power allows, and at 4.6 on zeros).
 struct Costs {
     static constexpr Tile TILES[] = {{256, 256, 256, 2.2, 0.55, 0.785, 10.8},  // (stored by a round at once)
                                      {256, 128, 512, 6.5, 0.5, 0.85, 0.0124}, {128, 128, 512, 5, 0.2, 0.46, 0.01}, {64, 64, 1024, 4, 0.1, 0.4, 0.003}};
     static constexpr int64_t STEP = I8_STEP, MOST_STEPS = I8_MOST_STEPS;
 };
 
-// Whether few_kernel serves, by rows and length alone: a reduction beyond that needs more than one workgroup's waves.
+// Whether few_kernel serves, by rows and length alone: a reduction beyond that needs more than one workgroup's waves.  us of the
+// product by itself, few_kernel / tiles, of 16, 32 and 64 rows: length 4096, 4096 wide 5.2/10.0, 6.2/11.5, 8.7/11.5; length 8192, 1024
+// wide 6.0/11.9, 7.7/10.5, 12.5/11.5; length 1024, 8192 wide 4.4/5.3, 5.3/5.3, 7.1/5.4.
 bool few(int64_t m, int64_t k) { return m <= 64 && i8_steps(k) <= 256; }
 
 // the products of a list that go in tiles, and the others
@@ -428,19 +449,19 @@ int launch_few(void (*kernel)(FewArgs), const FewArgs &g, int waves, int64_t lds
     AMSIM_HIP_CHECK(hipGetLastError());
     return AMSIM_OK;
 }
-// A wave for every step, and for 128 of the pieces of 8 values that are to be converted first.
+// A wave for every step, and for 128 of the pieces of 8 values that are to be converted first.  Eight waves for up to four rows
+// (one token of 4096 x 4096: 6.3 us, 7.0 with sixteen; of 8192 x 8192 12.8 and 15.2), sixteen for more (8 rows: 8.8 and 8.1).
 int few_waves(const FewArgs &g, int64_t pieces)
 {
+    const int most = g.rows <= 4 ? 8 : 16;
     int waves = 1;
-    while (waves < 16 && (waves < g.steps || 128 * waves < pieces)) waves *= 2;
+    while (waves < most && (waves < g.steps || 128 * waves < pieces)) waves *= 2;
     return waves;
 }
 template <typename X> int launch_raw(const FewArgs &g, hipStream_t stream)
 {
-    // (eight waves' sums of four fragments are 32 KB of LDS, sixteen waves' with the rest would be more than 64)
-    const int fragments = g.rows <= 16 ? 1 : g.rows <= 32 ? 2 : 4, waves = std::min(few_waves(g, g.rows * g.steps * 8), fragments == 4 ? 8 : 16);
-    const int64_t lds = std::max<int64_t>(g.steps * 4 * (g.rows | 1) * 16, waves * fragments * 1024);
-    return launch_few(fragments == 1 ? raw_kernel<X, 1> : fragments == 2 ? raw_kernel<X, 2> : raw_kernel<X, 4>, g, waves, lds, stream);
+    const int waves = few_waves(g, g.rows * g.steps * 8);
+    return launch_few(raw_kernel<X>, g, waves, std::max<int64_t>(g.steps * 4 * (g.rows | 1) * 16, waves * 1024), stream);
 }
 
 struct Product {
@@ -486,7 +507,7 @@ int products(const Product *list, int count, void *workspace, hipStream_t stream
         if (blocks >= (1ll << 22)) return fail(AMSIM_ERR_UNSUPPORTED, "int8: more tiles than one launch takes");
     }
     switch (p.tile) {
-    case 0: gemm_kernel<4, 8, 4, 2, 4, 2><<<(unsigned)blocks, 512, 0, stream>>>(jobs); break;
+    case 0: gemm_kernel<8, 4, 2, 4, 4, 2><<<(unsigned)blocks, 512, 0, stream>>>(jobs); break;
     case 1: gemm_kernel<8, 4, 2, 2, 3, 2><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
     case 2: gemm_kernel<4, 4, 2, 2, 4, 2><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
     default: gemm_kernel<2, 2, 2, 2, 4, 4><<<(unsigned)blocks, WG, 0, stream>>>(jobs); break;
@@ -519,12 +540,10 @@ int check_workspace(const void *workspace, size_t have, size_t need)
     return AMSIM_OK;
 }
 
-// Whether few rows are converted by every workgroup that multiplies them, not once ahead.
-bool converts_on_the_way(int64_t m, int64_t n, int64_t k)
-{
-    const int64_t values = m * i8_steps(k) * I8_STEP;
-    return m <= 64 && values * ceil_div64(n, 4096) <= RAW_VALUES;
-}
+// Whether few rows are converted by every workgroup that multiplies them, not once ahead.  us so, and ahead: one token of 4096
+// x 4096 6.3 and 8.5, 4 rows 6.5 and 8.4, 8 rows 7.8 and 8.2; 16 rows of 1024 x 1024 5.7 and 6.7, 32 rows 7.3 and 7.0; 64 rows of 512 x
+// 512 10.5 and 7.4 (a wave's rows wait for memory one after the other).
+bool converts_on_the_way(int64_t m, int64_t n, int64_t k) { return m <= RAW_ROWS && m * i8_steps(k) * I8_STEP * ceil_div64(n, 4096) <= RAW_VALUES; }
 
 size_t aligned(int64_t bytes) { return ((size_t)bytes + 255) / 256 * 256; }
 size_t operand_bytes(int64_t rows, int64_t length) { return aligned(i8_bytes(rows, length)); }
@@ -594,7 +613,8 @@ int amsim_i8_linear(const void *x, int dtype, int64_t row_stride, const void *w,
     }
     uint8_t *codes = (uint8_t *)workspace;
     float *scales = (float *)(codes + i8_code_bytes(m, k));
-    if (int rc = i8_convert_rows({x, nullptr, dtype, m, k, row_stride, nullptr, codes, nullptr, scales, nullptr, nullptr}, (hipStream_t)stream)) return rc;
+    const I8Rows job{x, nullptr, dtype, m, k, row_stride, nullptr, codes, nullptr, scales};
+    if (int rc = i8_convert(&job, nullptr, nullptr, (hipStream_t)stream)) return rc;
     return product({operand(codes, scales, m), operand(w, n, k), k, bias, bias_dtype, act, out, dtype}, codes + operand_bytes(m, k), (hipStream_t)stream);
 }
 
@@ -602,7 +622,7 @@ size_t amsim_i8_kept_bytes(int64_t rows, int64_t length) { return i8_extents_fit
 
 size_t amsim_i8_dense_workspace_bytes(int64_t m, int64_t n, int64_t k)
 {
-    return product_fits(m, n, k) ? operand_bytes(m, k) + operand_bytes(n, k) + aligned(4 * i8_columns_workspace(k, n)) + product_workspace(m, n, k) : 0;
+    return product_fits(m, n, k) ? operand_bytes(m, k) + operand_bytes(n, k) + aligned(4 * i8_partial_floats(k, n)) + product_workspace(m, n, k) : 0;
 }
 
 int amsim_i8_dense(const void *x, int dtype, int64_t row_stride, const void *kernel, int kernel_dtype, int64_t kernel_row_stride,
@@ -620,15 +640,14 @@ int amsim_i8_dense(const void *x, int dtype, int64_t row_stride, const void *ker
     if (int rc = check_workspace(workspace, workspace_bytes, amsim_i8_dense_workspace_bytes(m, n, k))) return rc;
     hipStream_t s = (hipStream_t)stream;
     uint8_t *x_rows = (uint8_t *)workspace, *kernel_columns = x_rows + operand_bytes(m, k);
-    float *columns = (float *)(kernel_columns + operand_bytes(n, k));
-    void *partial = (uint8_t *)columns + aligned(4 * i8_columns_workspace(k, n));
+    float *looked = (float *)(kernel_columns + operand_bytes(n, k));
+    void *partial = (uint8_t *)looked + aligned(4 * i8_partial_floats(k, n));
     // (where they are kept, the scales lie with the codes that are)
     float *x_scales = x_kept ? (float *)kept_scales(x_kept, k, m) : (float *)(x_rows + i8_code_bytes(m, k));
     float *kernel_scales = kernel_kept ? (float *)kept_scales(kernel_kept, k, n) : (float *)(kernel_columns + i8_code_bytes(n, k));
-    if (int rc = i8_convert_rows({x, nullptr, dtype, m, k, row_stride, nullptr, x_rows, (uint8_t *)x_kept, x_scales, nullptr, nullptr}, s)) return rc;
-    if (int rc = i8_convert_columns({kernel, nullptr, kernel_dtype, k, n, kernel_row_stride, nullptr, (uint8_t *)kernel_kept, kernel_columns, kernel_scales,
-                                     nullptr, 0, nullptr}, columns, s))
-        return rc;
+    const I8Rows rows{x, nullptr, dtype, m, k, row_stride, nullptr, x_rows, (uint8_t *)x_kept, x_scales};
+    const I8Columns columns{kernel, nullptr, kernel_dtype, k, n, kernel_row_stride, nullptr, (uint8_t *)kernel_kept, kernel_columns, kernel_scales, nullptr, 0};
+    if (int rc = i8_convert(&rows, &columns, looked, s)) return rc;
     return product({operand(x_rows, x_scales, m), operand(kernel_columns, kernel_scales, n), k, bias, bias_dtype, act, out, dtype}, partial, s);
 }
 
@@ -637,7 +656,7 @@ size_t amsim_i8_dense_grad_workspace_bytes(int64_t m, int64_t n, int64_t k)
     if (!product_fits(m, n, k) || !i8_extents_fit(k, n) || !i8_extents_fit(k, m)) return 0;
     const Extents e[2] = {{m, k, n}, {k, n, m}};
     // (the products of either gradient alone are planned by themselves)
-    return operand_bytes(m, n) + operand_bytes(n, m) + aligned(8 * ceil_div64(m, 16) * n) + aligned(4 * i8_columns_workspace(m, n))
+    return operand_bytes(m, n) + operand_bytes(n, m) + aligned(4 * i8_partial_floats(m, n))
          + std::max({products_workspace(e, 2), products_workspace(e, 1), products_workspace(e + 1, 1)});
 }
 
@@ -660,20 +679,14 @@ int amsim_i8_dense_grad(const void *grad, int dtype, int64_t row_stride, const v
     if (!grad_x && !grad_kernel && !grad_bias) return AMSIM_OK;
     hipStream_t s = (hipStream_t)stream;
     uint8_t *rows = (uint8_t *)workspace, *columns = rows + operand_bytes(m, n);
-    float *looked = (float *)(columns + operand_bytes(n, m)), *joined = (float *)((uint8_t *)looked + aligned(8 * ceil_div64(m, 16) * n));
-    void *partial = (uint8_t *)joined + aligned(4 * i8_columns_workspace(m, n));
+    float *looked = (float *)(columns + operand_bytes(n, m));
+    void *partial = (uint8_t *)looked + aligned(4 * i8_partial_floats(m, n));
     float *row_scales = (float *)(rows + i8_code_bytes(m, n)), *column_scales = (float *)(columns + i8_code_bytes(n, m));
-    const float *of_x = grad_kernel ? kept_scales(x_kept, k, m) : nullptr;
-    const bool by_columns = grad_kernel || grad_bias;
     // (the gradient's rows are converted with the kernel's scales on its columns, its columns with x's on its rows)
-    if (grad_x)
-        if (int rc = i8_convert_rows({grad, out, dtype, m, n, row_stride, kept_scales(kernel_kept, k, n), rows, nullptr, row_scales, of_x,
-                                      by_columns ? looked : nullptr}, s))
-            return rc;
-    if (by_columns)
-        if (int rc = i8_convert_columns({grad, out, dtype, m, n, row_stride, of_x, nullptr, grad_kernel ? columns : nullptr, column_scales, grad_bias,
-                                         bias_dtype, grad_x ? looked : nullptr}, joined, s))
-            return rc;
+    const I8Rows by_rows{grad, out, dtype, m, n, row_stride, grad_x ? kept_scales(kernel_kept, k, n) : nullptr, rows, nullptr, row_scales};
+    const I8Columns by_columns{grad, out, dtype, m, n, row_stride, grad_kernel ? kept_scales(x_kept, k, m) : nullptr, nullptr, grad_kernel ? columns : nullptr,
+                               column_scales, grad_bias, bias_dtype};
+    if (int rc = i8_convert(grad_x ? &by_rows : nullptr, grad_kernel || grad_bias ? &by_columns : nullptr, looked, s)) return rc;
     Product list[2];
     int count = 0;
     if (grad_x) list[count++] = {operand(rows, row_scales, m), operand(kernel_kept, nullptr, k), n, nullptr, 0, AMSIM_ACT_NONE, grad_x, dtype};

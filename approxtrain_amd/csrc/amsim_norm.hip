@@ -65,6 +65,7 @@ struct NormArgs {
     float *statistics;         // [rows][2], or null
     uint8_t *codes;            // [rows][pitch], or null
     float *scales;
+    bool around;
 };
 
 template <typename T, typename S>
@@ -83,18 +84,22 @@ __global__ __launch_bounds__(S::THREADS) void norm_kernel(NormArgs g)
         if (g.gamma) load_floats(g.gamma, g.param_dtype, c, cols - c, gamma[p]);
         if (g.beta) load_floats(g.beta, g.param_dtype, c, cols - c, beta[p]);
     }
-    for (int64_t row = place.first_row(); row < g.rows; row += place.rows_apart()) {
-        const T *x = (const T *)g.x + row * g.stride;
-        float v[PIECES][N], sum = 0.0f, squares = 0.0f, largest = 0.0f;
-        v4i raw[PIECES];
+    v4i raw[PIECES];
+    auto load = [&](int64_t row) {
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const int c = (p * S::LANES + place.lane) * N;
-            raw[p] = load_piece(x + c, cols - c);
+            raw[p] = load_piece((const T *)g.x + row * g.stride + c, row < g.rows ? cols - c : 0);
         }
+    };
+    load(place.first_row());
+    for (int64_t row = place.first_row(); row < g.rows; row += place.rows_apart()) {
+        float v[PIECES][N], sum = 0.0f, squares = 0.0f, largest = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) piece_floats<T>(raw[p], v[p]);
+        load(row + place.rows_apart());  // (the next row is under way while this one is worked on)
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            piece_floats<T>(raw[p], v[p]);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 sum += v[p][i];
@@ -123,7 +128,7 @@ __global__ __launch_bounds__(S::THREADS) void norm_kernel(NormArgs g)
             if (g.codes && c < pitch) store_codes(g.codes + row * pitch + c, v[p], r);
 #pragma unroll
             for (int i = 0; i < N; ++i) v[p][i] = __builtin_fmaf((v[p][i] - mean) * rstd, gamma[p][i], beta[p][i]);
-            store_piece(out + c, cols - c, v[p]);
+            store_piece(out + c, cols - c, v[p], g.around);
         }
         if (place.lane == 0) {
             if (g.statistics) g.statistics[2 * row] = mean, g.statistics[2 * row + 1] = rstd;
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs g)
             if (g.beta) load_floats(g.beta, g.param_dtype, c, cols - c, beta);
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = __builtin_fmaf((v[i] - mean) * rstd, gamma[i], beta[i]);
-            store_piece((T *)g.out + row * cols + c, cols - c, v);
+            store_piece((T *)g.out + row * cols + c, cols - c, v, g.around);
         }
         if (place.lane == 0) {
             if (g.statistics) g.statistics[2 * row] = mean, g.statistics[2 * row + 1] = rstd;
@@ -196,6 +201,7 @@ struct NormGradArgs {
     int param_dtype;
     void *grad_x;              // or null
     float *partial;            // [workgroups][2][cols]: of dgamma and dbeta, or null
+    bool around;
 };
 
 // x as it was given, or as it was kept
@@ -234,22 +240,31 @@ __global__ __launch_bounds__(S::THREADS) void norm_grad_kernel(NormGradArgs g)
         for (int i = 0; i < N; ++i) gamma[p][i] = 1.0f;
         if (g.gamma) load_floats(g.gamma, g.param_dtype, c, cols - c, gamma[p]);
     }
-    for (int64_t row = place.first_row(); row < g.rows; row += place.rows_apart()) {
-        const T *dy = (const T *)g.grad + row * g.stride;
-        const float mean = g.statistics[2 * row], rstd = g.statistics[2 * row + 1], scale = KEPT ? g.scales[row] : 0.0f;
-        v4i raw[PIECES];
-        decltype(load_input<T, KEPT>(g, 0, 0, 0)) raw_x[PIECES];
+    v4i raw[PIECES];
+    decltype(load_input<T, KEPT>(g, 0, 0, 0)) raw_x[PIECES];
+    float next_mean, next_rstd, next_scale;
+    auto load = [&](int64_t row) {
+        const int64_t at = row < g.rows ? row : 0;
+        next_mean = g.statistics[2 * at], next_rstd = g.statistics[2 * at + 1], next_scale = KEPT ? g.scales[at] : 0.0f;
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const int c = (p * S::LANES + place.lane) * N;
-            raw[p] = load_piece(dy + c, cols - c);
-            raw_x[p] = load_input<T, KEPT>(g, row, c, pitch);
+            raw[p] = load_piece((const T *)g.grad + row * g.stride + c, row < g.rows ? cols - c : 0);
+            raw_x[p] = load_input<T, KEPT>(g, at, c, pitch);
         }
+    };
+    load(place.first_row());
+    for (int64_t row = place.first_row(); row < g.rows; row += place.rows_apart()) {
+        const float mean = next_mean, rstd = next_rstd;
         float h[PIECES][N], d[PIECES][N], sum = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             piece_floats<T>(raw[p], d[p]);  // (zeros behind the row's end: nothing is added there)
-            input_floats<T, KEPT>(raw_x[p], scale, h[p]);
+            input_floats<T, KEPT>(raw_x[p], next_scale, h[p]);
+        }
+        load(row + place.rows_apart());  // (the next row is under way while this one is worked on)
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 h[p][i] = (h[p][i] - mean) * rstd;
@@ -269,7 +284,7 @@ __global__ __launch_bounds__(S::THREADS) void norm_grad_kernel(NormGradArgs g)
             const int c = (p * S::LANES + place.lane) * N;
 #pragma unroll
             for (int i = 0; i < N; ++i) d[p][i] = rstd * __builtin_fmaf(-dot, h[p][i], d[p][i] - sum);
-            store_piece(dx + c, cols - c, d[p]);
+            store_piece(dx + c, cols - c, d[p], g.around);
         }
     }
     if (!g.partial) return;
@@ -340,7 +355,7 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(NormGradArgs g)
             load(c);
 #pragma unroll
             for (int i = 0; i < N; ++i) d[i] = rstd * __builtin_fmaf(-dot, h[i], d[i] - sum);
-            store_piece((T *)g.grad_x + row * cols + c, cols - c, d);
+            store_piece((T *)g.grad_x + row * cols + c, cols - c, d, g.around);
         }
     }
 }
@@ -451,6 +466,7 @@ struct ActArgs {
     void *out;       // or null
     uint8_t *codes;  // or null
     float *scales;
+    bool around;
 };
 
 template <typename T, typename S, typename F>
@@ -461,12 +477,11 @@ __global__ __launch_bounds__(S::THREADS) void activation_kernel(ActArgs g)
     RowLanes<S::LANES> lanes = place.lanes();
     const int cols = (int)g.cols, pitch = (int)kept8_pitch(cols);
     for (int64_t row = place.first_row(); row < g.rows; row += place.rows_apart()) {
-        const T *x = (const T *)g.x + row * g.stride;
         v4i raw[PIECES];
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const int c = (p * S::LANES + place.lane) * N;
-            raw[p] = load_piece(x + c, cols - c);
+            raw[p] = load_piece((const T *)g.x + row * g.stride + c, cols - c);
         }
         if (g.codes) {
             float largest = 0.0f;
@@ -496,7 +511,7 @@ __global__ __launch_bounds__(S::THREADS) void activation_kernel(ActArgs g)
             piece_floats<T>(raw[p], v);
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = F::value(v[i]);
-            store_piece((T *)g.out + row * cols + c, cols - c, v);
+            store_piece((T *)g.out + row * cols + c, cols - c, v, g.around);
         }
     }
 }
@@ -526,7 +541,7 @@ __global__ __launch_bounds__(1024) void activation_long_kernel(ActArgs g)
             if (!g.out) continue;
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = F::value(v[i]);
-            store_piece((T *)g.out + row * cols + c, cols - c, v);
+            store_piece((T *)g.out + row * cols + c, cols - c, v, g.around);
         }
         if (g.codes && place.lane == 0) g.scales[row] = q8_scale(__float_as_uint(largest));
     }
@@ -539,6 +554,7 @@ struct ActGradArgs {
     const uint8_t *codes;
     const float *scales;
     void *grad_x;
+    bool around;
 };
 template <typename T, typename F, int LANES>
 __global__ __launch_bounds__(256) void activation_grad_kernel(ActGradArgs g)
@@ -559,23 +575,26 @@ __global__ __launch_bounds__(256) void activation_grad_kernel(ActGradArgs g)
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = d[i] * F::slope(v[i]);
             }
-            store_piece((T *)g.grad_x + row * cols + c, cols - c, v);
+            store_piece((T *)g.grad_x + row * cols + c, cols - c, v, g.around);
         }
     }
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 
-// workgroups that go over the rows in turn: what the card holds at once
+// Normalisation: workgroups that go over the rows in turn, as many as the card holds, with gamma and beta in registers.  An
+// activation's rows, which have nothing in common, are a workgroup each (16384 x 4096 bf16: 58 us, 69 by 2048 workgroups).
 template <typename S> unsigned workgroups(int64_t rows) { return (unsigned)std::min<int64_t>(ceil_div64(rows, S::ROWS), 256 * 2048 / S::THREADS); }
 unsigned long_workgroups(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 512); }
-// ... of the backward pass, each of which leaves 2 x cols sums to be added up
-constexpr int64_t GRAD_WORKGROUPS = 512, GRAD_SLABS = 64;
+// ... of the backward pass, each of which leaves 2 x cols sums to be added up: two to a CU, three where a row takes four waves
+// (16384 x 4096 bf16: 71.7 us with 768, 76 with 512, 89 with 1024, which leave a quarter of it for a second round; 8192 x 512
+// f32: 13.6, 14.1 with 768, 14.8 with 1024)
+constexpr int64_t GRAD_SLABS = 64;
 int64_t grad_parts(int64_t rows, int64_t cols)
 {
     if (cols > MOST_HELD) return std::min(rows, GRAD_SLABS);
     const int64_t at_once = cols <= 128 ? 16 : cols <= 1024 ? 4 : 1;
-    return std::min(ceil_div64(rows, at_once), GRAD_WORKGROUPS);
+    return std::min<int64_t>(ceil_div64(rows, at_once), cols > 1024 && cols <= 4096 ? 768 : 512);
 }
 
 template <typename T, bool KEPT> int launch_norm_grad(const NormGradArgs &g, hipStream_t stream)
@@ -604,7 +623,7 @@ template <typename F> int launch_activation(const ActArgs &g, int dtype, hipStre
         } else {
             with_shape(g.cols, [&](auto shape) {
                 using S = decltype(shape);
-                activation_kernel<T, S, F><<<workgroups<S>(g.rows), S::THREADS, 0, stream>>>(g);
+                activation_kernel<T, S, F><<<(unsigned)std::min<int64_t>(ceil_div64(g.rows, S::ROWS), 1 << 20), S::THREADS, 0, stream>>>(g);
                 return 0;
             });
         }
@@ -637,6 +656,7 @@ int check_rows(const char *what, const void *x, int dtype, int64_t rows, int64_t
     if ((uintptr_t)x & (element_bytes(dtype) - 1)) return fail(AMSIM_ERR_INVALID, w + ": misaligned pointer");
     return AMSIM_OK;
 }
+bool around(int64_t rows, int64_t cols, int dtype) { return mx_goes_around((double)rows * (double)cols * element_bytes(dtype)); }
 bool off(const void *p, uintptr_t bytes) { return (uintptr_t)p & (bytes - 1); }
 uint8_t *codes_of(void *kept) { return (uint8_t *)kept; }
 float *scales_of(void *kept, int64_t rows, int64_t cols) { return kept ? (float *)((uint8_t *)kept + rows * kept8_pitch(cols)) : nullptr; }
@@ -659,7 +679,7 @@ int amsim_kept8_values(const void *kept, int64_t rows, int64_t cols, int dtype, 
     if (int rc = check_rows("kept8", out, dtype, rows, cols, cols)) return rc;
     if (!kept) return fail(AMSIM_ERR_INVALID, "kept8: null pointer");
     if (off(kept, 16)) return fail(AMSIM_ERR_INVALID, "kept8: misaligned pointer");
-    return launch_activation_grad<Linear>({nullptr, rows, cols, cols, codes_of((void *)kept), scales_of((void *)kept, rows, cols), out}, dtype, (hipStream_t)stream);
+    return launch_activation_grad<Linear>({nullptr, rows, cols, cols, codes_of((void *)kept), scales_of((void *)kept, rows, cols), out, around(rows, cols, dtype)}, dtype, (hipStream_t)stream);
 }
 
 int amsim_layer_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, const void *gamma, const void *beta, int param_dtype,
@@ -672,7 +692,7 @@ int amsim_layer_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64
     const uintptr_t element = element_bytes(dtype), param = element_bytes(param_dtype);
     if (off(out, element) || off(statistics, 4) || off(kept, 16) || (gamma && off(gamma, param)) || (beta && off(beta, param)))
         return fail(AMSIM_ERR_INVALID, "layer_norm: misaligned pointer");
-    const NormArgs g{x, rows, row_stride, cols, gamma, beta, param_dtype, (float)epsilon, out, statistics, codes_of(kept), scales_of(kept, rows, cols)};
+    const NormArgs g{x, rows, row_stride, cols, gamma, beta, param_dtype, (float)epsilon, out, statistics, codes_of(kept), scales_of(kept, rows, cols), around(rows, cols, dtype)};
     return with_type(dtype, [&](auto zero) {
         using T = decltype(zero);
         if (cols > MOST_HELD) {
@@ -714,7 +734,7 @@ int amsim_layer_norm_grad(const void *grad, int dtype, int64_t rows, int64_t col
         return fail(AMSIM_ERR_WORKSPACE, "layer_norm: workspace missing, misaligned or too small");
     if (!grad_x && !sums) return AMSIM_OK;
     const NormGradArgs g{grad, rows, row_stride, cols, x, x_row_stride, codes_of((void *)kept), scales_of((void *)kept, rows, cols), statistics, gamma,
-                         param_dtype, grad_x, sums ? (float *)workspace : nullptr};
+                         param_dtype, grad_x, sums ? (float *)workspace : nullptr, around(rows, cols, dtype)};
     const int rc = with_type(dtype, [&](auto zero) {
         using T = decltype(zero);
         return kept ? launch_norm_grad<T, true>(g, (hipStream_t)stream) : launch_norm_grad<T, false>(g, (hipStream_t)stream);
@@ -731,7 +751,7 @@ int amsim_activation(const void *x, int dtype, int64_t rows, int64_t cols, int64
     if (int rc = check_rows("activation", x, dtype, rows, cols, row_stride)) return rc;
     if (!out && !kept) return fail(AMSIM_ERR_INVALID, "activation: null pointer");
     if (off(out, element_bytes(dtype)) || off(kept, 16)) return fail(AMSIM_ERR_INVALID, "activation: misaligned pointer");
-    const ActArgs g{x, rows, row_stride, cols, out, codes_of(kept), scales_of(kept, rows, cols)};
+    const ActArgs g{x, rows, row_stride, cols, out, codes_of(kept), scales_of(kept, rows, cols), around(rows, cols, dtype)};
     switch (kind) {
     case AMSIM_ACT_NONE: return launch_activation<Linear>(g, dtype, (hipStream_t)stream);
     case AMSIM_ACT_GELU: return launch_activation<Gelu>(g, dtype, (hipStream_t)stream);
@@ -745,7 +765,7 @@ int amsim_activation_grad(const void *grad, int dtype, int64_t rows, int64_t col
     if (int rc = check_rows("activation", grad, dtype, rows, cols, row_stride)) return rc;
     if (!kept || !grad_x) return fail(AMSIM_ERR_INVALID, "activation: null pointer");
     if (off(kept, 16) || off(grad_x, element_bytes(dtype))) return fail(AMSIM_ERR_INVALID, "activation: misaligned pointer");
-    const ActGradArgs g{grad, rows, row_stride, cols, codes_of((void *)kept), scales_of((void *)kept, rows, cols), grad_x};
+    const ActGradArgs g{grad, rows, row_stride, cols, codes_of((void *)kept), scales_of((void *)kept, rows, cols), grad_x, around(rows, cols, dtype)};
     switch (kind) {
     case AMSIM_ACT_GELU: return launch_activation_grad<Gelu>(g, dtype, (hipStream_t)stream);
     case AMSIM_ACT_SWISH: return launch_activation_grad<Swish>(g, dtype, (hipStream_t)stream);

@@ -28,11 +28,14 @@ __device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_
 // The code of one value in the lowest byte: within 1.5 * 2^23 +- 2^22 a float's last place is 1, so that the sum's one
 // rounding, behind the exact product, is the rounding to an integer.
 __device__ __forceinline__ uint32_t q8_code(float v, float r) { return __float_as_uint(__builtin_fmaf(v, r, 12582912.0f)); }
+// the lowest bytes of four
+__device__ __forceinline__ uint32_t q8_pack(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    return __builtin_amdgcn_perm(b, a, 0x0c0c0400u) | __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+}
 __device__ __forceinline__ uint32_t q8_codes4(float a, float b, float c, float d, float r)
 {
-    const uint32_t low = __builtin_amdgcn_perm(q8_code(b, r), q8_code(a, r), 0x0c0c0400u);
-    const uint32_t high = __builtin_amdgcn_perm(q8_code(d, r), q8_code(c, r), 0x04000c0cu);
-    return low | high;
+    return q8_pack(q8_code(a, r), q8_code(b, r), q8_code(c, r), q8_code(d, r));
 }
 __device__ __forceinline__ float q8_value(uint32_t codes, int i, float s) { return (float)(int8_t)(codes >> 8 * i) * s; }
 
@@ -64,7 +67,8 @@ template <typename T> __device__ __forceinline__ void piece_floats(v4i raw, floa
 #pragma unroll
     for (int i = 0; i < PIECE<T>; ++i) v[i] = to_float(e[i]);
 }
-template <typename T> __device__ __forceinline__ void store_piece(T *p, int64_t count, const float (&v)[PIECE<T>])
+// (around: past the last-level cache, where it would not be when it is read next; mx_goes_around)
+template <typename T> __device__ __forceinline__ void store_piece(T *p, int64_t count, const float (&v)[PIECE<T>], bool around = false)
 {
     T e[PIECE<T>];
 #pragma unroll
@@ -72,7 +76,8 @@ template <typename T> __device__ __forceinline__ void store_piece(T *p, int64_t 
     if (count >= PIECE<T>) {
         v4i raw;
         __builtin_memcpy(&raw, e, 16);
-        store16(p, raw);
+        if (around) __builtin_nontemporal_store(raw, (v4i_anywhere *)p);
+        else store16(p, raw);
     } else {
 #pragma unroll
         for (int i = 0; i < PIECE<T>; ++i)

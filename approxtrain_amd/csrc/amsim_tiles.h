@@ -98,7 +98,7 @@ template <int SIZE> __device__ __forceinline__ void load_to_lds(const uint8_t *f
 // goes out in parts (16 rows of 32 bits or 32 of 16), so that its first stores are under way early: 4096^3 takes 37.2 us
 // so and 37.6 in one part; tiles of 128 and less, which have neighbours to hide behind, in one: 42.7 and 44.1.
 template <typename T, int FM, int FN> struct Rows {
-    static constexpr int COLUMNS = 16 * FN, STRIDE = COLUMNS * sizeof(T) + 16, AT_ONCE = FM * FN == 32 ? 32 / FN / sizeof(T) : FM;
+    static constexpr int COLUMNS = 16 * FN, STRIDE = COLUMNS * sizeof(T) + 16, AT_ONCE = FM * FN >= 32 ? 32 / FN / sizeof(T) : FM;
     static constexpr int BYTES = 16 * AT_ONCE * STRIDE;
 };
 // value(i, j, e): of the lane's row in fragment i of the rows, its e-th column in fragment j of the columns.
@@ -187,7 +187,11 @@ template <typename Costs> Plan make_plan(const Extents *e, int count)
 {
     Plan best{-1, {}};
     double least = 0;
+#ifndef X_TILE
+#define X_TILE i
+#endif
     for (int i = 0; i < 4; ++i) {
+        if (i != X_TILE) continue;
         Plan p{i, {}};
         double tiles = 0, work = 0, longest = 0, more = 0;
         for (int j = 0; j < count; ++j) {

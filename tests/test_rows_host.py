@@ -17,7 +17,7 @@ def test_sizes():
     size = lib().amsim_kept8_bytes
     assert size(1, 1) == 20 and size(3, 16) == 3 * 20 and size(3, 17) == 3 * 36 and size(0, 4) == size(4, 0) == size(-1, 4) == size(1 << 31, 1) == 0
     ws = lib().amsim_layer_norm_grad_workspace_bytes
-    assert ws(1, 1) == 8 and ws(0, 4) == ws(4, -1) == 0 and ws(1 << 20, 4096) == 512 * 2 * 4096 * 4
+    assert ws(1, 1) == 8 and ws(0, 4) == ws(4, -1) == 0 and ws(1 << 20, 4096) == 768 * 2 * 4096 * 4
 
 
 def norm(x=A, dtype=0, rows=4, cols=4, stride=4, gamma=A, beta=A, param=0, eps=1e-3, out=A, stats=A, kept=A):
