@@ -14,7 +14,7 @@ namespace amsim {
 
 namespace {
 
-// A row over LANES lanes of EACH values: 16 lanes for short ones (four rows a wavefront), a wavefront, four, or sixteen.
+// A row over LANES lanes of EACH values: 16 lanes for short ones (four rows a wavefront), a wavefront, four, eight or sixteen.
 template <int LANES_, int EACH_> struct Shape {
     static constexpr int LANES = LANES_, EACH = EACH_, THREADS = LANES_ > 256 ? LANES_ : 256, ROWS = THREADS / LANES_;
     static constexpr int64_t HOLDS = (int64_t)LANES_ * EACH_;
@@ -28,7 +28,7 @@ template <typename Fn> int with_shape(int64_t cols, Fn &&fn)
     if (cols <= 1024) return fn(Shape<64, 16>{});
     if (cols <= 2048) return fn(Shape<256, 8>{});
     if (cols <= 4096) return fn(Shape<256, 16>{});
-    if (cols <= 8192) return fn(Shape<1024, 8>{});
+    if (cols <= 8192) return fn(Shape<512, 16>{});  // (1024 lanes of 8: 8192 x 8192 bf16 77 us, 53 so: two of them share a CU)
     return fn(Shape<1024, 16>{});
 }
 template <typename Fn> int with_type(int dtype, Fn &&fn)
@@ -253,8 +253,10 @@ __global__ __launch_bounds__(S::THREADS) void norm_grad_kernel(NormGradArgs g)
             raw_x[p] = load_input<T, KEPT>(g, at, c, pitch);
         }
     };
-    load(place.first_row());
+    constexpr bool AHEAD = S::LANES * S::EACH < 16384;  // (there are no registers for it in sixteen waves of 16 values)
+    if constexpr (AHEAD) load(place.first_row());
     for (int64_t row = place.first_row(); row < g.rows; row += place.rows_apart()) {
+        if constexpr (!AHEAD) load(row);
         const float mean = next_mean, rstd = next_rstd;
         float h[PIECES][N], d[PIECES][N], sum = 0.0f, dot = 0.0f;
 #pragma unroll
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(S::THREADS) void norm_grad_kernel(NormGradArgs g)
             piece_floats<T>(raw[p], d[p]);  // (zeros behind the row's end: nothing is added there)
             input_floats<T, KEPT>(raw_x[p], next_scale, h[p]);
         }
-        load(row + place.rows_apart());  // (the next row is under way while this one is worked on)
+        if constexpr (AHEAD) load(row + place.rows_apart());  // (the next row is under way while this one is worked on)
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
 #pragma unroll
@@ -582,19 +584,32 @@ __global__ __launch_bounds__(256) void activation_grad_kernel(ActGradArgs g)
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 
-// Normalisation: workgroups that go over the rows in turn, as many as the card holds, with gamma and beta in registers.  An
-// activation's rows, which have nothing in common, are a workgroup each (16384 x 4096 bf16: 58 us, 69 by 2048 workgroups).
-template <typename S> unsigned workgroups(int64_t rows) { return (unsigned)std::min<int64_t>(ceil_div64(rows, S::ROWS), 256 * 2048 / S::THREADS); }
+// Workgroups of a normalisation, which go over the rows in turn with gamma and beta in registers: as many as the card holds at
+// once, so that none waits for a second round (16384 x 2048 bf16: 31 us with 1792, 34 with 1024; 8192 x 8192: 53 with 512, 59 with 1024),
+// but two rounds of them where four waves hold a row of 16 values a lane (16384 x 4096 bf16, forward and backward: 131 us with 2048, 138
+// with 1024; 8192 x 4096 75 and 74).  An activation's rows, which have nothing in common, are a workgroup each (16384 x 4096 bf16: 58
+// us, 69 by 2048 workgroups).
+template <typename S> unsigned workgroups(int64_t rows)
+{
+    const int to_a_cu = S::LANES > 256 ? 1024 / S::LANES : S::EACH == 8 ? 7 : S::LANES == 64 ? 4 : 8;
+    return (unsigned)std::min<int64_t>(ceil_div64(rows, S::ROWS), 256 * to_a_cu);
+}
 unsigned long_workgroups(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 512); }
-// ... of the backward pass, each of which leaves 2 x cols sums to be added up: two to a CU, three where a row takes four waves
-// (16384 x 4096 bf16: 71.7 us with 768, 76 with 512, 89 with 1024, which leave a quarter of it for a second round; 8192 x 512
-// f32: 13.6, 14.1 with 768, 14.8 with 1024)
+// ... of the backward pass, each of which leaves 2 x cols sums to be added up: as many as the card holds, but at least four
+// rows, or groups of rows, to each (65536 x 512 bf16: 45 us with 1280, 57 with 512; 16384 x 4096 bf16: 72 with 768, 89 with 1024; 8192 x
+// 512 f32: 13.8 with 512, 15.3 with 1280).
 constexpr int64_t GRAD_SLABS = 64;
 int64_t grad_parts(int64_t rows, int64_t cols)
 {
     if (cols > MOST_HELD) return std::min(rows, GRAD_SLABS);
-    const int64_t at_once = cols <= 128 ? 16 : cols <= 1024 ? 4 : 1;
-    return std::min<int64_t>(ceil_div64(rows, at_once), cols > 1024 && cols <= 4096 ? 768 : 512);
+    int64_t parts = 0;
+    with_shape(cols, [&](auto shape) {
+        using S = decltype(shape);
+        const int64_t groups = ceil_div64(rows, S::ROWS), held = 256 * (S::LANES > 256 ? 1 : S::EACH == 8 ? 5 : 3);
+        parts = std::min({groups, held, std::max<int64_t>(256, groups / 4)});
+        return 0;
+    });
+    return parts;
 }
 
 template <typename T, bool KEPT> int launch_norm_grad(const NormGradArgs &g, hipStream_t stream)
