@@ -462,10 +462,11 @@ template <typename Fn> int with_type(int dtype, Fn &&fn)
 }
 
 // Slabs of rows that are looked through: enough workgroups for the card beside those that convert rows, few enough for
-// every wavefront that converts columns to join them by itself.
+// every wavefront that converts columns to join them by itself (to quantise the columns of 16384 x 1000 bf16 takes 24.1 us
+// with 64 slabs, 28.9 with 32, 29.8 with 256; a training step of 8192 x 512 x 512 62 with 64, 64 with 128).
 int64_t slab_rows(int64_t rows, int64_t cols)
 {
-    const int64_t slabs = std::min(ceil_div64(rows, 64), std::max<int64_t>(16, 128 / ceil_div64(cols, 256)));
+    const int64_t slabs = std::min(ceil_div64(rows, 64), std::max<int64_t>(16, std::min<int64_t>(64, 128 / ceil_div64(cols, 512))));
     return ceil_div64(rows, slabs);
 }
 

@@ -504,7 +504,9 @@ int products(const Product *list, int count, void *workspace, hipStream_t stream
         if (j == 0) jobs.blocks = (unsigned)std::min<int64_t>(o.tiles_m * o.tiles_n * o.splits, 1 << 30);
         blocks += o.tiles_m * o.tiles_n * o.splits;
         if (o.splits > 1) f.blocks[j] = (unsigned)ceil_div64(t[j].m * ceil_div64(t[j].n, 4), FINISH_WG);
-        if (blocks >= (1ll << 22)) return fail(AMSIM_ERR_UNSUPPORTED, "int8: more tiles than one launch takes");
+        // (a launch has less than 2^32 threads)
+        if (blocks >= (1ll << 22) || (o.splits > 1 && ceil_div64(t[j].m * ceil_div64(t[j].n, 4), FINISH_WG) >= (1ll << 23)))
+            return fail(AMSIM_ERR_UNSUPPORTED, "int8: more tiles than one launch takes");
     }
     switch (p.tile) {
     case 0: gemm_kernel<8, 4, 2, 4, 4, 2><<<(unsigned)blocks, 512, 0, stream>>>(jobs); break;

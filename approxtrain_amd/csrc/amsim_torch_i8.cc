@@ -148,6 +148,15 @@ struct LinearI8 : torch::autograd::Function<LinearI8> {
             if (want_bias) grads[2] = m ? at::empty({n}, like.dtype(bias_type)) : at::zeros({n}, like.dtype(bias_type));
             if (m) {
                 const Source grad = row_source(g, "grad");
+                // (a hook may have brought back something else than was saved)
+                auto is = [&](const Tensor &t, size_t size) {
+                    return t.defined() && t.is_cuda() && t.get_device() == grad.t.get_device() && t.scalar_type() == at::kByte && t.is_contiguous() && t.numel() == (int64_t)size;
+                };
+                TORCH_CHECK((!want_kernel || is(saved[0], amsim_i8_kept_bytes(k, m))) && (!want_x || is(saved[1], amsim_i8_kept_bytes(k, n)))
+                                && (!saved[2].defined() || (saved[2].is_cuda() && saved[2].get_device() == grad.t.get_device() && saved[2].scalar_type() == g.scalar_type()
+                                                            && saved[2].is_contiguous() && saved[2].sizes() == g.sizes()))
+                                && grad.rows == m && grad.cols == n,
+                            "what lineari8 kept for its backward pass came back in another form");
                 const size_t need = amsim_i8_dense_grad_workspace_bytes(m, n, k);
                 Tensor ws = bytes((int64_t)need, grad.t);
                 auto ptr = [](const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };

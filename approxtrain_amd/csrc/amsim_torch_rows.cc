@@ -60,6 +60,13 @@ void no_capture(int64_t eager, const char *call)
                                               "their gradients would be added: release it (its outputs and losses) before the capture");
 }
 
+// what a backward pass finds of what was saved (a hook may have brought back something else)
+void check_saved(bool good, const char *call) { TORCH_CHECK(good, "what ", call, " kept for its backward pass came back in another form"); }
+bool plain(const Tensor &t, const Tensor &like, at::ScalarType type, int64_t n)
+{
+    return t.defined() && t.is_cuda() && t.get_device() == like.get_device() && t.scalar_type() == type && t.is_contiguous() && t.numel() == n;
+}
+
 // ---- layer normalisation ------------------------------------------------------------------------------------------
 
 struct Normed {
@@ -112,6 +119,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             } else {
                 if (need_x) result[0] = like_rows(*g);
                 const std::optional<Source> x = kept ? std::nullopt : rows_of(saved[1], "x");
+                check_saved(g->cols == f[7] && plain(saved[0], g->t, at::kFloat, 2 * g->rows)
+                                && (kept ? plain(saved[1], g->t, at::kByte, (int64_t)amsim_kept8_bytes(g->rows, g->cols))
+                                         : x->rows == g->rows && x->cols == g->cols && x->dtype == g->dtype && x->t.get_device() == g->t.get_device()),
+                            "layernorm");
                 const Bias gamma = f[3] ? parameters(saved[2], std::nullopt, given[0]).gamma : Bias{};
                 const size_t need = need_gamma || need_beta ? amsim_layer_norm_grad_workspace_bytes(g->rows, g->cols) : 0;
                 Tensor ws;
@@ -187,6 +198,7 @@ struct ActivationI8 : torch::autograd::Function<ActivationI8> {
             at::AutoGradMode off(false);
             const std::optional<Source> g = rows_of(given[0], "grad");
             result[0] = g ? like_rows(*g) : at::empty(given[0].sizes(), given[0].options());
+            if (g) check_saved(plain(saved[0], g->t, at::kByte, (int64_t)amsim_kept8_bytes(g->rows, g->cols)), "activationi8");
             if (g)
                 check_in_graph(amsim_activation_grad(g->t.data_ptr(), g->dtype, g->rows, g->cols, g->stride, saved[0].data_ptr(), (int)f[0],
                                                      result[0].data_ptr(), stream()));

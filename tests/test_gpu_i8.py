@@ -207,6 +207,21 @@ def test_training_step_in_large_tiles():
     check_train(make((2100, 1100), "bf16", 1), make((1100, 1300), "f32", 2, 0.1), make((1300,), "f32", 3), make((2100, 1300), "bf16", 4, 0.01))
 
 
+def test_training_step_of_more_tokens_than_one_sum_has():
+    m, n, k = 150000, 33, 40
+    assert plan((k, n, m))[2] >= 2
+    check_train(make((m, k), "bf16", 1), make((k, n), "f32", 2, 0.1), make((n,), "f32", 3), make((m, n), "bf16", 4, 0.01))
+
+
+def test_what_comes_back_in_another_form_is_refused():
+    x, kernel = make((40, 60), "f32", 1).cuda().requires_grad_(), make((60, 30), "f32", 2).cuda().requires_grad_()
+    for other in (lambda t: t[:-1], lambda t: t.cpu(), lambda t: t.view(torch.int8)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+            out = math_ops.lineari8(x, kernel)
+        with pytest.raises(RuntimeError, match="in another form"):
+            out.sum().backward()
+
+
 def test_asked_for_some_gradients():
     x, kernel, bias, dy = make((150, 200), "bf16", 1).cuda(), make((200, 90), "f32", 2).cuda(), make((90,), "f32", 3).cuda(), make((150, 90), "bf16", 4).cuda()
     _, want = train(x, kernel, bias, dy)
@@ -432,6 +447,30 @@ def test_products_on_another_stream():
                 got.append(functors.int8_linear(x, w))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i % 3]) for i, g in enumerate(got))
+
+
+def test_offsets_past_32_bits():
+    """Operands of more than 2^32 bytes, results of more than 2^31 elements: their last rows are those of the rows by themselves."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(70016, 65536, dtype=torch.float16, device="cuda")  # 9.2 GB, 4.6 GB of codes
+    x.normal_(generator=g)
+    few = x[-64:].clone()
+    w = functors.int8_quantize(torch.randn((65536, 20), device="cuda", generator=g), 0)
+    q = functors.int8_quantize(x)
+    assert q.nbytes() > 1 << 32
+    want = functors.int8_linear(few, w)
+    assert torch.equal(functors.int8_matmul(q, w, dtype=torch.float16)[-64:], want)
+    assert torch.equal(functors.int8_linear(x, w)[-64:], want)
+    assert torch.equal(q.dequantize(torch.float16)[-64:], functors.int8_quantize(few).dequantize(torch.float16))
+    del q
+    torch.cuda.empty_cache()
+    by_columns = functors.int8_quantize(x, 0)  # the last columns', of all rows
+    assert torch.equal(by_columns.dequantize(torch.float16)[-64:], functors.int8_quantize(x[:, -64:], 0).dequantize(torch.float16))
+    del by_columns, x
+    torch.cuda.empty_cache()
+    a, b = torch.randn((70016, 64), device="cuda", generator=g), torch.randn((64, 40000), device="cuda", generator=g)
+    wide = functors.int8_quantize(b, 0)
+    assert torch.equal(functors.int8_linear(a.bfloat16(), wide)[-64:], functors.int8_linear(a[-64:].bfloat16(), wide))
 
 
 def test_status_of_the_library_is_raised():

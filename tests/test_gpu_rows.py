@@ -345,6 +345,32 @@ def test_refusals(call, error):
         call(make(5, 40, "f32", 1).cuda())
 
 
+def test_what_comes_back_in_another_form_is_refused():
+    x = make(20, 64, "f32", 1).cuda().requires_grad_()
+    for call in (lambda: math_ops.layernorm(x), lambda: math_ops.layernorm(x, keep_bits=8), lambda: math_ops.activationi8(x, "gelu")):
+        for other in (lambda t: t[:-1], lambda t: t.cpu(), lambda t: t.double()):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+                out = call()
+            with pytest.raises((RuntimeError, TypeError)):
+                out.sum().backward()
+
+
+@pytest.mark.parametrize("cols", [8192, 20000])
+def test_offsets_past_32_bits(cols):
+    """Tensors of more than 2^32 elements: their last rows are those of the rows by themselves."""
+    rows = (1 << 32) // cols + 100
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    few = x[-50:].clone()
+    gamma, beta = (t.cuda() for t in vectors(cols, 3))
+    assert torch.equal(functors.layer_norm(x, gamma, beta)[-50:], functors.layer_norm(few, gamma, beta))
+    assert torch.equal(functors.keep8(x).values()[-50:], functors.keep8(few).values())
+    for call in (lambda t: math_ops.layernorm(t, gamma, beta, keep_bits=8), lambda t: math_ops.layernorm(t, gamma, beta), lambda t: math_ops.activationi8(t, "swish")):
+        a, b = x.requires_grad_(), few.requires_grad_()
+        big, = torch.autograd.grad(call(a), [a], x.detach())
+        assert torch.equal(big[-50:], torch.autograd.grad(call(b), [b], few.detach())[0])
+        del big
+
+
 def test_layer():
     layer = layers.LayerNormalization(keep_bits=8)
     x = make(30, 200, "bf16", 1).cuda().requires_grad_()
