@@ -321,17 +321,19 @@ template <typename T, bool MASK> __device__ __forceinline__ void look_through(co
     }
 }
 
-// How rows are converted: by sixteen with 0 to 8 units of a wave held, or by themselves.
-constexpr int LANES_64 = -1, LANES_512 = -2, LANES_512_TWICE = -3, LANES_512_AGAIN = -4;
+// How rows are converted: by sixteen with 0 to 8 units of a wave held, or by themselves.  Eight units by themselves have a CU's
+// registers (4096 x 4096 bf16: a serving call 72.0 us, 73.8 in half of them); beside a look they leave half to it (a training
+// step of 4096^3 274 us, 285 else, and 290 in launches of their own).
+constexpr int EIGHT_ALONE = 9, LANES_64 = -1, LANES_512 = -2, LANES_512_TWICE = -3, LANES_512_AGAIN = -4;
 
 // A conversion along rows, a look through columns, or both beside each other (the two do not wait for each other).
 constexpr int LDS_FLOATS = 2 * WAVES * 64 * PIECE<__bf16>;
-template <typename T, int HOW, bool MASK> __global__ __launch_bounds__(WG, HOW == 8 && sizeof(T) == 4 ? 2 : 4) void rows_and_look_kernel(I8Rows rows, unsigned row_blocks, Look look)
+template <typename T, int HOW, bool MASK> __global__ __launch_bounds__(WG, HOW == EIGHT_ALONE || (HOW == 8 && sizeof(T) == 4) ? 2 : 4) void rows_and_look_kernel(I8Rows rows, unsigned row_blocks, Look look)
 {
     __shared__ __attribute__((aligned(16))) float lds[LDS_FLOATS];
     static_assert(LDS_FLOATS >= WAVES * (CORNER + 16), "");
     if (blockIdx.x < row_blocks) {
-        if constexpr (HOW >= 0) convert_rows<T, HOW, MASK>(rows, (uint32_t *)lds);
+        if constexpr (HOW >= 0) convert_rows<T, (HOW == EIGHT_ALONE ? 8 : HOW), MASK>(rows, (uint32_t *)lds);
         else if constexpr (HOW == LANES_64) convert_single_rows<T, 64, 16, MASK>(rows, lds);
         else if constexpr (HOW == LANES_512) convert_single_rows<T, 512, 8, MASK>(rows, lds);
         else if constexpr (HOW == LANES_512_TWICE) convert_single_rows<T, 512, 16, MASK>(rows, lds);
@@ -508,7 +510,7 @@ int i8_convert(const I8Rows *rows, const I8Columns *columns, float *partial, hip
             const auto launch = rows && single_rows(j) ? j.cols <= 1024 ? launch_rows_and_look<T, LANES_64> : j.cols <= 4096 ? launch_rows_and_look<T, LANES_512>
                                   : j.cols <= 8192 ? launch_rows_and_look<T, LANES_512_TWICE> : launch_rows_and_look<T, LANES_512_AGAIN>
                               : each <= 1 ? launch_rows_and_look<T, 1> : each == 2 ? launch_rows_and_look<T, 2> : each <= 4 ? launch_rows_and_look<T, 4>
-                              : each <= 8 ? launch_rows_and_look<T, 8> : launch_rows_and_look<T, 0>;
+                              : each <= 8 ? columns ? launch_rows_and_look<T, 8> : launch_rows_and_look<T, EIGHT_ALONE> : launch_rows_and_look<T, 0>;
             launch(j, (unsigned)row_blocks, look, (unsigned)look_blocks, stream);
             AMSIM_HIP_CHECK(hipGetLastError());
             return (int)AMSIM_OK;
