@@ -358,7 +358,7 @@ __global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
     finish_few(g, ends, blockIdx.x, (v4i *)converted, acc, row_scales);
 }
 
-// The sums of split reductions, added in 64 bits.
+// The sums of split reductions, added in 64 bits (2 x 512 x 512 4.0 us: a launch).
 constexpr int FINISH_WG = 256;
 struct FinishArgs {
     GemmJobs products;

