@@ -749,7 +749,7 @@ int amsim_layer_norm_grad(const void *grad, int dtype, int64_t rows, int64_t col
         || (grad_beta && off(grad_beta, param)))
         return fail(AMSIM_ERR_INVALID, "layer_norm: misaligned pointer");
     const bool sums = grad_gamma || grad_beta;
-    if (sums && cols >= 1 << 26) return fail(AMSIM_ERR_UNSUPPORTED, "layer_norm: more columns than one launch sums");
+    if (sums && cols >= 1 << 25) return fail(AMSIM_ERR_UNSUPPORTED, "layer_norm: more columns than one launch sums");
     if (sums && (!workspace || workspace_bytes < amsim_layer_norm_grad_workspace_bytes(rows, cols) || off(workspace, 256)))
         return fail(AMSIM_ERR_WORKSPACE, "layer_norm: workspace missing, misaligned or too small");
     if (!grad_x && !sums) return AMSIM_OK;

@@ -8,11 +8,15 @@ namespace {
 
 // ---- arguments ----------------------------------------------------------------------------------------------------
 
-// [..., cols] as a matrix of rows; nothing where there are no rows
-std::optional<Source> rows_of(const Tensor &x, const char *name)
+void check_rows(const Tensor &x, const char *name)
 {
     known(on_device(x, name).scalar_type(), name);
     if (x.dim() < 1 || x.size(-1) == 0) value_error(std::string(name) + " has no last axis to go along");
+}
+// [..., cols] as a matrix of rows; nothing where there are no rows
+std::optional<Source> rows_of(const Tensor &x, const char *name)
+{
+    check_rows(x, name);
     if (x.numel() == 0) return std::nullopt;
     return row_source(x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}), name);
 }
@@ -54,10 +58,13 @@ Tensor kept_buffer(const Source &s)
 // in a backward pass errors are the engine's to report
 void check_in_graph(int status) { TORCH_CHECK(status == 0, "amsim status ", status, ": ", amsim_last_error()); }
 
-void no_capture(int64_t eager, const char *call)
+// eager: of the inputs, by their edges, those whose gradients are added on the default stream
+void no_capture(AutogradContext *ctx, int64_t eager, const char *call)
 {
-    TORCH_CHECK(!eager || !capturing(), call, "'s backward pass is captured while a graph of the same leaves lives that was made on the default stream, where "
-                                              "their gradients would be added: release it (its outputs and losses) before the capture");
+    for (int i = 0; i < 3; ++i)
+        TORCH_CHECK(!(eager >> i & 1) || !ctx->needs_input_grad(i) || !capturing(), call, 
+                    "'s backward pass is captured while a graph of the same leaves lives that was made on the default stream, where "
+                    "their gradients would be added: release it (its outputs and losses) before the capture");
 }
 
 // what a backward pass finds of what was saved (a hook may have brought back something else)
@@ -104,8 +111,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     {
         const variable_list saved = ctx->get_saved_variables();
         const std::vector<int64_t> f = ctx->saved_data["shape"].toIntVector();
-        no_capture(f[5], "layernorm");
-        const bool need_x = f[0] && ctx->needs_input_grad(0), need_gamma = f[1], need_beta = f[2], kept = f[4];
+        no_capture(ctx, f[5], "layernorm");
+        // (an input that is None has no edge: beta's is the second where there is no gamma)
+        const bool need_x = f[0] && ctx->needs_input_grad(0), need_gamma = f[1] && ctx->needs_input_grad(1), need_beta = f[2] && ctx->needs_input_grad(1 + f[3]), kept = f[4];
         const at::ScalarType type = (at::ScalarType)f[6];
         variable_list result(6);
         {
@@ -151,9 +159,15 @@ Tensor layernorm(py::handle x_, py::handle gamma_, py::handle beta_, double epsi
         const std::optional<Source> s = rows_of(x, "x");
         return s ? shaped(norm(*s, p, epsilon, false, false).out, x) : at::empty(x.sizes(), x.options());
     }
-    parameters(gamma, beta, x);
-    rows_of(x.detach(), "x");
-    const int64_t eager = capturing() && (adds_on_default_stream(x) || (gamma && adds_on_default_stream(*gamma)) || (beta && adds_on_default_stream(*beta)));
+    check_rows(x, "x");
+    if (gamma) on_device(*gamma, "gamma");
+    if (beta) on_device(*beta, "beta");
+    int64_t eager = 0;
+    if (capturing()) {
+        eager = adds_on_default_stream(x);
+        if (gamma) eager |= adds_on_default_stream(*gamma) << 1;
+        if (beta) eager |= adds_on_default_stream(*beta) << (1 + gamma.has_value());
+    }
     if (x.dim() == 2) return LayerNorm::apply(x, gamma, beta, epsilon, keep, eager);
     return LayerNorm::apply(x.reshape({x.numel() ? -1 : 0, x.size(-1)}), gamma, beta, epsilon, keep, eager).reshape(x.sizes());
 }
@@ -192,7 +206,7 @@ struct ActivationI8 : torch::autograd::Function<ActivationI8> {
     {
         const variable_list saved = ctx->get_saved_variables();
         const std::vector<int64_t> f = ctx->saved_data["shape"].toIntVector();
-        no_capture(f[1], "activationi8");
+        no_capture(ctx, f[1], "activationi8");
         variable_list result(3);
         {
             at::AutoGradMode off(false);
@@ -219,7 +233,7 @@ Tensor activationi8(py::handle x_, int kind)
         check(amsim_activation(s->t.data_ptr(), s->dtype, s->rows, s->cols, s->stride, kind, out.data_ptr(), nullptr, stream()));
         return shaped(out, x);
     }
-    rows_of(x.detach(), "x");
+    check_rows(x, "x");
     const int64_t eager = capturing() && adds_on_default_stream(x);
     if (x.dim() == 2) return ActivationI8::apply(x, (int64_t)kind, eager);
     return ActivationI8::apply(x.reshape({x.numel() ? -1 : 0, x.size(-1)}), (int64_t)kind, eager).reshape(x.sizes());

@@ -314,6 +314,27 @@ def test_a_backward_pass_captured_beside_an_eager_graph_is_an_error():
         del alive
 
 
+def test_a_captured_gradient_beside_an_eager_graph_of_leaves_that_are_not_asked_for():
+    x = make(20, 64, "f32", 1).cuda()
+    gamma = torch.ones(64, device="cuda", requires_grad=True)
+    beta = torch.zeros(64, device="cuda", requires_grad=True)
+    alive = (gamma * 1, beta * 1)  # noqa: F841  (their gradients would be added on the default stream)
+    dy = torch.randn(20, 64, device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        leaf = x.clone().requires_grad_()
+        want = torch.autograd.grad(math_ops.layernorm(leaf, gamma, beta), [leaf], dy)[0]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        got, = torch.autograd.grad(math_ops.layernorm(leaf, gamma, beta), [leaf], dy)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_gradients_of_gradients_are_refused():
     x = make(5, 40, "f32", 1).cuda().requires_grad_()
     for y in (math_ops.layernorm(x), math_ops.activationi8(x, "gelu")):
