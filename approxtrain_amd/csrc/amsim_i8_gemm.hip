@@ -273,85 +273,96 @@ __global__ __launch_bounds__(1024) void few_kernel(FewArgs g)
     finish_few(g, ends, blockIdx.x, sums, acc, g.a.scales);
 }
 
-// Up to 16 rows as they come: every workgroup converts them for itself, into LDS, while its first loads of b are
-// under way.  A row belongs to a group of waves (all of them for one row, one from nine rows on), whose lanes hold
-// its pieces of 8 values in registers between the search for the largest and the codes.
-constexpr int64_t RAW_ROWS = 16, RAW_VALUES = 32768;  // rows, and rows x length (in whole steps), that it converts
-template <typename X>
-__global__ __launch_bounds__(1024) void raw_kernel(FewArgs g)
+// FA fragments of rows as they come: every workgroup converts them for itself, into LDS, while its first loads of b are
+// under way.  Its threads take the rows' pieces of 8 values in turn and hold them between the search for the largest,
+// which meets in LDS (a step is 8 pieces, so that 8 neighbouring lanes are of one row), and the codes.
+constexpr int64_t RAW_VALUES = 32768;  // rows x length (in whole steps) that it converts
+template <typename X, int FA>
+__global__ __launch_bounds__(FA == 4 ? 512 : 1024) void raw_kernel(FewArgs g)
 {
+    constexpr int HELD = FA == 4 ? 8 : 4;  // pieces of a thread: what RAW_VALUES come to; if there are more they are read again
     extern __shared__ __attribute__((aligned(16))) uint8_t converted[];  // codes [16 values][row][16 bytes]; then the sums
-    __shared__ uint32_t largest_of[2][16];
-    __shared__ float row_scales[RAW_ROWS];
+    __shared__ uint32_t largest[16 * FA];
+    __shared__ float row_scales[16 * FA];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int rows = (int)g.rows, apart = rows | 1, pieces = (int)g.steps * 8;  // (an odd distance: a row's 16 values lie in different banks)
     FewSteps b;
     b.load(g, blockIdx.x, wave, waves);
     FewEnds ends;
     ends.load(g, blockIdx.x);
-    int together = waves;  // waves to a row: a power of two
-    while (together > 1 && together * rows > waves) together /= 2;
-    const int group = wave / together, groups = waves / together, first = wave % together * 64 + lane;
-    for (int round = 0; round * groups < rows; ++round) {
-        const int r = round * groups + group;
-        const X *p = (const X *)g.x + r * g.row_stride;
-        constexpr int HELD = 4;  // (32 values a lane are what RAW_VALUES come to; others are read again)
-        X v[HELD][8], more[8];
-        auto load = [&](int at, X (&to)[8]) {
-            const int64_t count = r < rows && at < pieces ? g.k - 8 * at : 0;
+    const int down = blockDim.x / pieces, across = blockDim.x % pieces, row0 = threadIdx.x / pieces, at0 = threadIdx.x % pieces;
+    struct Piece {
+        int row, at;
+    };
+    auto next = [&](Piece &p) {
+        p.row += down, p.at += across;
+        if (p.at >= pieces) p.at -= pieces, ++p.row;
+    };
+    auto load = [&](Piece p, X (&v)[8]) {
+        const int64_t count = p.row < rows ? g.k - 8 * p.at : 0;
+        const X *x = (const X *)g.x + p.row * g.row_stride + 8 * p.at;
 #pragma unroll
-            for (int h = 0; h < 8; h += PIECE<X>) {
-                const v4i raw = load_piece(p + 8 * at + h, count - h);
-                __builtin_memcpy(&to[h], &raw, 16);
-            }
-        };
-        uint32_t largest = 0;
-        auto look = [&](const X (&of)[8]) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) largest = max(largest, magnitude_bits(to_float(of[e])));
-        };
-#pragma unroll
-        for (int j = 0; j < HELD; ++j) load(first + j * together * 64, v[j]);
-#pragma unroll
-        for (int j = 0; j < HELD; ++j) look(v[j]);
-        for (int at = first + HELD * together * 64; at < pieces; at += together * 64) {
-            load(at, more);
-            look(more);
+        for (int h = 0; h < 8; h += PIECE<X>) {
+            const v4i raw = load_piece(x + h, count - h);
+            __builtin_memcpy(&v[h], &raw, 16);
         }
-        largest = __float_as_uint(over_lanes<MaxOf, 64>(__uint_as_float(largest)));
-        if (together > 1) {  // (the same in every wave)
-            uint32_t *of = largest_of[round & 1];  // (who writes one half has met everybody since it was read)
-            if (lane == 0) of[wave] = largest;
-            __syncthreads();
-            for (int w = 0; w < together; ++w) largest = max(largest, of[group * together + w]);
-        }
-        if (r >= rows) continue;
-        if (first == 0) row_scales[r] = q8_scale(largest);
-        const float multiplier = q8_multiplier(largest);
-        auto store = [&](int at, const X (&of)[8]) {
-            if (at >= pieces) return;
-            float f[8];
+    };
+    auto look = [&](Piece p, const X (&v)[8]) {
+        uint32_t m = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = to_float(of[e]);
-            store_codes(converted + (at / 2 * apart + r) * 16 + at % 2 * 8, f, multiplier);
-        };
+        for (int e = 0; e < 8; ++e) m = max(m, magnitude_bits(to_float(v[e])));
+        float f = __uint_as_float(m);
+        f = with_dpp<MaxOf, 0xb1>(f);
+        f = with_dpp<MaxOf, 0x4e>(f);
+        f = with_dpp<MaxOf, 0x141>(f);
+        if (lane % 8 == 0 && p.row < rows) atomicMax(&largest[p.row], __float_as_uint(f));  // (of LDS; the largest of any order)
+    };
+    auto store = [&](Piece p, const X (&v)[8]) {
+        if (p.row >= rows) return;
+        float f[8];
 #pragma unroll
-        for (int j = 0; j < HELD; ++j) store(first + j * together * 64, v[j]);
-        for (int at = first + HELD * together * 64; at < pieces; at += together * 64) {
-            load(at, more);
-            store(at, more);
-        }
+        for (int e = 0; e < 8; ++e) f[e] = to_float(v[e]);
+        store_codes(converted + (p.at / 2 * apart + p.row) * 16 + p.at % 2 * 8, f, q8_multiplier(largest[p.row]));
+    };
+    X held[HELD][8];
+    Piece piece{row0, at0};
+#pragma unroll
+    for (int j = 0; j < HELD; ++j, next(piece)) load(piece, held[j]);
+    const Piece rest = piece;  // behind what is held
+    if (threadIdx.x < 16 * FA) largest[threadIdx.x] = 0;
+    __syncthreads();
+    piece = {row0, at0};
+#pragma unroll
+    for (int j = 0; j < HELD; ++j, next(piece)) look(piece, held[j]);
+    // (all lanes of a wave go round: its neighbours' maxima are read across lanes)
+    for (Piece p = rest; __any(p.row < rows); next(p)) {
+        X v[8];
+        load(p, v);
+        look(p, v);
     }
     __syncthreads();
-    const int row = min(lane % 16, rows - 1);  // (results of rows that do not exist are not stored)
-    v4i acc[1] = {};
+    if (threadIdx.x < rows) row_scales[threadIdx.x] = q8_scale(largest[threadIdx.x]);
+    piece = {row0, at0};
+#pragma unroll
+    for (int j = 0; j < HELD; ++j, next(piece)) store(piece, held[j]);
+    for (Piece p = rest; p.row < rows; next(p)) {
+        X v[8];
+        load(p, v);
+        store(p, v);
+    }
+    __syncthreads();
+    int row[FA];
+#pragma unroll
+    for (int i = 0; i < FA; ++i) row[i] = min(16 * i + lane % 16, rows - 1);  // (results of rows that do not exist are not stored)
+    v4i acc[FA] = {};
     for (int64_t s = wave; s < g.steps; s += AHEAD * waves) {
         if (s != wave) b.load(g, blockIdx.x, s, waves);
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) {
             const int t = (int)s + h * waves;
             if (t >= g.steps) break;
-            acc[0] = mfma(b.codes[h], *(const v4i *)(converted + ((4 * t + lane / 16) * apart + row) * 16), acc[0]);
+#pragma unroll
+            for (int i = 0; i < FA; ++i) acc[i] = mfma(b.codes[h], *(const v4i *)(converted + ((4 * t + lane / 16) * apart + row[i]) * 16), acc[i]);
         }
     }
     __syncthreads();  // (the sums take the place of what was converted)
@@ -460,8 +471,10 @@ int few_waves(const FewArgs &g, int64_t pieces)
 }
 template <typename X> int launch_raw(const FewArgs &g, hipStream_t stream)
 {
-    const int waves = few_waves(g, g.rows * g.steps * 8);
-    return launch_few(raw_kernel<X>, g, waves, std::max<int64_t>(g.steps * 4 * (g.rows | 1) * 16, waves * 1024), stream);
+    // (eight waves' sums of four fragments are 32 KB of LDS, sixteen waves' with the rest would be more than 64)
+    const int fragments = g.rows <= 16 ? 1 : g.rows <= 32 ? 2 : 4, waves = std::min(few_waves(g, g.rows * g.steps * 8), fragments == 4 ? 8 : 16);
+    const int64_t lds = std::max<int64_t>(g.steps * 4 * (g.rows | 1) * 16, waves * fragments * 1024);
+    return launch_few(fragments == 1 ? raw_kernel<X, 1> : fragments == 2 ? raw_kernel<X, 2> : raw_kernel<X, 4>, g, waves, lds, stream);
 }
 
 struct Product {
@@ -542,10 +555,10 @@ int check_workspace(const void *workspace, size_t have, size_t need)
     return AMSIM_OK;
 }
 
-// Whether few rows are converted by every workgroup that multiplies them, not once ahead.  us so, and ahead: one token of 4096
-// x 4096 6.3 and 8.5, 4 rows 6.5 and 8.4, 8 rows 7.8 and 8.2; 16 rows of 1024 x 1024 5.7 and 6.7, 32 rows 7.3 and 7.0; 64 rows of 512 x
-// 512 10.5 and 7.4 (a wave's rows wait for memory one after the other).
-bool converts_on_the_way(int64_t m, int64_t n, int64_t k) { return m <= RAW_ROWS && m * i8_steps(k) * I8_STEP * ceil_div64(n, 4096) <= RAW_VALUES; }
+// Whether few rows are converted by every workgroup that multiplies them, not once ahead, by a launch more of the device and of
+// the host.  us so, and ahead, the device alone: one token of 4096 x 4096 6.5 and 8.8, 4 rows 7.1 and 8.7, 8 rows 8.3 and 8.4; 24 rows of
+// 224 x 54 5.9 and 7.5, 32 rows of 1024 x 4096 7.9 and 7.5, 64 rows of 512 x 512 7.2 and 8.0, of 512 x 4096 8.1 and 7.7.
+bool converts_on_the_way(int64_t m, int64_t n, int64_t k) { return m <= 64 && m * i8_steps(k) * I8_STEP * ceil_div64(n, 4096) <= RAW_VALUES; }
 
 size_t aligned(int64_t bytes) { return ((size_t)bytes + 255) / 256 * 256; }
 size_t operand_bytes(int64_t rows, int64_t length) { return aligned(i8_bytes(rows, length)); }
