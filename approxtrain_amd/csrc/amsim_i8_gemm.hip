@@ -38,13 +38,16 @@ struct GemmJobs {
     unsigned blocks;         // of the first
 };
 
-// The smaller scale first: then no step leaves the range of 32 bits unless the result does (a whole number is 0 or at
-// least 1).  A NaN on either side stays one.
-__device__ __forceinline__ float scaled(float sum, float a, float b)
+// sum * a * b, two roundings, that leaves the range of 32 bits only where the result does.  Within 2^-60 .. 2^60 either product
+// does so by itself (a whole number is 0 or from 1 to 2^31); other scales are multiplied as fractions, their powers of two
+// applied behind, which moves no rounding: a result does not depend on which way its neighbours go.  A NaN stays one.
+__device__ __forceinline__ bool plain_scale(float s) { return s >= 0x1p-60f && s <= 0x1p60f; }
+__device__ __forceinline__ float scaled_any(float sum, float a, float b)
 {
-    const float low = a < b ? a : b, high = a < b ? b : a;
-    return sum * low * high;
+    const int ea = __builtin_amdgcn_frexp_expf(a), eb = __builtin_amdgcn_frexp_expf(b);
+    return __builtin_amdgcn_ldexpf(sum * __builtin_amdgcn_frexp_mantf(a) * __builtin_amdgcn_frexp_mantf(b), ea + eb);
 }
+__device__ __forceinline__ float scaled(float sum, float a, float b) { return plain_scale(a) && plain_scale(b) ? sum * a * b : scaled_any(sum, a, b); }
 
 __device__ __forceinline__ v4i mfma(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
@@ -171,10 +174,22 @@ __global__ __launch_bounds__(64 * WM * WN, RESIDENT) void gemm_kernel(GemmJobs j
             sb[j][e] = scale_of(g.b.scales, n, g.b.rows);
             bias[j][e] = g.bias && n < g.b.rows ? load_as_float(g.bias, g.bias_dtype, n) : 0.0f;
         }
+    bool plain = true;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) plain = plain && plain_scale(sa[i]);
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) plain = plain && plain_scale(sb[j][e]);
+    plain = __all(plain);
     auto store = [&](auto zero, auto *out) {
         using T = decltype(zero);
-        store_tile<T, FM, FN>(mine, [&](int i, int j, int e) { return from_float<T>(activate(scaled((float)acc[i][j][e], sa[i], sb[j][e]) + bias[j][e], g.act)); }, out,
-                              m0, n0, g.a.rows, g.b.rows, g.around);
+        auto tile = [&](auto &&scale) {
+            store_tile<T, FM, FN>(mine, [&](int i, int j, int e) { return from_float<T>(activate(scale((float)acc[i][j][e], sa[i], sb[j][e]) + bias[j][e], g.act)); }, out,
+                                  m0, n0, g.a.rows, g.b.rows, g.around);
+        };
+        if (plain) tile([](float sum, float a, float b) { return sum * a * b; });
+        else tile([](float sum, float a, float b) { return scaled_any(sum, a, b); });
     };
     if (g.out_dtype == AMSIM_DTYPE_F32) store(0.0f, (float *)g.out);
     else if (g.out_dtype == AMSIM_DTYPE_BF16) store((__bf16)0.0f, (__bf16 *)g.out);
@@ -229,8 +244,12 @@ __device__ __forceinline__ void finish_few(const FewArgs &g, const FewEnds &ends
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int64_t n = f * 16 + lane / 16 * 4, N = g.b.rows;
     float sa[FA];
+    bool plain = true;
 #pragma unroll
-    for (int i = 0; i < FA; ++i) sa[i] = scale_of(row_scales, 16 * i + lane % 16, g.rows);
+    for (int i = 0; i < FA; ++i) sa[i] = scale_of(row_scales, 16 * i + lane % 16, g.rows), plain = plain && plain_scale(sa[i]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) plain = plain && plain_scale(ends.scale[e]);
+    plain = __all(plain);
 #pragma unroll
     for (int i = 0; i < FA; ++i) sums[(wave * FA + i) * 64 + lane] = acc[i];
     __syncthreads();
@@ -243,7 +262,7 @@ __device__ __forceinline__ void finish_few(const FewArgs &g, const FewEnds &ends
         if (m >= g.rows || n >= N) continue;
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = scaled((float)z[e], sa[i], ends.scale[e]) + ends.bias[e];
+        for (int e = 0; e < 4; ++e) v[e] = (plain ? (float)z[e] * sa[i] * ends.scale[e] : scaled_any((float)z[e], sa[i], ends.scale[e])) + ends.bias[e];
         finish4(nullptr, 0, g.act, g.out, g.out_dtype, m, n, N, v);
     }
 }

@@ -110,6 +110,30 @@ def test_largest_and_smallest_scales():
     close(got, want)
 
 
+@pytest.mark.parametrize("m,n", [(40, 33), (200, 150), (600, 1300)])
+def test_scales_of_every_size_beside_each_other(m, n):
+    """Rows and columns from 1e-36 to 1e36: each result is its own definition's, and the same with whatever stands beside it."""
+    x, w = make((m, 96), "f32", 1), make((n, 96), "f32", 2)
+    x *= 10.0 ** torch.randint(-18, 19, (m, 1), generator=torch.Generator().manual_seed(3)).float()
+    w *= 10.0 ** torch.randint(-18, 19, (n, 1), generator=torch.Generator().manual_seed(4)).float()
+    x[::7] *= 1e18
+    x[3::7] *= 1e-18
+    a, b = functors.int8_quantize(x.cuda()), functors.int8_quantize(w.cuda())
+    (qa, sa), (qb, sb) = ref.int8(x), ref.int8(w)
+    want = (qa @ qb.t()) * sa * sb.t()
+    assert (sa < 1e-34).any() and (sa > 1e30).any()
+    got = functors.int8_matmul(a, b)
+    # (from 2^128 on no numbers of 32 bits; four roundings below it either may come out)
+    beyond, at_most = want.abs() >= 2.0 ** 128 * (1 + 4 * ref.U), want.abs() >= 2.0 ** 128 * (1 - 4 * ref.U)
+    assert torch.isinf(got.cpu()[beyond]).all()
+    close(torch.where(at_most.cuda(), 0.0, got), torch.where(at_most, 0.0, want))
+    for row in (0, 3, 5, m - 1):
+        assert torch.equal(functors.int8_matmul(functors.int8_quantize(x[row:row + 1].cuda()), b)[0], got[row])
+    calm = (sb[:, 0] > 2.0 ** -50) & (sb[:, 0] < 2.0 ** 50)
+    few = functors.int8_quantize(w[calm].cuda())
+    assert torch.equal(functors.int8_matmul(a, few), got[:, calm.cuda()])
+
+
 PRODUCTS = [(1, 1, 1), (1, 4096, 64), (1, 10, 70), (2, 33, 9000), (3, 1000, 4096), (5, 17, 6000), (8, 130, 4096), (9, 257, 3600), (13, 1003, 2051), (16, 64, 16384),
             (17, 100, 16384), (31, 77, 1000), (33, 200, 990), (48, 513, 640), (64, 40, 512), (64, 300, 4000), (65, 64, 64), (64, 10, 16385), (100, 10, 40000),
             (129, 300, 784), (257, 515, 129), (1000, 1003, 333), (2048, 2048, 200), (300, 5000, 70), (4099, 17, 260)]
