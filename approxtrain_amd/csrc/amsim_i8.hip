@@ -117,13 +117,20 @@ template <typename T, int HELD, bool MASK> __device__ __forceinline__ void conve
     const T *x = (const T *)g.x, *positive = (const T *)g.positive;
     v4i held[HELD ? HELD : 1][U::LOADS];
     uint32_t largest[U::LOADS] = {};
-    // what the unit's values are as codes are made of them
+    // What the unit's values are as codes are made of them.  The columns' factors come by way of LDS where rows are held (from
+    // memory, twice for every unit, they took 10 us of 4096 x 4096's 22).
+    float *factors = (float *)(lds + WAVES * (CORNER + 16));
     auto floats = [&](const v4i &raw, int64_t col0, float (&v)[U::N]) {
         piece_floats<T>(raw, v);
         if (g.col_factor) {
             float f[U::N];
             const int64_t c = col0 + unit_col<T>();
-            load_floats(g.col_factor, AMSIM_DTYPE_F32, c, g.cols - c, f);
+            if constexpr (HELD > 0) {
+#pragma unroll
+                for (int e = 0; e < U::N; e += 4) __builtin_memcpy(f + e, __builtin_assume_aligned(factors + c + e, 16), 16);
+            } else {
+                load_floats(g.col_factor, AMSIM_DTYPE_F32, c, g.cols - c, f);
+            }
 #pragma unroll
             for (int e = 0; e < U::N; ++e) v[e] *= f[e];
         }
@@ -140,6 +147,13 @@ template <typename T, int HELD, bool MASK> __device__ __forceinline__ void conve
     if constexpr (HELD > 0) {
 #pragma unroll
         for (int h = 0; h < HELD; ++h) load_unit<MASK>(x, positive, g.rows, g.cols, g.row_stride, row0, (wave + h * WAVES) * 64, held[h]);
+        if (g.col_factor) {
+            for (int64_t c = threadIdx.x * 4; c < units * 64; c += WG * 4) {
+                const v4i f = load_piece(g.col_factor + c, g.cols - c);
+                __builtin_memcpy(__builtin_assume_aligned(factors + c, 16), &f, 16);
+            }
+            __syncthreads();
+        }
 #pragma unroll
         for (int h = 0; h < HELD; ++h)
             if (wave + h * WAVES < units) look(held[h], (wave + h * WAVES) * 64);
@@ -332,7 +346,7 @@ constexpr int LDS_FLOATS = 2 * WAVES * 64 * PIECE<__bf16>;
 template <typename T, int HOW, bool MASK> __global__ __launch_bounds__(WG, HOW == EIGHT_ALONE || (HOW == 8 && sizeof(T) == 4) ? 2 : 4) void rows_and_look_kernel(I8Rows rows, unsigned row_blocks, Look look)
 {
     __shared__ __attribute__((aligned(16))) float lds[LDS_FLOATS];
-    static_assert(LDS_FLOATS >= WAVES * (CORNER + 16), "");
+    static_assert(LDS_FLOATS >= WAVES * (CORNER + 16) + WAVES * 8 * 64, "");
     if (blockIdx.x < row_blocks) {
         if constexpr (HOW >= 0) convert_rows<T, (HOW == EIGHT_ALONE ? 8 : HOW), MASK>(rows, (uint32_t *)lds);
         else if constexpr (HOW == LANES_64) convert_single_rows<T, 64, 16, MASK>(rows, lds);
@@ -390,6 +404,14 @@ __global__ __launch_bounds__(256) void columns_kernel(I8Columns g, const float *
     if (codes)
 #pragma unroll
         for (int q = 0; q < 4; ++q) load_unit<MASK>((const T *)g.x, (const T *)g.positive, g.rows, g.cols, g.row_stride, step * 64 + 16 * q, col0, raw[q]);
+    float factor[4][U::LOADS];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < U::LOADS; ++i) {
+            const int64_t r = step * 64 + 16 * q + unit_row<T>(i);
+            factor[q][i] = g.row_factor && r < g.rows ? g.row_factor[r] : 1.0f;
+        }
     if (step == 0 && g.sums) {
         const v4f s = over_slabs<SumOf>(partial + g.cols, slabs, g.cols, col0);
         if (lane < 16)
@@ -421,8 +443,7 @@ __global__ __launch_bounds__(256) void columns_kernel(I8Columns g, const float *
         Codes<U::N> unit;
 #pragma unroll
         for (int i = 0; i < U::LOADS; ++i) {
-            const int64_t r = row0 + unit_row<T>(i);
-            const float f = g.row_factor && r < g.rows ? g.row_factor[r] : 1.0f;
+            const float f = factor[q][i];
             float v[U::N];
             piece_floats<T>(raw[q][i], v);
 #pragma unroll
