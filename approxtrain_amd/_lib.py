@@ -90,7 +90,7 @@ SIGNATURES = {
     "amsim_mxfp4_dense": (_i, [_p, _i, _i64] * 2 + [_i64] * 3 + [_p, _i, _i] + [_p] * 4 + [_sz, _p]),
     "amsim_mxfp4_dense_grad_workspace_bytes": (_sz, [_i64] * 3),
     "amsim_mxfp4_dense_grad": (_i, [_p, _i, _i64] + [_p] * 3 + [_i64] * 3 + [_p, _p, _i, _p, _i, _p, _sz, _p]),
-    "amsim_i8_operand_bytes": (_sz, [_i64] * 2),
+    "amsim_i8_operand_workspace_bytes": (_sz, [_i64] * 2),
     "amsim_i8_quantize_workspace_bytes": (_sz, [_i64] * 2),
     "amsim_i8_quantize": (_i, [_p, _i, _i64, _i64, _i64, _p, _p, _p, _sz, _p]),
     "amsim_i8_dequantize": (_i, [_p, _i64, _i64, _i, _p, _p]),
@@ -98,14 +98,14 @@ SIGNATURES = {
     "amsim_i8_matmul": (_i, [_p, _p, _i64, _i64, _i64, _p, _i, _i, _p, _i, _p, _sz, _p]),
     "amsim_i8_linear_workspace_bytes": (_sz, [_i64] * 3),
     "amsim_i8_linear": (_i, [_p, _i, _i64, _p, _i64, _i64, _i64, _p, _i, _i, _p, _p, _sz, _p]),
-    "amsim_i8_kept_bytes": (_sz, [_i64] * 2),
+    "amsim_i8_kept_workspace_bytes": (_sz, [_i64] * 2),
     "amsim_i8_dense_workspace_bytes": (_sz, [_i64] * 3),
     "amsim_i8_dense": (_i, [_p, _i, _i64] * 2 + [_i64] * 3 + [_p, _i, _i] + [_p] * 4 + [_sz, _p]),
     "amsim_i8_dense_grad_workspace_bytes": (_sz, [_i64] * 3),
     "amsim_i8_dense_grad": (_i, [_p, _i, _i64] + [_p] * 3 + [_i64] * 3 + [_p, _p, _i, _p, _i, _p, _sz, _p]),
-    "amsim_kept8_bytes": (_sz, [_i64] * 2),
+    "amsim_kept8_workspace_bytes": (_sz, [_i64] * 2),
     "amsim_kept8_values": (_i, [_p, _i64, _i64, _i, _p, _p]),
-    "amsim_layer_norm": (_i, [_p, _i, _i64, _i64, _i64, _p, _p, _i, C.c_double, _p, _f, _p, _p]),
+    "amsim_layer_norm": (_i, [_p, _i, _i64, _i64, _i64, _p, _p, _i, C.c_float, _p, _f, _p, _p]),
     "amsim_layer_norm_grad_workspace_bytes": (_sz, [_i64] * 2),
     "amsim_layer_norm_grad": (_i, [_p, _i, _i64, _i64, _i64, _p, _i64, _p, _f, _p, _i, _p, _p, _p, _p, _sz, _p]),
     "amsim_activation": (_i, [_p, _i, _i64, _i64, _i64, _i, _p, _p, _p]),

@@ -554,7 +554,7 @@ using namespace amsim;
 
 extern "C" {
 
-size_t amsim_i8_operand_bytes(int64_t rows, int64_t length)
+size_t amsim_i8_operand_workspace_bytes(int64_t rows, int64_t length)
 {
     return i8_extents_fit(rows, length) && rows && length ? (size_t)i8_bytes(rows, length) : 0;
 }

@@ -652,7 +652,7 @@ int amsim_i8_linear(const void *x, int dtype, int64_t row_stride, const void *w,
     return product({operand(codes, scales, m), operand(w, n, k), k, bias, bias_dtype, act, out, dtype}, codes + operand_bytes(m, k), (hipStream_t)stream);
 }
 
-size_t amsim_i8_kept_bytes(int64_t rows, int64_t length) { return i8_extents_fit(rows, length) && rows && length ? kept_bytes(rows, length) : 0; }
+size_t amsim_i8_kept_workspace_bytes(int64_t rows, int64_t length) { return i8_extents_fit(rows, length) && rows && length ? kept_bytes(rows, length) : 0; }
 
 size_t amsim_i8_dense_workspace_bytes(int64_t m, int64_t n, int64_t k)
 {

@@ -689,7 +689,7 @@ using namespace amsim;
 
 extern "C" {
 
-size_t amsim_kept8_bytes(int64_t rows, int64_t cols)
+size_t amsim_kept8_workspace_bytes(int64_t rows, int64_t cols)
 {
     return mx_extents_fit(rows, cols) && rows && cols ? (size_t)kept8_bytes(rows, cols) : 0;
 }
@@ -703,7 +703,7 @@ int amsim_kept8_values(const void *kept, int64_t rows, int64_t cols, int dtype, 
 }
 
 int amsim_layer_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, const void *gamma, const void *beta, int param_dtype,
-                     double epsilon, void *out, float *statistics, void *kept, void *stream)
+                     float epsilon, void *out, float *statistics, void *kept, void *stream)
 {
     if (int rc = check_rows("layer_norm", x, dtype, rows, cols, row_stride)) return rc;
     if ((gamma || beta) && !known_dtype(param_dtype)) return fail(AMSIM_ERR_INVALID, "layer_norm: unknown element type");
@@ -712,7 +712,7 @@ int amsim_layer_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64
     const uintptr_t element = element_bytes(dtype), param = element_bytes(param_dtype);
     if (off(out, element) || off(statistics, 4) || off(kept, 16) || (gamma && off(gamma, param)) || (beta && off(beta, param)))
         return fail(AMSIM_ERR_INVALID, "layer_norm: misaligned pointer");
-    const NormArgs g{x, rows, row_stride, cols, gamma, beta, param_dtype, (float)epsilon, out, statistics, codes_of(kept), scales_of(kept, rows, cols), around(rows, cols, dtype)};
+    const NormArgs g{x, rows, row_stride, cols, gamma, beta, param_dtype, epsilon, out, statistics, codes_of(kept), scales_of(kept, rows, cols), around(rows, cols, dtype)};
     return with_type(dtype, [&](auto zero) {
         using T = decltype(zero);
         if (cols > MOST_HELD) {

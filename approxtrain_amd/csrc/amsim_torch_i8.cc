@@ -8,7 +8,7 @@ namespace {
 
 int64_t operand_bytes(int64_t rows, int64_t length)
 {
-    const size_t n = amsim_i8_operand_bytes(rows, length);
+    const size_t n = amsim_i8_operand_workspace_bytes(rows, length);
     if (n == 0) value_error("a " + std::to_string(rows) + " x " + std::to_string(length) + " tensor is out of the 8-bit products' range");
     return (int64_t)n;
 }
@@ -102,12 +102,12 @@ Forward dense(const Tensor &given, const Tensor &given_kernel, const std::option
     const int64_t m = x.rows, k = x.cols, n = kernel.cols;
     const Bias add = bias_of(bias, n, x.t);
     operand_bytes(m, k), operand_bytes(n, k);
-    if (keep_kernel && !amsim_i8_kept_bytes(k, n)) value_error("a layer of " + std::to_string(n) + " units is out of the 8-bit products' range");
-    if (keep_x && !amsim_i8_kept_bytes(k, m)) value_error("a batch of " + std::to_string(m) + " rows is out of the 8-bit products' range");
+    if (keep_kernel && !amsim_i8_kept_workspace_bytes(k, n)) value_error("a layer of " + std::to_string(n) + " units is out of the 8-bit products' range");
+    if (keep_x && !amsim_i8_kept_workspace_bytes(k, m)) value_error("a batch of " + std::to_string(m) + " rows is out of the 8-bit products' range");
     const size_t need = amsim_i8_dense_workspace_bytes(m, n, k);
     Forward f{matrix(m, n, x.t, x.t.scalar_type()), Tensor(), Tensor()};
-    if (keep_x) f.x_kept = bytes((int64_t)amsim_i8_kept_bytes(k, m), x.t);
-    if (keep_kernel) f.kernel_kept = bytes((int64_t)amsim_i8_kept_bytes(k, n), x.t);
+    if (keep_x) f.x_kept = bytes((int64_t)amsim_i8_kept_workspace_bytes(k, m), x.t);
+    if (keep_kernel) f.kernel_kept = bytes((int64_t)amsim_i8_kept_workspace_bytes(k, n), x.t);
     Tensor ws = bytes((int64_t)need, x.t);
     check(amsim_i8_dense(x.t.data_ptr(), x.dtype, x.stride, kernel.t.data_ptr(), kernel.dtype, kernel.stride, m, n, k, add.ptr(), add.dtype, act,
                          f.out.data_ptr(), keep_x ? f.x_kept.data_ptr() : nullptr, keep_kernel ? f.kernel_kept.data_ptr() : nullptr, ws.data_ptr(), need, stream()));
@@ -152,7 +152,7 @@ struct LinearI8 : torch::autograd::Function<LinearI8> {
                 auto is = [&](const Tensor &t, size_t size) {
                     return t.defined() && t.is_cuda() && t.get_device() == grad.t.get_device() && t.scalar_type() == at::kByte && t.is_contiguous() && t.numel() == (int64_t)size;
                 };
-                TORCH_CHECK((!want_kernel || is(saved[0], amsim_i8_kept_bytes(k, m))) && (!want_x || is(saved[1], amsim_i8_kept_bytes(k, n)))
+                TORCH_CHECK((!want_kernel || is(saved[0], amsim_i8_kept_workspace_bytes(k, m))) && (!want_x || is(saved[1], amsim_i8_kept_workspace_bytes(k, n)))
                                 && (!saved[2].defined() || (saved[2].is_cuda() && saved[2].get_device() == grad.t.get_device() && saved[2].scalar_type() == g.scalar_type()
                                                             && saved[2].is_contiguous() && saved[2].sizes() == g.sizes()))
                                 && grad.rows == m && grad.cols == n,

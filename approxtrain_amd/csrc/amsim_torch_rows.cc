@@ -42,15 +42,14 @@ Parameters parameters(const std::optional<Tensor> &gamma, const std::optional<Te
     if (gamma && beta && p.gamma.dtype != p.beta.dtype) type_error("gamma and beta must be of one type");
     return p;
 }
-float epsilon_of(double epsilon)
+void check_epsilon(double epsilon)
 {
     if (!(epsilon >= 0)) value_error("epsilon must not be negative");
-    return (float)epsilon;
 }
 
 Tensor kept_buffer(const Source &s)
 {
-    const size_t n = amsim_kept8_bytes(s.rows, s.cols);
+    const size_t n = amsim_kept8_workspace_bytes(s.rows, s.cols);
     if (n == 0) value_error("a " + std::to_string(s.rows) + " x " + std::to_string(s.cols) + " tensor is out of range");
     return bytes((int64_t)n, s.t);
 }
@@ -82,7 +81,7 @@ struct Normed {
 Normed norm(const Source &s, const Parameters &p, double epsilon, bool statistics, bool keep)
 {
     Normed n{like_rows(s), statistics ? matrix(s.rows, 2, s.t, at::kFloat) : Tensor(), keep ? kept_buffer(s) : Tensor()};
-    check(amsim_layer_norm(s.t.data_ptr(), s.dtype, s.rows, s.cols, s.stride, p.gamma.ptr(), p.beta.ptr(), p.dtype(), epsilon, n.out.data_ptr(),
+    check(amsim_layer_norm(s.t.data_ptr(), s.dtype, s.rows, s.cols, s.stride, p.gamma.ptr(), p.beta.ptr(), p.dtype(), (float)epsilon, n.out.data_ptr(),
                            statistics ? (float *)n.statistics.data_ptr() : nullptr, keep ? n.kept.data_ptr() : nullptr, stream()));
     return n;
 }
@@ -128,7 +127,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                 if (need_x) result[0] = like_rows(*g);
                 const std::optional<Source> x = kept ? std::nullopt : rows_of(saved[1], "x");
                 check_saved(g->cols == f[7] && plain(saved[0], g->t, at::kFloat, 2 * g->rows)
-                                && (kept ? plain(saved[1], g->t, at::kByte, (int64_t)amsim_kept8_bytes(g->rows, g->cols))
+                                && (kept ? plain(saved[1], g->t, at::kByte, (int64_t)amsim_kept8_workspace_bytes(g->rows, g->cols))
                                          : x->rows == g->rows && x->cols == g->cols && x->dtype == g->dtype && x->t.get_device() == g->t.get_device()),
                             "layernorm");
                 const Bias gamma = f[3] ? parameters(saved[2], std::nullopt, given[0]).gamma : Bias{};
@@ -152,7 +151,7 @@ Tensor layernorm(py::handle x_, py::handle gamma_, py::handle beta_, double epsi
     const std::optional<Tensor> gamma = maybe_tensor(gamma_, "gamma"), beta = maybe_tensor(beta_, "beta");
     if (x._fw_grad(0).defined() || (gamma && gamma->_fw_grad(0).defined()) || (beta && beta->_fw_grad(0).defined()))
         type_error("layernorm has no forward-mode derivative");
-    epsilon_of(epsilon);
+    check_epsilon(epsilon);
     auto requires = [](const std::optional<Tensor> &t) { return t && t->requires_grad(); };
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || requires(gamma) || requires(beta))) {
         const Parameters p = parameters(gamma, beta, x);
@@ -179,7 +178,7 @@ Tensor layer_norm(py::handle x_, py::handle gamma_, py::handle beta_, double eps
     no_derivative(x, "x", "layer_norm", "layernorm");
     if (gamma) no_derivative(*gamma, "gamma", "layer_norm", "layernorm");
     if (beta) no_derivative(*beta, "beta", "layer_norm", "layernorm");
-    epsilon_of(epsilon);
+    check_epsilon(epsilon);
     const Parameters p = parameters(gamma, beta, x);
     const std::optional<Source> s = rows_of(x, "x");
     return s ? shaped(norm(*s, p, epsilon, false, false).out, x) : at::empty(x.sizes(), x.options());
@@ -212,7 +211,7 @@ struct ActivationI8 : torch::autograd::Function<ActivationI8> {
             at::AutoGradMode off(false);
             const std::optional<Source> g = rows_of(given[0], "grad");
             result[0] = g ? like_rows(*g) : at::empty(given[0].sizes(), given[0].options());
-            if (g) check_saved(plain(saved[0], g->t, at::kByte, (int64_t)amsim_kept8_bytes(g->rows, g->cols)), "activationi8");
+            if (g) check_saved(plain(saved[0], g->t, at::kByte, (int64_t)amsim_kept8_workspace_bytes(g->rows, g->cols)), "activationi8");
             if (g)
                 check_in_graph(amsim_activation_grad(g->t.data_ptr(), g->dtype, g->rows, g->cols, g->stride, saved[0].data_ptr(), (int)f[0],
                                                      result[0].data_ptr(), stream()));
@@ -256,7 +255,7 @@ py::tuple keep8(py::handle x_)
 Tensor kept8_values(py::handle data_, int64_t rows, int64_t cols, py::handle dtype)
 {
     const Tensor &data = on_device(tensor(data_, "kept"), "kept");
-    const size_t need = amsim_kept8_bytes(rows, cols);
+    const size_t need = amsim_kept8_workspace_bytes(rows, cols);
     if (need == 0 || data.scalar_type() != at::kByte || !data.is_contiguous() || data.numel() != (int64_t)need)
         value_error("kept's data are not those of a " + std::to_string(rows) + " x " + std::to_string(cols) + " tensor");
     at::ScalarType t;

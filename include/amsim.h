@@ -352,7 +352,7 @@ int amsim_mxfp4_dense_grad(const void *grad, int dtype, int64_t row_stride, cons
  * reduction axis, and a scale for each row: of the row's largest magnitude a = max(|x|, 2^-119) the multiplier 127 / a and the
  * scale a / 127, rounded to 32 bits each; a value's code is the integer nearest to its exact product with the
  * multiplier (ties to even) and stands for code * scale.  A row that holds an infinity or a NaN has the scale NaN.  Operands are
- * opaque, amsim_i8_operand_bytes long (0: extents out of range, lengths above 2^21 among them) and start on 16-byte boundaries.
+ * opaque, amsim_i8_operand_workspace_bytes long (0: extents out of range, lengths above 2^21 among them) and start on 16-byte boundaries.
  *
  * amsim_i8_quantize: x[rows][cols] of `dtype`, rows row_stride elements apart, to an operand of its rows (rows x cols), of
  * its columns (cols x rows, for which the workspace is), or both; a direction that is not wanted is NULL.
@@ -360,7 +360,7 @@ int amsim_mxfp4_dense_grad(const void *grad, int dtype, int64_t row_stride, cons
  * amsim_i8_matmul: out[m][n] = act(sum_k a[m][k] b[n][k] + bias[n]), the sum over the codes exact, rounded to 32 bits, scaled,
  * and rounded to out_dtype once; bias may be NULL.  amsim_i8_linear: the same with a = x[m][k], quantised on the way.  Out
  * starts on a 16-byte boundary, the workspace on a 256-byte one.  Empty extents are refused (AMSIM_ERR_INVALID). */
-size_t amsim_i8_operand_bytes(int64_t rows, int64_t length);
+size_t amsim_i8_operand_workspace_bytes(int64_t rows, int64_t length);
 size_t amsim_i8_quantize_workspace_bytes(int64_t rows, int64_t cols);
 int amsim_i8_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void *by_rows,
                       void *by_columns, void *workspace, size_t workspace_bytes, void *stream);
@@ -375,14 +375,14 @@ int amsim_i8_linear(const void *x, int dtype, int64_t row_stride, const void *w,
 
 /* The training step of a dense layer in 8 bits, which keeps a byte of each activation.  amsim_i8_dense: out[m][n] = act(
  * x[m][k] kernel[k][n] + bias), x quantised by rows (scales sx), the kernel by columns (sw); for the backward pass
- * it keeps the codes that were multiplied, with their scales, in x_kept (amsim_i8_kept_bytes(k, m)) and kernel_kept
- * (amsim_i8_kept_bytes(k, n)), either of which may be NULL.  amsim_i8_dense_grad, for a gradient[m][n] of x's type: with
+ * it keeps the codes that were multiplied, with their scales, in x_kept (amsim_i8_kept_workspace_bytes(k, m)) and kernel_kept
+ * (amsim_i8_kept_workspace_bytes(k, n)), either of which may be NULL.  amsim_i8_dense_grad, for a gradient[m][n] of x's type: with
  * out (the forward pass's, for the rectifier) not NULL the gradient counts as zero where out is not above zero; the kept scales
  * go onto the gradient (each product rounded to 32 bits) before that is quantised, so that the kept codes are multiplied as
  * they are: grad_x[m][k] = Q(gradient[m][n] sw[n]) along n by the kernel's codes, grad_kernel[k][n] = x's codes by
  * Q(gradient[m][n] sx[m]) along m, and grad_bias[n] the sums of the gradient's columns in 32 bits, each in its tensor's type
  * and each NULL if not wanted.  No result depends on the order of arrival. */
-size_t amsim_i8_kept_bytes(int64_t rows, int64_t length);
+size_t amsim_i8_kept_workspace_bytes(int64_t rows, int64_t length);
 size_t amsim_i8_dense_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int amsim_i8_dense(const void *x, int dtype, int64_t row_stride, const void *kernel, int kernel_dtype,
                    int64_t kernel_row_stride, int64_t m, int64_t n, int64_t k, const void *bias, int bias_dtype, int act,
@@ -397,7 +397,7 @@ int amsim_i8_dense_grad(const void *grad, int dtype, int64_t row_stride, const v
  * What a backward pass needs of a tensor, a byte for each value: of a row's largest magnitude a = max(|x|, 2^-119) the
  * multiplier 127 / a and the scale a / 127, rounded to 32 bits each; a value's code is the integer nearest to its exact
  * product with the multiplier (ties to even) and stands for code * scale.  A row that holds an infinity or a NaN reads
- * back as NaN.  `kept` is opaque, amsim_kept8_bytes long (0: extents out of range) and starts on a 16-byte boundary.
+ * back as NaN.  `kept` is opaque, amsim_kept8_workspace_bytes long (0: extents out of range) and starts on a 16-byte boundary.
  *
  * amsim_layer_norm: out = (x - mean) / sqrt(var + epsilon) * gamma + beta over each row of x[rows][cols] (rows row_stride
  * elements apart; out is contiguous, of x's type); gamma and beta, of param_dtype, may be NULL.  For the backward pass:
@@ -406,10 +406,10 @@ int amsim_i8_dense_grad(const void *grad, int dtype, int64_t row_stride, const v
  * grad_beta of param_dtype, each NULL if not wanted; the workspace, 256-byte aligned, is for the latter two.
  * amsim_activation: out = f(x), f GELU, SWISH or NONE; out or kept may be NULL.  amsim_activation_grad: grad_x = grad
  * f'(kept's values).  amsim_kept8_values: those values.  No result depends on the order of arrival. */
-size_t amsim_kept8_bytes(int64_t rows, int64_t cols);
+size_t amsim_kept8_workspace_bytes(int64_t rows, int64_t cols);
 int amsim_kept8_values(const void *kept, int64_t rows, int64_t cols, int dtype, void *out, void *stream);
 int amsim_layer_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, const void *gamma,
-                     const void *beta, int param_dtype, double epsilon, void *out, float *statistics, void *kept,
+                     const void *beta, int param_dtype, float epsilon, void *out, float *statistics, void *kept,
                      void *stream);
 size_t amsim_layer_norm_grad_workspace_bytes(int64_t rows, int64_t cols);
 int amsim_layer_norm_grad(const void *grad, int dtype, int64_t rows, int64_t cols, int64_t row_stride, const void *x,

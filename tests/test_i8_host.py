@@ -14,12 +14,12 @@ def lib():
 
 
 def test_operand_sizes():
-    size = lib().amsim_i8_operand_bytes
+    size = lib().amsim_i8_operand_workspace_bytes
     assert size(1, 1) == 1024 + 4 and size(16, 64) == 1024 + 64 and size(17, 65) == 2 * 2 * 1024 + 68
     assert size(4096, 4096) == 4096 * 4096 + 4 * 4096
     assert size(1, 1 << 21) == (1 << 15) * 1024 + 4 and size(1, (1 << 21) + 1) == 0
     assert size(-1, 5) == size(5, -1) == size(0, 5) == size(5, 0) == size(1 << 31, 1) == 0
-    kept = lib().amsim_i8_kept_bytes
+    kept = lib().amsim_i8_kept_workspace_bytes
     assert kept(17, 65) == 4 * 1024 + 4 * 65 and kept(0, 4) == 0 and kept(4, 1 << 22) == 0
 
 

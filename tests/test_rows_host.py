@@ -14,7 +14,7 @@ def lib():
 
 
 def test_sizes():
-    size = lib().amsim_kept8_bytes
+    size = lib().amsim_kept8_workspace_bytes
     assert size(1, 1) == 20 and size(3, 16) == 3 * 20 and size(3, 17) == 3 * 36 and size(0, 4) == size(4, 0) == size(-1, 4) == size(1 << 31, 1) == 0
     ws = lib().amsim_layer_norm_grad_workspace_bytes
     assert ws(1, 1) == 8 and ws(0, 4) == ws(4, -1) == 0 and ws(1 << 20, 4096) == 768 * 2 * 4096 * 4
