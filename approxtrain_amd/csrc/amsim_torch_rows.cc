@@ -61,7 +61,7 @@ void check_in_graph(int status) { TORCH_CHECK(status == 0, "amsim status ", stat
 void no_capture(AutogradContext *ctx, int64_t eager, const char *call)
 {
     for (int i = 0; i < 3; ++i)
-        TORCH_CHECK(!(eager >> i & 1) || !ctx->needs_input_grad(i) || !capturing(), call, 
+        TORCH_CHECK(!(eager >> i & 1) || !ctx->needs_input_grad(i) || !capturing(), call,
                     "'s backward pass is captured while a graph of the same leaves lives that was made on the default stream, where "
                     "their gradients would be added: release it (its outputs and losses) before the capture");
 }
@@ -126,7 +126,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             } else {
                 if (need_x) result[0] = like_rows(*g);
                 const std::optional<Source> x = kept ? std::nullopt : rows_of(saved[1], "x");
-                check_saved(g->cols == f[7] && plain(saved[0], g->t, at::kFloat, 2 * g->rows)
+                check_saved(g->cols == f[7] && (!f[3] || (saved[2].defined() && saved[2].scalar_type() == type)) && plain(saved[0], g->t, at::kFloat, 2 * g->rows)
                                 && (kept ? plain(saved[1], g->t, at::kByte, (int64_t)amsim_kept8_workspace_bytes(g->rows, g->cols))
                                          : x->rows == g->rows && x->cols == g->cols && x->dtype == g->dtype && x->t.get_device() == g->t.get_device()),
                             "layernorm");
