@@ -87,31 +87,41 @@ Tensor i8_linear(py::handle given, py::handle data, int64_t n, int64_t k, py::ha
 
 // ---- the training step of a layer -------------------------------------------------------------------------------
 
-struct Forward {
-    Tensor out, x_kept, kernel_kept;
+// What is kept of x and of the kernel, one behind the other in a buffer.
+struct Kept {
+    int64_t x, kernel;  // bytes of either, 0 where it is not kept
+    Kept(int64_t m, int64_t n, int64_t k, bool keep_x, bool keep_kernel)
+        : x(keep_x ? (int64_t)amsim_i8_kept_workspace_bytes(k, m) : 0), kernel(keep_kernel ? (int64_t)amsim_i8_kept_workspace_bytes(k, n) : 0)
+    {
+    }
+    int64_t first() const { return (x + 15) / 16 * 16; }
+    int64_t all() const { return first() + kernel; }
+    uint8_t *of_x(const Tensor &t) const { return x ? (uint8_t *)t.data_ptr() : nullptr; }
+    uint8_t *of_kernel(const Tensor &t) const { return kernel ? (uint8_t *)t.data_ptr() + first() : nullptr; }
 };
-Forward dense(const Tensor &given, const Tensor &given_kernel, const std::optional<Tensor> &bias, int act, bool keep_x, bool keep_kernel)
+
+// (the result, what is kept)
+std::pair<Tensor, Tensor> dense(const Tensor &given, const Tensor &given_kernel, const std::optional<Tensor> &bias, int act, bool keep_x, bool keep_kernel)
 {
     const Source kernel = row_source(given_kernel, "kernel");
     if (given.size(0) == 0) {  // (a batch of nothing, as a router may leave to an expert)
         known(on_device(given, "x").scalar_type(), "x");
         bias_of(bias, kernel.cols, given);
-        return {matrix(0, kernel.cols, given, given.scalar_type()), bytes(0, given), bytes(0, given)};
+        return {matrix(0, kernel.cols, given, given.scalar_type()), bytes(0, given)};
     }
     const Source x = row_source(given, "x");
     const int64_t m = x.rows, k = x.cols, n = kernel.cols;
     const Bias add = bias_of(bias, n, x.t);
     operand_bytes(m, k), operand_bytes(n, k);
-    if (keep_kernel && !amsim_i8_kept_workspace_bytes(k, n)) value_error("a layer of " + std::to_string(n) + " units is out of the 8-bit products' range");
-    if (keep_x && !amsim_i8_kept_workspace_bytes(k, m)) value_error("a batch of " + std::to_string(m) + " rows is out of the 8-bit products' range");
+    const Kept keep(m, n, k, keep_x, keep_kernel);
+    if (keep_kernel && !keep.kernel) value_error("a layer of " + std::to_string(n) + " units is out of the 8-bit products' range");
+    if (keep_x && !keep.x) value_error("a batch of " + std::to_string(m) + " rows is out of the 8-bit products' range");
     const size_t need = amsim_i8_dense_workspace_bytes(m, n, k);
-    Forward f{matrix(m, n, x.t, x.t.scalar_type()), Tensor(), Tensor()};
-    if (keep_x) f.x_kept = bytes((int64_t)amsim_i8_kept_workspace_bytes(k, m), x.t);
-    if (keep_kernel) f.kernel_kept = bytes((int64_t)amsim_i8_kept_workspace_bytes(k, n), x.t);
-    Tensor ws = bytes((int64_t)need, x.t);
+    Tensor out = matrix(m, n, x.t, x.t.scalar_type()), kept, ws = bytes((int64_t)need, x.t);
+    if (keep.all()) kept = bytes(keep.all(), x.t);
     check(amsim_i8_dense(x.t.data_ptr(), x.dtype, x.stride, kernel.t.data_ptr(), kernel.dtype, kernel.stride, m, n, k, add.ptr(), add.dtype, act,
-                         f.out.data_ptr(), keep_x ? f.x_kept.data_ptr() : nullptr, keep_kernel ? f.kernel_kept.data_ptr() : nullptr, ws.data_ptr(), need, stream()));
-    return f;
+                         out.data_ptr(), keep.of_x(kept), keep.of_kernel(kept), ws.data_ptr(), need, stream()));
+    return {out, kept};
 }
 
 // x is kept as the codes that were multiplied, a byte for each value, and so is the kernel; the backward pass multiplies
@@ -120,11 +130,11 @@ struct LinearI8 : torch::autograd::Function<LinearI8> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &kernel, const std::optional<Tensor> &bias, int64_t act, int64_t eager)
     {
         const bool need_x = x.requires_grad(), need_kernel = kernel.requires_grad();
-        const Forward f = dense(x, kernel, bias, (int)act, need_kernel, need_x);
-        ctx->save_for_backward({need_kernel ? f.x_kept : Tensor(), need_x ? f.kernel_kept : Tensor(), act == AMSIM_ACT_RELU ? f.out : Tensor()});
+        auto [out, kept] = dense(x, kernel, bias, (int)act, need_kernel, need_x);
+        ctx->save_for_backward(act == AMSIM_ACT_RELU ? variable_list{kept, out} : variable_list{kept});
         ctx->saved_data["shape"] = std::vector<int64_t>{x.size(0), x.size(1), kernel.size(1), need_x, need_kernel, (int64_t)kernel.scalar_type(),
                                                         bias && bias->requires_grad() ? (int64_t)bias->scalar_type() : -1, eager};
-        return f.out;
+        return out;
     }
 
     static variable_list backward(AutogradContext *ctx, const variable_list &given)
@@ -148,19 +158,18 @@ struct LinearI8 : torch::autograd::Function<LinearI8> {
             if (want_bias) grads[2] = m ? at::empty({n}, like.dtype(bias_type)) : at::zeros({n}, like.dtype(bias_type));
             if (m) {
                 const Source grad = row_source(g, "grad");
+                const Kept keep(m, n, k, s[4], s[3]);
+                const Tensor &kept = saved[0], none, &out = saved.size() > 1 ? saved[1] : none;
                 // (a hook may have brought back something else than was saved)
-                auto is = [&](const Tensor &t, size_t size) {
-                    return t.defined() && t.is_cuda() && t.get_device() == grad.t.get_device() && t.scalar_type() == at::kByte && t.is_contiguous() && t.numel() == (int64_t)size;
+                auto is = [&](const Tensor &t, at::ScalarType type, int64_t size) {
+                    return t.defined() && t.is_cuda() && t.get_device() == grad.t.get_device() && t.scalar_type() == type && t.is_contiguous() && t.numel() == size;
                 };
-                TORCH_CHECK((!want_kernel || is(saved[0], amsim_i8_kept_workspace_bytes(k, m))) && (!want_x || is(saved[1], amsim_i8_kept_workspace_bytes(k, n)))
-                                && (!saved[2].defined() || (saved[2].is_cuda() && saved[2].get_device() == grad.t.get_device() && saved[2].scalar_type() == g.scalar_type()
-                                                            && saved[2].is_contiguous() && saved[2].sizes() == g.sizes()))
-                                && grad.rows == m && grad.cols == n,
+                TORCH_CHECK((!keep.all() || is(kept, at::kByte, keep.all())) && (!out.defined() || is(out, g.scalar_type(), m * n)) && grad.rows == m && grad.cols == n,
                             "what lineari8 kept for its backward pass came back in another form");
                 const size_t need = amsim_i8_dense_grad_workspace_bytes(m, n, k);
                 Tensor ws = bytes((int64_t)need, grad.t);
                 auto ptr = [](const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
-                const int status = amsim_i8_dense_grad(grad.t.data_ptr(), grad.dtype, grad.stride, ptr(saved[2]), ptr(saved[0]), ptr(saved[1]), m, n, k, ptr(grads[0]),
+                const int status = amsim_i8_dense_grad(grad.t.data_ptr(), grad.dtype, grad.stride, ptr(out), keep.of_x(kept), keep.of_kernel(kept), m, n, k, ptr(grads[0]),
                                                        ptr(grads[1]), code_of(kernel_type), ptr(grads[2]), code_of(bias_type), ws.data_ptr(), need, stream());
                 TORCH_CHECK(status == 0, "amsim status ", status, ": ", amsim_last_error());
             }
@@ -182,7 +191,7 @@ Tensor lineari8(py::handle x_, py::handle kernel_, py::handle bias_, int act)
     const Tensor flat = x.dim() == 2 ? x : x.reshape({x.numel() ? -1 : 0, x.size(-1)});
     const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || kernel.requires_grad() || (bias && bias->requires_grad()));
     const int64_t eager = graph && capturing() ? adds_on_default_stream(x) | adds_on_default_stream(kernel) << 1 | (bias && adds_on_default_stream(*bias)) << 2 : 0;
-    const Tensor out = graph ? LinearI8::apply(flat, kernel, bias, (int64_t)act, eager) : dense(flat, kernel, bias, act, false, false).out;
+    const Tensor out = graph ? LinearI8::apply(flat, kernel, bias, (int64_t)act, eager) : dense(flat, kernel, bias, act, false, false).first;
     if (x.dim() == 2) return out;
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
     shape.back() = kernel.size(1);
