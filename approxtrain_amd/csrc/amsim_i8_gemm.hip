@@ -279,14 +279,19 @@ __global__ __launch_bounds__(1024) void few_kernel(FewArgs g)
     for (int64_t s = wave; s < g.steps; s += AHEAD * waves) {
         FewSteps b;
         b.load(g, blockIdx.x, s, waves);
+        // The rows' codes with them, all at once: a step's loads in their turn would each be a trip to the L2 (64 rows by
+        // 4096 x 4096: 9.5 us that way, 7.7 this; 16 rows by 4096 x 4096 5.8 and 5.7).
+        v4i a[AHEAD][FA];
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) {
-            const int64_t t = s + h * waves;
-            if (t >= g.steps) break;
-            v4i a[FA];
+            const int64_t t = min<int64_t>(s + h * waves, g.steps - 1);
 #pragma unroll
-            for (int i = 0; i < FA; ++i) a[i] = *(const v4i *)(g.a.codes + ((min<int64_t>(i, g.a.fragments - 1) * g.steps + t) * 64 + lane) * 16);
-            for_each<FA>([&](auto i) { acc[i.value] = mfma(b.codes[h], a[i.value], acc[i.value]); });
+            for (int i = 0; i < FA; ++i) a[h][i] = *(const v4i *)(g.a.codes + ((min<int64_t>(i, g.a.fragments - 1) * g.steps + t) * 64 + lane) * 16);
+        }
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h) {
+            if (s + h * waves >= g.steps) break;
+            for_each<FA>([&](auto i) { acc[i.value] = mfma(b.codes[h], a[h][i.value], acc[i.value]); });
         }
     }
     finish_few(g, ends, blockIdx.x, sums, acc, g.a.scales);
@@ -441,17 +446,19 @@ struct Costs {
     static constexpr int64_t STEP = I8_STEP, MOST_STEPS = I8_MOST_STEPS;
 };
 
-// Whether few_kernel serves, by rows and length alone: a reduction beyond that needs more than one workgroup's waves.  us of the
-// product by itself, few_kernel / tiles, of 16, 32 and 64 rows: length 4096, 4096 wide 5.2/10.0, 6.2/11.5, 8.7/11.5; length 8192, 1024
-// wide 6.0/11.9, 7.7/10.5, 12.5/11.5; length 1024, 8192 wide 4.4/5.3, 5.3/5.3, 7.1/5.4.
-bool few(int64_t m, int64_t k) { return m <= 64 && i8_steps(k) <= 256; }
+// Whether few_kernel serves: a reduction beyond that needs more than one workgroup's waves, and a wider result has every workgroup
+// fetch the rows again for 16 columns.  us of the product by itself, few_kernel / tiles, of 16, 32 and 64 rows: length 4096, 4096 wide
+// 6.0/10.7, 6.2/11.0, 7.6/11.6; length 8192, 1024 wide 6.0/12.3, 7.1/11.1, 10.1/12.3; length 1024, 8192 wide 5.0/5.5, 5.2/5.8, 6.4/5.9,
+// 32768 wide 12.2/9.5, 15.1/9.7, -; length 4096, 32768 wide 32.9/28.8, 38.7/30.7, 51.0/30.9; length 16384, 1024 wide 8.9/14.5,
+// 11.1/15.1, 17.4/15.4.
+bool few(const Extents &e) { return e.m <= 64 && e.n <= 8192 && i8_steps(e.k) <= 256; }
 
 // the products of a list that go in tiles, and the others
 int tiled(const Extents *e, int count, Extents *out, int *which)
 {
     int n = 0;
     for (int j = 0; j < count; ++j)
-        if (!few(e[j].m, e[j].k)) out[n] = e[j], which[n++] = j;
+        if (!few(e[j])) out[n] = e[j], which[n++] = j;
     return n;
 }
 
@@ -514,7 +521,7 @@ int products(const Product *list, int count, void *workspace, hipStream_t stream
     const int n = tiled(e, count, t, which);
     for (int j = 0; j < count; ++j) {
         const Product &q = list[j];
-        if (!few(e[j].m, e[j].k)) continue;
+        if (!few(e[j])) continue;
         const FewArgs f{q.b, q.a, nullptr, 0, q.a.rows, q.k, i8_steps(q.k), q.bias, q.bias_dtype, q.act, q.out_dtype, q.out};
         if (int rc = launch_few(q.a.rows <= 16 ? few_kernel<1> : q.a.rows <= 32 ? few_kernel<2> : few_kernel<4>, f, few_waves(f, 0), 0, stream)) return rc;
     }

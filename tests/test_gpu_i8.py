@@ -135,7 +135,7 @@ def test_scales_of_every_size_beside_each_other(m, n):
 
 
 PRODUCTS = [(1, 1, 1), (1, 4096, 64), (1, 10, 70), (2, 33, 9000), (3, 1000, 4096), (5, 17, 6000), (8, 130, 4096), (9, 257, 3600), (13, 1003, 2051), (16, 64, 16384),
-            (17, 100, 16384), (31, 77, 1000), (33, 200, 990), (48, 513, 640), (64, 40, 512), (64, 300, 4000), (65, 64, 64), (64, 10, 16385), (100, 10, 40000),
+            (17, 100, 16384), (31, 77, 1000), (33, 200, 990), (48, 513, 640), (64, 40, 512), (64, 300, 4000), (65, 64, 64), (64, 10, 16385), (64, 8192, 192), (64, 8193, 192), (5, 8200, 1100), (100, 10, 40000),
             (129, 300, 784), (257, 515, 129), (1000, 1003, 333), (2048, 2048, 200), (300, 5000, 70), (4099, 17, 260)]
 
 
