@@ -417,24 +417,28 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(ColumnSums g)
 
 // ---- activations whose input is kept -------------------------------------------------------------------------------------
 
-// Phi(-|x|) = exp(-x^2 / 2) R(|x|), R by a polynomial in 1 / (1 + 0.3 |x|), least in its largest relative error, 1.6e-7, on
-// |x| <= 14.5 (the coefficients: weighted least squares on the scaled complementary error function, the weights raised
-// where the error was largest).  With the roundings Phi is within 2.5e-7.  Some 25 instructions, two of them at a quarter
-// rate: the language's erfcf takes so many more that the vector units, not memory, would be the bound.
+// Phi(-t) = exp(-t^2 / 2) R(t), t = |x|, and R(t) = 1/2 + w Q(w) in w = t / (1 + t / 4): what the reciprocal and Q are off by
+// counts with w, so that next to zero little is left of it.  Q's coefficients: least largest relative error of R on t <= 14.5
+// (least squares on the scaled complementary error function, the weights raised where the error was largest, one coefficient
+// after the other rounded to 32 bits), 2.1e-8.  Below -13.2, where the gelu is less than 2^-126, it comes out as zero.  Largest relative errors measured over 2^20 values
+// each: the gelu on -1 .. 0 3.1e-7, on -4 .. -1 1.2e-6, on -12 .. -4 9.2e-6 (the exponent's rounding), above zero 2e-7; in elementary
+// 32-bit operations with the language's erfcf 2.8e-7, 1.2e-6, 1.1e-5 and 2.3e-7.  Some 26 instructions, two of them at a
+// quarter rate: erfcf takes so many more that the vector units, not memory, would be the bound.
 struct Gelu {
     static __device__ __forceinline__ void parts(float x, float &phi, float &density)
     {
-        const float t = fabsf(x), u = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3f, t, 1.0f));
-        float p = 0.03542371094226837f;
-        p = __builtin_fmaf(p, u, -0.15615835785865784f);
-        p = __builtin_fmaf(p, u, 0.2045566290616989f);
-        p = __builtin_fmaf(p, u, -0.05203388258814812f);
-        p = __builtin_fmaf(p, u, 0.12769170105457306f);
-        p = __builtin_fmaf(p, u, 0.10017596930265427f);
-        p = __builtin_fmaf(p, u, 0.12071213126182556f);
-        p = __builtin_fmaf(p, u, 0.11963200569152832f);
+        const float t = fminf(fabsf(x), 15.0f), w = t * __builtin_amdgcn_rcpf(__builtin_fmaf(0.25f, t, 1.0f));
+        float q = -1.278699954809781e-07f;
+        q = __builtin_fmaf(q, w, 1.6464955479023047e-06f);
+        q = __builtin_fmaf(q, w, -2.7883238544745836e-06f);
+        q = __builtin_fmaf(q, w, -5.159039574209601e-05f);
+        q = __builtin_fmaf(q, w, 0.00010789257066790015f);
+        q = __builtin_fmaf(q, w, 0.003397819586098194f);
+        q = __builtin_fmaf(q, w, -0.032908763736486435f);
+        q = __builtin_fmaf(q, w, 0.15026246011257172f);
+        q = __builtin_fmaf(q, w, -0.3989420533180237f);
         const float e = __builtin_amdgcn_exp2f(t * t * -0.72134752f);
-        const float tail = u * p * e;
+        const float tail = __builtin_fmaf(q, w, 0.5f) * e;
         phi = x < 0.0f ? tail : 1.0f - tail;
         density = e * 0.39894228f;
     }
@@ -451,13 +455,33 @@ struct Gelu {
         return __builtin_fmaf(x, density, phi);
     }
 };
+// With e = exp(-x) the swish is x / (1 + e), its slope s + x s (1 - s) of s = 1 / (1 + e); 1 - s is e s where s is near one.  exp2's argument is rounded, which
+// would cost as many last places as x is large: what was lost is put back by the first term of its series.  The
+// reciprocal, a last place off by itself, is corrected by its residual.  Beyond 64 the one or the other of 1 and e is nothing beside the other,
+// and exp(x) is held 2^64 times as large, or it would be zero from -88 on, where the swish itself is so only from -104 on.
+// The swish in 32 bits is within 2.2e-7 of itself from -87 on; without the corrections within 3.9e-6, and in 16 bits 5.9375 went to its
+// farther neighbour.
 struct Swish {
-    static __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f)); }
-    static __device__ __forceinline__ float value(float x) { return x * sigmoid(x); }
+    static constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596299e-8f, LN2 = 0.693147182f;
+    // exp2(x log2(e) + more)
+    static __device__ __forceinline__ float exponential(float x, float more)
+    {
+        const float a = x * LOG2E, rest = __builtin_fmaf(x, LOG2E_REST, __builtin_fmaf(x, LOG2E, -a)), e = __builtin_amdgcn_exp2f(a + more);
+        return __builtin_fmaf(e, rest * LN2, e);
+    }
+    static __device__ __forceinline__ bool far(float x) { return fabsf(x) > 64.0f; }
+    static __device__ __forceinline__ float far_exponential(float x) { return exponential(fmaxf(x, -200.0f), 64.0f); }  // (2^64 exp(x))
+    static __device__ __forceinline__ float value(float x)
+    {
+        if (far(x)) return x > 0.0f ? x : x * far_exponential(x) * 0x1p-64f;
+        const float d = 1.0f + exponential(-x, 0.0f), r = __builtin_amdgcn_rcpf(d), q = x * r;
+        return __builtin_fmaf(__builtin_fmaf(-d, q, x), r, q);
+    }
     static __device__ __forceinline__ float slope(float x)
     {
-        const float s = sigmoid(x);
-        return __builtin_fmaf(x * s, 1.0f - s, s);
+        if (far(x)) return x > 0.0f ? 1.0f : (1.0f + x) * far_exponential(x) * 0x1p-64f;
+        const float e = exponential(-x, 0.0f), d = 1.0f + e, r = __builtin_amdgcn_rcpf(d), s = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+        return __builtin_fmaf(x * s, x < 1.0f ? 1.0f - s : e * s, s);
     }
 };
 struct Linear {  // (nothing but the keeping)
