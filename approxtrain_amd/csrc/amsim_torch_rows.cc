@@ -125,11 +125,13 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                 if (need_x) result[0] = at::empty(given[0].sizes(), given[0].options());
             } else {
                 if (need_x) result[0] = like_rows(*g);
-                const std::optional<Source> x = kept ? std::nullopt : rows_of(saved[1], "x");
+                const Tensor &of_x = saved[1];
                 check_saved(g->cols == f[7] && (!f[3] || (saved[2].defined() && saved[2].scalar_type() == type)) && plain(saved[0], g->t, at::kFloat, 2 * g->rows)
-                                && (kept ? plain(saved[1], g->t, at::kByte, (int64_t)amsim_kept8_workspace_bytes(g->rows, g->cols))
-                                         : x->rows == g->rows && x->cols == g->cols && x->dtype == g->dtype && x->t.get_device() == g->t.get_device()),
+                                && (kept ? plain(of_x, g->t, at::kByte, (int64_t)amsim_kept8_workspace_bytes(g->rows, g->cols))
+                                         : of_x.defined() && of_x.is_cuda() && of_x.layout() == at::kStrided && of_x.get_device() == g->t.get_device()
+                                               && of_x.scalar_type() == g->t.scalar_type() && of_x.dim() == 2 && of_x.size(0) == g->rows && of_x.size(1) == g->cols),
                             "layernorm");
+                const std::optional<Source> x = kept ? std::nullopt : rows_of(of_x, "x");
                 const Bias gamma = f[3] ? parameters(saved[2], std::nullopt, given[0]).gamma : Bias{};
                 const size_t need = need_gamma || need_beta ? amsim_layer_norm_grad_workspace_bytes(g->rows, g->cols) : 0;
                 Tensor ws;
