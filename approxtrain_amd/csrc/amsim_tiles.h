@@ -187,11 +187,7 @@ template <typename Costs> Plan make_plan(const Extents *e, int count)
 {
     Plan best{-1, {}};
     double least = 0;
-#ifndef X_TILE
-#define X_TILE i
-#endif
     for (int i = 0; i < 4; ++i) {
-        if (i != X_TILE) continue;
         Plan p{i, {}};
         double tiles = 0, work = 0, longest = 0, more = 0;
         for (int j = 0; j < count; ++j) {
