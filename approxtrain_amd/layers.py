@@ -566,24 +566,37 @@ class packed_densei8(nn.Module):
         return out
 
 
-class LayerNormalization(nn.Module):
-    """Layer normalisation over the last axis with the Keras layer's vocabulary (``epsilon, center, scale`` and the
-    initializers of ``beta`` and ``gamma``); the parameters are 32-bit floats, activations float32, bfloat16 or float16.
-    ``keep_bits=8`` keeps the input for the backward pass in 8 bits (``math_ops.layernorm``)."""
+class LayerNormalization(nn.Module, _KerasLayerArgs):
+    """Layer normalisation over the last axis with the Keras layer's vocabulary (``axis, epsilon, center, scale``, the
+    initializers, regularizers and constraints of ``beta`` and ``gamma``, and what every layer takes besides); the
+    parameters are 32-bit floats, activations float32, bfloat16 or float16.  ``axis``: -1, or the last axis's index, by itself or
+    in a list.  ``keep_bits=8`` keeps the input for the backward pass in 8 bits (``math_ops.layernorm``)."""
 
     def __init__(self, axis=-1, epsilon=1e-3, center=True, scale=True, beta_initializer="zeros", gamma_initializer="ones", keep_bits=None,
-                 input_dim=None):
+                 input_dim=None, beta_regularizer=None, gamma_regularizer=None, beta_constraint=None, gamma_constraint=None, **kwargs):
         super().__init__()
-        if axis != -1:
-            raise ValueError("only the last axis (-1) is normalised")
+        if isinstance(axis, (list, tuple)) and len(axis) == 1:
+            axis, = axis
+        if not isinstance(axis, int) or axis < -1 or axis == 0:
+            raise ValueError("only the last axis is normalised: -1, or its index")
         if not epsilon >= 0:
             raise ValueError("epsilon must not be negative")
         if keep_bits not in (None, 8):
             raise ValueError("keep_bits must be None or 8")
-        self.epsilon, self.center, self.scale, self.keep_bits = epsilon, center, scale, keep_bits
+        for what, f in (("beta_regularizer", beta_regularizer), ("gamma_regularizer", gamma_regularizer), ("beta_constraint", beta_constraint),
+                        ("gamma_constraint", gamma_constraint)):
+            if f is not None and not callable(f):
+                raise ValueError(f"{what} must be a callable or None")
+        activity_regularizer = kwargs.pop("activity_regularizer", None)
+        input_shape = self._keras_args(None, None, activity_regularizer, None, None, kwargs)
+        self.axis, self.epsilon, self.center, self.scale, self.keep_bits = axis, epsilon, center, scale, keep_bits
         self.beta_initializer, self.gamma_initializer = beta_initializer, gamma_initializer
+        self.beta_regularizer, self.gamma_regularizer = beta_regularizer, gamma_regularizer
+        self.beta_constraint, self.gamma_constraint = beta_constraint, gamma_constraint
         self.gamma = None
         self.beta = None
+        if input_dim is None and input_shape is not None:
+            input_dim = input_shape[-1]
         if input_dim is not None:
             self.build(input_dim)
 
@@ -592,14 +605,31 @@ class LayerNormalization(nn.Module):
             self.gamma = nn.Parameter(_initialize_(torch.empty(input_dim, device=device), self.gamma_initializer, input_dim, input_dim))
         if self.center:
             self.beta = nn.Parameter(_initialize_(torch.empty(input_dim, device=device), self.beta_initializer, input_dim, input_dim))
+        self._finish_build()
 
     def forward(self, inputs):
+        if self.axis not in (-1, inputs.dim() - 1):
+            raise ValueError(f"only the last axis is normalised: axis {self.axis} is not that of a tensor of {inputs.dim()} axes")
         if (self.scale and self.gamma is None) or (self.center and self.beta is None):
             self.build(inputs.shape[-1], inputs.device)
-        return layernorm(inputs, self.gamma, self.beta, self.epsilon, self.keep_bits)
+        return self._track_activity(layernorm(inputs, self.gamma, self.beta, self.epsilon, self.keep_bits))
+
+    def losses(self):
+        """Regularization terms of this layer (Keras ``layer.losses``), to be added to the objective."""
+        out = [f(p) for f, p in ((self.gamma_regularizer, self.gamma), (self.beta_regularizer, self.beta)) if f is not None and p is not None]
+        if self._activity_loss is not None:
+            out.append(self._activity_loss)
+        return out
+
+    def apply_constraints(self):
+        """Projects gamma and beta through their constraints (Keras does so after each update)."""
+        with torch.no_grad():
+            for f, p in ((self.gamma_constraint, self.gamma), (self.beta_constraint, self.beta)):
+                if f is not None and p is not None:
+                    p.copy_(f(p))
 
     def get_config(self):
-        return {"epsilon": self.epsilon, "center": self.center, "scale": self.scale, "keep_bits": self.keep_bits}
+        return {"axis": self.axis, "epsilon": self.epsilon, "center": self.center, "scale": self.scale, "keep_bits": self.keep_bits}
 
 
 class _Attention(torch.autograd.Function):
