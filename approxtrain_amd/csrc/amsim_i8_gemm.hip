@@ -692,13 +692,16 @@ int amsim_i8_dense(const void *x, int dtype, int64_t row_stride, const void *ker
     return product({operand(x_rows, x_scales, m), operand(kernel_columns, kernel_scales, n), k, bias, bias_dtype, act, out, dtype}, partial, s);
 }
 
+static size_t gradient_columns_bytes(int64_t m, int64_t n, int64_t k) { return i8_extents_fit(k, m) ? operand_bytes(n, m) : 0; }
+
 size_t amsim_i8_dense_grad_workspace_bytes(int64_t m, int64_t n, int64_t k)
 {
-    if (!product_fits(m, n, k) || !i8_extents_fit(k, n) || !i8_extents_fit(k, m)) return 0;
+    if (!product_fits(m, n, k)) return 0;
+    // (the products of either gradient alone are planned by themselves, and one whose reduction is too long is not asked for)
     const Extents e[2] = {{m, k, n}, {k, n, m}};
-    // (the products of either gradient alone are planned by themselves)
-    return operand_bytes(m, n) + operand_bytes(n, m) + aligned(4 * i8_partial_floats(m, n))
-         + std::max({products_workspace(e, 2), products_workspace(e, 1), products_workspace(e + 1, 1)});
+    const bool of_x = i8_extents_fit(k, n), of_kernel = i8_extents_fit(k, m);
+    return operand_bytes(m, n) + gradient_columns_bytes(m, n, k) + aligned(4 * i8_partial_floats(m, n))
+         + std::max({of_x && of_kernel ? products_workspace(e, 2) : 0, of_x ? products_workspace(e, 1) : 0, of_kernel ? products_workspace(e + 1, 1) : 0});
 }
 
 int amsim_i8_dense_grad(const void *grad, int dtype, int64_t row_stride, const void *out, const void *x_kept, const void *kernel_kept,
@@ -707,7 +710,7 @@ int amsim_i8_dense_grad(const void *grad, int dtype, int64_t row_stride, const v
 {
     if (!known_dtype(dtype) || (grad_kernel && !known_dtype(kernel_dtype)) || (grad_bias && !known_dtype(bias_dtype)))
         return fail(AMSIM_ERR_INVALID, "int8: unknown element type");
-    if (!i8_extents_fit(m, k) || !i8_extents_fit(n, k) || !mx_extents_fit(m, n) || !i8_extents_fit(k, n) || !i8_extents_fit(k, m))
+    if (!i8_extents_fit(m, k) || !i8_extents_fit(n, k) || !mx_extents_fit(m, n) || (grad_x && !i8_extents_fit(k, n)) || (grad_kernel && !i8_extents_fit(k, m)))
         return fail(AMSIM_ERR_UNSUPPORTED, "int8: extents out of range");
     if (m == 0 || n == 0 || k == 0) return fail(AMSIM_ERR_INVALID, "int8: empty product");
     if (row_stride < n && m > 1) return fail(AMSIM_ERR_INVALID, "int8: rows overlap");
@@ -720,7 +723,7 @@ int amsim_i8_dense_grad(const void *grad, int dtype, int64_t row_stride, const v
     if (!grad_x && !grad_kernel && !grad_bias) return AMSIM_OK;
     hipStream_t s = (hipStream_t)stream;
     uint8_t *rows = (uint8_t *)workspace, *columns = rows + operand_bytes(m, n);
-    float *looked = (float *)(columns + operand_bytes(n, m));
+    float *looked = (float *)(columns + gradient_columns_bytes(m, n, k));
     void *partial = (uint8_t *)looked + aligned(4 * i8_partial_floats(m, n));
     float *row_scales = (float *)(rows + i8_code_bytes(m, n)), *column_scales = (float *)(columns + i8_code_bytes(n, m));
     // (the gradient's rows are converted with the kernel's scales on its columns, its columns with x's on its rows)

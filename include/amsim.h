@@ -381,7 +381,8 @@ int amsim_i8_linear(const void *x, int dtype, int64_t row_stride, const void *w,
  * go onto the gradient (each product rounded to 32 bits) before that is quantised, so that the kept codes are multiplied as
  * they are: grad_x[m][k] = Q(gradient[m][n] sw[n]) along n by the kernel's codes, grad_kernel[k][n] = x's codes by
  * Q(gradient[m][n] sx[m]) along m, and grad_bias[n] the sums of the gradient's columns in 32 bits, each in its tensor's type
- * and each NULL if not wanted.  No result depends on the order of arrival. */
+ * and each NULL if not wanted (grad_x has to be where n is above 2^21, grad_kernel where m is: the reductions' lengths).  No
+ * result depends on the order of arrival. */
 size_t amsim_i8_kept_workspace_bytes(int64_t rows, int64_t length);
 size_t amsim_i8_dense_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int amsim_i8_dense(const void *x, int dtype, int64_t row_stride, const void *kernel, int kernel_dtype,
