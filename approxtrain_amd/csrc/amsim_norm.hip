@@ -420,47 +420,51 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(ColumnSums g)
 // Phi(-t) = exp(-t^2 / 2) R(t), t = |x|, and R(t) = 1/2 + w Q(w) in w = t / (1 + t / 4): what the reciprocal and Q are off by
 // counts with w, so that next to zero little is left of it.  Q's coefficients: least largest relative error of R on t <= 14.5
 // (least squares on the scaled complementary error function, the weights raised where the error was largest, one coefficient
-// after the other rounded to 32 bits), 2.1e-8.  Below -13.2, where the gelu is less than 2^-126, it comes out as zero.  Largest relative errors measured over 2^20 values
-// each: the gelu on -1 .. 0 3.1e-7, on -4 .. -1 1.2e-6, on -12 .. -4 9.2e-6 (the exponent's rounding), above zero 2e-7; in elementary
-// 32-bit operations with the language's erfcf 2.8e-7, 1.2e-6, 1.1e-5 and 2.3e-7.  Some 26 instructions, two of them at a
-// quarter rate: erfcf takes so many more that the vector units, not memory, would be the bound.
+// after the other rounded to 32 bits), 2.1e-8.  Below -13.2, where the gelu is less than 2^-126, it comes out as zero.
+// Largest relative errors, of 2^20 values each: on -1 .. 0 3.0e-7, on -4 .. -1 1.1e-6, on -12 .. -4 8.8e-6 (the exponent's
+// rounding), above zero 2.0e-7; in elementary 32-bit operations with the language's erfcf 2.8e-7, 1.1e-6, 1.1e-5 and 2.3e-7.
+// Some 20 instructions, two of them at a quarter rate: of 16-bit tensors the vector units are the bound, and erfcf takes so
+// many more that they would be of 32-bit ones.
 struct Gelu {
-    static __device__ __forceinline__ void parts(float x, float &phi, float &density)
-    {
-        const float t = fminf(fabsf(x), 15.0f), w = t * __builtin_amdgcn_rcpf(__builtin_fmaf(0.25f, t, 1.0f));
-        float q = -1.278699954809781e-07f;
-        q = __builtin_fmaf(q, w, 1.6464955479023047e-06f);
-        q = __builtin_fmaf(q, w, -2.7883238544745836e-06f);
-        q = __builtin_fmaf(q, w, -5.159039574209601e-05f);
-        q = __builtin_fmaf(q, w, 0.00010789257066790015f);
-        q = __builtin_fmaf(q, w, 0.003397819586098194f);
-        q = __builtin_fmaf(q, w, -0.032908763736486435f);
-        q = __builtin_fmaf(q, w, 0.15026246011257172f);
-        q = __builtin_fmaf(q, w, -0.3989420533180237f);
-        const float e = __builtin_amdgcn_exp2f(t * t * -0.72134752f);
-        const float tail = __builtin_fmaf(q, w, 0.5f) * e;
-        phi = x < 0.0f ? tail : 1.0f - tail;
-        density = e * 0.39894228f;
-    }
+    // R(t) and exp(-t^2 / 2)
+    struct Parts {
+        float r, e;
+        __device__ __forceinline__ explicit Parts(float x)
+        {
+            const float t = fminf(fabsf(x), 15.0f), w = t * __builtin_amdgcn_rcpf(__builtin_fmaf(0.25f, t, 1.0f));
+            float q = -1.278699954809781e-07f;
+            q = __builtin_fmaf(q, w, 1.6464955479023047e-06f);
+            q = __builtin_fmaf(q, w, -2.7883238544745836e-06f);
+            q = __builtin_fmaf(q, w, -5.159039574209601e-05f);
+            q = __builtin_fmaf(q, w, 0.00010789257066790015f);
+            q = __builtin_fmaf(q, w, 0.003397819586098194f);
+            q = __builtin_fmaf(q, w, -0.032908763736486435f);
+            q = __builtin_fmaf(q, w, 0.15026246011257172f);
+            q = __builtin_fmaf(q, w, -0.3989420533180237f);
+            r = __builtin_fmaf(q, w, 0.5f);
+            e = __builtin_amdgcn_exp2f(t * t * -0.72134752f);
+        }
+    };
     static __device__ __forceinline__ float value(float x)
     {
-        float phi, density;
-        parts(x, phi, density);
-        return x * phi;
+        const Parts p(x);
+        const float tail = p.r * p.e;
+        return x * (x < 0.0f ? tail : 1.0f - tail);
     }
+    // Phi(x) + x phi(x) = 1 + e (|x| / sqrt(2 pi) - R) above zero, 1 less that below
     static __device__ __forceinline__ float slope(float x)
     {
-        float phi, density;
-        parts(x, phi, density);
-        return __builtin_fmaf(x, density, phi);
+        const Parts p(x);
+        const float above = p.e * __builtin_fmaf(0.39894228f, fabsf(x), -p.r);
+        return x < 0.0f ? -above : 1.0f + above;
     }
 };
-// With e = exp(-x) the swish is x / (1 + e), its slope s + x s (1 - s) of s = 1 / (1 + e); 1 - s is e s where s is near one.  exp2's argument is rounded, which
-// would cost as many last places as x is large: what was lost is put back by the first term of its series.  The
-// reciprocal, a last place off by itself, is corrected by its residual.  Beyond 64 the one or the other of 1 and e is nothing beside the other,
-// and exp(x) is held 2^64 times as large, or it would be zero from -88 on, where the swish itself is so only from -104 on.
-// The swish in 32 bits is within 2.2e-7 of itself from -87 on; without the corrections within 3.9e-6, and in 16 bits 5.9375 went to its
-// farther neighbour.
+// With e = exp(-x) the swish is x / (1 + e), its slope s + x s (1 - s) of s = 1 / (1 + e); 1 - s is e s where s is near one.
+// exp2's argument is rounded, which would cost as many last places as x is large: what was lost is put back by the first
+// term of its series.  The reciprocal, a last place off by itself, is corrected by its residual.  Beyond 64 the one or the
+// other of 1 and e is nothing beside the other, and exp(x) is held 2^64 times as large, or it would be zero from -88 on, where
+// the swish itself is so only from -104 on.  In 32 bits the swish is within 2.2e-7 of itself from -87 on; without the
+// corrections within 3.9e-6, and in 16 bits 5.9375 went to its farther neighbour.
 struct Swish {
     static constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596299e-8f, LN2 = 0.693147182f;
     // exp2(x log2(e) + more)

@@ -96,8 +96,9 @@ def lineari8(x, kernel, bias=None, activation=None):
     The backward pass keeps the integers that were multiplied, a byte for each value of x, and multiplies them by the
     gradient in 8 bits: the kernel's scales go onto the gradient before it is quantised by token (x's gradient), x's before
     it is quantised by unit (the kernel's); the bias's is summed in 32 bits.  A sum has at most 2^21 terms: of more rows no
-    kernel's gradient is given, of more units no x's.  Of no rows the result is empty and the weights' gradients are zeros.  (Gradients of gradients are not provided, and a backward pass cannot be captured while a graph of
-    the same leaves from the default stream lives.)"""
+    kernel's gradient is given, of more units no x's.  Of no rows the result is empty and the weights' gradients are zeros.
+    (Gradients of gradients are not provided, and a backward pass cannot be captured while a graph of the same leaves from
+    the default stream lives.)"""
     return functors._native().lineari8(x, kernel, bias, functors._activation(activation))
 
 
