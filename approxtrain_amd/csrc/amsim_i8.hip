@@ -115,7 +115,7 @@ template <typename Op> __device__ __forceinline__ v4f over_slabs(const float *pa
 }
 
 // A workgroup of four waves takes 64 rows (a step of the columns' operand), four units in turn to a wave, whose loads are under
-// way while the slabs are joined.  Look and conversion of 4096 x 4096 to columns: f32 31 us (150 MB), bf16 23; 784 x 300 f32 9.4.
+// way while the slabs are joined.  Look and conversion of 4096 x 4096 to columns: f32 32 us (150 MB), bf16 23; 784 x 300 f32 9.7.
 template <typename T, bool MASK>
 __global__ __launch_bounds__(256) void columns_kernel(I8Columns g, const float *partial, int64_t slabs)
 {

@@ -280,7 +280,7 @@ __global__ __launch_bounds__(1024) void few_kernel(FewArgs g)
         FewSteps b;
         b.load(g, blockIdx.x, s, waves);
         // The rows' codes with them, all at once: a step's loads in their turn would each be a trip to the L2 (64 rows by
-        // 4096 x 4096: 9.5 us that way, 7.7 this; 16 rows by 4096 x 4096 5.8 and 5.7).
+        // 4096 x 4096 took 9.5 us that way and take 7.8 this; 16 rows 5.5 either way).
         v4i a[AHEAD][FA];
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) {
@@ -447,10 +447,13 @@ struct Costs {
 };
 
 // Whether few_kernel serves: a reduction beyond that needs more than one workgroup's waves, and a wider result has every workgroup
-// fetch the rows again for 16 columns.  us of the product by itself, few_kernel / tiles, of 16, 32 and 64 rows: length 4096, 4096 wide
-// 6.0/10.7, 6.2/11.0, 7.6/11.6; length 8192, 1024 wide 6.0/12.3, 7.1/11.1, 10.1/12.3; length 1024, 8192 wide 5.0/5.5, 5.2/5.8, 6.4/5.9,
-// 32768 wide 12.2/9.5, 15.1/9.7, -; length 4096, 32768 wide 32.9/28.8, 38.7/30.7, 51.0/30.9; length 16384, 1024 wide 8.9/14.5,
-// 11.1/15.1, 17.4/15.4.
+// fetch the rows again for 16 columns.  us of the product by itself, few_kernel / tiles, of 16, 32 and 64 rows:
+//   length 1024    8192 wide 4.8/5.2, 5.4/5.6, 6.2/6.1       32768 wide 12.2/9.5, 15.1/9.7, -
+//   length 4096    4096 wide 5.5/10.2, 6.9/10.7, 7.8/11.6    8192 wide 8.3/11.7, 8.7/11.7, 11.2/11.7    32768 wide 32.9/28.8, 38.7/30.7, 51.0/30.9
+//   length 8192    1024 wide 6.2/12.2, 7.6/10.7, 10.1/11.9   8192 wide 13.3/16.6, 13.9/17.0, 18.2/17.9
+//   length 16384   1024 wide 8.9/14.4, 11.2/15.1, 17.4/15.4  4096 wide 12.7/17.6, 13.9/18.3, 19.1/18.9  8192 wide 34.4/41.8, 39.8/42.5, 51.2/43.5
+// The three bounds take the quicker up to 32 rows, and of 64 up to a length of 8192 (within 2 %); 64 rows of the longest take up to
+// 1.18 times as long as in tiles.
 bool few(const Extents &e) { return e.m <= 64 && e.n <= 8192 && i8_steps(e.k) <= 256; }
 
 // the products of a list that go in tiles, and the others
@@ -487,7 +490,8 @@ int launch_few(void (*kernel)(FewArgs), const FewArgs &g, int waves, int64_t lds
     return AMSIM_OK;
 }
 // A wave for every step, and for 128 of the pieces of 8 values that are to be converted first.  Eight waves for up to four rows
-// (one token of 4096 x 4096: 6.3 us, 7.0 with sixteen; of 8192 x 8192 12.8 and 15.2), sixteen for more (8 rows: 8.8 and 8.1).
+// (calls in a row, us: one token of 4096 x 4096 6.8, 7.3 with sixteen; of 8192 x 8192 13.6 and 15.7), sixteen for more (8 rows: 8.5,
+// 10.1 with eight).
 int few_waves(const FewArgs &g, int64_t pieces)
 {
     const int most = g.rows <= 4 ? 8 : 16;
@@ -582,8 +586,9 @@ int check_workspace(const void *workspace, size_t have, size_t need)
 }
 
 // Whether few rows are converted by every workgroup that multiplies them, not once ahead, by a launch more of the device and of
-// the host.  us so, and ahead, the device alone: one token of 4096 x 4096 6.5 and 8.8, 4 rows 7.1 and 8.7, 8 rows 8.3 and 8.4; 24 rows of
-// 224 x 54 5.9 and 7.5, 32 rows of 1024 x 4096 7.9 and 7.5, 64 rows of 512 x 512 7.2 and 8.0, of 512 x 4096 8.1 and 7.7.
+// the host.  us so, and ahead, calls in a row: one token of 4096 x 4096 6.8 and 9.3, 4 rows 7.2 and 9.0, 8 rows 8.7 and 8.9; one of
+// 8192 x 8192 13.8 and 15.6; 13 rows of 2051 x 1003 in 32 bits 7.2 and 7.7; 24 rows of 224 x 54 6.0 and 7.6, 32 rows of 1024 x 1024 7.4 and
+// 8.4, of 1024 x 4096 7.9 and 8.0, 64 rows of 512 x 512 8.0 and 7.7, of 512 x 4096 8.3 and 7.8.
 bool converts_on_the_way(int64_t m, int64_t n, int64_t k) { return m <= 64 && m * i8_steps(k) * I8_STEP * ceil_div64(n, 4096) <= RAW_VALUES; }
 
 size_t aligned(int64_t bytes) { return ((size_t)bytes + 255) / 256 * 256; }

@@ -135,10 +135,11 @@ template <typename T, typename C> int launch(const I8Rows *rows, const I8Columns
 
 }  // namespace
 
-// us of a call so, and in two launches (all on the device): gradients of a 128 x 784 x 300 layer 9.7 and 15.7, a training step of 64 x 100 x
-// 100 22 and 33, of 256 x 512 x 512 25 and 31, columns of 512 x 512 bf16 7.7 and 9.5, of 250 x 8000 f32 5.3 and 10.0; but of 784 x 300
-// 11.6 and 9.5, of 1000 x 1000 12.9 and 9.6: few workgroups read long columns twice.  Up to 2^18 values that is less than the
-// launch that the host saves (2.5 us), for which such layers' steps wait.
+// us of a call so, and in two launches, calls in a row: gradients of a 128 x 784 x 300 layer 10.2 and 15.7, a training step of 64 x 100 x
+// 100 21 and 32, of 256 x 512 x 512 24 and 32, columns of 512 x 512 bf16 8.1 and 9.5, of 250 x 8000 f32 6.2 and 10.0; but of 784 x 300
+// 11.7 and 9.7, the forward pass of 128 x 784 x 300 18.2 and 16.5, columns of 1000 x 250 15.7 and 11.0: few workgroups read long columns
+// twice.  Up to 2^18 values they take one launch all the same: a training step of such layers waits for the host, which saves
+// 2.5 us with it.  (A captured step does not wait so, and is 2 to 5 us slower for it.)
 bool i8_small(const I8Rows *rows, const I8Columns &columns)
 {
     if (columns.rows > 512 && (columns.rows > 1024 || columns.rows * columns.cols > 1 << 18)) return false;

@@ -53,8 +53,8 @@ template <typename S> struct Place {
     const Place<S> place{(int)threadIdx.x % S::LANES, (int)threadIdx.x / S::LANES, part_}
 
 // ---- layer norm, forward ----------------------------------------------------------------------------------------------
-// Moves each value twice, and a byte more where it is kept: 16384 x 4096 bf16 53 us (268 MB, 5.1 TB/s), kept 62 to 65 (335 MB); 256 x
-// 512 f32 3.4, the latency of a load, two sums over the lanes and a store.
+// Moves each value twice, and a byte more where it is kept: 16384 x 4096 bf16 54 us (268 MB, 5.0 TB/s), kept 62 to 66 (335 MB); 256 x
+// 512 f32 3.3, the latency of a load, two sums over the lanes and a store.
 
 struct NormArgs {
     const void *x;
@@ -139,7 +139,8 @@ __global__ __launch_bounds__(S::THREADS) void norm_kernel(NormArgs g)
     }
 }
 
-// rows that no workgroup holds: read for the sum, for the squares, and for the results
+// rows that no workgroup holds: read for the sum, for the squares, and for the results (2048 x 32768 bf16 101 us, kept 112; as many values in
+// rows of 16384 that are held 60)
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs g)
 {
@@ -227,7 +228,7 @@ template <typename T, bool KEPT, typename Raw> __device__ __forceinline__ void i
 
 // dx needs two sums over the row, which meet in one pass over the lanes.  The gradients of gamma and beta: a lane adds up its
 // columns over the rows that it sees; a workgroup's go to memory once, and column_sums_kernel adds those in their order.
-// 16384 x 4096 bf16 from x 88 us, from 8 bits 72 (335 MB and 25 of sums, 5.0 TB/s), the sums' launch 5 to 6.
+// 16384 x 4096 bf16 with the sums' launch, 5 to 6 us of it: from x 87 us (403 MB and 25 of sums, 4.9 TB/s), from 8 bits 73 (335 and 25).
 template <typename T, typename S, bool KEPT>
 __global__ __launch_bounds__(S::THREADS) void norm_grad_kernel(NormGradArgs g)
 {
@@ -327,7 +328,8 @@ __global__ __launch_bounds__(S::THREADS) void norm_grad_kernel(NormGradArgs g)
     }
 }
 
-// rows that no workgroup holds: dx by rows, dgamma and dbeta by columns, a slab of rows to a workgroup
+// rows that no workgroup holds: dx by rows, dgamma and dbeta by columns, a slab of rows to a workgroup (2048 x 32768 bf16 from x 171 us, from 8
+// bits 143: gradient and input are read three times; as many values in rows of 16384 from x 90)
 template <typename T, bool KEPT>
 __global__ __launch_bounds__(1024) void norm_grad_long_kernel(NormGradArgs g)
 {
@@ -493,8 +495,9 @@ struct Linear {  // (nothing but the keeping)
     static __device__ __forceinline__ float slope(float) { return 1.0f; }
 };
 
-// A row's values stay as they came between the search for the largest, the codes and the function: 16384 x 4096 bf16 58 us
-// (335 MB, 5.8 TB/s; a quarter of the vector units' time), 8192 x 2048 f32 27.
+// A row's values stay as they came between the search for the largest, the codes and the function.  16384 x 4096 bf16 gelu 61 to 64 us
+// (335 MB): the vector units are the bound, 34 instructions of four cycles for 64 values, 1.41e8 of the SIMDs' 1.44e8 cycles;
+// swish 58.  8192 x 2048 f32 27 (151 MB, 5.5 TB/s), the vector units half of it.  Rows past 16384 are read twice: 2048 x 32768 bf16 88.
 struct ActArgs {
     const void *x;
     int64_t rows, stride, cols;
@@ -582,7 +585,8 @@ __global__ __launch_bounds__(1024) void activation_long_kernel(ActArgs g)
     }
 }
 
-// dx = dy f'(what was kept); without dy: what was kept.  Bound by memory: 16384 x 4096 bf16 60 us (335 MB, 5.5 TB/s).
+// dx = dy f'(what was kept); without dy: what was kept.  16384 x 4096 bf16 gelu 64 us (335 MB), again 33 instructions a value; 8192 x 2048
+// f32 29, bound by memory (151 MB, 5.2 TB/s).
 struct ActGradArgs {
     const void *grad;  // or null
     int64_t rows, stride, cols;
@@ -628,9 +632,11 @@ template <typename S> unsigned workgroups(int64_t rows)
     return (unsigned)std::min<int64_t>(ceil_div64(rows, S::ROWS), 256 * to_a_cu);
 }
 unsigned long_workgroups(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 512); }
-// ... of the backward pass, each of which leaves 2 x cols sums to be added up: as many as the card holds, but at least four
-// rows, or groups of rows, to each (65536 x 512 bf16: 45 us with 1280, 57 with 512; 16384 x 4096 bf16: 72 with 768, 89 with 1024; 8192 x
-// 512 f32: 13.8 with 512, 15.3 with 1280).
+// ... of the backward pass, each of which leaves 2 x cols sums to be added up: as many as the card holds, from 1024 rows (or groups of
+// rows) on at least four to each, below that up to 256 workgroups, of one row each up to 256 rows (65536 x 512 bf16: 45 us with 1280,
+// 57 with 512; 16384 x 4096 bf16: 72 with 768, 89 with 1024; 8192 x 512 f32: 13.8 with 512, 15.3 with 1280).  Few wide rows so write
+// more sums than they have values: 256 x 16384 bf16 21 us, 34 MB of sums written and read beside 25 MB of tensors; 512 x 16384 25, 256 x 8192
+// 13, 512 x 8192 15, 1024 x 8192 19.
 constexpr int64_t GRAD_SLABS = 64;
 int64_t grad_parts(int64_t rows, int64_t cols)
 {
