@@ -425,8 +425,8 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(ColumnSums g)
 // after the other rounded to 32 bits), 2.1e-8.  Below -13.2, where the gelu is less than 2^-126, it comes out as zero.
 // Largest relative errors, of 2^20 values each: on -1 .. 0 3.0e-7, on -4 .. -1 1.1e-6, on -12 .. -4 8.8e-6 (the exponent's
 // rounding), above zero 2.0e-7; in elementary 32-bit operations with the language's erfcf 2.8e-7, 1.1e-6, 1.1e-5 and 2.3e-7.
-// Some 20 instructions, two of them at a quarter rate: of 16-bit tensors the vector units are the bound, and erfcf takes so
-// many more that they would be of 32-bit ones.
+// Some 20 instructions, two of them at a quarter rate: with 16-bit tensors the vector units are about as busy as memory, and
+// erfcf takes so many more that they would be the bound of 32-bit ones too.
 struct Gelu {
     // R(t) and exp(-t^2 / 2)
     struct Parts {
@@ -496,8 +496,9 @@ struct Linear {  // (nothing but the keeping)
 };
 
 // A row's values stay as they came between the search for the largest, the codes and the function.  16384 x 4096 bf16 gelu 61 to 64 us
-// (335 MB): the vector units are the bound, 34 instructions of four cycles for 64 values, 1.41e8 of the SIMDs' 1.44e8 cycles;
-// swish 58.  8192 x 2048 f32 27 (151 MB, 5.5 TB/s), the vector units half of it.  Rows past 16384 are read twice: 2048 x 32768 bf16 88.
+// (335 MB, 5.2 to 5.5 TB/s) beside 34 vector instructions for 64 values, of two cycles each, or four with a literal: most of the
+// SIMDs' time; swish 58.  8192 x 2048 f32 27 (151 MB, 5.5 TB/s), the vector units at most half of it.  Rows past 16384 are read
+// twice: 2048 x 32768 bf16 88.
 struct ActArgs {
     const void *x;
     int64_t rows, stride, cols;
@@ -585,8 +586,8 @@ __global__ __launch_bounds__(1024) void activation_long_kernel(ActArgs g)
     }
 }
 
-// dx = dy f'(what was kept); without dy: what was kept.  16384 x 4096 bf16 gelu 64 us (335 MB), again 33 instructions a value; 8192 x 2048
-// f32 29, bound by memory (151 MB, 5.2 TB/s).
+// dx = dy f'(what was kept); without dy: what was kept.  16384 x 4096 bf16 gelu 64 us (335 MB), 33 instructions a value; it took 69 where
+// the slope had one more.  8192 x 2048 f32 29, bound by memory (151 MB, 5.2 TB/s).
 struct ActGradArgs {
     const void *grad;  // or null
     int64_t rows, stride, cols;
